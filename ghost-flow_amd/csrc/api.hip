@@ -128,6 +128,91 @@ int sgemm_common(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, floa
 
 }  // namespace
 
+namespace {
+
+int elem_bytes(int dtype) { return dtype == GFH_F32 ? 4 : 2; }
+
+// The checks that both calls over a paged cache make of it and of the batch.
+int check_paged(const char *who, const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads) {
+    if (!kv) return set_error(GFH_NULL_POINTER, "%s: kv is NULL", who);
+    const bool types = kv->dtype == GFH_F16 || kv->dtype == GFH_BF16 || kv->dtype == GFH_F32;
+    if (!types || !(dtype == kv->dtype || (dtype == GFH_F32 && kv->dtype == GFH_BF16)))
+        return set_error(GFH_INVALID_DATA,
+                         "%s: activations of dtype %d over a cache of dtype %d (the same, or f32 over bf16)", who,
+                         dtype, kv->dtype);
+    if (kv->head_dim < 8 || kv->head_dim > 128 || kv->head_dim % 8 != 0)
+        return set_error(GFH_INVALID_SHAPE, "%s: head_dim %lld must be a multiple of 8 in [8, 128]", who,
+                         (long long)kv->head_dim);
+    if (heads <= 0 || kv->kv_heads <= 0 || heads > 65535 || heads % kv->kv_heads != 0)
+        return set_error(GFH_INVALID_SHAPE, "%s: %lld heads must be a multiple of %lld kv_heads", who,
+                         (long long)heads, (long long)kv->kv_heads);
+    constexpr int64_t kMost = (int64_t)1 << 30;
+    if (kv->num_pages < 0 || kv->num_pages > kMaxDim || kv->page_size < 1 || kv->page_size > kMost ||
+        kv->max_pages < 0 || kv->max_pages > kMost || kv->max_pages * kv->page_size > kMost)
+        return set_error(GFH_INVALID_SHAPE, "%s: num_pages=%lld page_size=%lld max_pages=%lld out of range", who,
+                         (long long)kv->num_pages, (long long)kv->page_size, (long long)kv->max_pages);
+    if (tokens < 0 || tokens > kMost || kv->num_seqs < 0 || kv->num_seqs > (1 << 22) || tokens * heads > kMost)
+        return set_error(GFH_INVALID_SHAPE, "%s: tokens=%lld heads=%lld num_seqs=%lld out of range", who,
+                         (long long)tokens, (long long)heads, (long long)kv->num_seqs);
+    if (kv->table_stride < kv->max_pages)
+        return set_error(GFH_INVALID_SHAPE, "%s: table_stride %lld is below max_pages %lld", who,
+                         (long long)kv->table_stride, (long long)kv->max_pages);
+    const int64_t whole = 16 / elem_bytes(kv->dtype);
+    if (kv->page_stride < 0 || kv->row_stride < 0 || kv->head_stride < 0 || kv->page_stride % whole ||
+        kv->row_stride % whole || kv->head_stride % whole)
+        return set_error(GFH_INVALID_SHAPE, "%s: page, row and head strides must be whole 16-byte steps", who);
+    return GFH_SUCCESS;
+}
+
+int check_paged_memory(const char *who, const gfh_paged_kv *kv) {
+    int64_t e = 0, a, b, c;
+    if (kv->num_pages > 0) {
+        if (!mul_ok(kv->num_pages - 1, kv->page_stride, &a) || !mul_ok(kv->page_size - 1, kv->row_stride, &b) ||
+            !mul_ok(kv->kv_heads - 1, kv->head_stride, &c) || !count_ok({a + b, 4}) || !count_ok({a + b + c, 4}))
+            return set_error(GFH_INVALID_SHAPE, "%s: cache extent overflows", who);
+        e = a + b + c + kv->head_dim;
+    }
+    int64_t t;
+    if (!extent2d(kv->num_seqs, kv->max_pages, kv->table_stride, &t))
+        return set_error(GFH_INVALID_SHAPE, "%s: page_table extent overflows", who);
+    const size_t eb = (size_t)elem_bytes(kv->dtype);
+    GFH_TRY(require_range(kv->k_pages, (size_t)e * eb, "k_pages"));
+    GFH_TRY(require_range(kv->v_pages, (size_t)e * eb, "v_pages"));
+    GFH_TRY(require_range(kv->page_table, (size_t)t * 4, "page_table"));
+    GFH_TRY(require_range(kv->kv_lens, (size_t)kv->num_seqs * 4, "kv_lens"));
+    GFH_TRY(require_range(kv->q_offsets, (size_t)(kv->num_seqs + 1) * 4, "q_offsets"));
+    GFH_TRY(optional_range(kv->status, 4, "status"));
+    if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages))
+        return set_error(GFH_INVALID_DATA, "%s: k_pages and v_pages must be 16-byte aligned", who);
+    return GFH_SUCCESS;
+}
+
+// rows of `heads` heads, ld elements apart, whole 16-byte steps
+int check_rows(const char *who, const void *p, const char *name, int dtype, int64_t tokens, int64_t heads, int64_t d,
+               int64_t ld) {
+    int64_t e;
+    if (ld < heads * d || ld % (16 / elem_bytes(dtype)) != 0)
+        return set_error(GFH_INVALID_SHAPE, "%s: rows of %s, %lld apart, must be whole 16-byte steps >= %lld", who,
+                         name, (long long)ld, (long long)(heads * d));
+    if (!extent2d(tokens, heads * d, ld, &e))
+        return set_error(GFH_INVALID_SHAPE, "%s: extent of %s overflows", who, name);
+    GFH_TRY(require_range(p, (size_t)e * elem_bytes(dtype), name));
+    if (!aligned16(p)) return set_error(GFH_INVALID_DATA, "%s: %s must be 16-byte aligned", who, name);
+    return GFH_SUCCESS;
+}
+
+PagedAttnDesc paged_attn_desc(const gfh_paged_kv &kv, int64_t tokens, int64_t heads, int64_t max_kv_len) {
+    PagedAttnDesc d;
+    d.kv = kv;
+    d.tokens = tokens;
+    d.heads = heads;
+    const int64_t capacity = kv.max_pages * kv.page_size;
+    d.max_kv_len = max_kv_len <= 0 || max_kv_len > capacity ? capacity : max_kv_len;
+    return d;
+}
+
+}  // namespace
+
 extern "C" {
 
 GFH_API int gfh_init(void) {
@@ -861,6 +946,96 @@ GFH_API int gfh_swiglu_i8(const float *x, int64_t m, int64_t hidden, int64_t int
         d.y = y;
         d.h = h;
         return launch_swiglu_i8(d, ws.ptr(), s);
+    });
+}
+
+GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads, const void *q,
+                             int64_t ldq, void *q_out, int64_t ldqo, const void *k, int64_t ldk, const void *v,
+                             int64_t ldv, const float *rope_cos, const float *rope_sin, int64_t rope_rows,
+                             int64_t rotary_dim, int interleaved, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "paged_append";
+        GFH_TRY(check_paged(who, kv, dtype, tokens, heads));
+        if (!q != !q_out) return set_error(GFH_NULL_POINTER, "%s: q and q_out are given together", who);
+        if (!rope_cos != !rope_sin)
+            return set_error(GFH_NULL_POINTER, "%s: rope_cos and rope_sin are given together", who);
+        const int64_t capacity = kv->max_pages * kv->page_size;
+        if (rope_cos && (rotary_dim < 8 || rotary_dim % 8 != 0 || rotary_dim > kv->head_dim))
+            return set_error(GFH_INVALID_SHAPE, "%s: rotary_dim %lld must be a multiple of 8 in [8, head_dim]", who,
+                             (long long)rotary_dim);
+        if (rope_cos && (rope_rows < capacity || rope_rows > ((int64_t)1 << 40)))
+            return set_error(GFH_INVALID_SHAPE, "%s: angles of %lld positions, the page table holds %lld", who,
+                             (long long)rope_rows, (long long)capacity);
+        if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
+        GFH_TRY(check_paged_memory(who, kv));
+        if (q) {
+            GFH_TRY(check_rows(who, q, "q", dtype, tokens, heads, kv->head_dim, ldq));
+            GFH_TRY(check_rows(who, q_out, "q_out", dtype, tokens, heads, kv->head_dim, ldqo));
+            if (q == q_out && ldq != ldqo)
+                return set_error(GFH_INVALID_SHAPE, "%s: q_out on q needs the same rows", who);
+        }
+        GFH_TRY(check_rows(who, k, "k", dtype, tokens, kv->kv_heads, kv->head_dim, ldk));
+        GFH_TRY(check_rows(who, v, "v", dtype, tokens, kv->kv_heads, kv->head_dim, ldv));
+        if (rope_cos) {
+            GFH_TRY(require_range(rope_cos, (size_t)rope_rows * (rotary_dim / 2) * 4, "rope_cos"));
+            GFH_TRY(require_range(rope_sin, (size_t)rope_rows * (rotary_dim / 2) * 4, "rope_sin"));
+            if (!aligned16(rope_cos) || !aligned16(rope_sin))
+                return set_error(GFH_INVALID_DATA, "%s: rope_cos and rope_sin must be 16-byte aligned", who);
+        }
+        GFH_TRY(ensure_init());
+        PagedAppendDesc d;
+        d.kv = *kv;
+        d.dtype = dtype;
+        d.tokens = tokens;
+        d.heads = heads;
+        d.q = q, d.k = k, d.v = v;
+        d.q_out = q_out;
+        d.ldq = ldq, d.ldqo = ldqo, d.ldk = ldk, d.ldv = ldv;
+        d.cos = rope_cos, d.sin = rope_sin;
+        d.rotary_dim = rotary_dim;
+        d.interleaved = interleaved != 0;
+        return launch_paged_append(d, as_stream(stream));
+    });
+}
+
+GFH_API size_t gfh_paged_attention_workspace_size(const gfh_paged_kv *kv, int64_t tokens, int64_t heads,
+                                                  int64_t max_kv_len) {
+    if (!kv || check_paged("paged_attention", kv, kv->dtype, tokens, heads) != GFH_SUCCESS || tokens == 0 ||
+        kv->num_seqs == 0)
+        return 0;
+    return paged_attention_workspace_bytes(paged_attn_desc(*kv, tokens, heads, max_kv_len));
+}
+
+GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads, const void *q,
+                                int64_t ldq, void *out, int64_t ldo, float scale, int causal, int64_t window,
+                                int64_t max_kv_len, void *workspace, size_t workspace_bytes, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "paged_attention";
+        GFH_TRY(check_paged(who, kv, dtype, tokens, heads));
+        if (window < 0) return set_error(GFH_INVALID_SHAPE, "%s: window %lld", who, (long long)window);
+        if (!std::isfinite(scale)) return set_error(GFH_INVALID_DATA, "%s: scale is not finite", who);
+        if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
+        GFH_TRY(check_paged_memory(who, kv));
+        GFH_TRY(check_rows(who, q, "q", dtype, tokens, heads, kv->head_dim, ldq));
+        GFH_TRY(check_rows(who, out, "out", dtype, tokens, heads, kv->head_dim, ldo));
+        if (q == out && ldq != ldo) return set_error(GFH_INVALID_SHAPE, "%s: out on q needs the same rows", who);
+        if (workspace && !aligned16(workspace))
+            return set_error(GFH_INVALID_DATA, "%s: the workspace must be 16-byte aligned", who);
+        GFH_TRY(ensure_init());
+        PagedAttnDesc d = paged_attn_desc(*kv, tokens, heads, max_kv_len);
+        d.dtype = dtype;
+        d.q = q;
+        d.ldq = ldq;
+        d.out = out;
+        d.ldo = ldo;
+        d.scale = scale;
+        d.causal = causal != 0;
+        d.window = window;
+        hipStream_t s = as_stream(stream);
+        Scratch ws;
+        const size_t need = paged_attention_workspace_bytes(d);
+        if (need) GFH_TRY(ws.acquire(workspace, workspace_bytes, need, s));
+        return launch_paged_attention(d, ws.ptr(), s);
     });
 }
 

@@ -6,6 +6,8 @@
 
 #include <cstdint>
 
+#include "ghostflow_hip.h"
+
 namespace gfh {
 
 struct SgemmDesc {
@@ -173,6 +175,42 @@ struct KvAttnDesc {
     bool causal = false;
 };
 int launch_kv_attention(const KvAttnDesc &d, hipStream_t s);
+
+// A ragged batch over a cache in pages (paged_kv.hpp, ghostflow_hip.h); dtype
+// is the activations' type, strides are in elements.
+namespace paged {
+struct View;
+}
+paged::View paged_view(const gfh_paged_kv &kv, int64_t tokens, int64_t heads);
+// paged_append.hip: q is nullable, cos / sin nullable (nothing is turned).
+struct PagedAppendDesc {
+    gfh_paged_kv kv{};
+    int dtype = 0;
+    int64_t tokens = 0, heads = 0;
+    const void *q = nullptr, *k = nullptr, *v = nullptr;
+    void *q_out = nullptr;
+    int64_t ldq = 0, ldqo = 0, ldk = 0, ldv = 0;
+    const float *cos = nullptr, *sin = nullptr;
+    int64_t rotary_dim = 0;
+    bool interleaved = false;
+};
+int launch_paged_append(const PagedAppendDesc &d, hipStream_t s);
+// paged_attention.hip: max_kv_len in [0, capacity] is what the work is split
+// by; any length is served.  window 0: none.
+struct PagedAttnDesc {
+    gfh_paged_kv kv{};
+    int dtype = 0;
+    int64_t tokens = 0, heads = 0;
+    const void *q = nullptr;
+    int64_t ldq = 0;
+    void *out = nullptr;
+    int64_t ldo = 0;
+    float scale = 1.f;
+    bool causal = false;
+    int64_t window = 0, max_kv_len = 0;
+};
+size_t paged_attention_workspace_bytes(const PagedAttnDesc &d);
+int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t s);
 
 // mha.hip: MultiHeadAttention::forward_with_cache over a [b, capacity, e]
 // K/V cache; the workspace holds the projected queries and the attention

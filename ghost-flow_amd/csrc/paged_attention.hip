@@ -1,0 +1,1116 @@
+// paged_attention.hip -- attention of a ragged batch's new tokens (one each,
+// or chunks of a prompt) over a key/value cache in pages (paged_kv.hpp).
+//
+//   S = scale q . k,  P = softmax over the keys the token sees,  O = P V
+//
+// A token at position p sees key j of its sequence when j < kv_len, j <= p if
+// causal, j > p - window if there is a window; a token that sees none gets 0.
+// The G = heads / kv_heads query heads of a key/value head read the same keys,
+// so the rows of a product are (token, head of the group) pairs: row R = token
+// * G + g, and a tile is BM consecutive rows of one sequence and key/value
+// head.  Tiles lie at multiples of BM rows of the whole batch: tile j of
+// sequence s has the number j + s, which no other tile has (a sequence starts
+// in the tile row where the one before ends, or later), so a workgroup finds
+// its sequence with one search for the largest s with offset(s) G / BM + s <=
+// number, and the host needs no length.
+//
+// Softmax online in base 2, statistics and sums in fp32: the running maximum
+// is of the raw dot products, a probability is exp2(s c - m c + bias) with c =
+// |scale| log2 e (the sign of the scale is on q).  The bias (14 for f16, 16
+// where P is split) keeps small probabilities normal in their 16-bit form and
+// cancels in O / l.  Long axes are split over workgroups; a second kernel joins
+// the parts in their order, so results do not depend on timing.
+//
+// Rows of the cache past the last key and pages outside the cache read as
+// zeros.  A masked key must not reach a row even when its value is not
+// finite (0 * inf): a tile that holds keys which some of its rows do not see
+// is searched for such values, and its workgroup then redoes its rows one by
+// one over the keys they see (slow_rows).
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "paged_kv.hpp"
+#include "paged_types.hpp"
+#include "split_bf16.hpp"
+
+namespace gfh {
+namespace {
+
+using paged::View;
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void *lds_ptr_t;
+typedef __attribute__((address_space(1))) void *glb_ptr_t;
+
+struct AttnParams {
+    View c;
+    const char *q;
+    char *out;
+    int64_t ldq, ldo;  // elements between tokens
+    float sc2;         // |scale| log2 e
+    bool negate;       // scale < 0
+    bool causal;
+    int window;  // 0: none
+    int ntiles, nsplit, chunk;
+    int min_rows, max_rows;  // sequences this launch takes: rows = tokens * group
+    float *acc;   // [tokens * heads][nsplit][d] parts, where nsplit > 1
+    float2 *ml;   // [tokens * heads][nsplit] their maximum (scaled) and sum
+};
+
+// A workgroup's rows [r0, r1) and the keys [lo, hi) that any of them sees.
+struct Rows {
+    int r0, r1, base;   // base: the tile's first row, r0 >= base
+    int q_last;         // position of the sequence's token t is t + q_last
+    int kv_len;
+    int lo, hi;
+};
+
+__device__ __forceinline__ bool find_rows(const AttnParams &p, int number, int bm, int lane, Rows &t) {
+    const View &c = p.c;
+    const int n = paged::wave_leading(c.num_seqs, lane, [&](int s) {
+        return (int)((unsigned)(paged::offset_at(c, s) * c.group) / (unsigned)bm) + s <= number;
+    });
+    if (n == 0) return false;
+    const int s = n - 1;
+    const int o0 = paged::offset_at(c, s), o1 = max(o0, paged::offset_at(c, s + 1));
+    t.base = (number - s) * bm;
+    t.r0 = max(o0 * c.group, t.base);
+    t.r1 = min(o1 * c.group, t.base + bm);
+    const int rows = (o1 - o0) * c.group;
+    if (t.r0 >= t.r1 || rows < p.min_rows || rows > p.max_rows) return false;
+    t.kv_len = paged::length_at(c, s);
+    t.q_last = t.kv_len - o1;
+    const int first = t.r0 / c.group + t.q_last, last = (t.r1 - 1) / c.group + t.q_last;
+    t.hi = max(0, p.causal ? min(t.kv_len, last + 1) : t.kv_len);
+    t.lo = p.window ? min(t.hi, max(0, first - p.window + 1)) : 0;
+    return true;
+}
+// (the sequence again, for its row of the table)
+__device__ __forceinline__ int seq_of(const AttnParams &p, int number, const Rows &t, int bm) {
+    return number - t.base / bm;
+}
+
+// The splits that have keys (at least one, which writes rows without any).
+__device__ __forceinline__ int active_splits(const AttnParams &p, const Rows &t) {
+    return max(1, min(p.nsplit, (t.hi - t.lo + p.chunk - 1) / p.chunk));
+}
+
+// The keys [jmin, jmax] that row r of the batch sees.
+__device__ __forceinline__ void row_keys(const AttnParams &p, const Rows &t, int r, int &jmin, int &jmax) {
+    const bool ok = r >= t.r0 && r < t.r1;
+    const int pos = r / p.c.group + t.q_last;
+    jmax = !ok ? -1 : p.causal ? min(pos, t.kv_len - 1) : t.kv_len - 1;
+    jmin = ok && p.window ? pos - p.window + 1 : 0;
+}
+
+template <typename T>
+__device__ __forceinline__ const T *q_row(const AttnParams &p, int r, int kvh) {
+    const int tok = r / p.c.group, g = r - tok * p.c.group;
+    return reinterpret_cast<const T *>(p.q) + tok * p.ldq + (int64_t)(kvh * p.c.group + g) * p.c.d;
+}
+template <typename T>
+__device__ __forceinline__ T *out_row(const AttnParams &p, int r, int kvh) {
+    const int tok = r / p.c.group, g = r - tok * p.c.group;
+    return reinterpret_cast<T *>(p.out) + tok * p.ldo + (int64_t)(kvh * p.c.group + g) * p.c.d;
+}
+__device__ __forceinline__ int64_t part_row(const AttnParams &p, int r, int kvh) {
+    const int tok = r / p.c.group, g = r - tok * p.c.group;
+    return (int64_t)tok * p.c.heads + kvh * p.c.group + g;
+}
+
+// The rows of a tile one by one, a wave each, over the keys [b, e) that each
+// sees, in fp32: for the inputs named above.
+template <typename TA, typename TC>
+__device__ __forceinline__ void slow_rows(const AttnParams &p, const Rows &t, int seq, int kvh, int b, int e,
+                                                    int split, bool parts, float bias, int wave, int nwaves,
+                                                    int lane) {
+    const View &c = p.c;
+    for (int r = t.r0 + wave; r < t.r1; r += nwaves) {
+        int jmin, jmax;
+        row_keys(p, t, r, jmin, jmax);
+        const TA *q = q_row<TA>(p, r, kvh);
+        float qv[2], acc[2] = {0.f, 0.f}, m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) qv[i] = lane + 64 * i < c.d ? (float)q[lane + 64 * i] * (p.negate ? -1.f : 1.f) : 0.f;
+        for (int j = max(b, jmin); j < min(e, jmax + 1); ++j) {
+            const int pg = paged::page_of(c, j), page = c.table[seq * c.table_stride + pg];
+            const bool ok = page >= 0 && page < c.num_pages;
+            const int64_t at = ok ? page * c.page_stride + (int64_t)(j - pg * c.page_size) * c.row_stride +
+                                        kvh * c.head_stride
+                                  : 0;
+            float kv[2], vv[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const bool in = ok && lane + 64 * i < c.d;
+                kv[i] = in ? (float)reinterpret_cast<const TC *>(c.k)[at + lane + 64 * i] : 0.f;
+                vv[i] = in ? (float)reinterpret_cast<const TC *>(c.v)[at + lane + 64 * i] : 0.f;
+            }
+            const float s = wave_sum(fmaf(qv[1], kv[1], qv[0] * kv[0])) * p.sc2;
+            const float m_new = max_nan(m, s);
+            if (m_new == -INFINITY) continue;
+            if (m_new != m_new) {  // so is the row
+                m = l = acc[0] = acc[1] = m_new;
+                break;
+            }
+            const float alpha = exp2f(m - m_new), w = exp2f(s - m_new + bias);
+            l = fmaf(l, alpha, w);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) acc[i] = fmaf(acc[i], alpha, w * vv[i]);
+            m = m_new;
+        }
+        if (parts) {
+            const int64_t at = part_row(p, r, kvh) * p.nsplit + split;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (lane + 64 * i < c.d) p.acc[at * c.d + lane + 64 * i] = acc[i];
+            if (lane == 0) p.ml[at] = make_float2(m, l);
+        } else {
+            const float inv = m == -INFINITY ? 0.f : 1.0f / l;
+            TA *o = out_row<TA>(p, r, kvh);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (lane + 64 * i < c.d) o[lane + 64 * i] = (TA)(acc[i] * inv);
+        }
+    }
+}
+
+// ---- 16-bit types ---------------------------------------------------------------
+
+template <typename T>
+struct Half;
+template <>
+struct Half<__bf16> {
+    typedef bf16x2 v2;
+    typedef bf16x4 v4;
+    typedef bf16x8 v8;
+    static constexpr uint32_t kExp = 0x7f80u;
+    static constexpr float kBias = 0.f;
+    static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Half<_Float16> {
+    typedef f16x2 v2;
+    typedef f16x4 v4;
+    typedef f16x8 v8;
+    static constexpr uint32_t kExp = 0x7c00u;
+    static constexpr float kBias = 14.f;
+    static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// (x, y) as 16-bit pairs: one rounded to nearest (NP = 1), or their three
+// bf16 pieces (split_bf16.hpp).
+template <typename T, int NP>
+__device__ __forceinline__ void pieces2(float x, float y, uint32_t (&w)[NP]) {
+    if constexpr (NP == 1) {
+        const f32x2 v = {x, y};
+        w[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, typename Half<T>::v2));
+    } else {
+        split2(x, y, w[0], w[1], w[2]);
+    }
+}
+
+// Where a 16-byte chunk of a K or V row lies in LDS: rows of DP elements, the
+// chunk's number XORed with bits of its key so that
+//  * a K fragment read (16 or 32 keys at one chunk) and
+//  * a transposing V read (4 keys x 16 dims per 16 lanes, groups 4 keys or 16
+//    dims apart)
+// fall on all banks evenly.
+template <int DP>
+__device__ __forceinline__ int swz_k(int key) {
+    return DP == 128 ? key & 15 : (key >> 1) & 7;
+}
+template <int DP>
+__device__ __forceinline__ int swz_v(int key) {
+    return DP == 128 ? ((key & 3) << 2) ^ (((key >> 2) & 1) << 1) : (((key >> 1) & 1) << 2) ^ (((key >> 2) & 1) << 1);
+}
+
+__device__ __attribute__((aligned(16))) uint32_t g_zero_chunk[4];
+
+constexpr int kMaxPages = 1024;  // page offsets held in LDS: keys per pass >= kMaxPages
+
+// Byte offsets of the pages of keys [b, e) into LDS, -1 for a page outside
+// the cache; returns the end of the keys they cover.
+__device__ __forceinline__ int stage_pages(const View &c, int seq, int b, int e, int elem, int64_t *lds, int tid,
+                                           int nthreads) {
+    const int p0 = paged::page_of(c, b);
+    const int n = min(kMaxPages, paged::page_of(c, e - 1) - p0 + 1);
+    for (int i = tid; i < n; i += nthreads) {
+        const int page = c.table[seq * c.table_stride + p0 + i];
+        const bool ok = page >= 0 && page < c.num_pages;
+        if (!ok) paged::raise(c, paged::kBadPage);
+        lds[i] = ok ? page * c.page_stride * elem : -1;
+    }
+    return (int)min((int64_t)e, (int64_t)(p0 + n) * c.page_size);
+}
+
+// One wave's requests for KEYS keys from k0 of K and V straight into LDS (16
+// bytes per lane; keys from e on and dims past d read zeros).
+template <int DP, int KEYS, int WAVES>
+__device__ __forceinline__ void request(const View &c, int kvh, const int64_t *pages, int p0, int k0, int e, char *kl,
+                                        char *vl, int wave, int lane) {
+    constexpr int kRowChunks = DP / 8, kRowsPer = 64 / kRowChunks;
+    constexpr int kInstr = KEYS / kRowsPer / WAVES;
+    static_assert(kInstr * kRowsPer * WAVES == KEYS, "whole instructions per wave");
+#pragma unroll
+    for (int i = 0; i < kInstr; ++i) {
+        const int ins = wave * kInstr + i;
+        const int row = ins * kRowsPer + lane / kRowChunks, ch = lane % kRowChunks;
+        const int key = min(k0 + row, e - 1), pg = paged::page_of(c, key);
+        const int64_t off = pages[pg - p0];
+        const int64_t at = off + 2 * ((int64_t)(key - pg * c.page_size) * c.row_stride + kvh * c.head_stride);
+        const bool ok = k0 + row < e && off >= 0;
+        const int ck = ch ^ swz_k<DP>(row), cv = ch ^ swz_v<DP>(row);
+        const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
+        const char *ks = ok && ck * 8 < c.d ? c.k + at + ck * 16 : zero;
+        const char *vs = ok && cv * 8 < c.d ? c.v + at + cv * 16 : zero;
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)ks, (lds_ptr_t)(kl + ins * 1024), 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)vs, (lds_ptr_t)(vl + ins * 1024), 16, 0, 0);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ typename Half<T>::v4 read_tr(const char *lds) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(typename Half<T>::v4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                        (__attribute__((address_space(3))) s4 *)(lds)));
+}
+// Four A operands of a decode tile at once: dims 16 i .. of keys 4 h .. + 3
+// and, BYTES further, keys 16 + 4 h .. + 3, at[i] each.  (The builtin waits
+// for every request to LDS first, which here are the next tile's; this waits
+// for its own reads alone.)
+template <int BYTES, typename V8>
+__device__ __forceinline__ void read_tr4(const char *lds, const int (&at)[4], V8 (&v)[4]) {
+    typedef int i2 __attribute__((ext_vector_type(2)));
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char *)lds;
+    i2 a[4], b[4];
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\t"
+        "ds_read_b64_tr_b16 %1, %8 offset:%c12\n\t"
+        "ds_read_b64_tr_b16 %2, %9\n\t"
+        "ds_read_b64_tr_b16 %3, %9 offset:%c12\n\t"
+        "ds_read_b64_tr_b16 %4, %10\n\t"
+        "ds_read_b64_tr_b16 %5, %10 offset:%c12\n\t"
+        "ds_read_b64_tr_b16 %6, %11\n\t"
+        "ds_read_b64_tr_b16 %7, %11 offset:%c12\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(a[0]), "=&v"(b[0]), "=&v"(a[1]), "=&v"(b[1]), "=&v"(a[2]), "=&v"(b[2]), "=&v"(a[3]), "=&v"(b[3])
+        : "v"(base + at[0]), "v"(base + at[1]), "v"(base + at[2]), "v"(base + at[3]), "n"(BYTES)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v[i] = __builtin_bit_cast(V8, __builtin_shufflevector(a[i], b[i], 0, 1, 2, 3));
+}
+template <typename V8, typename V4>
+__device__ __forceinline__ V8 join(V4 a, V4 b) {
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+    constexpr uint32_t e = Half<T>::kExp;
+    return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// Whether x holds in any lane of the workgroup (a barrier on either side: the
+// caller may reuse its LDS).
+template <int WAVES>
+__device__ __forceinline__ bool any_wave(bool x, int *flags, int wave, int lane) {
+    const bool mine = __any(x);
+    if (lane == 0) flags[wave] = mine;
+    __syncthreads();
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) any |= flags[w] != 0;
+    return any;
+}
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N < 64, "vmcnt has six bits");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+// The rows of q as B operands: lane (c, h) holds dims STEP u + 8 h .. + 7 of
+// row c, as NP pieces; dims past d and rows out of the tile are zero.
+template <typename TA, typename T, int NU, int STEP, int NP>
+__device__ __forceinline__ void load_q(const AttnParams &p, const Rows &t, int r, int kvh, int h,
+                                       typename Half<T>::v8 (&qf)[NU][NP]) {
+    const bool ok = r >= t.r0 && r < t.r1;
+    const TA *q = q_row<TA>(p, ok ? r : t.r0, kvh);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const int dim = STEP * u + 8 * h;
+        float x[8];
+        load_vec<8>(q + (dim < p.c.d ? dim : 0), x);
+        uint32_t w[NP][4];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = ok && dim < p.c.d ? x[e] : 0.f;
+            x[e] = p.negate ? -x[e] : x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            uint32_t two[NP];
+            pieces2<T, NP>(x[2 * e], x[2 * e + 1], two);
+            if constexpr (NP > 1) {
+                // an infinite leading piece leaves nothing
+                const bool i0 = !(fabsf(x[2 * e]) < INFINITY), i1 = !(fabsf(x[2 * e + 1]) < INFINITY);
+                const uint32_t keep = (i0 ? 0u : 0xffffu) | (i1 ? 0u : 0xffff0000u);
+#pragma unroll
+                for (int n = 1; n < NP; ++n) two[n] &= keep;
+            }
+#pragma unroll
+            for (int n = 0; n < NP; ++n) w[n][e] = two[n];
+        }
+#pragma unroll
+        for (int n = 0; n < NP; ++n) {
+            const i32x4 v = {(int)w[n][0], (int)w[n][1], (int)w[n][2], (int)w[n][3]};
+            qf[u][n] = __builtin_bit_cast(typename Half<T>::v8, v);
+        }
+    }
+}
+
+// ---- few rows: decode --------------------------------------------------------------
+//
+// A tile of 16 rows, WAVES waves that take 32-key tiles in turn, each with a
+// ring of two K / V tiles of its own in LDS (no barrier in the loop) and its
+// own softmax state; the states are joined in LDS at the end.  S^T = K . Q^T
+// on 16x16x32: lane (c = l % 16, h = l / 16) holds keys 16 kb + 4 h + r of row
+// c, which are its B operand of O^T = V^T . P^T when V^T takes the keys in the
+// same order (two transposing reads: keys 4 h .., 16 + 4 h ..).
+template <typename TA, typename T, int DP, int NP, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) {
+    using H = Half<T>;
+    using v8 = typename H::v8;
+    constexpr int NU = DP / 32, NB = DP / 16, kTile = 32 * DP * 2;
+    constexpr int kOps = 2 * 32 * DP / 512;  // requests per tile and wave
+    constexpr float kBias = NP > 1 ? 16.f : H::kBias;
+    // wave, stage, K / V.  (One array for all: with several the compiler tells
+    // them apart and waits for every request before any read of the rings.)
+    constexpr int kRing = WAVES * 4 * kTile;
+    __shared__ __attribute__((aligned(1024))) char lds[kRing + kMaxPages * 8 + 64];
+    int64_t *const pages = reinterpret_cast<int64_t *>(lds + kRing);
+    int *const flags = reinterpret_cast<int *>(lds + kRing + kMaxPages * 8);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    const int id = xcd_chunked(blockIdx.x, gridDim.x);
+    const int split = id % p.nsplit, kvh = (id / p.nsplit) % p.c.hkv, number = id / p.nsplit / p.c.hkv;
+    Rows t;
+    if (!find_rows(p, number, 16, lane, t)) return;
+    const int nact = active_splits(p, t);
+    if (split >= nact) return;
+    const int seq = seq_of(p, number, t, 16);
+    const int b = t.lo + split * p.chunk, e = split == p.nsplit - 1 ? t.hi : min(t.hi, b + p.chunk);
+
+    const int r = t.base + c;
+    int jmin, jmax;
+    row_keys(p, t, r, jmin, jmax);
+    v8 qf[NU][NP];
+    load_q<TA, T, NU, 32, NP>(p, t, r, kvh, h, qf);
+    // keys that every row sees: [all_lo, all_hi)
+    int x0, x1, y0, y1;
+    row_keys(p, t, t.r0, x0, x1);
+    row_keys(p, t, t.r1 - 1, y0, y1);
+    const int all_lo = y0, all_hi = x1 + 1;
+
+    f32x4 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    bool odd = false;
+
+    for (int pb = b; pb < e;) {
+        const int p0 = paged::page_of(p.c, pb);
+        __syncthreads();  // every wave is done with the pages before
+        const int pe = stage_pages(p.c, seq, pb, e, 2, pages, tid, 64 * WAVES);
+        __syncthreads();
+        const int n = (pe - pb + 31) / 32;  // tiles of this pass; this wave's: wave, wave + WAVES, ..
+        char *const ring = lds + wave * 4 * kTile;
+        if (wave < n)
+            request<DP, 32, 1>(p.c, kvh, pages, p0, pb + 32 * wave, pe, ring, ring + kTile, 0, lane);
+        int st = 0;
+        for (int i = wave; i < n; i += WAVES, st ^= 1) {
+            // (past the last tile: the last key again, into the free stage)
+            const int k0 = pb + 32 * i, kn = min(k0 + 32 * WAVES, pe - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            request<DP, 32, 1>(p.c, kvh, pages, p0, kn, pe, ring + (st ^ 1) * 2 * kTile,
+                               ring + (st ^ 1) * 2 * kTile + kTile, 0, lane);
+            __builtin_amdgcn_sched_barrier(0);
+            wait_vm<kOps>();
+            __builtin_amdgcn_sched_barrier(0);
+            const char *kt = ring + st * 2 * kTile, *vt = kt + kTile;
+            f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const v8 kf = *reinterpret_cast<const v8 *>(kt + (kb * 16 + c) * DP * 2 +
+                                                                (((4 * u + h) ^ swz_k<DP>(kb * 16 + c)) << 4));
+#pragma unroll
+                    for (int q = NP - 1; q >= 0; --q) s[kb] = H::mfma16(kf, qf[u][q], s[kb]);
+                }
+            if (k0 < all_lo || k0 + 32 > min(all_hi, pe)) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int j = k0 + 16 * kb + 4 * h + x;
+                        s[kb][x] = j >= jmin && j <= jmax && j < pe ? s[kb][x] : -INFINITY;
+                    }
+                const uint32_t *w = reinterpret_cast<const uint32_t *>(vt);
+#pragma unroll 4
+                for (int x = 0; x < kTile / 256; ++x) odd |= not_finite<T>(w[x * 64 + lane]);
+            }
+            float mb = max_nan(max_nan(max_nan(s[0][0], s[0][1]), max_nan(s[0][2], s[0][3])),
+                               max_nan(max_nan(s[1][0], s[1][1]), max_nan(s[1][2], s[1][3])));
+            const float m_new = max_nan(m, quarter_max_nan(mb));
+            // (an infinite key meets q's pieces with either sign, or a zero one)
+            if (NP > 1) odd |= jmax >= 0 && m_new != m_new;
+            const float mc = m_new == -INFINITY ? 0.f : m_new * p.sc2;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * p.sc2 - mc);
+            float pv[8], sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                pv[x] = __builtin_amdgcn_exp2f(fmaf(s[x >> 2][x & 3], p.sc2, kBias - mc));
+                sum += pv[x];
+            }
+            l = fmaf(l, alpha, sum);
+            m = m_new;
+#pragma unroll
+            for (int i2 = 0; i2 < NB; ++i2) o[i2] *= alpha;
+            uint32_t pw[NP][4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                uint32_t two[NP];
+                pieces2<T, NP>(pv[2 * x], pv[2 * x + 1], two);
+#pragma unroll
+                for (int q = 0; q < NP; ++q) pw[q][x] = two[q];
+            }
+            v8 pf[NP];
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                const i32x4 v = {(int)pw[q][0], (int)pw[q][1], (int)pw[q][2], (int)pw[q][3]};
+                pf[q] = __builtin_bit_cast(v8, v);
+            }
+            const int key = 4 * h + (c >> 2);
+#pragma unroll
+            for (int i4 = 0; i4 < NB; i4 += 4) {
+                int at[4];
+                v8 vf[4];
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    at[x] = key * DP * 2 + (((2 * (i4 + x) + ((c & 3) >> 1)) ^ swz_v<DP>(key)) << 4) + (c & 1) * 8;
+                read_tr4<16 * DP * 2>(vt, at, vf);
+#pragma unroll
+                for (int q = NP - 1; q >= 0; --q)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[i4 + x] = H::mfma16(vf[x], pf[q], o[i4 + x]);
+            }
+        }
+        wait_vm<0>();  // nothing is still on its way into the ring
+        pb = pe;
+    }
+
+    // Join the waves: states into LDS (over the rings), then thread i takes
+    // 4 dims of a row.
+    l = quarter_sum(l);
+    const float mt = m == -INFINITY ? m : m * p.sc2;
+    constexpr int kRow = DP + 4;
+    static_assert(WAVES * 16 * (kRow + 2) * 4 <= kRing, "states over the rings");
+    float *const accs = reinterpret_cast<float *>(lds);
+    float2 *const mls = reinterpret_cast<float2 *>(accs + WAVES * 16 * kRow);
+    if (any_wave<WAVES>(odd, flags, wave, lane)) {
+        slow_rows<TA, T>(p, t, seq, kvh, b, e, split, nact > 1, kBias, wave, WAVES, lane);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i) *reinterpret_cast<f32x4 *>(accs + (wave * 16 + c) * kRow + 16 * i + 4 * h) = o[i];
+    if (h == 0) mls[wave * 16 + c] = make_float2(mt, l);
+    __syncthreads();
+    for (int i = tid; i < 16 * DP / 4; i += 64 * WAVES) {
+        const int row = i / (DP / 4), dim = 4 * (i % (DP / 4));
+        const int rr = t.base + row;
+        if (rr < t.r0 || rr >= t.r1 || dim >= p.c.d) continue;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) M = max_nan(M, mls[w * 16 + row].x);
+        f32x4 A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float2 x = mls[w * 16 + row];
+            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
+            L = fmaf(x.y, f, L);
+            A += *reinterpret_cast<const f32x4 *>(accs + (w * 16 + row) * kRow + dim) * f;
+        }
+        if (nact > 1) {
+            const int64_t at = part_row(p, rr, kvh) * p.nsplit + split;
+            *reinterpret_cast<f32x4 *>(p.acc + at * p.c.d + dim) = A;
+            if (dim == 0) p.ml[at] = make_float2(M, L);
+        } else {
+            const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+            const float y[4] = {A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv};
+            store_vec<4>(out_row<TA>(p, rr, kvh) + dim, y);
+        }
+    }
+}
+
+// ---- many rows: chunks of prompts ---------------------------------------------------
+//
+// A tile of 128 rows, four waves of 32; K and V tiles of 64 keys, two stages
+// in LDS filled while the tile before is computed, one barrier per tile.  S^T =
+// K . Q^T on 32x32x16: lane (c = l % 32, h = l / 32) holds keys 32 kb + 8 (r /
+// 4) + 4 h + r % 4 of row c; registers 8 t .. 8 t + 7 are its B operand of O^T
+// = V^T . P^T for the 16 keys 16 t .. when V^T takes them in that order.
+template <typename TA, typename T, int DP, int ND, int NP>
+__global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnParams p) {
+    using H = Half<T>;
+    using v8 = typename H::v8;
+    constexpr int NU = 2 * ND, NB = ND, kTile = 64 * DP * 2;  // ND: 32-dim blocks computed
+    constexpr float kBias = NP > 1 ? 16.f : H::kBias;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * kTile + kMaxPages * 8 + 64];  // stage, K / V; pages; flags
+    int64_t *const pages = reinterpret_cast<int64_t *>(lds + 4 * kTile);
+    int *const flags = reinterpret_cast<int *>(lds + 4 * kTile + kMaxPages * 8);
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, h = lane >> 5;
+    const int id = xcd_chunked(blockIdx.x, gridDim.x);
+    // (tiles of one key/value head side by side: they read the same keys)
+    const int number = p.ntiles - 1 - id % p.ntiles, rest = id / p.ntiles;
+    const int split = rest % p.nsplit, kvh = rest / p.nsplit;
+    Rows t;
+    if (!find_rows(p, number, 128, lane, t)) return;
+    const int nact = active_splits(p, t);
+    if (split >= nact) return;
+    const int seq = seq_of(p, number, t, 128);
+    const int b = t.lo + split * p.chunk, e = split == p.nsplit - 1 ? t.hi : min(t.hi, b + p.chunk);
+
+    const int r = t.base + 32 * wave + c;
+    int jmin, jmax;
+    row_keys(p, t, r, jmin, jmax);
+    v8 qf[NU][NP];
+    load_q<TA, T, NU, 16, NP>(p, t, r, kvh, h, qf);
+    // this wave's rows, the keys [any_lo, any_hi) that any of them sees and
+    // [all_lo, all_hi) that all of them see
+    const int w0 = max(t.r0, t.base + 32 * wave), w1 = min(t.r1, t.base + 32 * wave + 32);
+    const bool live = w0 < w1;
+    int any_lo, any_hi, all_lo, all_hi;
+    row_keys(p, t, live ? w0 : t.r0, any_lo, all_hi);
+    row_keys(p, t, live ? w1 - 1 : t.r0, all_lo, any_hi);
+    ++all_hi, ++any_hi;
+
+    f32x16 o[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    bool odd = false;
+
+    for (int pb = b; pb < e;) {
+        const int p0 = paged::page_of(p.c, pb);
+        __syncthreads();
+        const int pe = stage_pages(p.c, seq, pb, e, 2, pages, tid, 256);
+        __syncthreads();
+        const int n = (pe - pb + 63) / 64;
+        request<DP, 64, 4>(p.c, kvh, pages, p0, pb, pe, lds, lds + kTile, wave, lane);
+        for (int i = 0; i < n; ++i) {
+            const int k0 = pb + 64 * i, st = i & 1;
+            // The tile is there, and every wave is done with the one before: the
+            // next one's requests have the scores and the softmax of this one to
+            // arrive in (the compiler waits for them before the transposing
+            // reads of V).
+            wait_vm<0>();
+            __syncthreads();
+            if (i + 1 < n)
+                request<DP, 64, 4>(p.c, kvh, pages, p0, k0 + 64, pe, lds + (st ^ 1) * 2 * kTile,
+                                   lds + (st ^ 1) * 2 * kTile + kTile, wave, lane);
+            if (!live || k0 >= any_hi || k0 + 64 <= any_lo) continue;
+            const char *kt = lds + st * 2 * kTile, *vt = kt + kTile;
+            f32x16 s[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) s[kb][x] = 0.f;
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const v8 kf = *reinterpret_cast<const v8 *>(kt + (kb * 32 + c) * DP * 2 +
+                                                                (((2 * u + h) ^ swz_k<DP>(c)) << 4));
+#pragma unroll
+                    for (int q = NP - 1; q >= 0; --q) s[kb] = H::mfma32(kf, qf[u][q], s[kb]);
+                }
+            if (k0 < all_lo || k0 + 64 > min(all_hi, pe)) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const int j = k0 + 32 * kb + 8 * (x >> 2) + 4 * h + (x & 3);
+                        s[kb][x] = j >= jmin && j <= jmax && j < pe ? s[kb][x] : -INFINITY;
+                    }
+                const uint32_t *w = reinterpret_cast<const uint32_t *>(vt);
+#pragma unroll 4
+                for (int x = 0; x < kTile / 256; ++x) odd |= not_finite<T>(w[x * 64 + lane]);
+            }
+            float mb = max_nan(s[0][0], s[1][0]);
+#pragma unroll
+            for (int x = 1; x < 16; ++x) mb = max_nan(mb, max_nan(s[0][x], s[1][x]));
+            {
+                const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mb), __float_as_uint(mb), false, false);
+                mb = max_nan(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+            }
+            const float m_new = max_nan(m, mb);
+            // (an infinite key meets q's pieces with either sign, or a zero one)
+            if (NP > 1) odd |= jmax >= 0 && m_new != m_new;
+            const float mc = m_new == -INFINITY ? 0.f : m_new * p.sc2;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * p.sc2 - mc);
+            float sum = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    s[kb][x] = __builtin_amdgcn_exp2f(fmaf(s[kb][x], p.sc2, kBias - mc));
+                    sum += s[kb][x];
+                }
+            l = fmaf(l, alpha, sum);
+            if (__any(!(m_new == m))) {
+#pragma unroll
+                for (int i2 = 0; i2 < NB; ++i2) o[i2] *= alpha;
+            }
+            m = m_new;
+            const int key = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {  // 16 keys from 32 kb + 16 x
+                    uint32_t pw[NP][4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        uint32_t two[NP];
+                        pieces2<T, NP>(s[kb][8 * x + 2 * y], s[kb][8 * x + 2 * y + 1], two);
+#pragma unroll
+                        for (int q = 0; q < NP; ++q) pw[q][y] = two[q];
+                    }
+                    v8 pf[NP];
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) {
+                        const i32x4 v = {(int)pw[q][0], (int)pw[q][1], (int)pw[q][2], (int)pw[q][3]};
+                        pf[q] = __builtin_bit_cast(v8, v);
+                    }
+#pragma unroll
+                    for (int i2 = 0; i2 < NB; ++i2) {
+                        const int ch = 4 * i2 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                        const char *at = vt + (32 * kb + 16 * x + key) * DP * 2 + (lane & 1) * 8;
+                        const v8 vf = join<v8>(read_tr<T>(at + ((ch ^ swz_v<DP>(key)) << 4)),
+                                               read_tr<T>(at + 8 * DP * 2 + ((ch ^ swz_v<DP>(key + 8)) << 4)));
+#pragma unroll
+                        for (int q = NP - 1; q >= 0; --q) o[i2] = H::mfma32(vf, pf[q], o[i2]);
+                    }
+                }
+        }
+        pb = pe;
+    }
+
+    if (any_wave<4>(odd, flags, wave, lane)) {
+        slow_rows<TA, T>(p, t, seq, kvh, b, e, split, nact > 1, kBias, wave, 4, lane);
+        return;
+    }
+    {
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+        l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    }
+    if (r < t.r0 || r >= t.r1) return;
+    if (nact > 1) {
+        const int64_t at = part_row(p, r, kvh) * p.nsplit + split;
+        if (h == 0) p.ml[at] = make_float2(m == -INFINITY ? m : m * p.sc2, l);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int dim = 32 * i + 8 * x + 4 * h;
+                if (dim < p.c.d)
+                    *reinterpret_cast<f32x4 *>(p.acc + at * p.c.d + dim) =
+                        f32x4{o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]};
+            }
+    } else {
+        const float inv = m == -INFINITY ? 0.f : 1.0f / l;
+        TA *row = out_row<TA>(p, r, kvh);
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int dim = 32 * i + 8 * x + 4 * h;
+                const float y[4] = {o[i][4 * x] * inv, o[i][4 * x + 1] * inv, o[i][4 * x + 2] * inv, o[i][4 * x + 3] * inv};
+                if (dim < p.c.d) store_vec<4>(row + dim, y);
+            }
+    }
+}
+
+// ---- fp32 cache -------------------------------------------------------------------
+//
+// A tile of 16 rows, four waves that take 16-key tiles in turn, K and V straight
+// into registers and both products on f32 MFMA (16x16x4).  K: lane (c, h) loads
+// dims 16 u + 4 h .. + 3 of key c, and product e of step u takes dim 16 u + 4 h
+// + e of quarter h on both sides.  V: lane (c, h) loads dims 64 v + 4 c .. + 3 of
+// key 4 h + x; product (v, e, x) takes dim 64 v + 4 i + e as its row i.
+template <int DP>
+__global__ __launch_bounds__(256) void paged_f32_kernel(AttnParams p) {
+    constexpr int NU = DP / 16, NV = DP / 64;
+    __shared__ __attribute__((aligned(16))) float accs[4 * 16 * (DP + 4)];
+    __shared__ float2 mls[4 * 16];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    const int id = xcd_chunked(blockIdx.x, gridDim.x);
+    const int split = id % p.nsplit, kvh = (id / p.nsplit) % p.c.hkv, number = id / p.nsplit / p.c.hkv;
+    Rows t;
+    if (!find_rows(p, number, 16, lane, t)) return;
+    const int nact = active_splits(p, t);
+    if (split >= nact) return;
+    const int seq = seq_of(p, number, t, 16);
+    const int b = t.lo + split * p.chunk, e = split == p.nsplit - 1 ? t.hi : min(t.hi, b + p.chunk);
+    const int r = t.base + c;
+    int jmin, jmax;
+    row_keys(p, t, r, jmin, jmax);
+    const bool row_ok = r >= t.r0 && r < t.r1;
+    f32x4 qv[NU];
+    {
+        const float *q = q_row<float>(p, row_ok ? r : t.r0, kvh);
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int dim = 16 * u + 4 * h;
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(q + (dim < p.c.d ? dim : 0));
+            qv[u] = row_ok && dim < p.c.d ? (p.negate ? -x : x) : f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    int x0, x1, y0, y1;
+    row_keys(p, t, t.r0, x0, x1);
+    row_keys(p, t, t.r1 - 1, y0, y1);
+    const int all_lo = y0, all_hi = x1 + 1;
+
+    f32x4 o[NV][4];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[v][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    bool odd = false;
+    const View &cc = p.c;
+    // float offset of key j's row, -1 outside the cache
+    auto row_at = [&](int j) __attribute__((always_inline)) -> int64_t {
+        const int pg = paged::page_of(cc, j), page = cc.table[seq * cc.table_stride + pg];
+        const bool ok = page >= 0 && page < cc.num_pages;
+        if (!ok) paged::raise(cc, paged::kBadPage);
+        return ok ? page * cc.page_stride + (int64_t)(j - pg * cc.page_size) * cc.row_stride + kvh * cc.head_stride : -1;
+    };
+    const float *K = reinterpret_cast<const float *>(cc.k), *V = reinterpret_cast<const float *>(cc.v);
+    for (int k0 = b + 16 * wave; k0 < e; k0 += 64) {
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        const int64_t ka = k0 + c < e ? row_at(k0 + c) : -1;
+        f32x4 kr[NU], vr[4][NV];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int dim = 16 * u + 4 * h;
+            kr[u] = ka >= 0 && dim < cc.d ? *reinterpret_cast<const f32x4 *>(K + ka + dim) : zero;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int j = k0 + 4 * h + x;
+            const int64_t va = j < e ? row_at(j) : -1;
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                const int dim = 64 * v + 4 * c;
+                vr[x][v] = va >= 0 && dim < cc.d ? *reinterpret_cast<const f32x4 *>(V + va + dim) : zero;
+            }
+        }
+        f32x4 s = zero;
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[u][x], qv[u][x], s, 0, 0, 0);
+        if (k0 < all_lo || k0 + 16 > min(all_hi, e)) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int j = k0 + 4 * h + x;
+                s[x] = j >= jmin && j <= jmax && j < e ? s[x] : -INFINITY;
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) odd |= !(fabsf(vr[x][v][y]) < INFINITY);
+            }
+        }
+        const float m_new = max_nan(m, quarter_max_nan(max_nan(max_nan(s[0], s[1]), max_nan(s[2], s[3]))));
+        const float mc = m_new == -INFINITY ? 0.f : m_new * p.sc2;
+        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * p.sc2 - mc);
+        float sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], p.sc2, -mc));
+            sum += s[x];
+        }
+        l = fmaf(l, alpha, sum);
+        m = m_new;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                o[v][y] *= alpha;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) o[v][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[x][v][y], s[x], o[v][y], 0, 0, 0);
+            }
+    }
+    l = quarter_sum(l);
+    odd = __syncthreads_or(odd);
+    if (odd) {
+        slow_rows<float, float>(p, t, seq, kvh, b, e, split, nact > 1, 0.f, wave, 4, lane);
+        return;
+    }
+    constexpr int kRow = DP + 4;
+    // o[v][y], register x: dim 64 v + 4 (4 h + x) + y of row c
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            *reinterpret_cast<f32x4 *>(accs + (wave * 16 + c) * kRow + 64 * v + 16 * h + 4 * x) =
+                f32x4{o[v][0][x], o[v][1][x], o[v][2][x], o[v][3][x]};
+    if (h == 0) mls[wave * 16 + c] = make_float2(m == -INFINITY ? m : m * p.sc2, l);
+    __syncthreads();
+    for (int i = tid; i < 16 * DP / 4; i += 256) {
+        const int row = i / (DP / 4), dim = 4 * (i % (DP / 4));
+        const int rr = t.base + row;
+        if (rr < t.r0 || rr >= t.r1 || dim >= cc.d) continue;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = max_nan(M, mls[w * 16 + row].x);
+        f32x4 A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 x = mls[w * 16 + row];
+            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
+            L = fmaf(x.y, f, L);
+            A += *reinterpret_cast<const f32x4 *>(accs + (w * 16 + row) * kRow + dim) * f;
+        }
+        if (nact > 1) {
+            const int64_t at = part_row(p, rr, kvh) * p.nsplit + split;
+            *reinterpret_cast<f32x4 *>(p.acc + at * cc.d + dim) = A;
+            if (dim == 0) p.ml[at] = make_float2(M, L);
+        } else {
+            const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+            *reinterpret_cast<f32x4 *>(out_row<float>(p, rr, kvh) + dim) = A * inv;
+        }
+    }
+}
+
+// ---- the parts of split rows, in their order ------------------------------------------
+
+// Eight lanes per 32 dims: a wave takes 64 / (d / 4) rows, 4 dims per lane.
+template <typename TA>
+__global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int bm) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    // one (token, key/value head) per wave: its group of rows, whose tiles are
+    // found like the attention kernels' own
+    const int tok = wave / p.c.hkv, kvh = wave % p.c.hkv;
+    if (tok >= p.c.tokens) return;
+    const View &c = p.c;
+    const int n = paged::wave_leading(c.num_seqs + 1, lane, [&](int s) { return paged::offset_at(c, s) <= tok; });
+    if (n == 0 || n > c.num_seqs) return;
+    const int lanes = c.d / 4;  // per row; d <= 128
+    const int per = 64 / lanes;
+    for (int g0 = 0; g0 < c.group; g0 += per) {
+        // (the group's rows may lie in different tiles)
+        for (int i = 0; i < per; ++i) {
+            const int g = g0 + i;
+            if (g >= c.group) break;
+            const int r = tok * c.group + g;
+            Rows t;
+            if (!find_rows(p, r / bm + n - 1, bm, lane, t)) continue;
+            const int nact = active_splits(p, t);
+            if (nact <= 1 || lane / lanes != i || lane >= lanes * per) continue;
+            const int dim = 4 * (lane % lanes);
+            const int64_t at = part_row(p, r, kvh) * p.nsplit;
+            float M = -INFINITY, L = 0.f;
+            f32x4 A = {0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < nact; ++s) M = max_nan(M, p.ml[at + s].x);
+            for (int s = 0; s < nact; ++s) {
+                const float2 x = p.ml[at + s];
+                const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
+                L = fmaf(x.y, f, L);
+                A += *reinterpret_cast<const f32x4 *>(p.acc + (at + s) * c.d + dim) * f;
+            }
+            const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+            const float y[4] = {A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv};
+            store_vec<4>(out_row<TA>(p, r, kvh) + dim, y);
+        }
+    }
+}
+
+// What a call launches: a few-row launch, a chunk launch or both.
+struct Plan {
+    bool few, chunk;
+    int few_max;  // rows of the longest sequence the few-row launch takes
+    int few_split, few_chunk, chunk_split, chunk_chunk;
+    int64_t part_floats;
+};
+
+constexpr int kDecodeWaves = 2;
+constexpr int kAll = INT32_MAX;
+
+Plan make_plan(const PagedAttnDesc &d) {
+    Plan pl{};
+    const int64_t group = d.heads / d.kv.kv_heads;
+    const int64_t rows = d.tokens * group;
+    const bool f32 = d.kv.dtype == GFH_F32;
+    pl.few_max = 32;
+    pl.few = f32 || d.kv.num_seqs > 1 || rows <= pl.few_max;
+    pl.chunk = !f32 && rows > pl.few_max && d.tokens > d.kv.num_seqs;
+    if (!pl.chunk) pl.few_max = kAll;
+    const int64_t cus = device_cu_count();
+    auto cut = [&](int64_t tiles, int64_t target, int64_t least, int64_t unit, int &nsplit, int &chunk) {
+        const int64_t items = std::max<int64_t>(1, tiles * d.kv.kv_heads);
+        const int64_t kv = std::max<int64_t>(1, d.max_kv_len);
+        int64_t ch = std::max(least, (items * kv + target - 1) / target);
+        ch = (ch + unit - 1) / unit * unit;
+        nsplit = (int)std::min<int64_t>((kv + ch - 1) / ch, 256);
+        ch = std::max(ch, (kv + nsplit - 1) / nsplit);
+        chunk = (int)std::min<int64_t>((ch + unit - 1) / unit * unit, (int64_t)1 << 30);
+    };
+    cut(std::min(d.kv.num_seqs, d.tokens) + rows / 16, 4 * cus, 256, 64, pl.few_split, pl.few_chunk);
+    cut(rows / 128 + 1, 2 * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
+    int64_t most = 1;
+    if (pl.few) most = std::max<int64_t>(most, pl.few_split);
+    if (pl.chunk) most = std::max<int64_t>(most, pl.chunk_split);
+    pl.part_floats = most > 1 ? d.tokens * d.heads * most * (d.kv.head_dim + 2) : 0;
+    return pl;
+}
+
+}  // namespace
+
+View paged_view(const gfh_paged_kv &kv, int64_t tokens, int64_t heads) {
+    View c{};
+    c.k = static_cast<char *>(kv.k_pages);
+    c.v = static_cast<char *>(kv.v_pages);
+    c.num_pages = kv.num_pages;
+    c.page_stride = kv.page_stride, c.row_stride = kv.row_stride, c.head_stride = kv.head_stride;
+    c.table = kv.page_table;
+    c.table_stride = kv.table_stride;
+    c.kv_lens = kv.kv_lens, c.q_offsets = kv.q_offsets;
+    c.status = kv.status;
+    c.page_size = (int)kv.page_size;
+    c.page_shift = (kv.page_size & (kv.page_size - 1)) == 0 ? __builtin_ctzll(kv.page_size) : -1;
+    c.capacity = (int)(kv.max_pages * kv.page_size);
+    c.num_seqs = (int)kv.num_seqs;
+    c.tokens = (int)tokens;
+    c.heads = (int)heads;
+    c.hkv = (int)kv.kv_heads;
+    c.group = (int)(heads / kv.kv_heads);
+    c.d = (int)kv.head_dim;
+    return c;
+}
+
+size_t paged_attention_workspace_bytes(const PagedAttnDesc &d) { return (size_t)make_plan(d).part_floats * 4; }
+
+int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t s) {
+    const Plan pl = make_plan(d);
+    AttnParams p{};
+    p.c = paged_view(d.kv, d.tokens, d.heads);
+    p.q = static_cast<const char *>(d.q);
+    p.out = static_cast<char *>(d.out);
+    p.ldq = d.ldq, p.ldo = d.ldo;
+    // (a scale of 0 keeps masked scores at -inf)
+    p.sc2 = d.scale == 0.f ? 1e-38f : std::fabs(d.scale) * 0x1.715476p+0f;
+    p.negate = d.scale < 0.f;
+    p.causal = d.causal;
+    p.window = d.window >= p.c.capacity ? 0 : (int)d.window;
+    const int64_t rows = d.tokens * p.c.group;
+    const dim3 join((unsigned)((d.tokens * p.c.hkv + 3) / 4));
+    auto run = [&](int bm, int nsplit, int chunk, int min_rows, int max_rows, auto &&kernel) -> int {
+        p.ntiles = (int)((rows - 1) / bm + d.kv.num_seqs);
+        p.nsplit = nsplit, p.chunk = chunk, p.min_rows = min_rows, p.max_rows = max_rows;
+        p.acc = static_cast<float *>(workspace);
+        p.ml = reinterpret_cast<float2 *>(p.acc + d.tokens * d.heads * nsplit * d.kv.head_dim);
+        const int64_t blocks = (int64_t)p.ntiles * p.c.hkv * nsplit;
+        if (blocks > (int64_t)1 << 23) return set_error(GFH_INVALID_SHAPE, "paged_attention: grid too large");
+        kernel(dim3((unsigned)blocks));
+        GFH_TRY(check_launch("paged_attention"));
+        if (nsplit > 1) {
+            if (d.dtype == GFH_F32)
+                hipLaunchKernelGGL(paged_join_kernel<float>, join, dim3(256), 0, s, p, bm);
+            else if (d.dtype == GFH_BF16)
+                hipLaunchKernelGGL(paged_join_kernel<__bf16>, join, dim3(256), 0, s, p, bm);
+            else
+                hipLaunchKernelGGL(paged_join_kernel<_Float16>, join, dim3(256), 0, s, p, bm);
+            GFH_TRY(check_launch("paged_attention (join)"));
+        }
+        return GFH_SUCCESS;
+    };
+    const int64_t hd = d.kv.head_dim;
+    auto few = [&](dim3 grid) {
+        auto go = [&](auto ta, auto t, auto np) {
+            using TA = decltype(ta);
+            using T = decltype(t);
+            constexpr int NP = decltype(np)::value;
+            constexpr int W = kDecodeWaves;
+            if (hd <= 64)
+                hipLaunchKernelGGL((paged_decode_kernel<TA, T, 64, NP, W>), grid, dim3(64 * W), 0, s, p);
+            else
+                hipLaunchKernelGGL((paged_decode_kernel<TA, T, 128, NP, W>), grid, dim3(64 * W), 0, s, p);
+        };
+        using One = std::integral_constant<int, 1>;
+        using Three = std::integral_constant<int, 3>;
+        if (d.kv.dtype == GFH_F32) {
+            if (hd <= 64)
+                hipLaunchKernelGGL(paged_f32_kernel<64>, grid, dim3(256), 0, s, p);
+            else
+                hipLaunchKernelGGL(paged_f32_kernel<128>, grid, dim3(256), 0, s, p);
+        } else if (d.dtype == GFH_F32)
+            go(float{}, __bf16{}, Three{});
+        else if (d.dtype == GFH_BF16)
+            go(__bf16{}, __bf16{}, One{});
+        else
+            go(_Float16{}, _Float16{}, One{});
+    };
+    auto many = [&](dim3 grid) {
+        auto go = [&](auto ta, auto t, auto np) {
+            using TA = decltype(ta);
+            using T = decltype(t);
+            constexpr int NP = decltype(np)::value;
+            if (hd <= 64)
+                hipLaunchKernelGGL((paged_chunk_kernel<TA, T, 64, 2, NP>), grid, dim3(256), 0, s, p);
+            else if (hd <= 96)
+                hipLaunchKernelGGL((paged_chunk_kernel<TA, T, 128, 3, NP>), grid, dim3(256), 0, s, p);
+            else
+                hipLaunchKernelGGL((paged_chunk_kernel<TA, T, 128, 4, NP>), grid, dim3(256), 0, s, p);
+        };
+        using One = std::integral_constant<int, 1>;
+        using Three = std::integral_constant<int, 3>;
+        if (d.dtype == GFH_F32)
+            go(float{}, __bf16{}, Three{});
+        else if (d.dtype == GFH_BF16)
+            go(__bf16{}, __bf16{}, One{});
+        else
+            go(_Float16{}, _Float16{}, One{});
+    };
+    if (pl.chunk) GFH_TRY(run(128, pl.chunk_split, pl.chunk_chunk, pl.few ? pl.few_max + 1 : 0, kAll, many));
+    if (pl.few) GFH_TRY(run(16, pl.few_split, pl.few_chunk, 0, pl.few_max, few));
+    return GFH_SUCCESS;
+}
+
+}  // namespace gfh

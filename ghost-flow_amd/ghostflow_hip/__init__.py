@@ -24,6 +24,9 @@ from .ops import (  # noqa: F401
     mha_forward_cached,
     mha_forward_with_cache,
     mha_workspace_size,
+    paged_append,
+    paged_attention,
+    paged_attention_workspace_size,
     qlinear,
     qlinear_dynamic,
     qswiglu,

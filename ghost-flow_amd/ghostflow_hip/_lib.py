@@ -31,6 +31,9 @@ STATUS_NAMES = {
     UNKNOWN: "Unknown",
 }
 
+# Element types (gfh_dtype): the dtype bytes of a state dict.
+F16, BF16, F32 = 0, 1, 2
+
 _p = C.c_void_p
 _i = C.c_int
 _i64 = C.c_int64
@@ -68,6 +71,10 @@ SIGNATURES = {
     "gfh_mha_workspace_size": (_sz, [_i64, _i64, _i64]),
     "gfh_mha_forward_with_cache_f32": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _p,
                                             _i64, _i, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _sz, _p]),
+    "gfh_paged_append": (_i, [_p, _i, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i,
+                              _p]),
+    "gfh_paged_attention_workspace_size": (_sz, [_p, _i64, _i64, _i64]),
+    "gfh_paged_attention": (_i, [_p, _i, _i64, _i64, _p, _i64, _p, _i64, _f, _i, _i64, _i64, _p, _sz, _p]),
     "gfh_silu_mul_f32": (_i, [_p, _p, _p, _i64, _p]),
     "gfh_state_dict_open": (_i, [C.c_char_p, C.POINTER(C.c_void_p)]),
     "gfh_state_dict_close": (None, [_p]),
@@ -113,6 +120,16 @@ class TensorEntry(C.Structure):
     _fields_ = [("name", C.c_char_p), ("kind", C.c_int), ("dtype", C.c_int), ("ndim", C.c_int),
                 ("dims", C.POINTER(C.c_int64)), ("data", C.c_void_p), ("scales", C.c_void_p),
                 ("zero_points", C.c_void_p), ("nscales", C.c_int64)]
+
+
+class PagedKv(C.Structure):
+    """gfh_paged_kv (include/ghostflow_hip.h)."""
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("dtype", C.c_int), ("num_pages", C.c_int64),
+                ("page_size", C.c_int64), ("kv_heads", C.c_int64), ("head_dim", C.c_int64),
+                ("page_stride", C.c_int64), ("row_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("page_table", C.c_void_p), ("max_pages", C.c_int64), ("table_stride", C.c_int64),
+                ("num_seqs", C.c_int64), ("kv_lens", C.c_void_p), ("q_offsets", C.c_void_p),
+                ("status", C.c_void_p)]
 
 
 def load():

@@ -7,6 +7,9 @@ library's status code and thread-local message when a call fails.
 """
 from __future__ import annotations
 
+from ctypes import byref as _byref
+from functools import lru_cache
+
 import torch
 
 from . import _lib
@@ -352,6 +355,7 @@ def kv_attention(q, k_cache, v_cache, kv_len, num_heads, *, scale=None, causal=F
     return (o, w) if want_weights else o
 
 
+@lru_cache(maxsize=None)
 def _inv_sqrt(d):
     """1.0f32 / (d as f32).sqrt() (attention.rs:19-20), in float32."""
     return float(torch.tensor(1.0, dtype=torch.float32) / torch.sqrt(torch.tensor(float(d), dtype=torch.float32)))
@@ -416,6 +420,146 @@ def mha_forward_with_cache(query, key, value, wq, bq, wk, bk, wv, bv, wo, bo, nu
     k_new = kc[:, p:].reshape(b, sk, num_heads, d).transpose(1, 2)
     v_new = vc[:, p:].reshape(b, sk, num_heads, d).transpose(1, 2)
     return out, w, k_new, v_new
+
+
+# ---- key/value cache in pages ---------------------------------------------------
+
+_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
+def _dtype(t, name):
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return d
+
+
+def _rows(t, name, dtype, tokens, heads, d):
+    """Elements between the tokens of t [tokens, heads, d] (heads and dims
+    contiguous)."""
+    if not t.is_cuda:
+        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be a device tensor")
+    if t.dtype != dtype:
+        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != (tokens, heads, d):
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be [{tokens}, {heads}, {d}], got {list(t.shape)}")
+    ld, hs, ds = t.stride()
+    if (d > 1 and ds != 1) or (heads > 1 and hs != d):
+        raise GhostFlowError(_lib.INVALID_DATA, f"{name}: the heads of a token must be contiguous")
+    return ld if tokens > 1 else heads * d
+
+
+def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, tokens_on):
+    for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if not t.is_cuda or t.device != tokens_on:
+            raise GhostFlowError(_lib.INVALID_DATA, f"{n} must be on {tokens_on}")
+        if t.dim() != 4 or t.shape != k_pages.shape or t.dtype != k_pages.dtype or t.stride() != k_pages.stride():
+            raise GhostFlowError(_lib.INVALID_SHAPE, "k_pages and v_pages must be [pages, page_size, kv_heads, "
+                                 "head_dim], of one type and with one layout")
+    dt = _dtype(k_pages, "k_pages")
+    pages, page_size, hkv, d = k_pages.shape
+    sp, sr, sh, sd = k_pages.stride()
+    if d > 1 and sd != 1:
+        raise GhostFlowError(_lib.INVALID_DATA, "the dims of k_pages must be contiguous")
+    for t, n in ((page_table, "page_table"), (q_offsets, "q_offsets"), (kv_lens, "kv_lens"), (status, "status")):
+        if t is None and n == "status":
+            continue
+        if not t.is_cuda or t.device != tokens_on or t.dtype != torch.int32:
+            raise GhostFlowError(_lib.INVALID_DATA, f"{n} must be an int32 tensor on {tokens_on}")
+        if t.numel() > 1 and t.stride(-1) != 1:
+            raise GhostFlowError(_lib.INVALID_DATA, f"{n} must be contiguous")
+    seqs = kv_lens.numel()
+    if page_table.dim() != 2 or page_table.shape[0] != seqs or kv_lens.dim() != 1 or tuple(q_offsets.shape) != (seqs + 1,):
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"page_table [seqs, pages], q_offsets [seqs + 1] and kv_lens [seqs], "
+                             f"got {list(page_table.shape)}, {list(q_offsets.shape)}, {list(kv_lens.shape)}")
+    width = page_table.shape[1]
+    # (a stride over a single element says nothing)
+    return _lib.PagedKv(k_pages.data_ptr(), v_pages.data_ptr(), dt, pages, page_size, hkv, d, sp if pages > 1 else 0,
+                        sr if page_size > 1 else 0, sh if hkv > 1 else 0, page_table.data_ptr(), width,
+                        page_table.stride(0) if seqs > 1 else width, seqs, kv_lens.data_ptr(), q_offsets.data_ptr(),
+                        _ptr(status))
+
+
+def paged_append(k_pages, v_pages, page_table, q_offsets, kv_lens, k, v, *, q=None, q_out=None, cos=None, sin=None,
+                 interleaved=False, status=None):
+    """Writes the new tokens' k and v [tokens, kv_heads, head_dim] into their
+    sequences' pages [pages, page_size, kv_heads, head_dim], k turned by the
+    rotary tables cos / sin [positions, rotary_dim / 2] (fp32) at the tokens'
+    positions, and returns q [tokens, heads, head_dim] turned the same way
+    (into q_out, which may be q; None without q).  gfh_paged_kv in
+    ghostflow_hip.h says what page_table [seqs, pages], q_offsets [seqs + 1],
+    kv_lens [seqs] (the new tokens included) and status (all int32) are."""
+    tokens, hkv, d = k.shape if k.dim() == 3 else (0, 0, 0)
+    dt = _dtype(k, "k")
+    kv = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, k.device)
+    if (hkv, d) != (kv.kv_heads, kv.head_dim):
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"k must be [tokens, {kv.kv_heads}, {kv.head_dim}], got {list(k.shape)}")
+    ldk = _rows(k, "k", k.dtype, tokens, hkv, d)
+    ldv = _rows(v, "v", k.dtype, tokens, hkv, d)
+    heads, ldq, ldqo = hkv, 0, 0
+    if q is not None:
+        heads = q.shape[1] if q.dim() == 3 else 0
+        ldq = _rows(q, "q", k.dtype, tokens, heads, d)
+        if q_out is None:
+            q_out = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
+        ldqo = _rows(q_out, "q_out", k.dtype, tokens, heads, d)
+    elif q_out is not None:
+        raise GhostFlowError(_lib.INVALID_DATA, "q_out without q")
+    rows = half = 0
+    if (cos is None) != (sin is None):
+        raise GhostFlowError(_lib.INVALID_DATA, "cos and sin are given together")
+    if cos is not None:
+        _need(cos, torch.float32, "cos")
+        _need(sin, torch.float32, "sin")
+        if cos.dim() != 2 or cos.shape != sin.shape:
+            raise GhostFlowError(_lib.INVALID_SHAPE, "cos and sin must be [positions, rotary_dim / 2]")
+        rows, half = cos.shape
+    _same_device(k.device, v, q, q_out, cos, sin)
+    with torch.cuda.device(k.device):
+        _check(lib().gfh_paged_append(_byref(kv), dt, tokens, heads, _ptr(q), ldq, _ptr(q_out), ldqo, k.data_ptr(), ldk,
+                                      v.data_ptr(), ldv, _ptr(cos), _ptr(sin), rows, 2 * half, int(bool(interleaved)),
+                                      _stream(k.device)))
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, *, scale=None, causal=True, window=0,
+                    max_kv_len=None, out=None, workspace=None, status=None):
+    """Attention of the new tokens q [tokens, heads, head_dim] over their
+    sequences' pages (arguments as paged_append's): token at position p sees
+    the keys j < kv_len, j <= p if causal, j > p - window if window.  Returns
+    out like q (which may be q); rows behind the last sequence are left as
+    they are, and zero in an out made here.  max_kv_len: the batch's longest
+    length where the caller knows it."""
+    if q.dim() != 3:
+        raise GhostFlowError(_lib.INVALID_SHAPE, "q must be [tokens, heads, head_dim]")
+    tokens, heads, d = q.shape
+    kv = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, q.device)
+    dt = _dtype(q, "q")
+    ldq = _rows(q, "q", q.dtype, tokens, heads, kv.head_dim)
+    if out is None:
+        out = torch.zeros((tokens, heads, d), dtype=q.dtype, device=q.device)
+    ldo = _rows(out, "out", q.dtype, tokens, heads, d)
+    if scale is None:
+        scale = _inv_sqrt(d)
+    _same_device(q.device, out, workspace)
+    ws, ws_bytes = _workspace(workspace)
+    with torch.cuda.device(q.device):
+        _check(lib().gfh_paged_attention(_byref(kv), dt, tokens, heads, q.data_ptr(), ldq, out.data_ptr(), ldo,
+                                         float(scale), int(bool(causal)), int(window), int(max_kv_len or 0), ws,
+                                         ws_bytes, _stream(q.device)))
+    return out
+
+
+def paged_attention_workspace_size(q, k_pages, v_pages, page_table, q_offsets, kv_lens, max_kv_len=None) -> int:
+    """Bytes of paged_attention's workspace for these arguments."""
+    kv = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, None, q.device)
+    return int(lib().gfh_paged_attention_workspace_size(_byref(kv), q.shape[0], q.shape[1], int(max_kv_len or 0)))
+
+
+def _same_device(dev, *tensors):
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise GhostFlowError(_lib.INVALID_DATA, f"all tensors must be on {dev}, one is on {t.device}")
 
 
 # ---- SwiGLU feed-forward block (ghostflow-nn/src/llama.rs:259-287) -------------

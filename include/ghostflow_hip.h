@@ -354,6 +354,87 @@ GFH_API int gfh_mha_forward_with_cache_f32(
     int64_t sq, int64_t sk, int64_t e, int64_t h, void *workspace,
     size_t workspace_bytes, gfh_stream_t stream);
 
+/* ---- key/value cache in pages -------------------------------------------- */
+
+/* Element types of activations and caches: the dtype bytes of the state dict
+ * (ghostflow-core/src/serialize.rs:188-215). */
+typedef enum gfh_dtype { GFH_F16 = 0, GFH_BF16 = 1, GFH_F32 = 2 } gfh_dtype;
+
+/* A key/value cache in pages and the ragged batch of a step (host struct of
+ * device pointers; no counterpart in the reference, whose cache is the copied
+ * past_key / past_value of attention.rs:100-144).
+ *   k_pages, v_pages  num_pages pages of page_size rows; row r of page p,
+ *                     key/value head hh, at p * page_stride + r * row_stride +
+ *                     hh * head_stride elements; the head_dim dims are
+ *                     contiguous
+ *   page_table        [num_seqs, table_stride], the first max_pages entries of
+ *                     a row are used: position j of sequence s is row
+ *                     j % page_size of page page_table[s, j / page_size]
+ *   q_offsets         [num_seqs + 1], rising: rows q_offsets[s] ..
+ *                     q_offsets[s + 1] - 1 of the new tokens belong to
+ *                     sequence s; rows behind the last (padding) are left alone
+ *   kv_lens           [num_seqs] positions of the sequence, the new tokens
+ *                     included: new token i is position kv_lens[s] - q_len + i
+ *   status            nullable; see below
+ * page_table, q_offsets and kv_lens are read by the kernels only, so a captured
+ * call can be replayed after they change.  What the host cannot check the
+ * kernels do: a length outside [0, max_pages * page_size], or a token whose
+ * position is, sets bit 0 of *status, a page outside [0, num_pages) bit 1.
+ * Such tokens and pages are not written; such a page reads as zeros; a length
+ * is clamped.  The caller clears *status.
+ * head_dim is a multiple of 8 in [8, 128]; max_pages * page_size is at most
+ * 2^30; pages are 16-byte aligned, the strides' bytes multiples of 16.  Pages
+ * may be shared by sequences (a common prefix) as long as a call writes no row
+ * twice. */
+typedef struct gfh_paged_kv {
+    void *k_pages, *v_pages;
+    int dtype; /* gfh_dtype of the cache */
+    int64_t num_pages, page_size, kv_heads, head_dim;
+    int64_t page_stride, row_stride, head_stride;
+    const int32_t *page_table;
+    int64_t max_pages, table_stride;
+    int64_t num_seqs;
+    const int32_t *kv_lens, *q_offsets;
+    int32_t *status;
+} gfh_paged_kv;
+
+/* The new tokens' keys and values into their pages, rotated on the way:
+ *   q [tokens, heads, head_dim], k, v [tokens, kv_heads, head_dim] of type
+ *   dtype, rows ldq / ldk / ldv elements apart; q_out like q, rows ldqo apart
+ *   (q_out may be q with ldqo = ldq; q and q_out may be NULL together);
+ *   rope_cos, rope_sin [rope_rows, rotary_dim / 2] fp32 tables by position
+ *   (NULL together: nothing is turned); rope_rows >= max_pages * page_size.
+ * Pair j of a head is dims (j, j + rotary_dim / 2), or (2j, 2j + 1) if
+ * interleaved: a' = a cos - b sin, b' = b cos + a sin, in fp32, rounded once.
+ * Dims from rotary_dim on, and v, are copied.  rotary_dim % 8 == 0.
+ * dtype is the cache's, or GFH_F32 over a GFH_BF16 cache. */
+GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads,
+                             const void *q, int64_t ldq, void *q_out, int64_t ldqo,
+                             const void *k, int64_t ldk, const void *v, int64_t ldv,
+                             const float *rope_cos, const float *rope_sin, int64_t rope_rows,
+                             int64_t rotary_dim, int interleaved, gfh_stream_t stream);
+
+/* Attention of the new tokens over their sequences' pages:
+ *   out[t, hh] = softmax(scale * q[t, hh] . K) . V
+ * over the keys j < kv_lens[s] of key/value head hh / (heads / kv_heads), and
+ * for the token at position p: j <= p if causal, j > p - window if window > 0.
+ * A token that sees no key gets zeros.  q [tokens, heads, head_dim], rows ldq
+ * apart, out the same, rows ldo apart (out may be q with ldo = ldq), of type
+ * dtype as in gfh_paged_append.  Sums and softmax in fp32; out is rounded once
+ * (fp32 q over a bf16 cache: fp32 products of the stored values).
+ * max_kv_len: the longest length of the batch as far as the caller knows (0:
+ * max_pages * page_size); the work is split by it, the results hold for any
+ * length.  workspace (nullable, 16-byte aligned) of at least
+ * gfh_paged_attention_workspace_size(...) bytes holds the parts of split rows;
+ * any contents.  Calls with NULL share the stream's block, so graphs that may
+ * run at the same time need workspaces of their own. */
+GFH_API size_t gfh_paged_attention_workspace_size(const gfh_paged_kv *kv, int64_t tokens, int64_t heads,
+                                                  int64_t max_kv_len);
+GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads,
+                                const void *q, int64_t ldq, void *out, int64_t ldo, float scale,
+                                int causal, int64_t window, int64_t max_kv_len, void *workspace,
+                                size_t workspace_bytes, gfh_stream_t stream);
+
 /* ---- SwiGLU feed-forward block ------------------------------------------ */
 
 /* out[i] = silu(gate[i]) * up[i], silu(v) = v / (1 + exp(-v)): the

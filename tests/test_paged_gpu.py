@@ -1,0 +1,323 @@
+"""Paged append (with rotary positions) and paged attention on the GPU against
+the plain form in 64 bits (_paged.py): types, head layouts, page sizes and
+layouts, ragged and empty sequences, windows, masked rows.  Rows of the pages
+that hold no position are NaN, so any use of them shows."""
+import pytest
+import torch
+
+import _paged as P
+
+pytestmark = pytest.mark.gpu
+
+
+def _gh():
+    import ghostflow_hip
+    return ghostflow_hip
+
+
+def _check(got, want, bound):
+    got = got.double().cpu()
+    live = ~torch.isnan(want)
+    err = (got - want).abs()
+    assert torch.isfinite(got[live]).all()
+    bad = live & (err > bound)
+    assert not bad.any(), (int(bad.sum()), float(err[bad].max()), float(bound[bad].min()))
+
+
+def _attend(dev, b, **kw):
+    gh = _gh()
+    x = P.to(b, dev)
+    out = torch.full_like(x["q"], 7.0)
+    hint = kw.pop("max_kv_len", None)
+    got = gh.paged_attention(x["q"], *P.args(x), out=out, max_kv_len=hint, **kw)
+    torch.cuda.synchronize()
+    return got
+
+
+# lengths: one token; decode; chunks that end inside pages and tiles; no past;
+# sequences without new tokens or without any position; more tokens than keys
+LENS = [
+    ([1], [1]),
+    ([1], [517]),
+    ([1, 1, 1, 1, 1], [33, 1, 700, 64, 129]),
+    ([5, 0, 1, 3], [5, 40, 65, 300]),
+    ([70, 1, 33], [70, 260, 100]),
+    ([200], [1000]),
+    ([0, 0, 2, 0], [10, 0, 9, 0]),
+    ([4, 9], [2, 0]),
+]
+HEADS = [(4, 4, 64), (8, 2, 128), (6, 1, 80), (3, 3, 8), (40, 2, 32), (7, 1, 128), (2, 2, 96)]
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("lens", LENS, ids=lambda v: "-".join(map(str, v[0])))
+def test_attention_lengths(torch_dev, types, lens):
+    for heads, kv_heads, d in ((8, 2, 128), (4, 4, 64)):
+        b = P.batch(*lens, heads=heads, kv_heads=kv_heads, d=d, page=16, types=types, seed=1)
+        _check(_attend(torch_dev, b), *P.attention(b))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("heads", HEADS, ids=lambda v: "-".join(map(str, v)))
+def test_attention_heads(torch_dev, types, heads):
+    h, hkv, d = heads
+    b = P.batch([1, 40, 3], [300, 90, 77], heads=h, kv_heads=hkv, d=d, page=16, types=types, seed=2)
+    _check(_attend(torch_dev, b), *P.attention(b))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("page", [1, 3, 16, 48, 64, 1000])
+@pytest.mark.parametrize("layout", ["rows", "heads", "pairs"])
+def test_attention_pages(torch_dev, types, page, layout):
+    b = P.batch([1, 50], [211, 333], heads=4, kv_heads=2, d=64, page=page, types=types, seed=3, layout=layout)
+    _check(_attend(torch_dev, b), *P.attention(b))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("causal,window", [(False, 0), (True, 1), (True, 20), (True, 128), (True, 10 ** 6), (False, 50)])
+def test_attention_masks(torch_dev, types, causal, window):
+    b = P.batch([1, 90, 2, 4], [400, 300, 2, 3], heads=4, kv_heads=1, d=128, page=16, types=types, seed=4)
+    _check(_attend(torch_dev, b, causal=causal, window=window), *P.attention(b, causal=causal, window=window))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("scale", [0.0, -0.125, 1.0, 1e-30])
+def test_attention_scales(torch_dev, types, scale):
+    b = P.batch([1, 60], [200, 150], heads=4, kv_heads=2, d=64, page=16, types=types, seed=5)
+    _check(_attend(torch_dev, b, scale=scale), *P.attention(b, scale=scale))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+def test_attention_long_axis_is_split_and_any_hint_is_right(torch_dev, types):
+    """Few rows over a long axis: the result holds whatever the caller says
+    about the longest length, and is the same bits every time."""
+    b = P.batch([1, 2, 30], [6001, 257, 3000], heads=4, kv_heads=2, d=128, page=16, types=types, seed=6)
+    want = P.attention(b)
+    for hint in (None, 6001, 100, 10 ** 9):
+        got = _attend(torch_dev, b, max_kv_len=hint)
+        _check(got, *want)
+        assert torch.equal(got, _attend(torch_dev, b, max_kv_len=hint))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+def test_attention_leaves_padding_and_serves_any_offsets(torch_dev, types):
+    """Rows behind the last sequence keep what they held; more sequences than
+    a wave has lanes, most without new tokens."""
+    b = P.batch([1, 40], [50, 60], heads=4, kv_heads=2, d=64, page=16, types=types, seed=7, pad=9)
+    got = _attend(torch_dev, b)
+    _check(got[:41], *(x[:41] for x in P.attention(b)))
+    assert (got[41:] == 7.0).all()
+    lens = [0 if s % 7 else 1 + s % 3 for s in range(300)]
+    b = P.batch(lens, [n + s % 50 for s, n in enumerate(lens)], heads=2, kv_heads=2, d=64, page=16, types=types, seed=8)
+    _check(_attend(torch_dev, b), *P.attention(b))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("which", ["k_pages", "v_pages"])
+def test_attention_masked_values_do_not_reach_a_row(torch_dev, types, value, which):
+    """A value that is not finite in a key that only later tokens see, or only
+    earlier ones (window): the others' rows stay as the plain form, which
+    leaves that key out, has them."""
+    b = P.batch([60, 1], [300, 200], heads=4, kv_heads=2, d=64, page=16, types=types, seed=9)
+    page, row = b["page_table"][0, 270 // 16].long(), 270 % 16
+    b[which][page, row, 1, 5] = value
+    for window in (0, 40):
+        want, bound = P.attention(b, window=window)
+        got = _attend(torch_dev, b, window=window).double().cpu()
+        sees = torch.zeros(61, 4, dtype=torch.bool)
+        for t in range(60):
+            p = 240 + t
+            sees[t, 2:] = p >= 270 and (not window or 270 > p - window)
+        fine = ~sees[..., None].expand_as(want)
+        assert (got - want).abs()[fine].le(bound[fine]).all()
+        # and the rows that see it are finite where the formula's are
+        assert torch.equal(torch.isfinite(got[~fine]), torch.isfinite(want[~fine]))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+def test_attention_strided_rows_and_in_place(torch_dev, types):
+    """q as a slice of a fused projection, out in a wider tensor; out on q."""
+    gh = _gh()
+    b = P.batch([1, 40, 5], [300, 90, 77], heads=4, kv_heads=2, d=64, page=16, types=types, seed=10)
+    want = P.attention(b)
+    x = P.to(b, torch_dev)
+    t = x["tokens"]
+    fused = torch.zeros(t, 8, 64, dtype=x["q"].dtype, device=torch_dev)
+    fused[:, 2:6] = x["q"]
+    wide = torch.zeros(t, 6, 64, dtype=x["q"].dtype, device=torch_dev)
+    gh.paged_attention(fused[:, 2:6], *P.args(x), out=wide[:, 1:5])
+    _check(wide[:, 1:5], *want)
+    assert (wide[:, 0] == 0).all() and (wide[:, 5] == 0).all()
+    same = x["q"].clone()
+    gh.paged_attention(same, *P.args(x), out=same)
+    _check(same, *want)
+
+
+@pytest.mark.parametrize("types", [("bf16", "bf16"), ("f32", "f32")], ids="/".join)
+def test_attention_shared_pages(torch_dev, types):
+    """Two sequences over one prefix."""
+    b = P.batch([3, 20], [200, 250], heads=4, kv_heads=2, d=64, page=16, types=types, seed=11)
+    b["page_table"][1, :6] = b["page_table"][0, :6]
+    _check(_attend(torch_dev, b), *P.attention(b))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+def test_bad_pages_and_lengths_are_reported(torch_dev, types):
+    """A page outside the cache is not touched and sets a bit of status; so
+    does a length the table cannot hold.  The other sequences are served."""
+    gh = _gh()
+    b = P.batch([1, 40, 2], [100, 90, 77], heads=4, kv_heads=2, d=64, page=16, types=types, seed=12)
+    want, bound = P.attention(b)
+    for bad in (-1, 10 ** 6):
+        c = dict(b, page_table=b["page_table"].clone())
+        c["page_table"][0, 2] = bad
+        x = P.to(c, torch_dev)
+        st = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+        got = gh.paged_attention(x["q"], *P.args(x), status=st)
+        assert int(st) == 2
+        _check(got[1:], want[1:], bound[1:])
+        st.zero_()
+        c["page_table"][0, 6] = bad  # where the new token goes
+        x = P.to(c, torch_dev)
+        gh.paged_append(*P.args(x), x["k"], x["v"], status=st)
+        assert int(st) == 2
+    for n in (-5, 10 ** 6):
+        c = dict(b, kv_lens=b["kv_lens"].clone())
+        c["kv_lens"][0] = n
+        x = P.to(c, torch_dev)
+        st = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+        got = gh.paged_attention(x["q"], *P.args(x), status=st)
+        assert int(st) & 1
+        _check(got[1:], want[1:], bound[1:])
+        st.zero_()
+        gh.paged_append(*P.args(x), x["k"], x["v"], status=st)
+        assert int(st) == 1
+
+
+# ---- append --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("rot,interleaved", [(0, False), (64, False), (64, True), (32, False), (24, True), (8, False)])
+@pytest.mark.parametrize("lens", [([1], [1]), ([1, 1, 1], [33, 1, 700]), ([5, 0, 30], [5, 40, 65])],
+                         ids=lambda v: "-".join(map(str, v[0])))
+def test_append(torch_dev, types, rot, interleaved, lens):
+    gh = _gh()
+    for heads, kv_heads, d, page, layout in ((4, 2, 64, 16, "rows"), (3, 1, 72, 5, "heads"), (8, 8, 128, 1, "pairs")):
+        b = P.batch(*lens, heads=heads, kv_heads=kv_heads, d=d, page=page, types=types, seed=20, pad=3, stale=9.0,
+                    layout=layout)
+        cos = sin = None
+        if rot:
+            cos, sin = P.angles(b["page_table"].shape[1] * page, rot)
+        x = P.to(b, torch_dev)
+        q_out = torch.full_like(x["q"], 5.0)
+        dc, ds = (None, None) if cos is None else (cos.to(torch_dev), sin.to(torch_dev))
+        r = gh.paged_append(*P.args(x), x["k"], x["v"], q=x["q"], q_out=q_out, cos=dc, sin=ds, interleaved=interleaved)
+        assert r is q_out
+        got_k, got_v, got_q = x["k_pages"].double().cpu(), x["v_pages"].double().cpu(), q_out.double().cpu()
+        want_k, want_v, want_q = b["k_pages"].double(), b["v_pages"].double(), torch.full_like(got_q, 5.0)
+        mag_k, mag_q = torch.zeros_like(want_k), torch.zeros_like(want_q)
+        for s in range(len(lens[0])):
+            a, e, n = int(b["q_offsets"][s]), int(b["q_offsets"][s + 1]), int(b["kv_lens"][s])
+            for t in range(a, e):
+                p = n - (e - t)
+                at = (b["page_table"][s, p // page].long(), p % page)
+                want_k[at] = P.turned(b["k"][t], p, cos, sin, interleaved)
+                want_v[at] = b["v"][t].double()
+                want_q[t] = P.turned(b["q"][t], p, cos, sin, interleaved)
+                # two products and a sum in fp32, of at most |a| + |b|
+                mag_k[at] = 2 * b["k"][t].abs().double().amax()
+                mag_q[t] = 2 * b["q"][t].abs().double().amax()
+        hc, ha = P.half_step(x["k_pages"].dtype), P.half_step(x["q"].dtype)
+        assert (got_k - want_k).abs().le(hc * want_k.abs() * (1 + 2 ** -10) + 2.0 ** -23 * mag_k).all()
+        assert (got_v - want_v).abs().le(hc * want_v.abs()).all()
+        assert (got_q - want_q).abs().le(ha * want_q.abs() * (1 + 2 ** -10) + 2.0 ** -23 * mag_q).all()
+
+
+def test_append_in_place_strided_and_without_q(torch_dev):
+    gh = _gh()
+    b = P.batch([1, 9], [20, 30], heads=4, kv_heads=2, d=64, page=16, types=("bf16", "bf16"), seed=21, stale=0.0)
+    cos, sin = (t.to(torch_dev) for t in P.angles(b["page_table"].shape[1] * 16, 64))
+    x = P.to(b, torch_dev)
+    q_out = gh.paged_append(*P.args(x), x["k"], x["v"], q=x["q"], cos=cos, sin=sin)
+    fused = torch.cat([x["q"], x["k"], x["v"]], 1)
+    y = P.to(b, torch_dev)
+    q = fused[:, :4]
+    assert gh.paged_append(*P.args(y), fused[:, 4:6], fused[:, 6:], q=q, q_out=q, cos=cos, sin=sin) is q
+    assert torch.equal(q, q_out) and torch.equal(x["k_pages"], y["k_pages"]) and torch.equal(x["v_pages"], y["v_pages"])
+    z = P.to(b, torch_dev)
+    assert gh.paged_append(*P.args(z), z["k"], z["v"], cos=cos, sin=sin) is None
+    assert torch.equal(x["k_pages"], z["k_pages"]) and torch.equal(x["v_pages"], z["v_pages"])
+
+
+# ---- together --------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+def test_chunks_then_tokens_give_what_one_prompt_gives(torch_dev, types):
+    """A prompt in one call, and in chunks followed by single tokens: append
+    and attend at every step.  The same keys and probabilities, in other
+    tiles: both within the bound of the plain form over the cache."""
+    gh = _gh()
+    n, page = 150, 16
+    b = P.batch([n], [n], heads=8, kv_heads=2, d=64, page=page, types=types, seed=22)
+    cos, sin = (t.to(torch_dev) for t in P.angles(b["page_table"].shape[1] * page, 64))
+    x = P.to(b, torch_dev)
+    q = gh.paged_append(*P.args(x), x["k"], x["v"], q=x["q"], cos=cos, sin=sin)
+    out = gh.paged_attention(q, *P.args(x))
+    host = dict(b, k_pages=x["k_pages"].cpu(), v_pages=x["v_pages"].cpu(), q=q.cpu())
+    want, bound = P.attention(host)
+    _check(out, want, bound)
+    y = P.to(b, torch_dev)
+    at = 0
+    for m in [64, 33, 20] + [1] * 33:
+        off = torch.tensor([0, m], dtype=torch.int32, device=torch_dev)
+        kl = torch.tensor([at + m], dtype=torch.int32, device=torch_dev)
+        cache = (y["k_pages"], y["v_pages"], y["page_table"], off, kl)
+        r = gh.paged_append(*cache, y["k"][at:at + m], y["v"][at:at + m], q=y["q"][at:at + m], cos=cos, sin=sin)
+        assert torch.equal(r, q[at:at + m])
+        _check(gh.paged_attention(r, *cache), want[at:at + m], bound[at:at + m])
+        at += m
+    assert torch.equal(x["k_pages"].nan_to_num(9), y["k_pages"].nan_to_num(9))
+
+
+def test_captured_step_follows_lengths_and_tables(torch_dev):
+    """A decode step captured once and replayed while the sequences grow, a
+    second graph with its own workspace beside it, eager work between."""
+    gh = _gh()
+    types = ("bf16", "bf16")
+    b = P.batch([1, 1, 1], [2000, 700, 60], heads=8, kv_heads=2, d=128, page=16, types=types, seed=23, stale=0.0)
+    x = P.to(b, torch_dev)
+    cos, sin = (t.to(torch_dev) for t in P.angles(b["page_table"].shape[1] * 16, 128))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    size = gh.paged_attention_workspace_size(x["q"], *P.args(x))
+    assert size > 0
+    ws = [torch.empty(size, dtype=torch.uint8, device=torch_dev) for _ in range(2)]
+    outs = [torch.empty_like(x["q"]) for _ in range(2)]
+    qs = [torch.empty_like(x["q"]) for _ in range(2)]
+
+    def step(i):
+        gh.paged_append(*P.args(x), x["k"], x["v"], q=x["q"], q_out=qs[i], cos=cos, sin=sin)
+        gh.paged_attention(qs[i], *P.args(x), out=outs[i], workspace=ws[i])
+
+    graphs = []
+    for i, s in enumerate(streams):
+        s.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            step(i)
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for rep in range(4):
+        x["kv_lens"].copy_(torch.tensor([1900 + 7 * rep, 650 + rep, 50 + rep], dtype=torch.int32))
+        x["q"].normal_()
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        want = gh.paged_attention(qs[0], *P.args(x))
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want) and torch.equal(got[1], want), rep
