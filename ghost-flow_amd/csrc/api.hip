@@ -132,6 +132,27 @@ namespace {
 
 int elem_bytes(int dtype) { return dtype == GFH_F32 ? 4 : 2; }
 
+// A 4-bit weight's sizes: [n, k] in groups of `group` columns.
+int check_w4(const char *who, int64_t n, int64_t k, int64_t group) {
+    if (n < 0 || k < 0 || n > kMaxDim || k > (int64_t)1 << 30 || k % 32 != 0)
+        return set_error(GFH_INVALID_SHAPE, "%s: n=%lld k=%lld out of range (k a multiple of 32)", who, (long long)n,
+                         (long long)k);
+    if (group < 32 || group > (int64_t)1 << 30 || group % 32 != 0)
+        return set_error(GFH_INVALID_SHAPE, "%s: group %lld must be a multiple of 32", who, (long long)group);
+    if (!count_ok({n, k, 4})) return set_error(GFH_INVALID_SHAPE, "%s: weight extent overflows", who);
+    return GFH_SUCCESS;
+}
+
+int check_w4_memory(const char *who, const uint8_t *codes, const float *scales, const uint8_t *zps, int64_t n, int64_t k,
+                    int64_t group) {
+    const size_t groups = (size_t)((k + group - 1) / group);
+    GFH_TRY(require_range(codes, (size_t)n * (size_t)k / 2, "codes"));
+    GFH_TRY(require_range(scales, (size_t)n * groups * 4, "scales"));
+    GFH_TRY(optional_range(zps, (size_t)n * groups, "zero_points"));
+    if (!aligned16(codes)) return set_error(GFH_INVALID_DATA, "%s: codes must be 16-byte aligned", who);
+    return GFH_SUCCESS;
+}
+
 // The checks that both calls over a paged cache make of it and of the batch.
 int check_paged(const char *who, const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads) {
     if (!kv) return set_error(GFH_NULL_POINTER, "%s: kv is NULL", who);
@@ -1036,6 +1057,89 @@ GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t token
         const size_t need = paged_attention_workspace_bytes(d);
         if (need) GFH_TRY(ws.acquire(workspace, workspace_bytes, need, s));
         return launch_paged_attention(d, ws.ptr(), s);
+    });
+}
+
+GFH_API int gfh_quantize_i4_grouped(const float *w, int64_t n, int64_t k, int64_t group, uint8_t *codes, float *scales,
+                                    uint8_t *zero_points, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "quantize_i4_grouped";
+        GFH_TRY(check_w4(who, n, k, group));
+        if (n == 0 || k == 0) return GFH_SUCCESS;
+        GFH_TRY(require_range(w, (size_t)n * (size_t)k * 4, "w"));
+        GFH_TRY(check_w4_memory(who, codes, scales, zero_points, n, k, group));
+        if (!aligned16(w)) return set_error(GFH_INVALID_DATA, "%s: w must be 16-byte aligned", who);
+        GFH_TRY(ensure_init());
+        return launch_quantize_w4(w, n, k, group, codes, scales, zero_points, as_stream(stream));
+    });
+}
+
+GFH_API int gfh_dequantize_i4_grouped(const uint8_t *codes, const float *scales, const uint8_t *zero_points, int64_t n,
+                                      int64_t k, int64_t group, float *out, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "dequantize_i4_grouped";
+        GFH_TRY(check_w4(who, n, k, group));
+        if (n == 0 || k == 0) return GFH_SUCCESS;
+        GFH_TRY(check_w4_memory(who, codes, scales, zero_points, n, k, group));
+        GFH_TRY(require_range(out, (size_t)n * (size_t)k * 4, "out"));
+        if (!aligned16(out)) return set_error(GFH_INVALID_DATA, "%s: out must be 16-byte aligned", who);
+        GFH_TRY(ensure_init());
+        return launch_dequantize_w4(codes, scales, zero_points, n, k, group, out, as_stream(stream));
+    });
+}
+
+GFH_API size_t gfh_linear_w4_workspace_size(int dtype, int64_t m, int64_t n, int64_t k) {
+    if ((dtype != GFH_F16 && dtype != GFH_BF16 && dtype != GFH_F32) || m <= 0 || n <= 0 || k <= 0 || m > (1 << 19) ||
+        check_w4("linear_w4", n, k, 32) != GFH_SUCCESS || !count_ok({m, n, 4096}))
+        return 0;
+    LinearW4Desc d;
+    d.dtype = dtype;
+    d.m = m, d.n = n, d.k = k;
+    return linear_w4_workspace_bytes(d);
+}
+
+GFH_API int gfh_linear_w4(int dtype, const void *x, int64_t ldx, const uint8_t *codes, const float *scales,
+                          const uint8_t *zero_points, const void *bias, void *y, int64_t ldy, int64_t m, int64_t n,
+                          int64_t k, int64_t group, void *workspace, size_t workspace_bytes, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "linear_w4";
+        if (dtype != GFH_F16 && dtype != GFH_BF16 && dtype != GFH_F32)
+            return set_error(GFH_INVALID_DATA, "%s: dtype %d", who, dtype);
+        GFH_TRY(check_w4(who, n, k, group));
+        if (m < 0 || m > (1 << 19) || !count_ok({m, n, 4096}))
+            return set_error(GFH_INVALID_SHAPE, "%s: m=%lld out of range", who, (long long)m);
+        if (ldx < k || ldy < n)
+            return set_error(GFH_INVALID_SHAPE, "%s: ldx=%lld ldy=%lld below k=%lld, n=%lld", who, (long long)ldx,
+                             (long long)ldy, (long long)k, (long long)n);
+        if (m == 0 || n == 0) return GFH_SUCCESS;
+        if (k == 0) return set_error(GFH_INVALID_SHAPE, "%s: no columns", who);
+        int64_t ex, ey;
+        if (!extent2d(m, k, ldx, &ex) || !extent2d(m, n, ldy, &ey))
+            return set_error(GFH_INVALID_SHAPE, "%s: operand extent overflows", who);
+        const size_t eb = (size_t)elem_bytes(dtype);
+        GFH_TRY(require_range(x, (size_t)ex * eb, "x"));
+        GFH_TRY(check_w4_memory(who, codes, scales, zero_points, n, k, group));
+        GFH_TRY(optional_range(bias, (size_t)n * eb, "bias"));
+        GFH_TRY(require_range(y, (size_t)ey * eb, "y"));
+        if (workspace && !aligned16(workspace))
+            return set_error(GFH_INVALID_DATA, "%s: the workspace must be 16-byte aligned", who);
+        GFH_TRY(ensure_init());
+        LinearW4Desc d;
+        d.dtype = dtype;
+        d.x = x;
+        d.ldx = ldx;
+        d.codes = codes;
+        d.scales = scales;
+        d.zps = zero_points;
+        d.bias = bias;
+        d.y = y;
+        d.ldy = ldy;
+        d.m = m, d.n = n, d.k = k, d.group = group;
+        hipStream_t s = as_stream(stream);
+        Scratch ws;
+        const size_t need = linear_w4_workspace_bytes(d);
+        if (need) GFH_TRY(ws.acquire(workspace, workspace_bytes, need, s));
+        return launch_linear_w4(d, ws.ptr(), s);
     });
 }
 

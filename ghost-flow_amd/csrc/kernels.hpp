@@ -212,6 +212,27 @@ struct PagedAttnDesc {
 size_t paged_attention_workspace_bytes(const PagedAttnDesc &d);
 int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t s);
 
+// w4.hip: 4-bit weights in groups of columns (codes [n, k / 2], scales and
+// zero points [n, ceil(k / group)], zps nullable), k and group multiples of 32.
+int launch_quantize_w4(const float *w, int64_t n, int64_t k, int64_t group, uint8_t *codes, float *scales, uint8_t *zps,
+                       hipStream_t s);
+int launch_dequantize_w4(const uint8_t *codes, const float *scales, const uint8_t *zps, int64_t n, int64_t k,
+                         int64_t group, float *out, hipStream_t s);
+struct LinearW4Desc {
+    int dtype = 0;  // of x, bias and y
+    const void *x = nullptr;
+    int64_t ldx = 0;
+    const uint8_t *codes = nullptr;
+    const float *scales = nullptr;
+    const uint8_t *zps = nullptr;
+    const void *bias = nullptr;
+    void *y = nullptr;
+    int64_t ldy = 0;
+    int64_t m = 0, n = 0, k = 0, group = 0;
+};
+size_t linear_w4_workspace_bytes(const LinearW4Desc &d);
+int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s);
+
 // mha.hip: MultiHeadAttention::forward_with_cache over a [b, capacity, e]
 // K/V cache; the workspace holds the projected queries and the attention
 // output (mha_workspace_bytes).

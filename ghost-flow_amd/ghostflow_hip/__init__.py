@@ -11,6 +11,7 @@ from .ops import (  # noqa: F401
     GhostFlowError,
     StateDict,
     dequantize,
+    dequantize_grouped_i4,
     flash_attention_blockwise,
     gemv_f32,
     gemv_w8,
@@ -18,6 +19,8 @@ from .ops import (  # noqa: F401
     kv_attention,
     lib,
     linear,
+    linear_w4,
+    linear_w4_workspace_size,
     load_state_dict,
     matmul,
     matmul_backward,
@@ -30,6 +33,7 @@ from .ops import (  # noqa: F401
     qlinear,
     qlinear_dynamic,
     qswiglu,
+    quantize_grouped_i4,
     quantize_per_channel,
     quantize_per_tensor,
     quantize_per_tensor_workspace_size,

@@ -66,6 +66,22 @@ def _need(t, dtype, name):
         raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be contiguous")
 
 
+_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
+def _dtype(t, name):
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return d
+
+
+def _same_device(dev, *tensors):
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise GhostFlowError(_lib.INVALID_DATA, f"all tensors must be on {dev}, one is on {t.device}")
+
+
 def lib():
     return _lib.load()
 
@@ -242,6 +258,91 @@ def qlinear_dynamic(x, qw, sw, w_rowsum, *, bias=None, out=None, workspace=None)
     ws_ptr, ws_bytes = _workspace(workspace)
     _check(lib().gfh_qlinear_dynamic_i8(x.data_ptr(), qw.data_ptr(), sw.data_ptr(), w_rowsum.data_ptr(),
                                         _ptr(bias), y.data_ptr(), m, n, k, ws_ptr, ws_bytes, _stream(x.device)))
+    return y
+
+
+# ---- 4-bit weights in groups ------------------------------------------------------
+
+def _groups(k, group_size):
+    return -(-k // group_size) if group_size > 0 else 0
+
+
+def quantize_grouped_i4(w, group_size=128, symmetric=True):
+    """4-bit codes [n, k / 2] (two per byte, even column low), fp32 scales
+    [n, groups] and zero points [n, groups] (bytes; None if symmetric) of a
+    Linear weight w [n, k], a scale per group of group_size columns; k and
+    group_size are multiples of 32.  gfh_quantize_i4_grouped in
+    ghostflow_hip.h has the formulas."""
+    _need(w, torch.float32, "w")
+    if w.dim() != 2:
+        raise GhostFlowError(_lib.INVALID_SHAPE, "w must be [n, k]")
+    n, k = w.shape
+    groups = _groups(k, group_size)
+    codes = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
+    scales = torch.empty((n, groups), dtype=torch.float32, device=w.device)
+    zps = None if symmetric else torch.empty((n, groups), dtype=torch.uint8, device=w.device)
+    with torch.cuda.device(w.device):
+        _check(lib().gfh_quantize_i4_grouped(w.data_ptr(), n, k, group_size, codes.data_ptr(), scales.data_ptr(),
+                                             _ptr(zps), _stream(w.device)))
+    return codes, scales, zps
+
+
+def _need_w4(codes, scales, zero_points, group_size):
+    _need(codes, torch.uint8, "codes")
+    _need(scales, torch.float32, "scales")
+    _need(zero_points, torch.uint8, "zero_points")
+    if codes.dim() != 2:
+        raise GhostFlowError(_lib.INVALID_SHAPE, "codes must be [n, k / 2]")
+    n, k = codes.shape[0], 2 * codes.shape[1]
+    want = (n, _groups(k, group_size))
+    for t, name in ((scales, "scales"), (zero_points, "zero_points")):
+        if t is not None and tuple(t.shape) != want:
+            raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be {list(want)} for groups of {group_size}, got "
+                                 f"{list(t.shape)}")
+    return n, k
+
+
+def dequantize_grouped_i4(codes, scales, zero_points=None, group_size=128):
+    """The weight [n, k] in fp32 that quantize_grouped_i4's result stands for."""
+    n, k = _need_w4(codes, scales, zero_points, group_size)
+    _same_device(codes.device, scales, zero_points)
+    out = torch.empty((n, k), dtype=torch.float32, device=codes.device)
+    with torch.cuda.device(codes.device):
+        _check(lib().gfh_dequantize_i4_grouped(codes.data_ptr(), scales.data_ptr(), _ptr(zero_points), n, k, group_size,
+                                               out.data_ptr(), _stream(codes.device)))
+    return out
+
+
+def linear_w4_workspace_size(m: int, n: int, k: int, dtype=torch.float32) -> int:
+    return int(lib().gfh_linear_w4_workspace_size(_DTYPES.get(dtype, -1), m, n, k))
+
+
+def linear_w4(x, codes, scales, zero_points=None, bias=None, *, group_size=128, out=None, workspace=None):
+    """Linear::forward (linear.rs:56-69) on a 4-bit weight: y = x . W'^T + bias
+    for x [m, k] (rows may be strided), of float32, bfloat16 or float16 like
+    bias and y."""
+    n, k = _need_w4(codes, scales, zero_points, group_size)
+    if not x.is_cuda:
+        raise GhostFlowError(_lib.INVALID_DATA, "x must be a device tensor")
+    dt = _dtype(x, "x")
+    if x.dim() != 2 or x.shape[1] != k:
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"x must be [m, {k}], got {list(x.shape)}")
+    m = x.shape[0]
+    if k > 1 and x.stride(1) != 1:
+        raise GhostFlowError(_lib.INVALID_DATA, "the columns of x must be contiguous")
+    _need(bias, x.dtype, "bias")
+    if bias is not None and tuple(bias.shape) != (n,):
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"bias must be [{n}], got {list(bias.shape)}")
+    y = torch.empty((m, n), dtype=x.dtype, device=x.device) if out is None else out
+    _need(y, x.dtype, "out")
+    if tuple(y.shape) != (m, n):
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"out must be [{m}, {n}], got {list(y.shape)}")
+    _same_device(x.device, codes, scales, zero_points, bias, y, workspace)
+    ws, ws_bytes = _workspace(workspace)
+    with torch.cuda.device(x.device):
+        _check(lib().gfh_linear_w4(dt, x.data_ptr(), x.stride(0) if m > 1 else k, codes.data_ptr(), scales.data_ptr(),
+                                   _ptr(zero_points), _ptr(bias), y.data_ptr(), n, m, n, k, group_size, ws, ws_bytes,
+                                   _stream(x.device)))
     return y
 
 
@@ -424,16 +525,6 @@ def mha_forward_with_cache(query, key, value, wq, bq, wk, bk, wv, bv, wo, bo, nu
 
 # ---- key/value cache in pages ---------------------------------------------------
 
-_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
-
-
-def _dtype(t, name):
-    d = _DTYPES.get(t.dtype)
-    if d is None:
-        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    return d
-
-
 def _rows(t, name, dtype, tokens, heads, d):
     """Elements between the tokens of t [tokens, heads, d] (heads and dims
     contiguous)."""
@@ -554,12 +645,6 @@ def paged_attention_workspace_size(q, k_pages, v_pages, page_table, q_offsets, k
     """Bytes of paged_attention's workspace for these arguments."""
     kv = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, None, q.device)
     return int(lib().gfh_paged_attention_workspace_size(_byref(kv), q.shape[0], q.shape[1], int(max_kv_len or 0)))
-
-
-def _same_device(dev, *tensors):
-    for t in tensors:
-        if t is not None and t.device != dev:
-            raise GhostFlowError(_lib.INVALID_DATA, f"all tensors must be on {dev}, one is on {t.device}")
 
 
 # ---- SwiGLU feed-forward block (ghostflow-nn/src/llama.rs:259-287) -------------

@@ -66,6 +66,10 @@ typedef enum gfh_status {
 
 typedef void *gfh_stream_t;
 
+/* Element types of activations and caches where a call takes several: the
+ * dtype bytes of the state dict (ghostflow-core/src/serialize.rs:188-215). */
+typedef enum gfh_dtype { GFH_F16 = 0, GFH_BF16 = 1, GFH_F32 = 2 } gfh_dtype;
+
 /* ---- library ----------------------------------------------------------- */
 
 /* Replaces ghostflow_init (ghostflow-ffi/src/lib.rs:60-64): checks that a
@@ -193,6 +197,43 @@ GFH_API int gfh_qlinear_dynamic_i8(const float *x, const int8_t *qw, const float
                                    const int32_t *w_rowsum, const float *bias, float *y,
                                    int64_t m, int64_t n, int64_t k, void *workspace,
                                    size_t workspace_bytes, gfh_stream_t stream);
+
+/* ---- 4-bit weights in groups ----------------------------------------------- */
+
+/* The reference's quantization stops at 8 bits; these are its two schemes
+ * (quantization.rs:77-153) on 16 levels, per group of `group` columns of a row
+ * of a Linear weight [n, k] ([out, in]):
+ *   codes  [n, k / 2], two per byte, the even column in the low four bits
+ *   scales [n, groups] fp32, groups = ceil(k / group) (the last may be shorter)
+ *   zero_points [n, groups] bytes 0 .. 15; NULL: symmetric
+ *   symmetric:  s = max|w| (1/7),  c = clamp(round(w / s), -8, 7) + 8,  w' = (c - 8) s
+ *   asymmetric: s = (max(w, 0) - min(w, 0)) (1/15),  z = clamp(round(-min(w, 0) / s), 0, 15),
+ *               c = clamp(round(w / s) + z, 0, 15),  w' = (c - z) s
+ * with the fp32 constants 1/7 and 1/15; round is half away from zero; a group
+ * without a range has s = 1; a NaN counts as 0; weights are finite otherwise.  k and group are multiples of 32;
+ * w, codes and out are 16-byte aligned. */
+GFH_API int gfh_quantize_i4_grouped(const float *w, int64_t n, int64_t k, int64_t group,
+                                    uint8_t *codes, float *scales, uint8_t *zero_points,
+                                    gfh_stream_t stream);
+GFH_API int gfh_dequantize_i4_grouped(const uint8_t *codes, const float *scales,
+                                      const uint8_t *zero_points, int64_t n, int64_t k,
+                                      int64_t group, float *out, gfh_stream_t stream);
+
+/* Linear on such a weight: y[m, n] = x[m, k] . w'^T + bias[n], the codes taken
+ * apart in registers.  x, bias (nullable) and y are of type dtype, rows of x
+ * ldx and of y ldy elements apart.  Products of x with (c - z) in fp32, a
+ * group's sum times its scale, sums in fp32, y rounded once.  fp32 x is carried
+ * with all its bits for m <= 4 and above with at least 33 bits below the largest
+ * magnitude of its row in each 256 columns; bf16 likewise (8 bits down to 2^-29
+ * of that).  An infinite or NaN x gives inf / NaN.  Meant for few rows (decode);
+ * any m is served.  y overlaps no input.
+ * workspace (nullable, 16-byte aligned) of at least
+ * gfh_linear_w4_workspace_size(...) bytes; any contents. */
+GFH_API size_t gfh_linear_w4_workspace_size(int dtype, int64_t m, int64_t n, int64_t k);
+GFH_API int gfh_linear_w4(int dtype, const void *x, int64_t ldx, const uint8_t *codes,
+                          const float *scales, const uint8_t *zero_points, const void *bias,
+                          void *y, int64_t ldy, int64_t m, int64_t n, int64_t k, int64_t group,
+                          void *workspace, size_t workspace_bytes, gfh_stream_t stream);
 
 /* ---- decode GEMV --------------------------------------------------------- */
 
@@ -355,10 +396,6 @@ GFH_API int gfh_mha_forward_with_cache_f32(
     size_t workspace_bytes, gfh_stream_t stream);
 
 /* ---- key/value cache in pages -------------------------------------------- */
-
-/* Element types of activations and caches: the dtype bytes of the state dict
- * (ghostflow-core/src/serialize.rs:188-215). */
-typedef enum gfh_dtype { GFH_F16 = 0, GFH_BF16 = 1, GFH_F32 = 2 } gfh_dtype;
 
 /* A key/value cache in pages and the ragged batch of a step (host struct of
  * device pointers; no counterpart in the reference, whose cache is the copied

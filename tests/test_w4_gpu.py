@@ -1,0 +1,194 @@
+"""4-bit weights in groups on the GPU: codes and back bit for bit against the
+scheme's arithmetic, Linear on them against 64 bits."""
+import pytest
+import torch
+
+import _w4 as W
+
+pytestmark = pytest.mark.gpu
+
+
+def _gh():
+    import ghostflow_hip
+    return ghostflow_hip
+
+
+@pytest.mark.parametrize("n,k,group", [(1, 32, 32), (7, 96, 32), (33, 416, 64), (5, 4096, 128), (3, 1000 * 32, 256),
+                                       (9, 320, 320), (4, 2080, 1024), (6, 672, 96), (2, 64, 4096)])
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_quantize_and_back(torch_dev, n, k, group, symmetric):
+    gh = _gh()
+    g = torch.Generator().manual_seed(k + group)
+    w = torch.randn(n, k, generator=g) * 0.02
+    w[0, :32] = 0.0                       # a group without a range (group 32)
+    w[-1] = w[-1].abs() + 0.01            # one sign only
+    w[n // 2, ::3] *= -1
+    w[:, 1] = torch.where(w[:, 1] == 0, 0.5, w[:, 1])
+    want = W.quantize(w, group, symmetric)
+    got = gh.quantize_grouped_i4(w.to(torch_dev), group, symmetric=symmetric)
+    for a, b in zip(got, want):
+        assert (a is None) == (b is None)
+        if a is not None:
+            assert torch.equal(a.cpu(), b)
+    back = gh.dequantize_grouped_i4(*got, group).cpu()
+    assert torch.equal(back, W.weight(*want, group).float())
+    # no further from the weight than half a step, where no code was clamped;
+    # the largest magnitude of a symmetric group is 7 steps, of an asymmetric
+    # one at most a step beyond the zero point's rounding
+    step = W.spread(want[1], k, group)
+    assert (back - w).abs().le(step * (0.5 if symmetric else 1.0) * (1 + 2 ** -20)).all()
+
+
+def test_quantize_borders_and_nan(torch_dev):
+    gh = _gh()
+    w = torch.zeros(4, 32)
+    w[0] = torch.arange(32) * 0.5 - 7.0        # ties between two codes, clamped above
+    w[0, 31] = 7.0
+    w[1, 3] = float("nan")
+    w[1, 4] = 3.5
+    w[2] = float("nan")
+    w[3, 0] = 1e-45
+    for symmetric in (True, False):
+        got = gh.quantize_grouped_i4(w.to(torch_dev), 32, symmetric=symmetric)
+        clean = w.nan_to_num(0.0)
+        want = W.quantize(clean, 32, symmetric)
+        assert torch.equal(got[0][:3].cpu(), want[0][:3]) and torch.equal(got[1][:3].cpu(), want[1][:3])
+        assert torch.isfinite(got[1]).all() and (got[1] > 0).all()
+
+
+def _linear(dev, x, wt, group, bias=None, **kw):
+    gh = _gh()
+    d = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    y = gh.linear_w4(d(x), d(wt[0]), d(wt[1]), d(wt[2]), d(bias), group_size=group, **kw)
+    torch.cuda.synchronize()
+    return y.cpu()
+
+
+SHAPES = [(1, 1, 32, 32), (2, 5, 64, 32), (3, 40, 1024, 128), (4, 4100, 96, 32), (1, 3000, 4096, 128),
+          (5, 33, 256, 64), (16, 100, 416, 32), (17, 64, 1024, 128), (33, 200, 800, 128), (50, 130, 2048, 64),
+          (64, 65, 544, 256), (80, 70, 320, 96), (6, 20, 20000 // 32 * 32, 128), (1, 9, 14336, 128),
+          (9, 700, 352, 1024), (130, 300, 288, 32)]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda v: "x".join(map(str, v)))
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_whole_numbers_are_exact(torch_dev, shape, kind, zeros):
+    """Whole x, scales that are powers of two: every sum is exact in fp32, so
+    the result is the 64-bit one rounded once."""
+    m, n, k, group = shape
+    g = torch.Generator().manual_seed(m * n + k)
+    wt = W.random_weight(n, k, group, zeros, seed=k + n, exact=True)
+    x = torch.randint(-3, 4, (m, k), generator=g).to(W.TYPES[kind])
+    bias = torch.randint(-9, 10, (n,), generator=g).to(W.TYPES[kind])
+    want = x.double() @ W.weight(*wt, group).t() + bias.double()
+    assert torch.equal(_linear(torch_dev, x, wt, group, bias), want.to(W.TYPES[kind]))
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda v: "x".join(map(str, v)))
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_linear_random(torch_dev, shape, kind):
+    """Sums of k fp32 products in any order: each of the at most k roundings of
+    a sum, and two more per product, is 2^-24 of no more than the sum of
+    magnitudes; one rounding to the output's type."""
+    m, n, k, group = shape
+    g = torch.Generator().manual_seed(m + n + k)
+    wt = W.random_weight(n, k, group, True, seed=k)
+    x = torch.randn(m, k, generator=g).to(W.TYPES[kind])
+    w = W.weight(*wt, group)
+    want = x.double() @ w.t()
+    size = x.double().abs() @ w.abs().t()
+    bound = (k + 2) * 2.0 ** -24 * size + torch.finfo(W.TYPES[kind]).eps / 2 * (want.abs() * (1 + 2 ** -9))
+    assert (_linear(torch_dev, x, wt, group).double() - want).abs().le(bound).all()
+
+
+@pytest.mark.parametrize("m", [1, 4, 7, 40])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_linear_rows_of_very_different_size(torch_dev, m, kind):
+    """Rows, and slices of a row, that lie powers of two apart keep their own
+    relative accuracy (relative to their own magnitudes)."""
+    k, n, group = 1024, 48, 64
+    g = torch.Generator().manual_seed(m)
+    wt = W.random_weight(n, k, group, True, seed=3)
+    x = torch.randn(m, k, generator=g)
+    x *= 2.0 ** torch.linspace(-100, 90, m).round()[:, None]
+    x = x.to(W.TYPES[kind])
+    w = W.weight(*wt, group)
+    want = x.double() @ w.t()
+    size = x.double().abs() @ w.abs().t()
+    bound = (k + 2) * 2.0 ** -24 * size + torch.finfo(W.TYPES[kind]).eps / 2 * want.abs() * (1 + 2 ** -9)
+    assert (_linear(torch_dev, x, wt, group).double() - want).abs().le(bound).all()
+
+
+@pytest.mark.parametrize("m", [1, 3, 6, 50])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_linear_values_that_are_not_finite_stay_in_their_row(torch_dev, m, kind, value):
+    k, n, group = 512, 40, 128
+    g = torch.Generator().manual_seed(m)
+    wt = W.random_weight(n, k, group, False, seed=4)
+    x = torch.randn(m, k, generator=g).to(W.TYPES[kind])
+    ref = _linear(torch_dev, x, wt, group)
+    x[m - 1, 77] = value
+    got = _linear(torch_dev, x, wt, group)
+    assert torch.equal(got[:m - 1], ref[:m - 1])
+    c = W.unpack(wt[0])[:, 77].int() - 8
+    if value != value:
+        assert torch.isnan(got[m - 1]).all()
+    else:
+        assert torch.isinf(got[m - 1][c > 0]).all() and (got[m - 1][c > 0] > 0).all()
+        assert (got[m - 1][c < 0] < 0).all() and torch.isnan(got[m - 1][c == 0]).all()
+
+
+@pytest.mark.parametrize("m", [1, 20])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_linear_strided_rows_and_out(torch_dev, m, kind):
+    gh = _gh()
+    k, n, group = 640, 50, 32
+    wt = [None if t is None else t.to(torch_dev) for t in W.random_weight(n, k, group, True, seed=5)]
+    wide = torch.randn(m, k + 37, device=torch_dev).to(W.TYPES[kind])
+    for at in (0, 1, 8, 37):  # 16-byte aligned rows and others
+        x = wide[:, at:at + k]
+        want = gh.linear_w4(x.contiguous(), *wt, group_size=group)
+        out = torch.empty_like(want)
+        assert gh.linear_w4(x, *wt, group_size=group, out=out) is out
+        assert torch.equal(out, want)
+
+
+def test_linear_on_a_quantized_weight(torch_dev):
+    """quantize -> Linear is Linear on the dequantized weight."""
+    gh = _gh()
+    g = torch.Generator().manual_seed(6)
+    w = (torch.randn(300, 1088, generator=g) * 0.02).to(torch_dev)
+    for symmetric in (True, False):
+        q = gh.quantize_grouped_i4(w, 64, symmetric=symmetric)
+        back = gh.dequantize_grouped_i4(*q, 64).double().cpu()
+        for m in (1, 30):
+            x = torch.randn(m, 1088, generator=g)
+            y = gh.linear_w4(x.to(torch_dev), *q, group_size=64).double().cpu()
+            size = x.double().abs() @ back.abs().t()
+            assert (y - x.double() @ back.t()).abs().le(1091 * 2.0 ** -24 * size).all()
+
+
+def test_captured_linear_replays(torch_dev):
+    gh = _gh()
+    k, n, group = 4096, 512, 128
+    wt = [None if t is None else t.to(torch_dev) for t in W.random_weight(n, k, group, True, seed=7)]
+    x = torch.randn(16, k, device=torch_dev)
+    y = torch.empty(16, n, device=torch_dev)
+    size = gh.linear_w4_workspace_size(16, n, k)
+    assert size > 0
+    ws = torch.empty(size, dtype=torch.uint8, device=torch_dev)
+    s = torch.cuda.Stream()
+    g = torch.cuda.CUDAGraph()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(g, stream=s):
+        gh.linear_w4(x, *wt, group_size=group, out=y, workspace=ws)
+    for rep in range(4):
+        x.normal_()
+        ws.fill_(0xff)
+        want = gh.linear_w4(x, *wt, group_size=group)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want), rep
