@@ -7,7 +7,7 @@ library's status code and thread-local message when a call fails.
 """
 from __future__ import annotations
 
-from ctypes import byref as _byref
+import struct
 from functools import lru_cache
 
 import torch
@@ -80,6 +80,21 @@ def _same_device(dev, *tensors):
     for t in tensors:
         if t is not None and t.device != dev:
             raise GhostFlowError(_lib.INVALID_DATA, f"all tensors must be on {dev}, one is on {t.device}")
+
+
+def _call(dev, fn, *args):
+    """fn(*args, stream) on dev's current stream, with dev the current device
+    (a launch goes to the current one).  A call costs about as much host time
+    as a decode step's kernels take: the device is only switched where it has
+    to be, and the stream comes as its handle."""
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != _lib.SUCCESS:
+        _check(rc)
 
 
 def lib():
@@ -281,9 +296,8 @@ def quantize_grouped_i4(w, group_size=128, symmetric=True):
     codes = torch.empty((n, k // 2), dtype=torch.uint8, device=w.device)
     scales = torch.empty((n, groups), dtype=torch.float32, device=w.device)
     zps = None if symmetric else torch.empty((n, groups), dtype=torch.uint8, device=w.device)
-    with torch.cuda.device(w.device):
-        _check(lib().gfh_quantize_i4_grouped(w.data_ptr(), n, k, group_size, codes.data_ptr(), scales.data_ptr(),
-                                             _ptr(zps), _stream(w.device)))
+    _call(w.device, lib().gfh_quantize_i4_grouped, w.data_ptr(), n, k, group_size, codes.data_ptr(), scales.data_ptr(),
+          _ptr(zps))
     return codes, scales, zps
 
 
@@ -296,7 +310,7 @@ def _need_w4(codes, scales, zero_points, group_size):
     n, k = codes.shape[0], 2 * codes.shape[1]
     want = (n, _groups(k, group_size))
     for t, name in ((scales, "scales"), (zero_points, "zero_points")):
-        if t is not None and tuple(t.shape) != want:
+        if t is not None and t.shape != want:
             raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be {list(want)} for groups of {group_size}, got "
                                  f"{list(t.shape)}")
     return n, k
@@ -307,9 +321,8 @@ def dequantize_grouped_i4(codes, scales, zero_points=None, group_size=128):
     n, k = _need_w4(codes, scales, zero_points, group_size)
     _same_device(codes.device, scales, zero_points)
     out = torch.empty((n, k), dtype=torch.float32, device=codes.device)
-    with torch.cuda.device(codes.device):
-        _check(lib().gfh_dequantize_i4_grouped(codes.data_ptr(), scales.data_ptr(), _ptr(zero_points), n, k, group_size,
-                                               out.data_ptr(), _stream(codes.device)))
+    _call(codes.device, lib().gfh_dequantize_i4_grouped, codes.data_ptr(), scales.data_ptr(), _ptr(zero_points), n, k,
+          group_size, out.data_ptr())
     return out
 
 
@@ -339,10 +352,8 @@ def linear_w4(x, codes, scales, zero_points=None, bias=None, *, group_size=128, 
         raise GhostFlowError(_lib.INVALID_SHAPE, f"out must be [{m}, {n}], got {list(y.shape)}")
     _same_device(x.device, codes, scales, zero_points, bias, y, workspace)
     ws, ws_bytes = _workspace(workspace)
-    with torch.cuda.device(x.device):
-        _check(lib().gfh_linear_w4(dt, x.data_ptr(), x.stride(0) if m > 1 else k, codes.data_ptr(), scales.data_ptr(),
-                                   _ptr(zero_points), _ptr(bias), y.data_ptr(), n, m, n, k, group_size, ws, ws_bytes,
-                                   _stream(x.device)))
+    _call(x.device, lib().gfh_linear_w4, dt, x.data_ptr(), x.stride(0) if m > 1 else k, codes.data_ptr(),
+          scales.data_ptr(), _ptr(zero_points), _ptr(bias), y.data_ptr(), n, m, n, k, group_size, ws, ws_bytes)
     return y
 
 
@@ -525,50 +536,54 @@ def mha_forward_with_cache(query, key, value, wq, bq, wk, bk, wv, bv, wo, bo, nu
 
 # ---- key/value cache in pages ---------------------------------------------------
 
-def _rows(t, name, dtype, tokens, heads, d):
+def _rows(t, name, like, tokens, heads, d):
     """Elements between the tokens of t [tokens, heads, d] (heads and dims
-    contiguous)."""
-    if not t.is_cuda:
-        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be a device tensor")
-    if t.dtype != dtype:
-        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != (tokens, heads, d):
+    contiguous), of like's type and on its device."""
+    if t.dtype != like.dtype or t.device != like.device or not t.is_cuda:
+        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be {like.dtype} on {like.device} (a GPU), got {t.dtype} on "
+                             f"{t.device}")
+    if t.shape != (tokens, heads, d):
         raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be [{tokens}, {heads}, {d}], got {list(t.shape)}")
     ld, hs, ds = t.stride()
-    if (d > 1 and ds != 1) or (heads > 1 and hs != d):
+    if (ds != 1 and d > 1) or (hs != d and heads > 1):
         raise GhostFlowError(_lib.INVALID_DATA, f"{name}: the heads of a token must be contiguous")
     return ld if tokens > 1 else heads * d
 
 
-def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, tokens_on):
-    for t, n in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if not t.is_cuda or t.device != tokens_on:
-            raise GhostFlowError(_lib.INVALID_DATA, f"{n} must be on {tokens_on}")
-        if t.dim() != 4 or t.shape != k_pages.shape or t.dtype != k_pages.dtype or t.stride() != k_pages.stride():
-            raise GhostFlowError(_lib.INVALID_SHAPE, "k_pages and v_pages must be [pages, page_size, kv_heads, "
-                                 "head_dim], of one type and with one layout")
+_PAGED_KV = struct.Struct("@PPi7qP3qPPP")  # gfh_paged_kv; packed by hand, a ctypes Structure costs 3 us more
+
+
+def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
+    """(gfh_paged_kv, kv_heads, head_dim) of checked arguments."""
+    shape, stride = k_pages.shape, k_pages.stride()
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype != k_pages.dtype:
+        raise GhostFlowError(_lib.INVALID_SHAPE, "k_pages and v_pages must be [pages, page_size, kv_heads, head_dim], of "
+                             "one type and with one layout")
     dt = _dtype(k_pages, "k_pages")
-    pages, page_size, hkv, d = k_pages.shape
-    sp, sr, sh, sd = k_pages.stride()
-    if d > 1 and sd != 1:
+    pages, page_size, hkv, d = shape
+    sp, sr, sh, sd = stride
+    if sd != 1 and d > 1:
         raise GhostFlowError(_lib.INVALID_DATA, "the dims of k_pages must be contiguous")
-    for t, n in ((page_table, "page_table"), (q_offsets, "q_offsets"), (kv_lens, "kv_lens"), (status, "status")):
-        if t is None and n == "status":
-            continue
-        if not t.is_cuda or t.device != tokens_on or t.dtype != torch.int32:
-            raise GhostFlowError(_lib.INVALID_DATA, f"{n} must be an int32 tensor on {tokens_on}")
-        if t.numel() > 1 and t.stride(-1) != 1:
-            raise GhostFlowError(_lib.INVALID_DATA, f"{n} must be contiguous")
-    seqs = kv_lens.numel()
-    if page_table.dim() != 2 or page_table.shape[0] != seqs or kv_lens.dim() != 1 or tuple(q_offsets.shape) != (seqs + 1,):
+    if dev.type != "cuda" or k_pages.device != dev or v_pages.device != dev:
+        raise GhostFlowError(_lib.INVALID_DATA, f"k_pages and v_pages must be on {dev}, a GPU")
+    tshape, tstride = page_table.shape, page_table.stride()
+    seqs = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
+    if len(tshape) != 2 or tshape[0] != seqs or q_offsets.shape != (seqs + 1,):
         raise GhostFlowError(_lib.INVALID_SHAPE, f"page_table [seqs, pages], q_offsets [seqs + 1] and kv_lens [seqs], "
-                             f"got {list(page_table.shape)}, {list(q_offsets.shape)}, {list(kv_lens.shape)}")
-    width = page_table.shape[1]
+                             f"got {list(tshape)}, {list(q_offsets.shape)}, {list(kv_lens.shape)}")
+    width = tshape[1]
+    i32 = torch.int32
+    for t, n in ((page_table, "page_table"), (q_offsets, "q_offsets"), (kv_lens, "kv_lens")):
+        if t.dtype != i32 or t.device != dev or not (t.is_contiguous() or (t is page_table and tstride[1] == 1)):
+            raise GhostFlowError(_lib.INVALID_DATA, f"{n} must be a contiguous int32 tensor on {dev}")
+    if status is not None and (status.dtype != i32 or status.device != dev or status.numel() < 1):
+        raise GhostFlowError(_lib.INVALID_DATA, f"status must be an int32 tensor on {dev}")
     # (a stride over a single element says nothing)
-    return _lib.PagedKv(k_pages.data_ptr(), v_pages.data_ptr(), dt, pages, page_size, hkv, d, sp if pages > 1 else 0,
+    kv = _PAGED_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), dt, pages, page_size, hkv, d, sp if pages > 1 else 0,
                         sr if page_size > 1 else 0, sh if hkv > 1 else 0, page_table.data_ptr(), width,
-                        page_table.stride(0) if seqs > 1 else width, seqs, kv_lens.data_ptr(), q_offsets.data_ptr(),
-                        _ptr(status))
+                        tstride[0] if seqs > 1 else width, seqs, kv_lens.data_ptr(), q_offsets.data_ptr(),
+                        0 if status is None else status.data_ptr())
+    return kv, hkv, d
 
 
 def paged_append(k_pages, v_pages, page_table, q_offsets, kv_lens, k, v, *, q=None, q_out=None, cos=None, sin=None,
@@ -580,23 +595,23 @@ def paged_append(k_pages, v_pages, page_table, q_offsets, kv_lens, k, v, *, q=No
     (into q_out, which may be q; None without q).  gfh_paged_kv in
     ghostflow_hip.h says what page_table [seqs, pages], q_offsets [seqs + 1],
     kv_lens [seqs] (the new tokens included) and status (all int32) are."""
-    tokens, hkv, d = k.shape if k.dim() == 3 else (0, 0, 0)
+    dev = k.device
+    kv, hkv, d = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev)
     dt = _dtype(k, "k")
-    kv = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, k.device)
-    if (hkv, d) != (kv.kv_heads, kv.head_dim):
-        raise GhostFlowError(_lib.INVALID_SHAPE, f"k must be [tokens, {kv.kv_heads}, {kv.head_dim}], got {list(k.shape)}")
-    ldk = _rows(k, "k", k.dtype, tokens, hkv, d)
-    ldv = _rows(v, "v", k.dtype, tokens, hkv, d)
-    heads, ldq, ldqo = hkv, 0, 0
+    tokens = k.shape[0] if k.dim() else 0
+    ldk = _rows(k, "k", k, tokens, hkv, d)
+    ldv = _rows(v, "v", k, tokens, hkv, d)
+    heads, ldq, ldqo, qp, qop = hkv, 0, 0, None, None
     if q is not None:
         heads = q.shape[1] if q.dim() == 3 else 0
-        ldq = _rows(q, "q", k.dtype, tokens, heads, d)
+        ldq = _rows(q, "q", k, tokens, heads, d)
         if q_out is None:
-            q_out = torch.empty((tokens, heads, d), dtype=q.dtype, device=q.device)
-        ldqo = _rows(q_out, "q_out", k.dtype, tokens, heads, d)
+            q_out = torch.empty((tokens, heads, d), dtype=q.dtype, device=dev)
+        ldqo = _rows(q_out, "q_out", k, tokens, heads, d)
+        qp, qop = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise GhostFlowError(_lib.INVALID_DATA, "q_out without q")
-    rows = half = 0
+    rows, half, cp, sp = 0, 0, None, None
     if (cos is None) != (sin is None):
         raise GhostFlowError(_lib.INVALID_DATA, "cos and sin are given together")
     if cos is not None:
@@ -604,12 +619,11 @@ def paged_append(k_pages, v_pages, page_table, q_offsets, kv_lens, k, v, *, q=No
         _need(sin, torch.float32, "sin")
         if cos.dim() != 2 or cos.shape != sin.shape:
             raise GhostFlowError(_lib.INVALID_SHAPE, "cos and sin must be [positions, rotary_dim / 2]")
+        _same_device(dev, cos, sin)
         rows, half = cos.shape
-    _same_device(k.device, v, q, q_out, cos, sin)
-    with torch.cuda.device(k.device):
-        _check(lib().gfh_paged_append(_byref(kv), dt, tokens, heads, _ptr(q), ldq, _ptr(q_out), ldqo, k.data_ptr(), ldk,
-                                      v.data_ptr(), ldv, _ptr(cos), _ptr(sin), rows, 2 * half, int(bool(interleaved)),
-                                      _stream(k.device)))
+        cp, sp = cos.data_ptr(), sin.data_ptr()
+    _call(dev, lib().gfh_paged_append, kv, dt, tokens, heads, qp, ldq, qop, ldqo, k.data_ptr(), ldk, v.data_ptr(), ldv,
+          cp, sp, rows, 2 * half, 1 if interleaved else 0)
     return q_out
 
 
@@ -621,30 +635,31 @@ def paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, *, scal
     out like q (which may be q); rows behind the last sequence are left as
     they are, and zero in an out made here.  max_kv_len: the batch's longest
     length where the caller knows it."""
+    dev = q.device
+    kv, _, d = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev)
+    dt = _dtype(q, "q")
     if q.dim() != 3:
         raise GhostFlowError(_lib.INVALID_SHAPE, "q must be [tokens, heads, head_dim]")
-    tokens, heads, d = q.shape
-    kv = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, q.device)
-    dt = _dtype(q, "q")
-    ldq = _rows(q, "q", q.dtype, tokens, heads, kv.head_dim)
+    tokens, heads = q.shape[:2]
+    ldq = _rows(q, "q", q, tokens, heads, d)
     if out is None:
-        out = torch.zeros((tokens, heads, d), dtype=q.dtype, device=q.device)
-    ldo = _rows(out, "out", q.dtype, tokens, heads, d)
+        out = torch.zeros((tokens, heads, d), dtype=q.dtype, device=dev)
+    ldo = _rows(out, "out", q, tokens, heads, d)
     if scale is None:
         scale = _inv_sqrt(d)
-    _same_device(q.device, out, workspace)
-    ws, ws_bytes = _workspace(workspace)
-    with torch.cuda.device(q.device):
-        _check(lib().gfh_paged_attention(_byref(kv), dt, tokens, heads, q.data_ptr(), ldq, out.data_ptr(), ldo,
-                                         float(scale), int(bool(causal)), int(window), int(max_kv_len or 0), ws,
-                                         ws_bytes, _stream(q.device)))
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        _same_device(dev, workspace)
+        ws, ws_bytes = _workspace(workspace)
+    _call(dev, lib().gfh_paged_attention, kv, dt, tokens, heads, q.data_ptr(), ldq, out.data_ptr(), ldo, float(scale),
+          1 if causal else 0, int(window), int(max_kv_len or 0), ws, ws_bytes)
     return out
 
 
 def paged_attention_workspace_size(q, k_pages, v_pages, page_table, q_offsets, kv_lens, max_kv_len=None) -> int:
     """Bytes of paged_attention's workspace for these arguments."""
-    kv = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, None, q.device)
-    return int(lib().gfh_paged_attention_workspace_size(_byref(kv), q.shape[0], q.shape[1], int(max_kv_len or 0)))
+    kv, _, _ = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, None, q.device)
+    return int(lib().gfh_paged_attention_workspace_size(kv, q.shape[0], q.shape[1], int(max_kv_len or 0)))
 
 
 # ---- SwiGLU feed-forward block (ghostflow-nn/src/llama.rs:259-287) -------------

@@ -84,6 +84,16 @@ def test_workspace_size():
     assert 0 < few < most and most % 4 == 0
 
 
+def test_packed_struct():
+    """The wrappers pack gfh_paged_kv themselves."""
+    L, _ = _lib()
+    from ghostflow_hip import ops
+    assert ops._PAGED_KV.size == C.sizeof(L.PagedKv)
+    values = list(range(1, 18))
+    kv = L.PagedKv.from_buffer_copy(ops._PAGED_KV.pack(*values))
+    assert [getattr(kv, f) for f, _ in L.PagedKv._fields_] == values
+
+
 def test_python_checks():
     torch = pytest.importorskip("torch")
     import ghostflow_hip as gh
