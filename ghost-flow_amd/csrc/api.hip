@@ -222,13 +222,15 @@ int check_rows(const char *who, const void *p, const char *name, int dtype, int6
     return GFH_SUCCESS;
 }
 
-PagedAttnDesc paged_attn_desc(const gfh_paged_kv &kv, int64_t tokens, int64_t heads, int64_t max_kv_len) {
+PagedAttnDesc paged_attn_desc(const gfh_paged_kv &kv, int64_t tokens, int64_t heads, int64_t max_kv_len,
+                              int64_t window) {
     PagedAttnDesc d;
     d.kv = kv;
     d.tokens = tokens;
     d.heads = heads;
     const int64_t capacity = kv.max_pages * kv.page_size;
     d.max_kv_len = max_kv_len <= 0 || max_kv_len > capacity ? capacity : max_kv_len;
+    d.window = window >= capacity ? 0 : window;
     return d;
 }
 
@@ -1020,11 +1022,11 @@ GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, 
 }
 
 GFH_API size_t gfh_paged_attention_workspace_size(const gfh_paged_kv *kv, int64_t tokens, int64_t heads,
-                                                  int64_t max_kv_len) {
-    if (!kv || check_paged("paged_attention", kv, kv->dtype, tokens, heads) != GFH_SUCCESS || tokens == 0 ||
+                                                  int64_t window, int64_t max_kv_len) {
+    if (!kv || window < 0 || check_paged("paged_attention", kv, kv->dtype, tokens, heads) != GFH_SUCCESS || tokens == 0 ||
         kv->num_seqs == 0)
         return 0;
-    return paged_attention_workspace_bytes(paged_attn_desc(*kv, tokens, heads, max_kv_len));
+    return paged_attention_workspace_bytes(paged_attn_desc(*kv, tokens, heads, max_kv_len, window));
 }
 
 GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads, const void *q,
@@ -1043,7 +1045,7 @@ GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t token
         if (workspace && !aligned16(workspace))
             return set_error(GFH_INVALID_DATA, "%s: the workspace must be 16-byte aligned", who);
         GFH_TRY(ensure_init());
-        PagedAttnDesc d = paged_attn_desc(*kv, tokens, heads, max_kv_len);
+        PagedAttnDesc d = paged_attn_desc(*kv, tokens, heads, max_kv_len, window);
         d.dtype = dtype;
         d.q = q;
         d.ldq = ldq;
@@ -1051,7 +1053,6 @@ GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t token
         d.ldo = ldo;
         d.scale = scale;
         d.causal = causal != 0;
-        d.window = window;
         hipStream_t s = as_stream(stream);
         Scratch ws;
         const size_t need = paged_attention_workspace_bytes(d);
@@ -1088,13 +1089,13 @@ GFH_API int gfh_dequantize_i4_grouped(const uint8_t *codes, const float *scales,
     });
 }
 
-GFH_API size_t gfh_linear_w4_workspace_size(int dtype, int64_t m, int64_t n, int64_t k) {
+GFH_API size_t gfh_linear_w4_workspace_size(int dtype, int64_t m, int64_t n, int64_t k, int64_t group) {
     if ((dtype != GFH_F16 && dtype != GFH_BF16 && dtype != GFH_F32) || m <= 0 || n <= 0 || k <= 0 || m > (1 << 19) ||
-        check_w4("linear_w4", n, k, 32) != GFH_SUCCESS || !count_ok({m, n, 4096}))
+        check_w4("linear_w4", n, k, group) != GFH_SUCCESS || !count_ok({m, n, 4096}))
         return 0;
     LinearW4Desc d;
     d.dtype = dtype;
-    d.m = m, d.n = n, d.k = k;
+    d.m = m, d.n = n, d.k = k, d.group = group;
     return linear_w4_workspace_bytes(d);
 }
 

@@ -59,6 +59,7 @@ struct AttnParams {
     int window;  // 0: none
     int ntiles, nsplit, chunk;
     int min_rows, max_rows;  // sequences this launch takes: rows = tokens * group
+    bool direct;             // see find_rows
     float *acc;   // [tokens * heads][nsplit][d] parts, where nsplit > 1
     float2 *ml;   // [tokens * heads][nsplit] their maximum (scaled) and sum
 };
@@ -71,31 +72,51 @@ struct Rows {
     int lo, hi;
 };
 
-__device__ __forceinline__ bool find_rows(const AttnParams &p, int number, int bm, int lane, Rows &t) {
+// Tile `number` of sequence s, whose tokens are [o0, o1) and length kv_len.
+__device__ __forceinline__ bool rows_at(const AttnParams &p, int number, int s, int bm, int o0, int o1, int kv_len,
+                                        Rows &t) {
     const View &c = p.c;
-    const int n = paged::wave_leading(c.num_seqs, lane, [&](int s) {
-        return (int)((unsigned)(paged::offset_at(c, s) * c.group) / (unsigned)bm) + s <= number;
-    });
-    if (n == 0) return false;
-    const int s = n - 1;
-    const int o0 = paged::offset_at(c, s), o1 = max(o0, paged::offset_at(c, s + 1));
+    o1 = max(o0, o1);
     t.base = (number - s) * bm;
     t.r0 = max(o0 * c.group, t.base);
     t.r1 = min(o1 * c.group, t.base + bm);
     const int rows = (o1 - o0) * c.group;
     if (t.r0 >= t.r1 || rows < p.min_rows || rows > p.max_rows) return false;
-    t.kv_len = paged::length_at(c, s);
+    t.kv_len = kv_len;
     t.q_last = t.kv_len - o1;
     const int first = t.r0 / c.group + t.q_last, last = (t.r1 - 1) / c.group + t.q_last;
     t.hi = max(0, p.causal ? min(t.kv_len, last + 1) : t.kv_len);
     t.lo = p.window ? min(t.hi, max(0, first - p.window + 1)) : 0;
     return true;
 }
-// (the sequence again, for its row of the table)
-__device__ __forceinline__ int seq_of(const AttnParams &p, int number, const Rows &t, int bm) {
-    return number - t.base / bm;
+__device__ __forceinline__ bool rows_of(const AttnParams &p, int number, int s, int bm, Rows &t) {
+    return rows_at(p, number, s, bm, paged::offset_at(p.c, s), paged::offset_at(p.c, s + 1), paged::length_at(p.c, s), t);
 }
-
+// The tile of a workgroup of the few-row launches.  Where no sequence of the
+// launch has more than kFewRows rows (p.direct), a sequence has at most
+// kFewTiles tiles and the grid counts those; else it counts tile numbers.
+constexpr int kFewRows = 32, kFewTiles = 3;
+__device__ __forceinline__ bool find_rows(const AttnParams &p, int number, int bm, int lane, Rows &t, int &s) {
+    const View &c = p.c;
+    if (p.direct) {
+        s = number / kFewTiles;
+        return rows_of(p, paged::offset_at(c, s) * c.group / bm + s + number % kFewTiles, s, bm, t);
+    }
+    if (c.num_seqs < 64) {  // everything about the batch in one round of loads
+        const int off = paged::offset_at(c, min(lane, c.num_seqs));
+        const int len = paged::length_at(c, min(lane, c.num_seqs - 1));
+        const bool ok = lane < c.num_seqs && (int)((unsigned)(off * c.group) / (unsigned)bm) + lane <= number;
+        s = __popcll(__ballot(ok)) - 1;
+        if (s < 0) return false;
+        return rows_at(p, number, s, bm, __builtin_amdgcn_readlane(off, s), __builtin_amdgcn_readlane(off, s + 1),
+                       __builtin_amdgcn_readlane(len, s), t);
+    }
+    const int n = paged::wave_leading(c.num_seqs, lane, [&](int i) {
+        return (int)((unsigned)(paged::offset_at(c, i) * c.group) / (unsigned)bm) + i <= number;
+    });
+    s = n - 1;
+    return n > 0 && rows_of(p, number, s, bm, t);
+}
 // The splits that have keys (at least one, which writes rows without any).
 __device__ __forceinline__ int active_splits(const AttnParams &p, const Rows &t) {
     return max(1, min(p.nsplit, (t.hi - t.lo + p.chunk - 1) / p.chunk));
@@ -261,7 +282,7 @@ __device__ __forceinline__ int stage_pages(const View &c, int seq, int b, int e,
 
 // One wave's requests for KEYS keys from k0 of K and V straight into LDS (16
 // bytes per lane; keys from e on and dims past d read zeros).
-template <int DP, int KEYS, int WAVES>
+template <int DP, int KEYS, int WAVES, int HINT>
 __device__ __forceinline__ void request(const View &c, int kvh, const int64_t *pages, int p0, int k0, int e, char *kl,
                                         char *vl, int wave, int lane) {
     constexpr int kRowChunks = DP / 8, kRowsPer = 64 / kRowChunks;
@@ -279,9 +300,55 @@ __device__ __forceinline__ void request(const View &c, int kvh, const int64_t *p
         const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
         const char *ks = ok && ck * 8 < c.d ? c.k + at + ck * 16 : zero;
         const char *vs = ok && cv * 8 < c.d ? c.v + at + cv * 16 : zero;
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)ks, (lds_ptr_t)(kl + ins * 1024), 16, 0, HINT);
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)vs, (lds_ptr_t)(vl + ins * 1024), 16, 0, HINT);
+    }
+}
+
+// The same for the 64 keys of a whole tile whose 16 keys per wave (32 at DP = 64)
+// lie in one page: one page offset per wave, and per lane offsets that do not
+// change.  False (and nothing asked for) where they do not.
+template <int DP>
+struct Lanes {
+    static constexpr int kKeys = 16;  // per wave
+    static constexpr int kRowChunks = DP / 8, kRowsPer = 64 / kRowChunks, kInstr = kKeys / kRowsPer;
+    uint32_t k[kInstr], v[kInstr];  // bytes from the wave's first row, ~0: zeros
+    bool whole;                     // pages hold whole groups of a wave's keys
+
+    __device__ __forceinline__ Lanes(const View &c, int wave, int lane) {
+        whole = c.page_size % kKeys == 0 && c.row_stride < (int64_t)1 << 24;
+#pragma unroll
+        for (int i = 0; i < kInstr; ++i) {
+            const int row = (wave * kInstr + i) * kRowsPer + lane / kRowChunks, ch = lane % kRowChunks;
+            const uint32_t at = (uint32_t)(i * kRowsPer + lane / kRowChunks) * (uint32_t)c.row_stride * 2u;
+            const int ck = ch ^ swz_k<DP>(row), cv = ch ^ swz_v<DP>(row);
+            k[i] = ck * 8 < c.d ? at + ck * 16 : ~0u;
+            v[i] = cv * 8 < c.d ? at + cv * 16 : ~0u;
+        }
+    }
+};
+template <int DP>
+__device__ __forceinline__ bool request_tile(const View &c, const Lanes<DP> &ln, int kvh, const int64_t *pages, int p0,
+                                             int k0, int e, char *kl, char *vl, int wave) {
+    using L = Lanes<DP>;
+    if (!ln.whole || k0 + 64 > e || (k0 & (L::kKeys - 1))) return false;
+    const int key = k0 + wave * L::kKeys, pg = paged::page_of(c, key);
+    const int64_t off = pages[pg - p0];
+    const int lo = __builtin_amdgcn_readfirstlane((int)off), hi = __builtin_amdgcn_readfirstlane((int)(off >> 32));
+    if (hi < 0) return false;
+    const int64_t at = ((int64_t)hi << 32 | (uint32_t)lo) +
+                       2 * ((int64_t)(key - pg * c.page_size) * c.row_stride + kvh * c.head_stride);
+    const char *kb = c.k + at, *vb = c.v + at;
+    const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
+#pragma unroll
+    for (int i = 0; i < L::kInstr; ++i) {
+        const int ins = wave * L::kInstr + i;
+        const char *ks = ln.k[i] != ~0u ? kb + ln.k[i] : zero;
+        const char *vs = ln.v[i] != ~0u ? vb + ln.v[i] : zero;
         __builtin_amdgcn_global_load_lds((glb_ptr_t)ks, (lds_ptr_t)(kl + ins * 1024), 16, 0, 0);
         __builtin_amdgcn_global_load_lds((glb_ptr_t)vs, (lds_ptr_t)(vl + ins * 1024), 16, 0, 0);
     }
+    return true;
 }
 
 template <typename T>
@@ -386,6 +453,39 @@ __device__ __forceinline__ void load_q(const AttnParams &p, const Rows &t, int r
     }
 }
 
+// The waves' states of a 16-row tile from LDS (rows of DP + 4 floats, their
+// maximum and sum) to the tile's rows: thread i takes 4 dims of a row.
+template <typename TA, int DP, int WAVES>
+__device__ __forceinline__ void join_waves(const AttnParams &p, const Rows &t, int kvh, int split, bool parts,
+                                           const float *accs, const float2 *mls, int tid) {
+    constexpr int kRow = DP + 4;
+    for (int i = tid; i < 16 * DP / 4; i += 64 * WAVES) {
+        const int row = i / (DP / 4), dim = 4 * (i % (DP / 4));
+        const int rr = t.base + row;
+        if (rr < t.r0 || rr >= t.r1 || dim >= p.c.d) continue;
+        float M = -INFINITY, L = 0.f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) M = max_nan(M, mls[w * 16 + row].x);
+        f32x4 A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            const float2 x = mls[w * 16 + row];
+            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
+            L = fmaf(x.y, f, L);
+            A += *reinterpret_cast<const f32x4 *>(accs + (w * 16 + row) * kRow + dim) * f;
+        }
+        if (parts) {
+            const int64_t at = part_row(p, rr, kvh) * p.nsplit + split;
+            *reinterpret_cast<f32x4 *>(p.acc + at * p.c.d + dim) = A;
+            if (dim == 0) p.ml[at] = make_float2(M, L);
+        } else {
+            const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+            const float y[4] = {A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv};
+            store_vec<4>(out_row<TA>(p, rr, kvh) + dim, y);
+        }
+    }
+}
+
 // ---- few rows: decode --------------------------------------------------------------
 //
 // A tile of 16 rows, WAVES waves that take 32-key tiles in turn, each with a
@@ -410,13 +510,15 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, h = lane >> 4;
-    const int id = xcd_chunked(blockIdx.x, gridDim.x);
-    const int split = id % p.nsplit, kvh = (id / p.nsplit) % p.c.hkv, number = id / p.nsplit / p.c.hkv;
+    // Workgroups share no keys here, so they go round the XCDs as they come: a
+    // long sequence's then lie on all of them.
+    const int id = blockIdx.x;
+    const int kvh = id % p.c.hkv, split = (id / p.c.hkv) % p.nsplit, number = id / p.c.hkv / p.nsplit;
     Rows t;
-    if (!find_rows(p, number, 16, lane, t)) return;
+    int seq;
+    if (!find_rows(p, number, 16, lane, t, seq)) return;
     const int nact = active_splits(p, t);
     if (split >= nact) return;
-    const int seq = seq_of(p, number, t, 16);
     const int b = t.lo + split * p.chunk, e = split == p.nsplit - 1 ? t.hi : min(t.hi, b + p.chunk);
 
     const int r = t.base + c;
@@ -444,13 +546,13 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
         const int n = (pe - pb + 31) / 32;  // tiles of this pass; this wave's: wave, wave + WAVES, ..
         char *const ring = lds + wave * 4 * kTile;
         if (wave < n)
-            request<DP, 32, 1>(p.c, kvh, pages, p0, pb + 32 * wave, pe, ring, ring + kTile, 0, lane);
+            request<DP, 32, 1, kNtHint>(p.c, kvh, pages, p0, pb + 32 * wave, pe, ring, ring + kTile, 0, lane);
         int st = 0;
         for (int i = wave; i < n; i += WAVES, st ^= 1) {
             // (past the last tile: the last key again, into the free stage)
             const int k0 = pb + 32 * i, kn = min(k0 + 32 * WAVES, pe - 1);
             __builtin_amdgcn_sched_barrier(0);
-            request<DP, 32, 1>(p.c, kvh, pages, p0, kn, pe, ring + (st ^ 1) * 2 * kTile,
+            request<DP, 32, 1, kNtHint>(p.c, kvh, pages, p0, kn, pe, ring + (st ^ 1) * 2 * kTile,
                                ring + (st ^ 1) * 2 * kTile + kTile, 0, lane);
             __builtin_amdgcn_sched_barrier(0);
             wait_vm<kOps>();
@@ -544,31 +646,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     for (int i = 0; i < NB; ++i) *reinterpret_cast<f32x4 *>(accs + (wave * 16 + c) * kRow + 16 * i + 4 * h) = o[i];
     if (h == 0) mls[wave * 16 + c] = make_float2(mt, l);
     __syncthreads();
-    for (int i = tid; i < 16 * DP / 4; i += 64 * WAVES) {
-        const int row = i / (DP / 4), dim = 4 * (i % (DP / 4));
-        const int rr = t.base + row;
-        if (rr < t.r0 || rr >= t.r1 || dim >= p.c.d) continue;
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) M = max_nan(M, mls[w * 16 + row].x);
-        f32x4 A = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            const float2 x = mls[w * 16 + row];
-            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
-            L = fmaf(x.y, f, L);
-            A += *reinterpret_cast<const f32x4 *>(accs + (w * 16 + row) * kRow + dim) * f;
-        }
-        if (nact > 1) {
-            const int64_t at = part_row(p, rr, kvh) * p.nsplit + split;
-            *reinterpret_cast<f32x4 *>(p.acc + at * p.c.d + dim) = A;
-            if (dim == 0) p.ml[at] = make_float2(M, L);
-        } else {
-            const float inv = M == -INFINITY ? 0.f : 1.0f / L;
-            const float y[4] = {A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv};
-            store_vec<4>(out_row<TA>(p, rr, kvh) + dim, y);
-        }
-    }
+    join_waves<TA, DP, WAVES>(p, t, kvh, split, nact > 1, accs, mls, tid);
 }
 
 // ---- many rows: chunks of prompts ---------------------------------------------------
@@ -595,11 +673,12 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
     const int number = p.ntiles - 1 - id % p.ntiles, rest = id / p.ntiles;
     const int split = rest % p.nsplit, kvh = rest / p.nsplit;
     Rows t;
-    if (!find_rows(p, number, 128, lane, t)) return;
+    int seq;
+    if (!find_rows(p, number, 128, lane, t, seq)) return;
     const int nact = active_splits(p, t);
     if (split >= nact) return;
-    const int seq = seq_of(p, number, t, 128);
-    const int b = t.lo + split * p.chunk, e = split == p.nsplit - 1 ? t.hi : min(t.hi, b + p.chunk);
+    // (from a multiple of a tile, so that whole tiles lie in few pages)
+    const int b0 = t.lo & ~63, b = b0 + split * p.chunk, e = split == nact - 1 ? t.hi : b + p.chunk;
 
     const int r = t.base + 32 * wave + c;
     int jmin, jmax;
@@ -610,6 +689,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
     // [all_lo, all_hi) that all of them see
     const int w0 = max(t.r0, t.base + 32 * wave), w1 = min(t.r1, t.base + 32 * wave + 32);
     const bool live = w0 < w1;
+    const Lanes<DP> ln(p.c, wave, lane);
     int any_lo, any_hi, all_lo, all_hi;
     row_keys(p, t, live ? w0 : t.r0, any_lo, all_hi);
     row_keys(p, t, live ? w1 - 1 : t.r0, all_lo, any_hi);
@@ -629,7 +709,12 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
         const int pe = stage_pages(p.c, seq, pb, e, 2, pages, tid, 256);
         __syncthreads();
         const int n = (pe - pb + 63) / 64;
-        request<DP, 64, 4>(p.c, kvh, pages, p0, pb, pe, lds, lds + kTile, wave, lane);
+        auto ask = [&](int k0, int st) __attribute__((always_inline)) {
+            char *const to = lds + st * 2 * kTile;
+            if (!request_tile<DP>(p.c, ln, kvh, pages, p0, k0, pe, to, to + kTile, wave))
+                request<DP, 64, 4, 0>(p.c, kvh, pages, p0, k0, pe, to, to + kTile, wave, lane);
+        };
+        ask(pb, 0);
         for (int i = 0; i < n; ++i) {
             const int k0 = pb + 64 * i, st = i & 1;
             // The tile is there, and every wave is done with the one before: the
@@ -638,9 +723,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
             // reads of V).
             wait_vm<0>();
             __syncthreads();
-            if (i + 1 < n)
-                request<DP, 64, 4>(p.c, kvh, pages, p0, k0 + 64, pe, lds + (st ^ 1) * 2 * kTile,
-                                   lds + (st ^ 1) * 2 * kTile + kTile, wave, lane);
+            if (i + 1 < n) ask(k0 + 64, st ^ 1);
             if (!live || k0 >= any_hi || k0 + 64 <= any_lo) continue;
             const char *kt = lds + st * 2 * kTile, *vt = kt + kTile;
             f32x16 s[2];
@@ -648,15 +731,26 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int x = 0; x < 16; ++x) s[kb][x] = 0.f;
+            // (fragments are read two steps ahead of their products)
+            v8 kf[3][2];
+            auto read_k = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < NU; ++u)
+                for (int kb = 0; kb < 2; ++kb)
+                    kf[u % 3][kb] = *reinterpret_cast<const v8 *>(kt + (kb * 32 + c) * DP * 2 +
+                                                                  (((2 * u + h) ^ swz_k<DP>(c)) << 4));
+            };
+            read_k(0);
+            read_k(1);
 #pragma unroll
-                for (int kb = 0; kb < 2; ++kb) {
-                    const v8 kf = *reinterpret_cast<const v8 *>(kt + (kb * 32 + c) * DP * 2 +
-                                                                (((2 * u + h) ^ swz_k<DP>(c)) << 4));
+            for (int u = 0; u < NU; ++u) {
+                if (u + 2 < NU) read_k(u + 2);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int q = NP - 1; q >= 0; --q) s[kb] = H::mfma32(kf, qf[u][q], s[kb]);
-                }
+                for (int q = NP - 1; q >= 0; --q)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) s[kb] = H::mfma32(kf[u % 3][kb], qf[u][q], s[kb]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (k0 < all_lo || k0 + 64 > min(all_hi, pe)) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -695,11 +789,22 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
                 for (int i2 = 0; i2 < NB; ++i2) o[i2] *= alpha;
             }
             m = m_new;
+            // steps: 16 keys from 16 (n / NB), 32 dims from 32 (n % NB)
             const int key = 4 * h + ((lane & 15) >> 2);
+            v8 vf[3];
+            auto read_v = [&](int n) __attribute__((always_inline)) {
+                const int ch = 4 * (n % NB) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+                const char *at = vt + (16 * (n / NB) + key) * DP * 2 + (lane & 1) * 8 + ((ch ^ swz_v<DP>(key)) << 4);
+                vf[n % 3] = join<v8>(read_tr<T>(at), read_tr<T>(at + 8 * DP * 2));
+            };
+            read_v(0);
+            read_v(1);
+            v8 pf[NP];
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {  // 16 keys from 32 kb + 16 x
+            for (int n = 0; n < 4 * NB; ++n) {
+                if (n + 2 < 4 * NB) read_v(n + 2);
+                if (n % NB == 0) {
+                    const int kb = n / NB / 2, x = n / NB % 2;
                     uint32_t pw[NP][4];
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
@@ -708,22 +813,17 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
 #pragma unroll
                         for (int q = 0; q < NP; ++q) pw[q][y] = two[q];
                     }
-                    v8 pf[NP];
 #pragma unroll
                     for (int q = 0; q < NP; ++q) {
                         const i32x4 v = {(int)pw[q][0], (int)pw[q][1], (int)pw[q][2], (int)pw[q][3]};
                         pf[q] = __builtin_bit_cast(v8, v);
                     }
-#pragma unroll
-                    for (int i2 = 0; i2 < NB; ++i2) {
-                        const int ch = 4 * i2 + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-                        const char *at = vt + (32 * kb + 16 * x + key) * DP * 2 + (lane & 1) * 8;
-                        const v8 vf = join<v8>(read_tr<T>(at + ((ch ^ swz_v<DP>(key)) << 4)),
-                                               read_tr<T>(at + 8 * DP * 2 + ((ch ^ swz_v<DP>(key + 8)) << 4)));
-#pragma unroll
-                        for (int q = NP - 1; q >= 0; --q) o[i2] = H::mfma32(vf, pf[q], o[i2]);
-                    }
                 }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int q = NP - 1; q >= 0; --q) o[n % NB] = H::mfma32(vf[n % 3], pf[q], o[n % NB]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         pb = pe;
     }
@@ -766,25 +866,31 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
 // ---- fp32 cache -------------------------------------------------------------------
 //
 // A tile of 16 rows, four waves that take 16-key tiles in turn, K and V straight
-// into registers and both products on f32 MFMA (16x16x4).  K: lane (c, h) loads
-// dims 16 u + 4 h .. + 3 of key c, and product e of step u takes dim 16 u + 4 h
-// + e of quarter h on both sides.  V: lane (c, h) loads dims 64 v + 4 c .. + 3 of
-// key 4 h + x; product (v, e, x) takes dim 64 v + 4 i + e as its row i.
+// into registers (the next tile's while this one is computed) and both products
+// on f32 MFMA (16x16x4).  K: lane (c, h) loads dims 16 u + 4 h .. + 3 of key c,
+// and product e of step u takes dim 16 u + 4 h + e of quarter h on both sides.
+// V: lane (c, h) loads dims 64 v + 4 c .. + 3 of key 4 h + x; product (v, e, x)
+// takes dim 64 v + 4 i + e as its row i.
 template <int DP>
-__global__ __launch_bounds__(256) void paged_f32_kernel(AttnParams p) {
-    constexpr int NU = DP / 16, NV = DP / 64;
-    __shared__ __attribute__((aligned(16))) float accs[4 * 16 * (DP + 4)];
-    __shared__ float2 mls[4 * 16];
+__global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
+    constexpr int NU = DP / 16, NV = DP / 64, kRow = DP + 4;
+    constexpr int kStates = 4 * 16 * kRow * 4;
+    __shared__ __attribute__((aligned(16))) char lds[kStates + 4 * 16 * 8 + kMaxPages * 8 + 64];
+    float *const accs = reinterpret_cast<float *>(lds);
+    float2 *const mls = reinterpret_cast<float2 *>(lds + kStates);
+    int64_t *const pages = reinterpret_cast<int64_t *>(lds + kStates + 4 * 16 * 8);
+    int *const flags = reinterpret_cast<int *>(lds + kStates + 4 * 16 * 8 + kMaxPages * 8);
+    const View &cc = p.c;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, h = lane >> 4;
-    const int id = xcd_chunked(blockIdx.x, gridDim.x);
-    const int split = id % p.nsplit, kvh = (id / p.nsplit) % p.c.hkv, number = id / p.nsplit / p.c.hkv;
+    const int id = blockIdx.x;
+    const int kvh = id % cc.hkv, split = (id / cc.hkv) % p.nsplit, number = id / cc.hkv / p.nsplit;
     Rows t;
-    if (!find_rows(p, number, 16, lane, t)) return;
+    int seq;
+    if (!find_rows(p, number, 16, lane, t, seq)) return;
     const int nact = active_splits(p, t);
     if (split >= nact) return;
-    const int seq = seq_of(p, number, t, 16);
     const int b = t.lo + split * p.chunk, e = split == p.nsplit - 1 ? t.hi : min(t.hi, b + p.chunk);
     const int r = t.base + c;
     int jmin, jmax;
@@ -796,8 +902,8 @@ __global__ __launch_bounds__(256) void paged_f32_kernel(AttnParams p) {
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             const int dim = 16 * u + 4 * h;
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(q + (dim < p.c.d ? dim : 0));
-            qv[u] = row_ok && dim < p.c.d ? (p.negate ? -x : x) : f32x4{0.f, 0.f, 0.f, 0.f};
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(q + (dim < cc.d ? dim : 0));
+            qv[u] = row_ok && dim < cc.d ? (p.negate ? -x : x) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
     }
     int x0, x1, y0, y1;
@@ -812,77 +918,98 @@ __global__ __launch_bounds__(256) void paged_f32_kernel(AttnParams p) {
         for (int x = 0; x < 4; ++x) o[v][x] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     bool odd = false;
-    const View &cc = p.c;
-    // float offset of key j's row, -1 outside the cache
-    auto row_at = [&](int j) __attribute__((always_inline)) -> int64_t {
-        const int pg = paged::page_of(cc, j), page = cc.table[seq * cc.table_stride + pg];
-        const bool ok = page >= 0 && page < cc.num_pages;
-        if (!ok) paged::raise(cc, paged::kBadPage);
-        return ok ? page * cc.page_stride + (int64_t)(j - pg * cc.page_size) * cc.row_stride + kvh * cc.head_stride : -1;
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    struct Tile {
+        f32x4 k[NU], v[4][NV];
     };
-    const float *K = reinterpret_cast<const float *>(cc.k), *V = reinterpret_cast<const float *>(cc.v);
-    for (int k0 = b + 16 * wave; k0 < e; k0 += 64) {
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        const int64_t ka = k0 + c < e ? row_at(k0 + c) : -1;
-        f32x4 kr[NU], vr[4][NV];
+    for (int pb = b; pb < e;) {
+        const int p0 = paged::page_of(cc, pb);
+        __syncthreads();
+        const int pe = stage_pages(cc, seq, pb, e, 4, pages, tid, 256);
+        __syncthreads();
+        // byte offset of key j's row and head, -1 past the keys or outside the cache
+        auto row_at = [&](int j) __attribute__((always_inline)) -> int64_t {
+            const int jc = min(j, pe - 1), pg = paged::page_of(cc, jc);
+            const int64_t off = pages[pg - p0];
+            return j < pe && off >= 0
+                       ? off + 4 * ((int64_t)(jc - pg * cc.page_size) * cc.row_stride + kvh * cc.head_stride)
+                       : -1;
+        };
+        const f32x4 *const zeros = reinterpret_cast<const f32x4 *>(g_zero_chunk);
+        auto load = [&](int k0, Tile &f) __attribute__((always_inline)) {
+            const int64_t ka = row_at(k0 + c);
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const int dim = 16 * u + 4 * h;
-            kr[u] = ka >= 0 && dim < cc.d ? *reinterpret_cast<const f32x4 *>(K + ka + dim) : zero;
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int j = k0 + 4 * h + x;
-            const int64_t va = j < e ? row_at(j) : -1;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const int dim = 64 * v + 4 * c;
-                vr[x][v] = va >= 0 && dim < cc.d ? *reinterpret_cast<const f32x4 *>(V + va + dim) : zero;
+            for (int u = 0; u < NU; ++u) {
+                const int dim = 16 * u + 4 * h;
+                f.k[u] = __builtin_nontemporal_load(
+                    ka >= 0 && dim < cc.d ? reinterpret_cast<const f32x4 *>(cc.k + ka + 4 * dim) : zeros);
             }
-        }
-        f32x4 s = zero;
-#pragma unroll
-        for (int u = 0; u < NU; ++u)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kr[u][x], qv[u][x], s, 0, 0, 0);
-        if (k0 < all_lo || k0 + 16 > min(all_hi, e)) {
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const int j = k0 + 4 * h + x;
-                s[x] = j >= jmin && j <= jmax && j < e ? s[x] : -INFINITY;
+                const int64_t va = row_at(k0 + 4 * h + x);
+#pragma unroll
+                for (int v = 0; v < NV; ++v) {
+                    const int dim = 64 * v + 4 * c;
+                    f.v[x][v] = __builtin_nontemporal_load(
+                        va >= 0 && dim < cc.d ? reinterpret_cast<const f32x4 *>(cc.v + va + 4 * dim) : zeros);
+                }
+            }
+        };
+        Tile now, next;
+        int k0 = pb + 16 * wave;
+        if (k0 < pe) load(k0, next);
+#pragma unroll 1
+        for (; k0 < pe; k0 += 64) {
+            now = next;
+            __builtin_amdgcn_sched_barrier(0);
+            load(k0 + 64, next);
+            __builtin_amdgcn_sched_barrier(0);
+            f32x4 s = zero;
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s = __builtin_amdgcn_mfma_f32_16x16x4f32(now.k[u][x], qv[u][x], s, 0, 0, 0);
+            if (k0 < all_lo || k0 + 16 > min(all_hi, pe)) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int j = k0 + 4 * h + x;
+                    s[x] = j >= jmin && j <= jmax && j < pe ? s[x] : -INFINITY;
+#pragma unroll
+                    for (int v = 0; v < NV; ++v)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) odd |= !(fabsf(now.v[x][v][y]) < INFINITY);
+                }
+            }
+            const float m_new = max_nan(m, quarter_max_nan(max_nan(max_nan(s[0], s[1]), max_nan(s[2], s[3]))));
+            const float mc = m_new == -INFINITY ? 0.f : m_new * p.sc2;
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * p.sc2 - mc);
+            float sum = 0.f;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], p.sc2, -mc));
+                sum += s[x];
+            }
+            l = fmaf(l, alpha, sum);
+            m = m_new;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) o[v][y] *= alpha;
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
                 for (int v = 0; v < NV; ++v)
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) odd |= !(fabsf(vr[x][v][y]) < INFINITY);
-            }
+                    for (int y = 0; y < 4; ++y)
+                        o[v][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(now.v[x][v][y], s[x], o[v][y], 0, 0, 0);
         }
-        const float m_new = max_nan(m, quarter_max_nan(max_nan(max_nan(s[0], s[1]), max_nan(s[2], s[3]))));
-        const float mc = m_new == -INFINITY ? 0.f : m_new * p.sc2;
-        const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * p.sc2 - mc);
-        float sum = 0.f;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            s[x] = __builtin_amdgcn_exp2f(fmaf(s[x], p.sc2, -mc));
-            sum += s[x];
-        }
-        l = fmaf(l, alpha, sum);
-        m = m_new;
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                o[v][y] *= alpha;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) o[v][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(vr[x][v][y], s[x], o[v][y], 0, 0, 0);
-            }
+        pb = pe;
     }
     l = quarter_sum(l);
-    odd = __syncthreads_or(odd);
-    if (odd) {
+    if (any_wave<4>(odd, flags, wave, lane)) {
         slow_rows<float, float>(p, t, seq, kvh, b, e, split, nact > 1, 0.f, wave, 4, lane);
         return;
     }
-    constexpr int kRow = DP + 4;
     // o[v][y], register x: dim 64 v + 4 (4 h + x) + y of row c
 #pragma unroll
     for (int v = 0; v < NV; ++v)
@@ -892,85 +1019,83 @@ __global__ __launch_bounds__(256) void paged_f32_kernel(AttnParams p) {
                 f32x4{o[v][0][x], o[v][1][x], o[v][2][x], o[v][3][x]};
     if (h == 0) mls[wave * 16 + c] = make_float2(m == -INFINITY ? m : m * p.sc2, l);
     __syncthreads();
-    for (int i = tid; i < 16 * DP / 4; i += 256) {
-        const int row = i / (DP / 4), dim = 4 * (i % (DP / 4));
-        const int rr = t.base + row;
-        if (rr < t.r0 || rr >= t.r1 || dim >= cc.d) continue;
-        float M = -INFINITY, L = 0.f;
-#pragma unroll
-        for (int w = 0; w < 4; ++w) M = max_nan(M, mls[w * 16 + row].x);
-        f32x4 A = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float2 x = mls[w * 16 + row];
-            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
-            L = fmaf(x.y, f, L);
-            A += *reinterpret_cast<const f32x4 *>(accs + (w * 16 + row) * kRow + dim) * f;
-        }
-        if (nact > 1) {
-            const int64_t at = part_row(p, rr, kvh) * p.nsplit + split;
-            *reinterpret_cast<f32x4 *>(p.acc + at * cc.d + dim) = A;
-            if (dim == 0) p.ml[at] = make_float2(M, L);
-        } else {
-            const float inv = M == -INFINITY ? 0.f : 1.0f / L;
-            *reinterpret_cast<f32x4 *>(out_row<float>(p, rr, kvh) + dim) = A * inv;
-        }
-    }
+    join_waves<float, DP, 4>(p, t, kvh, split, nact > 1, accs, mls, tid);
 }
 
 // ---- the parts of split rows, in their order ------------------------------------------
 
-// Eight lanes per 32 dims: a wave takes 64 / (d / 4) rows, 4 dims per lane.
+// A wave per (token, head), or per row that a sequence of a direct launch can
+// have; two dims per lane.
 template <typename TA>
 __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int bm) {
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    // one (token, key/value head) per wave: its group of rows, whose tiles are
-    // found like the attention kernels' own
-    const int tok = wave / p.c.hkv, kvh = wave % p.c.hkv;
-    if (tok >= p.c.tokens) return;
     const View &c = p.c;
-    const int n = paged::wave_leading(c.num_seqs + 1, lane, [&](int s) { return paged::offset_at(c, s) <= tok; });
-    if (n == 0 || n > c.num_seqs) return;
-    const int lanes = c.d / 4;  // per row; d <= 128
-    const int per = 64 / lanes;
-    for (int g0 = 0; g0 < c.group; g0 += per) {
-        // (the group's rows may lie in different tiles)
-        for (int i = 0; i < per; ++i) {
-            const int g = g0 + i;
-            if (g >= c.group) break;
-            const int r = tok * c.group + g;
-            Rows t;
-            if (!find_rows(p, r / bm + n - 1, bm, lane, t)) continue;
-            const int nact = active_splits(p, t);
-            if (nact <= 1 || lane / lanes != i || lane >= lanes * per) continue;
-            const int dim = 4 * (lane % lanes);
-            const int64_t at = part_row(p, r, kvh) * p.nsplit;
-            float M = -INFINITY, L = 0.f;
-            f32x4 A = {0.f, 0.f, 0.f, 0.f};
-            for (int s = 0; s < nact; ++s) M = max_nan(M, p.ml[at + s].x);
-            for (int s = 0; s < nact; ++s) {
-                const float2 x = p.ml[at + s];
-                const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
-                L = fmaf(x.y, f, L);
-                A += *reinterpret_cast<const f32x4 *>(p.acc + (at + s) * c.d + dim) * f;
-            }
-            const float inv = M == -INFINITY ? 0.f : 1.0f / L;
-            const float y[4] = {A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv};
-            store_vec<4>(out_row<TA>(p, r, kvh) + dim, y);
+    const int lane = threadIdx.x & 63;
+    const int id = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    int s, kvh, r;
+    if (p.direct) {  // sequence, row of it, key/value head
+        kvh = id % c.hkv;
+        s = id / c.hkv / kFewRows;
+        if (s >= c.num_seqs) return;
+        r = paged::offset_at(c, s) * c.group + id / c.hkv % kFewRows;
+        if (r >= paged::offset_at(c, s + 1) * c.group) return;
+    } else {
+        const int tok = id / c.heads, head = id - tok * c.heads;
+        if (tok >= c.tokens) return;
+        const int n = paged::wave_leading(c.num_seqs + 1, lane, [&](int i) { return paged::offset_at(c, i) <= tok; });
+        if (n == 0 || n > c.num_seqs) return;
+        s = n - 1;
+        kvh = head / c.group;
+        r = tok * c.group + head - kvh * c.group;
+    }
+    Rows t;
+    if (!rows_of(p, r / bm + s, s, bm, t)) return;
+    const int nact = active_splits(p, t);
+    if (nact <= 1) return;
+    const int64_t at = part_row(p, r, kvh) * p.nsplit;
+    // the largest maximum: 64 splits at a time
+    float M = -INFINITY;
+    for (int i = lane; i < nact; i += 64) M = max_nan(M, p.ml[at + i].x);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) M = max_nan(M, __shfl_xor(M, o));
+    const int dim = min(2 * lane, c.d - 2);
+    float L = 0.f, a0 = 0.f, a1 = 0.f;
+    for (int s0 = 0; s0 < nact; s0 += 8) {
+        float2 ml[8], v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t part = at + min(s0 + i, nact - 1);
+            ml[i] = p.ml[part];
+            v[i] = *reinterpret_cast<const float2 *>(p.acc + part * c.d + dim);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (s0 + i >= nact || ml[i].x == -INFINITY) continue;  // no key of that part is seen
+            const float f = exp2f(ml[i].x - M);
+            L = fmaf(ml[i].y, f, L);
+            a0 = fmaf(v[i].x, f, a0);
+            a1 = fmaf(v[i].y, f, a1);
         }
     }
+    const float inv = M == -INFINITY ? 0.f : 1.0f / L;
+    const float y[2] = {a0 * inv, a1 * inv};
+    if (2 * lane < c.d) store_vec<2>(out_row<TA>(p, r, kvh) + dim, y);
 }
 
 // What a call launches: a few-row launch, a chunk launch or both.
 struct Plan {
     bool few, chunk;
+    bool wide;    // the few-row launch has wide workgroups
     int few_max;  // rows of the longest sequence the few-row launch takes
     int few_split, few_chunk, chunk_split, chunk_chunk;
     int64_t part_floats;
 };
 
-constexpr int kDecodeWaves = 2;
+// Waves of a few-row workgroup: two, so that two or more workgroups share a CU;
+// as many as the LDS takes where there are too few tiles to fill the CUs and a
+// length that such a workgroup walks in a few steps: no split and no second launch
+// (12 heads of 64 over 517 keys, f16: 8.6 us and 3.9 to join -> 9.2).
+constexpr int kDecodeWaves = 2, kWideWaves64 = 8, kWideWaves128 = 4;
+constexpr int kWideKeys = 96;  // per wave
 constexpr int kAll = INT32_MAX;
 
 Plan make_plan(const PagedAttnDesc &d) {
@@ -978,21 +1103,33 @@ Plan make_plan(const PagedAttnDesc &d) {
     const int64_t group = d.heads / d.kv.kv_heads;
     const int64_t rows = d.tokens * group;
     const bool f32 = d.kv.dtype == GFH_F32;
-    pl.few_max = 32;
+    pl.few_max = kFewRows;
     pl.few = f32 || d.kv.num_seqs > 1 || rows <= pl.few_max;
     pl.chunk = !f32 && rows > pl.few_max && d.tokens > d.kv.num_seqs;
     if (!pl.chunk) pl.few_max = kAll;
     const int64_t cus = device_cu_count();
     auto cut = [&](int64_t tiles, int64_t target, int64_t least, int64_t unit, int &nsplit, int &chunk) {
         const int64_t items = std::max<int64_t>(1, tiles * d.kv.kv_heads);
-        const int64_t kv = std::max<int64_t>(1, d.max_kv_len);
+        // keys that a tile sees at most
+        const int64_t kv = std::max<int64_t>(1, d.window > 0 ? std::min(d.max_kv_len, d.window + 127) : d.max_kv_len);
         int64_t ch = std::max(least, (items * kv + target - 1) / target);
         ch = (ch + unit - 1) / unit * unit;
-        nsplit = (int)std::min<int64_t>((kv + ch - 1) / ch, 256);
+        nsplit = (int)std::min<int64_t>((kv + ch / 2) / ch, 256);
+        nsplit = std::max(nsplit, 1);
         ch = std::max(ch, (kv + nsplit - 1) / nsplit);
         chunk = (int)std::min<int64_t>((ch + unit - 1) / unit * unit, (int64_t)1 << 30);
     };
-    cut(std::min(d.kv.num_seqs, d.tokens) + rows / 16, 4 * cus, 256, 64, pl.few_split, pl.few_chunk);
+    const int64_t few_tiles = std::min(d.kv.num_seqs, d.tokens) + (pl.chunk ? 0 : rows / 16);
+    // Workgroups of the few-row launch.  fp32: at least 384 keys each, four waves
+    // (4 sequences of up to 2047 keys, 32 heads of 128, us of the kernel by keys:
+    // 256 64.7, 384 53.2, 512 58.1).  16 bits: at least 128 keys each, six times as
+    // many as fit at once, for even ends (64 sequences of up to 4096 keys, 8 heads of
+    // 128: twice as many 148, four times 132, six times 125, eight times 131).
+    cut(few_tiles, (f32 ? 4 : 12) * cus, f32 ? 384 : 128, 64, pl.few_split, pl.few_chunk);
+    const int64_t wide_keys = kWideKeys * (d.kv.head_dim <= 64 ? kWideWaves64 : kWideWaves128);
+    pl.wide = !f32 && pl.few_split > 1 && few_tiles * d.kv.kv_heads <= cus &&
+              (d.window > 0 ? std::min(d.max_kv_len, d.window + 15) : d.max_kv_len) <= wide_keys;
+    if (pl.wide) pl.few_split = 1;
     cut(rows / 128 + 1, 2 * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
     int64_t most = 1;
     if (pl.few) most = std::max<int64_t>(most, pl.few_split);
@@ -1040,9 +1177,9 @@ int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t 
     p.causal = d.causal;
     p.window = d.window >= p.c.capacity ? 0 : (int)d.window;
     const int64_t rows = d.tokens * p.c.group;
-    const dim3 join((unsigned)((d.tokens * p.c.hkv + 3) / 4));
     auto run = [&](int bm, int nsplit, int chunk, int min_rows, int max_rows, auto &&kernel) -> int {
-        p.ntiles = (int)((rows - 1) / bm + d.kv.num_seqs);
+        p.direct = max_rows == kFewRows;
+        p.ntiles = p.direct ? kFewTiles * (int)d.kv.num_seqs : (int)((rows - 1) / bm + d.kv.num_seqs);
         p.nsplit = nsplit, p.chunk = chunk, p.min_rows = min_rows, p.max_rows = max_rows;
         p.acc = static_cast<float *>(workspace);
         p.ml = reinterpret_cast<float2 *>(p.acc + d.tokens * d.heads * nsplit * d.kv.head_dim);
@@ -1051,6 +1188,7 @@ int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t 
         kernel(dim3((unsigned)blocks));
         GFH_TRY(check_launch("paged_attention"));
         if (nsplit > 1) {
+            const dim3 join((unsigned)(((p.direct ? d.kv.num_seqs * kFewRows * p.c.hkv : d.tokens * d.heads) + 3) / 4));
             if (d.dtype == GFH_F32)
                 hipLaunchKernelGGL(paged_join_kernel<float>, join, dim3(256), 0, s, p, bm);
             else if (d.dtype == GFH_BF16)
@@ -1067,11 +1205,18 @@ int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t 
             using TA = decltype(ta);
             using T = decltype(t);
             constexpr int NP = decltype(np)::value;
-            constexpr int W = kDecodeWaves;
-            if (hd <= 64)
-                hipLaunchKernelGGL((paged_decode_kernel<TA, T, 64, NP, W>), grid, dim3(64 * W), 0, s, p);
-            else
-                hipLaunchKernelGGL((paged_decode_kernel<TA, T, 128, NP, W>), grid, dim3(64 * W), 0, s, p);
+            auto width = [&](auto dp, auto w) {
+                constexpr int DP = decltype(dp)::value, W = decltype(w)::value;
+                hipLaunchKernelGGL((paged_decode_kernel<TA, T, DP, NP, W>), grid, dim3(64 * W), 0, s, p);
+            };
+            using Two = std::integral_constant<int, kDecodeWaves>;
+            if (hd <= 64) {
+                using D = std::integral_constant<int, 64>;
+                pl.wide ? width(D{}, std::integral_constant<int, kWideWaves64>{}) : width(D{}, Two{});
+            } else {
+                using D = std::integral_constant<int, 128>;
+                pl.wide ? width(D{}, std::integral_constant<int, kWideWaves128>{}) : width(D{}, Two{});
+            }
         };
         using One = std::integral_constant<int, 1>;
         using Three = std::integral_constant<int, 3>;

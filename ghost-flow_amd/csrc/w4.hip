@@ -27,6 +27,7 @@
 namespace gfh {
 namespace {
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -130,7 +131,6 @@ struct W4LinearParams {
     float *part;  // [splits][m][n] where K is split
     int64_t ldx, ldy;
     int m, n, k, group, groups;
-    bool xvec;  // rows of x allow 16-byte loads
     int kper;   // columns per split
     int splits;
 };
@@ -139,8 +139,9 @@ struct W4LinearParams {
 struct Zero {
     f16x2 a, b;  // 1024 + z, -(64 + z)
     __device__ __forceinline__ explicit Zero(uint32_t z) {
-        a = __builtin_bit_cast(f16x2, 0x64006400u | z | z << 16);
-        b = __builtin_bit_cast(f16x2, 0xd400d400u | z << 4 | z << 20);
+        z |= z << 16;
+        a = __builtin_bit_cast(f16x2, 0x64006400u | z);
+        b = __builtin_bit_cast(f16x2, 0xd400d400u | z << 4);
     }
 };
 __device__ __forceinline__ void unpack8(uint32_t w, const Zero &z, f16x2 (&o)[4]) {
@@ -155,13 +156,30 @@ __device__ __forceinline__ void unpack8(uint32_t w, const Zero &z, f16x2 (&o)[4]
     }
 }
 
-template <int N, typename T>
-__device__ __forceinline__ void load_x(const T *p, bool vec, float (&v)[N]) {
-    if (vec) {
-        load_vec<N>(p, v);
-    } else {
+// Where row c of x's quarter h lies among a step's 64 operands in LDS: the 16
+// columns of a block row that one instruction writes then fall on all banks (they
+// would meet on a quarter of them), and a fragment read stays a permutation.
+__device__ __forceinline__ int x_slot(int step, int h, int c) { return h * 16 + (c ^ (4 * ((step & 1) * 2 + (h >> 1)))); }
+
+// 16 bytes from any address that an element may have.
+template <typename T>
+__device__ __forceinline__ i32x4 load16(const T *p) {
+    struct __attribute__((packed, aligned(sizeof(T)))) Any {
+        i32x4 v;
+    };
+    return reinterpret_cast<const Any *>(p)->v;
+}
+
+// 16 columns of x as fp32.
+template <typename T>
+__device__ __forceinline__ void load_x(const T *p, float (&v)[16]) {
+    constexpr int kPer = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(kPer)));
 #pragma unroll
-        for (int e = 0; e < N; ++e) v[e] = (float)p[e];
+    for (int i = 0; i < 16 / kPer; ++i) {
+        const vec t = __builtin_bit_cast(vec, load16(p + i * kPer));
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[i * kPer + e] = (float)t[e];
     }
 }
 
@@ -181,7 +199,7 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
     for (int i = 0; i < M; ++i)
 #pragma unroll
         for (int r = 0; r < R; ++r) acc[i][r] = 0.f;
-    uint2 c[R];
+    u32x2 c[R];
     float s[R];
     uint32_t z[R];
     auto fetch = [&](int j) __attribute__((always_inline)) {
@@ -189,7 +207,7 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int64_t row = min(n0 + r, p.n - 1);
-            c[r] = *reinterpret_cast<const uint2 *>(p.codes + (row * p.k + jc) / 2);
+            c[r] = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(p.codes + (row * p.k + jc) / 2));
             s[r] = p.scales[row * p.groups + g];
             z[r] = p.zps ? p.zps[row * p.groups + g] : 8;
         }
@@ -201,13 +219,13 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
 #pragma unroll
         for (int i = 0; i < M; ++i) {
             if (j < p.k) {
-                load_x<16>(x + min(i, p.m - 1) * p.ldx + j, p.xvec, xv[i]);
+                load_x(x + min(i, p.m - 1) * p.ldx + j, xv[i]);
             } else {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) xv[i][e] = 0.f;
             }
         }
-        uint2 cc[R];
+        u32x2 cc[R];
         float ss[R];
         uint32_t zz[R];
 #pragma unroll
@@ -219,8 +237,8 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
             f16x2 o[8];
             f16x2 (&o0)[4] = reinterpret_cast<f16x2 (&)[4]>(o[0]);
             f16x2 (&o1)[4] = reinterpret_cast<f16x2 (&)[4]>(o[4]);
-            unpack8(cc[r].x, zero, o0);
-            unpack8(cc[r].y, zero, o1);
+            unpack8(cc[r][0], zero, o0);
+            unpack8(cc[r][1], zero, o1);
 #pragma unroll
             for (int i = 0; i < M; ++i) {
                 float d = 0.f;
@@ -257,214 +275,310 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
 // 16) unpacks the codes of row c of W straight into its B operand and holds the
 // result's column c, so a group's scale is one value per lane.
 //
-// x goes through LDS as f16 in the codes' order (pairs 4 apart): f16 itself;
-// bf16 and fp32 after a scaling, per row and 256-column slice, by the power of
-// two that brings the largest magnitude to [2^14, 2^15), as one piece (bf16: 8
-// bits, exact above 2^-29 of the slice's largest) or three (fp32: 33 bits).  The
-// slice's sums are scaled back as they join.
+// Slices of 256 columns.  W comes by requests straight to LDS, a ring of kRing
+// slices per wave (eight rows of 128 bytes per instruction).  x goes through
+// registers into LDS, two buffers for the workgroup and one barrier per slice,
+// as f16 in the codes' order (pairs 4 apart): f16 itself; bf16 and fp32 after a
+// scaling, per row and slice, by the power of two that brings the largest
+// magnitude to [2^14, 2^15), as one piece (bf16: 8 bits, exact above 2^-29 of the
+// slice's largest) or three (fp32: 33 bits).  The slice's sums are scaled back as
+// they join.  Scales and zero points are looked up per 32 columns, two of a row's
+// eight per lane, and go round through LDS.
 //
-// Loads of 16 bytes give lane (c, h) columns 32 h .. of a 128-column block.
-// Where groups are whole blocks the products take them so (step t: columns 32 h
-// + 8 t of every h); else (T32) a 4 x 4 transposition over the four lanes of a row
-// makes step t the columns 32 t + 8 h, all of one group.
+// The loop is kept small: a launch that streams few slices spends its time on
+// instructions that no cache holds yet as much as on the weights (with the
+// slices unrolled, 16 KB of code: 18.0 us for 16 x 14336 x 4096, 8 of them
+// before the first slice).
 constexpr int kSlice = 256;
+typedef __attribute__((address_space(3))) void *lds_ptr_t;
+typedef __attribute__((address_space(1))) void *glb_ptr_t;
 
-template <typename T, int MB, int RT, bool T32>
-__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void w4_tiles_kernel(W4LinearParams p) {
-    constexpr int NP = std::is_same_v<T, float> ? 3 : 1;
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+    static_assert(N < 64, "vmcnt has six bits");
+    __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
+}
+
+// PER: 32-column steps per sum (4 where groups are whole 128-column blocks).
+template <typename T, int MB, bool ZP, int PER>
+__global__ __launch_bounds__(256, MB == 1 && sizeof(T) == 2 ? 2 : 1) void w4_tiles_kernel(W4LinearParams p) {
+    constexpr int NP = std::is_same_v<T, float> ? 3 : 1, RT = 2;
     constexpr bool SCALED = !std::is_same_v<T, _Float16>;
-    constexpr int NG = T32 ? 8 : 2;  // scales per slice
-    constexpr int kBuf = NP * MB * kSlice * 16 * 2;
-    __shared__ __attribute__((aligned(16))) char lds[2 * kBuf];
-    __shared__ __attribute__((aligned(16))) float back[2][MB * 16];
+    constexpr int kX = NP * MB * kSlice * 16 * 2;  // one buffer of x
+    constexpr int kW = RT * 16 * kSlice / 2;       // one slice of a wave's W
+    constexpr int kXLoads = sizeof(T);             // per thread and block
+    constexpr int kRing = 3;  // slices of W on their way or in use
+    // loads of one slice, in their order: x, scales, W
+    constexpr int kOps = MB * kXLoads + RT * (ZP ? 4 : 2) + 2 * RT;
+    constexpr int kTable = ZP ? 1536 : 512;  // of a tile: scales [16][8], then Zero [16][8]
+    __shared__ __attribute__((aligned(1024))) char lds[4 * kRing * kW + 2 * kX + 4 * RT * kTable + 2 * MB * 64];
+    char *const xbuf = lds + 4 * kRing * kW;
+    float *const backs = reinterpret_cast<float *>(xbuf + 2 * kX + 4 * RT * kTable);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, h = lane >> 4;
+    char *const ring = lds + wave * kRing * kW;
+    char *const sc = xbuf + 2 * kX + wave * RT * kTable;
     const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
     const int n0 = tile * 64 * RT + wave * 16 * RT, m0 = blockIdx.y * 16 * MB;
     const int k0 = split * p.kper, k1 = min(k0 + p.kper, p.k);
+    const int ns = (k1 - k0 + kSlice - 1) / kSlice;
     const T *x = static_cast<const T *>(p.x);
 
-    struct Set {
-        i32x4 w[RT][2];
-        float s[RT][NG];
-        uint32_t z[RT][NG];
+    // W: instruction i of a tile fills rows 8 i .. of it; lane l the chunk (l % 8)
+    // ^ row of row l / 8.  Rows past n are row n - 1, columns past k column 0 (they
+    // meet zeros of x).
+    const uint8_t *wsrc[RT][2];
+    int wcol[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = 8 * i + (lane >> 3);
+        wcol[i] = 32 * ((lane & 7) ^ (row & 7));
+#pragma unroll
+        for (int t = 0; t < RT; ++t) wsrc[t][i] = p.codes + (int64_t)min(n0 + 16 * t + row, p.n - 1) * (p.k / 2);
+    }
+    auto request_w = [&](int s) __attribute__((always_inline)) {
+        const int j = k0 + min(s, ns - 1) * kSlice;  // (past the end: the last slice again, never read)
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int col = j + wcol[i];
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)(wsrc[t][i] + (col < p.k ? col : 0) / 2),
+                                                 (lds_ptr_t)(ring + (s % kRing) * kW + (t * 2 + i) * 1024), 16, 0, kNtHint);
+            }
     };
-    auto fetch = [&](int j, Set &f) __attribute__((always_inline)) {
-        j = min(j, k1 - 1) & ~(kSlice - 1);
+    // scales of row c, steps 2 h and 2 h + 1 of the next slice to be asked for
+    int gi[2], rem[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int col = k0 + 64 * h + 32 * i;
+        gi[i] = col / p.group;
+        rem[i] = col - gi[i] * p.group;
+    }
+    const int gq = kSlice / p.group, gr = kSlice % p.group;
+    struct Scales {
+        float s[RT][2];
+        uint32_t z[RT][2];
+    } sa, sb;
+    auto fetch_s = [&](Scales &f) __attribute__((always_inline)) {
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
-            const int64_t row = min(n0 + 16 * t + c, p.n - 1);
+            const int64_t at = (int64_t)min(n0 + 16 * t + c, p.n - 1) * p.groups;
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int col = j + 128 * b + 32 * h;
-                f.w[t][b] = *reinterpret_cast<const i32x4 *>(p.codes + (row * p.k + (col < p.k ? col : 0)) / 2);
-            }
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const int64_t at = row * p.groups + min((j + (kSlice / NG) * g) / p.group, p.groups - 1);
-                f.s[t][g] = p.scales[at];
-                f.z[t][g] = p.zps ? p.zps[at] : 8;
+            for (int i = 0; i < 2; ++i) {
+                const int g = min(gi[i], p.groups - 1);
+                f.s[t][i] = p.scales[at + g];
+                if (ZP) f.z[t][i] = p.zps[at + g];
             }
         }
-    };
-    // x: thread (row tid / 16 of a block, 16 columns)
-    float xr[MB][16];
-    auto fetch_x = [&](int j) __attribute__((always_inline)) {
-        const int col = j + 16 * (tid & 15);
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
-            const int row = m0 + 16 * b + (tid >> 4);
-            if (row < p.m && col < k1) {
-                load_x<16>(x + row * p.ldx + col, p.xvec, xr[b]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) xr[b][e] = 0.f;
-            }
+        for (int i = 0; i < 2; ++i) {
+            gi[i] += gq;
+            rem[i] += gr;
+            if (rem[i] >= p.group) rem[i] -= p.group, ++gi[i];
         }
     };
-    auto stage_x = [&](int buf) __attribute__((always_inline)) {
+    // x: thread (row tid / 16 of a block, 16 columns), as loaded
+    i32x4 xa[MB][kXLoads], xb[MB][kXLoads];
+    auto fetch_x = [&](int s, i32x4 (&xr)[MB][kXLoads]) __attribute__((always_inline)) {
+        const int col = k0 + s * kSlice + 16 * (tid & 15);
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
+            const T *at = x + min(m0 + 16 * b + (tid >> 4), p.m - 1) * p.ldx + (col < k1 ? col : 0);
+#pragma unroll
+            for (int i = 0; i < kXLoads; ++i) xr[b][i] = load16(at + i * (16 / sizeof(T)));
+        }
+    };
+    auto stage_x = [&](int s, i32x4 (&xr)[MB][kXLoads]) __attribute__((always_inline)) {
+        char *const to = xbuf + (s & 1) * kX;
+        if (k0 + (s + 1) * kSlice > k1) {  // (rows past m are copies of the last, never stored)
+            const bool ok = k0 + s * kSlice + 16 * (tid & 15) < k1;
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int i = 0; i < kXLoads; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) xr[b][i][e] = ok ? xr[b][i][e] : 0;
+        }
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+            float v[16], up = 1.f;
             if constexpr (SCALED) {
-                // the largest finite magnitude's power of two
+                // the exponent of the largest finite magnitude
                 float big = 0.f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const float a = fabsf(xr[b][e]);
-                    big = fmaxf(big, a < INFINITY ? a : 0.f);
+                    if constexpr (sizeof(T) == 4) {
+                        const int w = xr[b][e / 4][e % 4];
+                        v[e] = __int_as_float(w);
+                    } else {
+                        const uint32_t w = (uint32_t)xr[b][e / 8][e % 8 / 2];
+                        v[e] = __uint_as_float(e % 2 ? w & 0xffff0000u : w << 16);
+                    }
+                    big = fmaxf(big, fabsf(v[e]));
+                }
+                if (__any(!(big < INFINITY)) || sizeof(T) == 4) {
+                    big = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) big = fmaxf(big, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.f);
                 }
                 big = fmaxf(big, dpp_mov<0xB1>(big));
                 big = fmaxf(big, dpp_mov<0x4E>(big));
                 big = fmaxf(big, dpp_mov<0x124>(big));
                 big = fmaxf(big, dpp_mov<0x128>(big));
-                const int e2 = big > 0.f ? min(14 - ilogbf(big), 126) : 0;
-                const float up = ldexpf(1.f, e2);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) xr[b][e] *= up;
-                if ((tid & 15) == 0) back[buf][16 * b + (tid >> 4)] = ldexpf(1.f, -e2);
+                const int e2 = big > 0.f ? min(15 - __builtin_amdgcn_frexp_expf(big), 126) : 0;
+                up = __builtin_ldexpf(1.f, e2);
+                if ((tid & 15) == 0) backs[(s & 1) * MB * 16 + 16 * b + (tid >> 4)] = __builtin_ldexpf(1.f, -e2);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int unit = 2 * (tid & 15) + u;  // of 8 columns
-                const int step = T32 ? unit / 4 : 4 * (unit / 16) + unit % 4, hh = T32 ? unit % 4 : (unit % 16) / 4;
-                char *at = lds + buf * kBuf + ((b * 8 + step) * 64 + hh * 16 + (tid >> 4)) * 16;
-                float v[8];
+                char *at = to + ((b * 8 + unit / 4) * 64 + x_slot(unit / 4, unit % 4, tid >> 4)) * 16;
+                if constexpr (!SCALED) {
+                    i32x4 o;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = xr[b][8 * u + (e >> 1) + 4 * (e & 1)];
-#pragma unroll
-                for (int q = 0; q < NP; ++q) {
-                    f16x8 o;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        o[e] = (_Float16)v[e];
-                        // (nothing is left of what is not finite)
-                        const float r = v[e] - (float)o[e];
-                        v[e] = fabsf(v[e]) < INFINITY ? r : 0.f;
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t lo = (uint32_t)xr[b][u][e], hi = (uint32_t)xr[b][u][e + 2];
+                        o[2 * e] = (int)__builtin_amdgcn_perm(hi, lo, 0x05040100u);
+                        o[2 * e + 1] = (int)__builtin_amdgcn_perm(hi, lo, 0x07060302u);
                     }
-                    *reinterpret_cast<f16x8 *>(at + q * MB * kSlice * 32) = o;
+                    *reinterpret_cast<i32x4 *>(at) = o;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) {
+                        i32x4 o;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float &v0 = v[8 * u + e], &v1 = v[8 * u + e + 4];
+                            if (q == 0 && NP > 1) v0 *= up, v1 *= up;
+                            const f16x2 two = NP > 1 ? f16x2{(_Float16)v0, (_Float16)v1}
+                                                     : f16x2{(_Float16)fmaf(v0, up, 0.f), (_Float16)fmaf(v1, up, 0.f)};
+                            o[e] = __builtin_bit_cast(int, two);
+                            if (q + 1 < NP) {
+                                // (nothing is left of what is not finite)
+                                const float r0 = v0 - (float)two[0], r1 = v1 - (float)two[1];
+                                v0 = fabsf(v0) < INFINITY ? r0 : 0.f;
+                                v1 = fabsf(v1) < INFINITY ? r1 : 0.f;
+                            }
+                        }
+                        *reinterpret_cast<i32x4 *>(at + q * MB * kSlice * 32) = o;
+                    }
                 }
             }
         }
     };
-    f32x4 acc[RT][MB], sum[RT][MB];
+    f32x4 acc[RT][MB], sum[RT][MB], g[RT][MB];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-        for (int b = 0; b < MB; ++b) acc[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto compute = [&](int buf, Set &f) __attribute__((always_inline)) {
-        if (SCALED) {
+        for (int b = 0; b < MB; ++b) acc[t][b] = sum[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // x and scales two slices ahead, W kRing - 1; every slice makes the same kOps
+    // loads in the same order, so the wait for its W is a constant.
+    fetch_x(0, xa);
+    fetch_x(1, xb);
+    fetch_s(sa);
+    fetch_s(sb);
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
+    for (int s = 0; s + 1 < kRing; ++s) request_w(s);
+    stage_x(0, xa);
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+#pragma unroll 1
+    for (int s = 0; s < ns; ++s) {
+        // this slice's scales into the wave's own table
 #pragma unroll
-                for (int b = 0; b < MB; ++b) sum[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < RT; ++t) {
+            *reinterpret_cast<float2 *>(sc + t * kTable + c * 32 + h * 8) = make_float2(sa.s[t][0], sa.s[t][1]);
+            if (ZP) {
+                Zero *const z = reinterpret_cast<Zero *>(sc + t * kTable + 512 + c * 64 + h * 16);
+                z[0] = Zero(sa.z[t][0]), z[1] = Zero(sa.z[t][1]);
+            }
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            uint32_t w[RT][4];
+        for (int b = 0; b < MB; ++b)
+#pragma unroll
+            for (int i = 0; i < kXLoads; ++i) xa[b][i] = xb[b][i];
+        sa = sb;
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_x(s + 2, xb);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_s(sb);
+        __builtin_amdgcn_sched_barrier(0);
+        request_w(s + kRing - 1);
+        __builtin_amdgcn_sched_barrier(0);
+        // W of slice s was asked for kRing - 1 slices ago; the first ones in a row
+        if (s == 0)
+            wait_vm<(kRing - 2) * 2 * RT + kOps>();
+        else
+            wait_vm<(kRing - 3) * 2 * RT + 2 * kOps>();
+        __builtin_amdgcn_sched_barrier(0);
+        const char *const wt = ring + (s % kRing) * kW;
+        const char *const xt = xbuf + (s & 1) * kX;
+        f32x4 sv[RT][2];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sv[t][i] = *reinterpret_cast<const f32x4 *>(sc + t * kTable + c * 32 + i * 16);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (e % PER == 0) {
+#pragma unroll
+                for (int t = 0; t < RT; ++t)
+#pragma unroll
+                    for (int b = 0; b < MB; ++b) g[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            f16x8 bw[RT];
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[t][e] = (uint32_t)f.w[t][k][e];
-                if (T32) {
-                    // register e of quarter h <-> register h of quarter e
-                    const auto a = __builtin_amdgcn_permlane32_swap(w[t][0], w[t][2], false, false);
-                    const auto d = __builtin_amdgcn_permlane32_swap(w[t][1], w[t][3], false, false);
-                    const auto u = __builtin_amdgcn_permlane16_swap(a[0], d[0], false, false);
-                    const auto v = __builtin_amdgcn_permlane16_swap(a[1], d[1], false, false);
-                    w[t][0] = u[0], w[t][1] = u[1], w[t][2] = v[0], w[t][3] = v[1];
-                }
+                const uint32_t w = *reinterpret_cast<const uint32_t *>(wt + t * 2048 + c * 128 + ((e ^ (c & 7)) << 4) + h * 4);
+                f16x2 o[4];
+                unpack8(w, ZP ? *reinterpret_cast<const Zero *>(sc + t * kTable + 512 + c * 64 + e * 8) : Zero(8), o);
+                bw[t] = __builtin_shufflevector(__builtin_shufflevector(o[0], o[1], 0, 1, 2, 3),
+                                                __builtin_shufflevector(o[2], o[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
             }
-            f32x4 g[RT][MB];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (T32 || e == 0) {
+            for (int b = 0; b < MB; ++b)
 #pragma unroll
-                    for (int t = 0; t < RT; ++t)
+                for (int q = NP - 1; q >= 0; --q) {
+                    const f16x8 a = *reinterpret_cast<const f16x8 *>(xt + q * MB * kSlice * 32 +
+                                                                     ((b * 8 + e) * 64 + x_slot(e, h, c)) * 16);
 #pragma unroll
-                        for (int b = 0; b < MB; ++b) g[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int t = 0; t < RT; ++t) g[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bw[t], g[t][b], 0, 0, 0);
                 }
-                const int gi = T32 ? 4 * k + e : k;
-                f16x8 bw[RT];
+            if (e % PER == PER - 1) {
 #pragma unroll
-                for (int t = 0; t < RT; ++t) {
-                    f16x2 o[4];
-                    unpack8(w[t][e], Zero(f.z[t][gi]), o);
-                    bw[t] = __builtin_shufflevector(__builtin_shufflevector(o[0], o[1], 0, 1, 2, 3),
-                                                    __builtin_shufflevector(o[2], o[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
-                }
+                for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int b = 0; b < MB; ++b)
+                    for (int b = 0; b < MB; ++b) {
+                        f32x4 &to = SCALED ? sum[t][b] : acc[t][b];
 #pragma unroll
-                    for (int q = NP - 1; q >= 0; --q) {
-                        const f16x8 a = *reinterpret_cast<const f16x8 *>(
-                            lds + buf * kBuf + q * MB * kSlice * 32 + ((b * 8 + 4 * k + e) * 64 + lane) * 16);
-#pragma unroll
-                        for (int t = 0; t < RT; ++t) g[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, bw[t], g[t][b], 0, 0, 0);
+                        for (int r = 0; r < 4; ++r) to[r] = fmaf(g[t][b][r], sv[t][e / 4][e % 4], to[r]);
                     }
-                if (T32 || e == 3) {
-#pragma unroll
-                    for (int t = 0; t < RT; ++t)
-#pragma unroll
-                        for (int b = 0; b < MB; ++b) {
-                            f32x4 &to = SCALED ? sum[t][b] : acc[t][b];
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) to[r] = fmaf(g[t][b][r], f.s[t][gi], to[r]);
-                        }
-                }
             }
         }
         if (SCALED) {
 #pragma unroll
             for (int b = 0; b < MB; ++b) {
-                const f32x4 s = *reinterpret_cast<const f32x4 *>(&back[buf][16 * b + 4 * h]);
+                const f32x4 f = *reinterpret_cast<const f32x4 *>(backs + (s & 1) * MB * 16 + 16 * b + 4 * h);
 #pragma unroll
-                for (int t = 0; t < RT; ++t)
+                for (int t = 0; t < RT; ++t) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[t][b][r] = fmaf(sum[t][b][r], s[r], acc[t][b][r]);
+                    for (int r = 0; r < 4; ++r) acc[t][b][r] = fmaf(sum[t][b][r], f[r], acc[t][b][r]);
+                    sum[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+                }
             }
         }
-    };
-    const int ns = (k1 - k0 + kSlice - 1) / kSlice;
-    Set f[2];
-    fetch_x(k0);
-    fetch(k0, f[0]);
-    fetch(k0 + kSlice, f[1]);
-    stage_x(0);
-    __syncthreads();
-    for (int i = 0; i < ns; i += 2) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            if (i + u < ns) {
-                const int j = k0 + (i + u) * kSlice;
-                if (i + u + 1 < ns) fetch_x(j + kSlice);
-                compute(u, f[u]);
-                fetch(j + 2 * kSlice, f[u]);
-                if (i + u + 1 < ns) stage_x(u ^ 1);
-                __syncthreads();
-            }
-        }
+        stage_x(s + 1, xa);
+        // every wave's x of the next slice is there, and is done with this one's
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
     }
+    wait_vm<0>();  // nothing is still on its way into the ring
     // lane (c, h), register r: row 4 h + r of x's block, row c of W's tile
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -513,10 +627,12 @@ W4Plan w4_plan(const LinearW4Desc &d) {
     const int64_t blocks = (d.m + 15) / 16;
     pl.mb = (int)std::min<int64_t>(blocks, d.dtype == GFH_F32 ? 2 : 4);
     if (pl.mb == 3) pl.mb = 4;
-    pl.rt = pl.mb == 1 ? 1 : 2;
+    pl.rt = 2;
     const int64_t tiles = (d.n + 64 * pl.rt - 1) / (64 * pl.rt) * ((d.m + 16 * pl.mb - 1) / (16 * pl.mb));
     const int64_t slices = (d.k + kSlice - 1) / kSlice;
-    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(2 * device_cu_count() / tiles, slices / 2));
+    // K is split as far as the workgroups that fit the CUs at once go
+    const int64_t slots = (pl.mb > 1 || d.dtype == GFH_F32 ? 1 : 2) * device_cu_count();
+    const int64_t want = std::max<int64_t>(1, std::min<int64_t>(slots / tiles, slices / 2));
     const int64_t per = (slices + want - 1) / want;
     pl.kper = (int)(per * kSlice);
     pl.splits = (int)((slices + per - 1) / per);
@@ -563,7 +679,6 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
     p.ldx = d.ldx, p.ldy = d.ldy;
     p.m = (int)d.m, p.n = (int)d.n, p.k = (int)d.k, p.group = (int)d.group;
     p.groups = (int)((d.k + d.group - 1) / d.group);
-    p.xvec = aligned16(d.x) && d.ldx % (d.dtype == GFH_F32 ? 4 : 8) == 0;
     p.part = static_cast<float *>(workspace);
     p.splits = 1;
     auto typed = [&](auto &&go) {
@@ -603,22 +718,25 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
     const dim3 grid((unsigned)gx, (unsigned)gy);
     typed([&](auto t) {
         using T = decltype(t);
-        auto go = [&](auto mb, auto rt) {
-            constexpr int MB = decltype(mb)::value, RT = decltype(rt)::value;
-            if (d.group % 128 == 0)
-                hipLaunchKernelGGL((w4_tiles_kernel<T, MB, RT, false>), grid, dim3(256), 0, s, p);
+        auto go = [&](auto mb, auto per) {
+            constexpr int MB = decltype(mb)::value, PER = decltype(per)::value;
+            if (d.zps)
+                hipLaunchKernelGGL((w4_tiles_kernel<T, MB, true, PER>), grid, dim3(256), 0, s, p);
             else
-                hipLaunchKernelGGL((w4_tiles_kernel<T, MB, RT, true>), grid, dim3(256), 0, s, p);
+                hipLaunchKernelGGL((w4_tiles_kernel<T, MB, false, PER>), grid, dim3(256), 0, s, p);
         };
-        using One = std::integral_constant<int, 1>;
-        using Two = std::integral_constant<int, 2>;
-        using Four = std::integral_constant<int, 4>;
-        if (pl.mb == 1)
-            go(One{}, One{});
-        else if (pl.mb == 2)
-            go(Two{}, Two{});
-        else if constexpr (!std::is_same_v<T, float>)
-            go(Four{}, Two{});
+        auto sized = [&](auto per) {
+            if (pl.mb == 1)
+                go(std::integral_constant<int, 1>{}, per);
+            else if (pl.mb == 2)
+                go(std::integral_constant<int, 2>{}, per);
+            else if constexpr (!std::is_same_v<T, float>)
+                go(std::integral_constant<int, 4>{}, per);
+        };
+        if (d.group % 128 == 0 || d.group >= d.k)
+            sized(std::integral_constant<int, 4>{});
+        else
+            sized(std::integral_constant<int, 1>{});
     });
     GFH_TRY(check_launch("linear_w4"));
     if (pl.splits > 1) {

@@ -61,7 +61,7 @@ SIGNATURES = {
     "gfh_qlinear_dynamic_i8": (_i, [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _sz, _p]),
     "gfh_quantize_i4_grouped": (_i, [_p, _i64, _i64, _i64, _p, _p, _p, _p]),
     "gfh_dequantize_i4_grouped": (_i, [_p, _p, _p, _i64, _i64, _i64, _p, _p]),
-    "gfh_linear_w4_workspace_size": (_sz, [_i, _i64, _i64, _i64]),
+    "gfh_linear_w4_workspace_size": (_sz, [_i, _i64, _i64, _i64, _i64]),
     "gfh_linear_w4": (_i, [_i, _p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _sz, _p]),
     "gfh_gemv_f32": (_i, [_p, _p, _p, _i64, _i64, _i64, _p]),
     "gfh_gemv_w8": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _p]),
@@ -77,7 +77,7 @@ SIGNATURES = {
                                             _i64, _i, _p, _p, _i64, _i64, _i64, _i64, _i64, _p, _sz, _p]),
     "gfh_paged_append": (_i, [_p, _i, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64, _i64, _i,
                               _p]),
-    "gfh_paged_attention_workspace_size": (_sz, [_p, _i64, _i64, _i64]),
+    "gfh_paged_attention_workspace_size": (_sz, [_p, _i64, _i64, _i64, _i64]),
     "gfh_paged_attention": (_i, [_p, _i, _i64, _i64, _p, _i64, _p, _i64, _f, _i, _i64, _i64, _p, _sz, _p]),
     "gfh_silu_mul_f32": (_i, [_p, _p, _p, _i64, _p]),
     "gfh_state_dict_open": (_i, [C.c_char_p, C.POINTER(C.c_void_p)]),

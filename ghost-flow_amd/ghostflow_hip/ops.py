@@ -326,8 +326,9 @@ def dequantize_grouped_i4(codes, scales, zero_points=None, group_size=128):
     return out
 
 
-def linear_w4_workspace_size(m: int, n: int, k: int, dtype=torch.float32) -> int:
-    return int(lib().gfh_linear_w4_workspace_size(_DTYPES.get(dtype, -1), m, n, k))
+def linear_w4_workspace_size(m: int, n: int, k: int, group_size: int = 128, dtype=torch.float32) -> int:
+    """Bytes of linear_w4's workspace for x [m, k] and a weight [n, k]."""
+    return int(lib().gfh_linear_w4_workspace_size(_DTYPES.get(dtype, -1), m, n, k, group_size))
 
 
 def linear_w4(x, codes, scales, zero_points=None, bias=None, *, group_size=128, out=None, workspace=None):
@@ -656,10 +657,12 @@ def paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, *, scal
     return out
 
 
-def paged_attention_workspace_size(q, k_pages, v_pages, page_table, q_offsets, kv_lens, max_kv_len=None) -> int:
+def paged_attention_workspace_size(q, k_pages, v_pages, page_table, q_offsets, kv_lens, window=0,
+                                   max_kv_len=None) -> int:
     """Bytes of paged_attention's workspace for these arguments."""
     kv, _, _ = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, None, q.device)
-    return int(lib().gfh_paged_attention_workspace_size(kv, q.shape[0], q.shape[1], int(max_kv_len or 0)))
+    return int(lib().gfh_paged_attention_workspace_size(kv, q.shape[0], q.shape[1], int(window),
+                                                          int(max_kv_len or 0)))
 
 
 # ---- SwiGLU feed-forward block (ghostflow-nn/src/llama.rs:259-287) -------------

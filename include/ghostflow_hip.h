@@ -229,7 +229,7 @@ GFH_API int gfh_dequantize_i4_grouped(const uint8_t *codes, const float *scales,
  * any m is served.  y overlaps no input.
  * workspace (nullable, 16-byte aligned) of at least
  * gfh_linear_w4_workspace_size(...) bytes; any contents. */
-GFH_API size_t gfh_linear_w4_workspace_size(int dtype, int64_t m, int64_t n, int64_t k);
+GFH_API size_t gfh_linear_w4_workspace_size(int dtype, int64_t m, int64_t n, int64_t k, int64_t group);
 GFH_API int gfh_linear_w4(int dtype, const void *x, int64_t ldx, const uint8_t *codes,
                           const float *scales, const uint8_t *zero_points, const void *bias,
                           void *y, int64_t ldy, int64_t m, int64_t n, int64_t k, int64_t group,
@@ -466,7 +466,7 @@ GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, 
  * any contents.  Calls with NULL share the stream's block, so graphs that may
  * run at the same time need workspaces of their own. */
 GFH_API size_t gfh_paged_attention_workspace_size(const gfh_paged_kv *kv, int64_t tokens, int64_t heads,
-                                                  int64_t max_kv_len);
+                                                  int64_t window, int64_t max_kv_len);
 GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads,
                                 const void *q, int64_t ldq, void *out, int64_t ldo, float scale,
                                 int causal, int64_t window, int64_t max_kv_len, void *workspace,

@@ -77,10 +77,10 @@ def test_calls():
 def test_workspace_size():
     L, lib = _lib()
     size = lib.gfh_paged_attention_workspace_size
-    assert size(C.byref(_kv(L, head_dim=7)), 1, 4, 0) == 0
-    assert size(C.byref(_kv(L)), 0, 4, 0) == 0
+    assert size(C.byref(_kv(L, head_dim=7)), 1, 4, 0, 0) == 0
+    assert size(C.byref(_kv(L)), 0, 4, 0, 0) == 0
     long = _kv(L, max_pages=4096, table_stride=4096)
-    few, most = size(C.byref(long), 1, 4, 2000), size(C.byref(long), 1, 4, 0)
+    few, most = size(C.byref(long), 1, 4, 0, 2000), size(C.byref(long), 1, 4, 0, 0)
     assert 0 < few < most and most % 4 == 0
 
 

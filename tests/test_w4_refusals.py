@@ -47,10 +47,10 @@ def test_empty_and_null():
 def test_workspace_size():
     L, lib = _lib()
     size = lib.gfh_linear_w4_workspace_size
-    assert size(2, 1, 4096, 4096) == 0          # the form for few rows has no parts
-    assert size(2, 16, 4096, 4096) % (16 * 4096 * 4) == 0
-    assert size(9, 16, 4096, 4096) == 0
-    assert size(2, 16, 4096, 40) == 0
+    assert size(2, 1, 4096, 4096, 128) == 0          # the form for few rows has no parts
+    assert size(2, 16, 4096, 4096, 128) % (16 * 4096 * 4) == 0
+    assert size(9, 16, 4096, 4096, 128) == 0
+    assert size(2, 16, 4096, 40, 128) == 0
 
 
 def test_python_checks():
