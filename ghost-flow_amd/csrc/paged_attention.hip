@@ -16,7 +16,7 @@
 //
 // Softmax online in base 2, statistics and sums in fp32: the running maximum
 // is of the raw dot products, a probability is exp2(s c - m c + bias) with c =
-// |scale| log2 e (the sign of the scale is on q).  The bias (14 for f16, 16
+// |scale| log2 e (the sign of the scale is on q).  The bias (14 or 9 for f16, 16
 // where P is split) keeps small probabilities normal in their 16-bit form and
 // cancels in O / l.  Long axes are split over workgroups; a second kernel joins
 // the parts in their order, so results do not depend on timing.
@@ -212,6 +212,10 @@ struct Half<__bf16> {
     typedef bf16x8 v8;
     static constexpr uint32_t kExp = 0x7f80u;
     static constexpr float kBias = 0.f;
+    // c + both halves of w
+    static __device__ __forceinline__ float add2(uint32_t w, float c) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, w), v2{(__bf16)1.f, (__bf16)1.f}, c, false);
+    }
     static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -226,6 +230,9 @@ struct Half<_Float16> {
     typedef f16x8 v8;
     static constexpr uint32_t kExp = 0x7c00u;
     static constexpr float kBias = 14.f;
+    static __device__ __forceinline__ float add2(uint32_t w, float c) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, w), v2{(_Float16)1.f, (_Float16)1.f}, c, false);
+    }
     static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -282,16 +289,15 @@ __device__ __forceinline__ int stage_pages(const View &c, int seq, int b, int e,
 
 // One wave's requests for KEYS keys from k0 of K and V straight into LDS (16
 // bytes per lane; keys from e on and dims past d read zeros).
-template <int DP, int KEYS, int WAVES, int HINT>
+template <int DP, int KEYS, int HINT>
 __device__ __forceinline__ void request(const View &c, int kvh, const int64_t *pages, int p0, int k0, int e, char *kl,
-                                        char *vl, int wave, int lane) {
+                                        char *vl, int lane) {
     constexpr int kRowChunks = DP / 8, kRowsPer = 64 / kRowChunks;
-    constexpr int kInstr = KEYS / kRowsPer / WAVES;
-    static_assert(kInstr * kRowsPer * WAVES == KEYS, "whole instructions per wave");
+    constexpr int kInstr = KEYS / kRowsPer;
+    static_assert(kInstr * kRowsPer == KEYS, "whole instructions");
 #pragma unroll
     for (int i = 0; i < kInstr; ++i) {
-        const int ins = wave * kInstr + i;
-        const int row = ins * kRowsPer + lane / kRowChunks, ch = lane % kRowChunks;
+        const int row = i * kRowsPer + lane / kRowChunks, ch = lane % kRowChunks;
         const int key = min(k0 + row, e - 1), pg = paged::page_of(c, key);
         const int64_t off = pages[pg - p0];
         const int64_t at = off + 2 * ((int64_t)(key - pg * c.page_size) * c.row_stride + kvh * c.head_stride);
@@ -300,23 +306,27 @@ __device__ __forceinline__ void request(const View &c, int kvh, const int64_t *p
         const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
         const char *ks = ok && ck * 8 < c.d ? c.k + at + ck * 16 : zero;
         const char *vs = ok && cv * 8 < c.d ? c.v + at + cv * 16 : zero;
-        __builtin_amdgcn_global_load_lds((glb_ptr_t)ks, (lds_ptr_t)(kl + ins * 1024), 16, 0, HINT);
-        __builtin_amdgcn_global_load_lds((glb_ptr_t)vs, (lds_ptr_t)(vl + ins * 1024), 16, 0, HINT);
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)ks, (lds_ptr_t)(kl + i * 1024), 16, 0, HINT);
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)vs, (lds_ptr_t)(vl + i * 1024), 16, 0, HINT);
     }
 }
 
-// The same for the 64 keys of a whole tile whose 16 keys per wave (32 at DP = 64)
-// lie in one page: one page offset per wave, and per lane offsets that do not
-// change.  False (and nothing asked for) where they do not.
-template <int DP>
+// The chunk kernels' requests for a 64-key tile, 64 / WAVES keys per wave.  Where
+// those lie in one page (a whole tile, at a multiple of them) that is one page
+// offset per wave, and offsets per lane that do not change; else every row is
+// looked up.
+template <int DP, int WAVES>
 struct Lanes {
-    static constexpr int kKeys = 16;  // per wave
+    static constexpr int kKeys = 64 / WAVES;
     static constexpr int kRowChunks = DP / 8, kRowsPer = 64 / kRowChunks, kInstr = kKeys / kRowsPer;
+    static_assert(kInstr >= 1, "whole instructions per wave");
     uint32_t k[kInstr], v[kInstr];  // bytes from the wave's first row, ~0: zeros
     bool whole;                     // pages hold whole groups of a wave's keys
+    bool full;                      // every lane has dims of the head
 
     __device__ __forceinline__ Lanes(const View &c, int wave, int lane) {
         whole = c.page_size % kKeys == 0 && c.row_stride < (int64_t)1 << 24;
+        full = c.d == DP;
 #pragma unroll
         for (int i = 0; i < kInstr; ++i) {
             const int row = (wave * kInstr + i) * kRowsPer + lane / kRowChunks, ch = lane % kRowChunks;
@@ -327,28 +337,53 @@ struct Lanes {
         }
     }
 };
-template <int DP>
-__device__ __forceinline__ bool request_tile(const View &c, const Lanes<DP> &ln, int kvh, const int64_t *pages, int p0,
-                                             int k0, int e, char *kl, char *vl, int wave) {
-    using L = Lanes<DP>;
-    if (!ln.whole || k0 + 64 > e || (k0 & (L::kKeys - 1))) return false;
-    const int key = k0 + wave * L::kKeys, pg = paged::page_of(c, key);
+// Where the wave's keys of the tile at k0 begin, in bytes from the cache's (same
+// for K and V), or -1 where they have to be looked up one by one.
+template <int DP, int WAVES>
+__device__ __forceinline__ int64_t locate_tile(const View &c, const Lanes<DP, WAVES> &ln, int kvh, const int64_t *pages,
+                                               int p0, int k0, int e, int wave) {
+    if (!ln.whole || k0 + 64 > e || (k0 & (ln.kKeys - 1)) != 0) return -1;
+    const int key = k0 + wave * ln.kKeys, pg = paged::page_of(c, key);
     const int64_t off = pages[pg - p0];
     const int lo = __builtin_amdgcn_readfirstlane((int)off), hi = __builtin_amdgcn_readfirstlane((int)(off >> 32));
-    if (hi < 0) return false;
-    const int64_t at = ((int64_t)hi << 32 | (uint32_t)lo) +
-                       2 * ((int64_t)(key - pg * c.page_size) * c.row_stride + kvh * c.head_stride);
-    const char *kb = c.k + at, *vb = c.v + at;
-    const char *zero = reinterpret_cast<const char *>(g_zero_chunk);
+    if (hi < 0) return -1;
+    return ((int64_t)hi << 32 | (uint32_t)lo) +
+           2 * ((int64_t)(key - pg * c.page_size) * c.row_stride + kvh * c.head_stride);
+}
+// One tile of K or V, located at `at`, into `to`.
+template <int DP, int WAVES, bool V>
+__device__ __forceinline__ void request_tile(const View &c, const Lanes<DP, WAVES> &ln, int64_t at, int kvh,
+                                             const int64_t *pages, int p0, int k0, int e, char *to, int wave, int lane) {
+    using L = Lanes<DP, WAVES>;
+    const char *const base = V ? c.v : c.k;
+    const char *const zero = reinterpret_cast<const char *>(g_zero_chunk);
+    if (at >= 0) {
+        if (ln.full) {
 #pragma unroll
+            for (int i = 0; i < L::kInstr; ++i)
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)(base + at + (V ? ln.v[i] : ln.k[i])),
+                                                 (lds_ptr_t)(to + (wave * L::kInstr + i) * 1024), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < L::kInstr; ++i) {
+                const uint32_t x = V ? ln.v[i] : ln.k[i];
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)(x != ~0u ? base + at + x : zero),
+                                                 (lds_ptr_t)(to + (wave * L::kInstr + i) * 1024), 16, 0, 0);
+            }
+        }
+        return;
+    }
+#pragma unroll 1
     for (int i = 0; i < L::kInstr; ++i) {
         const int ins = wave * L::kInstr + i;
-        const char *ks = ln.k[i] != ~0u ? kb + ln.k[i] : zero;
-        const char *vs = ln.v[i] != ~0u ? vb + ln.v[i] : zero;
-        __builtin_amdgcn_global_load_lds((glb_ptr_t)ks, (lds_ptr_t)(kl + ins * 1024), 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((glb_ptr_t)vs, (lds_ptr_t)(vl + ins * 1024), 16, 0, 0);
+        const int row = ins * L::kRowsPer + lane / L::kRowChunks, ch = lane % L::kRowChunks;
+        const int key = min(k0 + row, e - 1), pg = paged::page_of(c, key);
+        const int64_t off = pages[pg - p0];
+        const int64_t from = off + 2 * ((int64_t)(key - pg * c.page_size) * c.row_stride + kvh * c.head_stride);
+        const int cc = ch ^ (V ? swz_v<DP>(row) : swz_k<DP>(row));
+        const char *src = k0 + row < e && off >= 0 && cc * 8 < c.d ? base + from + cc * 16 : zero;
+        __builtin_amdgcn_global_load_lds((glb_ptr_t)src, (lds_ptr_t)(to + ins * 1024), 16, 0, 0);
     }
-    return true;
 }
 
 template <typename T>
@@ -546,14 +581,14 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
         const int n = (pe - pb + 31) / 32;  // tiles of this pass; this wave's: wave, wave + WAVES, ..
         char *const ring = lds + wave * 4 * kTile;
         if (wave < n)
-            request<DP, 32, 1, kNtHint>(p.c, kvh, pages, p0, pb + 32 * wave, pe, ring, ring + kTile, 0, lane);
+            request<DP, 32, kNtHint>(p.c, kvh, pages, p0, pb + 32 * wave, pe, ring, ring + kTile, lane);
         int st = 0;
         for (int i = wave; i < n; i += WAVES, st ^= 1) {
             // (past the last tile: the last key again, into the free stage)
             const int k0 = pb + 32 * i, kn = min(k0 + 32 * WAVES, pe - 1);
             __builtin_amdgcn_sched_barrier(0);
-            request<DP, 32, 1, kNtHint>(p.c, kvh, pages, p0, kn, pe, ring + (st ^ 1) * 2 * kTile,
-                               ring + (st ^ 1) * 2 * kTile + kTile, 0, lane);
+            request<DP, 32, kNtHint>(p.c, kvh, pages, p0, kn, pe, ring + (st ^ 1) * 2 * kTile,
+                               ring + (st ^ 1) * 2 * kTile + kTile, lane);
             __builtin_amdgcn_sched_barrier(0);
             wait_vm<kOps>();
             __builtin_amdgcn_sched_barrier(0);
@@ -649,6 +684,32 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     join_waves<TA, DP, WAVES>(p, t, kvh, split, nact > 1, accs, mls, tid);
 }
 
+// Row r of a chunk tile (lane half h holds dims 32 i + 8 x + 4 h .. + 3) to out or
+// to the parts.
+template <typename TA, int NB>
+__device__ __forceinline__ void store_rows(const AttnParams &p, const Rows &t, int kvh, int r, int h, int split,
+                                           bool parts, float m, float l, const f32x16 (&o)[NB]) {
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
+    l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    if (r < t.r0 || r >= t.r1) return;
+    const int64_t at = parts ? part_row(p, r, kvh) * p.nsplit + split : 0;
+    const float f = parts ? 1.f : m == -INFINITY ? 0.f : 1.0f / l;
+    if (parts && h == 0) p.ml[at] = make_float2(m == -INFINITY ? m : m * p.sc2, l);
+    TA *const row = out_row<TA>(p, r, kvh);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int dim = 32 * i + 8 * x + 4 * h;
+            if (dim >= p.c.d) continue;
+            const float y[4] = {o[i][4 * x] * f, o[i][4 * x + 1] * f, o[i][4 * x + 2] * f, o[i][4 * x + 3] * f};
+            if (parts)
+                store_vec<4>(p.acc + at * p.c.d + dim, y);
+            else
+                store_vec<4>(row + dim, y);
+        }
+}
+
 // ---- many rows: chunks of prompts ---------------------------------------------------
 //
 // A tile of 128 rows, four waves of 32; K and V tiles of 64 keys, two stages
@@ -656,12 +717,29 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
 // K . Q^T on 32x32x16: lane (c = l % 32, h = l / 32) holds keys 32 kb + 8 (r /
 // 4) + 4 h + r % 4 of row c; registers 8 t .. 8 t + 7 are its B operand of O^T
 // = V^T . P^T for the 16 keys 16 t .. when V^T takes them in that order.
+//
+// Bound by the matrix units and the vector ALU together: per tile a wave's
+// products take 1024 cycles, its 32 weights per lane some 850, and the two
+// waves that share a SIMD hide one in the other only in part.  So two
+// workgroups stay on a CU for every type, the products issue first, and the
+// softmax is kept short (bf16, 2048 tokens over 16384 keys, 32 heads over 8
+// of 128, 515 GFLOP; f32 over bf16, 27.5 GFLOP in three pieces each):
+//   the maximum followed at every tile, weights added singly    564 us
+//   the maximum followed late                                   560
+//   16-bit weights added in pairs (l sums what the product sees) 544
+//   products at the higher issue priority                       525, 980 TFLOP/s
+//   f32: one workgroup per CU, fragments two ahead              168
+//   f32: two per CU (q's pieces in 96 registers, one ahead)     131
+// Eight waves in two groups that alternate between products and softmax by
+// barriers were no faster (559 against 564).
 template <typename TA, typename T, int DP, int ND, int NP>
-__global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnParams p) {
+__global__ __launch_bounds__(256, 2) void paged_chunk_kernel(AttnParams p) {
     using H = Half<T>;
     using v8 = typename H::v8;
     constexpr int NU = 2 * ND, NB = ND, kTile = 64 * DP * 2;  // ND: 32-dim blocks computed
-    constexpr float kBias = NP > 1 ? 16.f : H::kBias;
+    constexpr float kLate = H::kBias != 0.f ? 6.f : 8.f;
+    constexpr float kBias = NP > 1 ? 16.f : H::kBias != 0.f ? 9.f : 0.f;
+    constexpr int kAheadK = NP > 1 ? 1 : 3, kAheadV = NP > 1 ? 1 : 5;  // steps that fragments are read ahead
     __shared__ __attribute__((aligned(1024))) char lds[4 * kTile + kMaxPages * 8 + 64];  // stage, K / V; pages; flags
     int64_t *const pages = reinterpret_cast<int64_t *>(lds + 4 * kTile);
     int *const flags = reinterpret_cast<int *>(lds + 4 * kTile + kMaxPages * 8);
@@ -689,7 +767,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
     // [all_lo, all_hi) that all of them see
     const int w0 = max(t.r0, t.base + 32 * wave), w1 = min(t.r1, t.base + 32 * wave + 32);
     const bool live = w0 < w1;
-    const Lanes<DP> ln(p.c, wave, lane);
+    const Lanes<DP, 4> ln(p.c, wave, lane);
     int any_lo, any_hi, all_lo, all_hi;
     row_keys(p, t, live ? w0 : t.r0, any_lo, all_hi);
     row_keys(p, t, live ? w1 - 1 : t.r0, all_lo, any_hi);
@@ -711,8 +789,9 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
         const int n = (pe - pb + 63) / 64;
         auto ask = [&](int k0, int st) __attribute__((always_inline)) {
             char *const to = lds + st * 2 * kTile;
-            if (!request_tile<DP>(p.c, ln, kvh, pages, p0, k0, pe, to, to + kTile, wave))
-                request<DP, 64, 4, 0>(p.c, kvh, pages, p0, k0, pe, to, to + kTile, wave, lane);
+            const int64_t at = locate_tile<DP, 4>(p.c, ln, kvh, pages, p0, k0, pe, wave);
+            request_tile<DP, 4, false>(p.c, ln, at, kvh, pages, p0, k0, pe, to, wave, lane);
+            request_tile<DP, 4, true>(p.c, ln, at, kvh, pages, p0, k0, pe, to + kTile, wave, lane);
         };
         ask(pb, 0);
         for (int i = 0; i < n; ++i) {
@@ -720,7 +799,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
             // The tile is there, and every wave is done with the one before: the
             // next one's requests have the scores and the softmax of this one to
             // arrive in (the compiler waits for them before the transposing
-            // reads of V).
+            // reads of V).  Priorities here are a wave's own, within its SIMD.
             wait_vm<0>();
             __syncthreads();
             if (i + 1 < n) ask(k0 + 64, st ^ 1);
@@ -731,24 +810,24 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int x = 0; x < 16; ++x) s[kb][x] = 0.f;
-            // (fragments are read two steps ahead of their products)
-            v8 kf[3][2];
+            // (fragments are read steps ahead of their products)
+            v8 kf[kAheadK + 1][2];
             auto read_k = [&](int u) __attribute__((always_inline)) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
-                    kf[u % 3][kb] = *reinterpret_cast<const v8 *>(kt + (kb * 32 + c) * DP * 2 +
+                    kf[u % (kAheadK + 1)][kb] = *reinterpret_cast<const v8 *>(kt + (kb * 32 + c) * DP * 2 +
                                                                   (((2 * u + h) ^ swz_k<DP>(c)) << 4));
             };
-            read_k(0);
-            read_k(1);
+#pragma unroll
+            for (int u = 0; u < kAheadK; ++u) read_k(u);
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
-                if (u + 2 < NU) read_k(u + 2);
+                if (u + kAheadK < NU) read_k(u + kAheadK);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int q = NP - 1; q >= 0; --q)
 #pragma unroll
-                    for (int kb = 0; kb < 2; ++kb) s[kb] = H::mfma32(kf[u % 3][kb], qf[u][q], s[kb]);
+                    for (int kb = 0; kb < 2; ++kb) s[kb] = H::mfma32(kf[u % (kAheadK + 1)][kb], qf[u][q], s[kb]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             if (k0 < all_lo || k0 + 64 > min(all_hi, pe)) {
@@ -763,6 +842,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
 #pragma unroll 4
                 for (int x = 0; x < kTile / 256; ++x) odd |= not_finite<T>(w[x * 64 + lane]);
             }
+            __builtin_amdgcn_s_setprio(0);
             float mb = max_nan(s[0][0], s[1][0]);
 #pragma unroll
             for (int x = 1; x < 16; ++x) mb = max_nan(mb, max_nan(s[0][x], s[1][x]));
@@ -773,36 +853,39 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
             const float m_new = max_nan(m, mb);
             // (an infinite key meets q's pieces with either sign, or a zero one)
             if (NP > 1) odd |= jmax >= 0 && m_new != m_new;
-            const float mc = m_new == -INFINITY ? 0.f : m_new * p.sc2;
-            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m * p.sc2 - mc);
-            float sum = 0.f;
+            // The maximum moves on only when some row's is 2^kLate behind: weights then
+            // reach 2^(kBias + kLate), within fp16's range too, and most tiles leave
+            // the sums unscaled.
+            if (__any(!((m_new - m) * p.sc2 <= kLate))) {
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * p.sc2);
+                l *= alpha;
+#pragma unroll
+                for (int i2 = 0; i2 < NB; ++i2) o[i2] *= alpha;
+                m = m_new;
+            }
+            const float mc = kBias - (m == -INFINITY ? 0.f : m * p.sc2);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    s[kb][x] = __builtin_amdgcn_exp2f(fmaf(s[kb][x], p.sc2, kBias - mc));
-                    sum += s[kb][x];
+                    s[kb][x] = __builtin_amdgcn_exp2f(fmaf(s[kb][x], p.sc2, mc));
+                    if (NP > 1) l += s[kb][x];
                 }
-            l = fmaf(l, alpha, sum);
-            if (__any(!(m_new == m))) {
-#pragma unroll
-                for (int i2 = 0; i2 < NB; ++i2) o[i2] *= alpha;
-            }
-            m = m_new;
+            __builtin_amdgcn_s_setprio(1);
             // steps: 16 keys from 16 (n / NB), 32 dims from 32 (n % NB)
             const int key = 4 * h + ((lane & 15) >> 2);
-            v8 vf[3];
+            v8 vf[kAheadV + 1];
             auto read_v = [&](int n) __attribute__((always_inline)) {
                 const int ch = 4 * (n % NB) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
                 const char *at = vt + (16 * (n / NB) + key) * DP * 2 + (lane & 1) * 8 + ((ch ^ swz_v<DP>(key)) << 4);
-                vf[n % 3] = join<v8>(read_tr<T>(at), read_tr<T>(at + 8 * DP * 2));
+                vf[n % (kAheadV + 1)] = join<v8>(read_tr<T>(at), read_tr<T>(at + 8 * DP * 2));
             };
-            read_v(0);
-            read_v(1);
+#pragma unroll
+            for (int n = 0; n < kAheadV; ++n) read_v(n);
             v8 pf[NP];
 #pragma unroll
             for (int n = 0; n < 4 * NB; ++n) {
-                if (n + 2 < 4 * NB) read_v(n + 2);
+                if (n + kAheadV < 4 * NB) read_v(n + kAheadV);
                 if (n % NB == 0) {
                     const int kb = n / NB / 2, x = n / NB % 2;
                     uint32_t pw[NP][4];
@@ -812,6 +895,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
                         pieces2<T, NP>(s[kb][8 * x + 2 * y], s[kb][8 * x + 2 * y + 1], two);
 #pragma unroll
                         for (int q = 0; q < NP; ++q) pw[q][y] = two[q];
+                        if (NP == 1) l = H::add2(two[0], l);
                     }
 #pragma unroll
                     for (int q = 0; q < NP; ++q) {
@@ -821,7 +905,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
                 }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int q = NP - 1; q >= 0; --q) o[n % NB] = H::mfma32(vf[n % 3], pf[q], o[n % NB]);
+                for (int q = NP - 1; q >= 0; --q) o[n % NB] = H::mfma32(vf[n % (kAheadV + 1)], pf[q], o[n % NB]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -832,35 +916,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void paged_chunk_kernel(AttnP
         slow_rows<TA, T>(p, t, seq, kvh, b, e, split, nact > 1, kBias, wave, 4, lane);
         return;
     }
-    {
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
-        l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
-    }
-    if (r < t.r0 || r >= t.r1) return;
-    if (nact > 1) {
-        const int64_t at = part_row(p, r, kvh) * p.nsplit + split;
-        if (h == 0) p.ml[at] = make_float2(m == -INFINITY ? m : m * p.sc2, l);
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int dim = 32 * i + 8 * x + 4 * h;
-                if (dim < p.c.d)
-                    *reinterpret_cast<f32x4 *>(p.acc + at * p.c.d + dim) =
-                        f32x4{o[i][4 * x], o[i][4 * x + 1], o[i][4 * x + 2], o[i][4 * x + 3]};
-            }
-    } else {
-        const float inv = m == -INFINITY ? 0.f : 1.0f / l;
-        TA *row = out_row<TA>(p, r, kvh);
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int dim = 32 * i + 8 * x + 4 * h;
-                const float y[4] = {o[i][4 * x] * inv, o[i][4 * x + 1] * inv, o[i][4 * x + 2] * inv, o[i][4 * x + 3] * inv};
-                if (dim < p.c.d) store_vec<4>(row + dim, y);
-            }
-    }
+    store_rows<TA, NB>(p, t, kvh, r, h, split, nact > 1, m, l, o);
 }
 
 // ---- fp32 cache -------------------------------------------------------------------
