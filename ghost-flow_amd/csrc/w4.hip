@@ -15,7 +15,8 @@
 // (c[n, j] - z[n, g]) + bias[n].  A code becomes an f16 exactly: 0x6400 | c is
 // 1024 + c (0x6400 | c << 4 is 1024 + 16 c), and one packed f16 operation takes
 // 1024 + z off, nine instructions for eight codes.  The scale multiplies a
-// group's finished sum in fp32.
+// group's finished sum in fp32.  Three kernels: VALU for one or two rows of x (fp32:
+// four), a stream of W for up to 16 rows of 16 bits, tiles for the rest.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,6 +31,7 @@ namespace {
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // ---- to codes and back ----------------------------------------------------------
 
@@ -133,6 +135,8 @@ struct W4LinearParams {
     int m, n, k, group, groups;
     int kper;   // columns per split
     int splits;
+    int steps;       // 32-column steps per group (more than there are: one group)
+    uint32_t magic;  // 2^32 / steps, rounded up
 };
 
 // Eight codes as f16 pairs (0, 4), (1, 5), (2, 6), (3, 7), z taken off.
@@ -270,10 +274,10 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
     }
 }
 
-// More rows on the matrix units: D = x . W^T by 16x16x32 f16.  A wave takes RT
-// tiles of 16 rows of W and MB blocks of 16 rows of x; lane (c = l % 16, h = l /
-// 16) unpacks the codes of row c of W straight into its B operand and holds the
-// result's column c, so a group's scale is one value per lane.
+// More rows on the matrix units: D = x . W^T by 16x16x32 f16.  A workgroup takes
+// 128 rows of W and MB blocks of 16 rows of x, a wave RT tiles of 16 rows of W;
+// lane (c = l % 16, h = l / 16) unpacks the codes of row c of W straight into its B
+// operand and holds the result's column c, so a group's scale is one value per lane.
 //
 // Slices of 256 columns.  W comes by requests straight to LDS, a ring of kRing
 // slices per wave (eight rows of 128 bytes per instruction).  x goes through
@@ -285,10 +289,10 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
 // they join.  Scales and zero points are looked up per 32 columns, two of a row's
 // eight per lane, and go round through LDS.
 //
-// The loop is kept small: a launch that streams few slices spends its time on
-// instructions that no cache holds yet as much as on the weights (with the
-// slices unrolled, 16 KB of code: 18.0 us for 16 x 14336 x 4096, 8 of them
-// before the first slice).
+// Bound by waits: a workgroup needs 4 us to its first slice and 1.5 us or more for
+// each (LDS reads, then the barrier), so two or more blocks of x take eight waves
+// of one tile each rather than four of two (f16, 50 x 4096 x 11008: 27.3 us against
+// 32.5 with the join).  K is split as far as the workgroups that fit the CUs go.
 constexpr int kSlice = 256;
 typedef __attribute__((address_space(3))) void *lds_ptr_t;
 typedef __attribute__((address_space(1))) void *glb_ptr_t;
@@ -301,26 +305,28 @@ __device__ __forceinline__ void wait_vm() {
 
 // PER: 32-column steps per sum (4 where groups are whole 128-column blocks).
 template <typename T, int MB, bool ZP, int PER>
-__global__ __launch_bounds__(256, MB == 1 && sizeof(T) == 2 ? 2 : 1) void w4_tiles_kernel(W4LinearParams p) {
-    constexpr int NP = std::is_same_v<T, float> ? 3 : 1, RT = 2;
+__global__ __launch_bounds__(MB == 1 ? 256 : 512, MB == 1 && sizeof(T) == 4 ? 1 : 2) void w4_tiles_kernel(W4LinearParams p) {
+    constexpr int NP = std::is_same_v<T, float> ? 3 : 1;
+    constexpr int NW = MB == 1 ? 4 : 8, RT = 8 / NW;  // waves, tiles of W each: 128 rows
+    constexpr int XB = MB * 4 / NW;                   // x: blocks per thread
     constexpr bool SCALED = !std::is_same_v<T, _Float16>;
     constexpr int kX = NP * MB * kSlice * 16 * 2;  // one buffer of x
     constexpr int kW = RT * 16 * kSlice / 2;       // one slice of a wave's W
     constexpr int kXLoads = sizeof(T);             // per thread and block
     constexpr int kRing = 3;  // slices of W on their way or in use
     // loads of one slice, in their order: x, scales, W
-    constexpr int kOps = MB * kXLoads + RT * (ZP ? 4 : 2) + 2 * RT;
+    constexpr int kOps = XB * kXLoads + RT * (ZP ? 4 : 2) + 2 * RT;
     constexpr int kTable = ZP ? 1536 : 512;  // of a tile: scales [16][8], then Zero [16][8]
-    __shared__ __attribute__((aligned(1024))) char lds[4 * kRing * kW + 2 * kX + 4 * RT * kTable + 2 * MB * 64];
-    char *const xbuf = lds + 4 * kRing * kW;
-    float *const backs = reinterpret_cast<float *>(xbuf + 2 * kX + 4 * RT * kTable);
+    __shared__ __attribute__((aligned(1024))) char lds[NW * kRing * kW + 2 * kX + 8 * kTable + 2 * MB * 64];
+    char *const xbuf = lds + NW * kRing * kW;
+    float *const backs = reinterpret_cast<float *>(xbuf + 2 * kX + 8 * kTable);
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, h = lane >> 4;
     char *const ring = lds + wave * kRing * kW;
     char *const sc = xbuf + 2 * kX + wave * RT * kTable;
     const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits;
-    const int n0 = tile * 64 * RT + wave * 16 * RT, m0 = blockIdx.y * 16 * MB;
+    const int n0 = tile * 128 + wave * 16 * RT, m0 = blockIdx.y * 16 * MB;
     const int k0 = split * p.kper, k1 = min(k0 + p.kper, p.k);
     const int ns = (k1 - k0 + kSlice - 1) / kSlice;
     const T *x = static_cast<const T *>(p.x);
@@ -380,29 +386,30 @@ __global__ __launch_bounds__(256, MB == 1 && sizeof(T) == 2 ? 2 : 1) void w4_til
         }
     };
     // x: thread (row tid / 16 of a block, 16 columns), as loaded
-    i32x4 xa[MB][kXLoads], xb[MB][kXLoads];
-    auto fetch_x = [&](int s, i32x4 (&xr)[MB][kXLoads]) __attribute__((always_inline)) {
+    i32x4 xa[XB][kXLoads], xb[XB][kXLoads];
+    const int xrow = tid >> 4;  // and 4 NW ..
+    auto fetch_x = [&](int s, i32x4 (&xr)[XB][kXLoads]) __attribute__((always_inline)) {
         const int col = k0 + s * kSlice + 16 * (tid & 15);
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
-            const T *at = x + min(m0 + 16 * b + (tid >> 4), p.m - 1) * p.ldx + (col < k1 ? col : 0);
+        for (int b = 0; b < XB; ++b) {
+            const T *at = x + min(m0 + 4 * NW * b + xrow, p.m - 1) * p.ldx + (col < k1 ? col : 0);
 #pragma unroll
             for (int i = 0; i < kXLoads; ++i) xr[b][i] = load16(at + i * (16 / sizeof(T)));
         }
     };
-    auto stage_x = [&](int s, i32x4 (&xr)[MB][kXLoads]) __attribute__((always_inline)) {
+    auto stage_x = [&](int s, i32x4 (&xr)[XB][kXLoads]) __attribute__((always_inline)) {
         char *const to = xbuf + (s & 1) * kX;
         if (k0 + (s + 1) * kSlice > k1) {  // (rows past m are copies of the last, never stored)
             const bool ok = k0 + s * kSlice + 16 * (tid & 15) < k1;
 #pragma unroll
-            for (int b = 0; b < MB; ++b)
+            for (int b = 0; b < XB; ++b)
 #pragma unroll
                 for (int i = 0; i < kXLoads; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) xr[b][i][e] = ok ? xr[b][i][e] : 0;
         }
 #pragma unroll
-        for (int b = 0; b < MB; ++b) {
+        for (int b = 0; b < XB; ++b) {
             float v[16], up = 1.f;
             if constexpr (SCALED) {
                 // the exponent of the largest finite magnitude
@@ -429,12 +436,12 @@ __global__ __launch_bounds__(256, MB == 1 && sizeof(T) == 2 ? 2 : 1) void w4_til
                 big = fmaxf(big, dpp_mov<0x128>(big));
                 const int e2 = big > 0.f ? min(15 - __builtin_amdgcn_frexp_expf(big), 126) : 0;
                 up = __builtin_ldexpf(1.f, e2);
-                if ((tid & 15) == 0) backs[(s & 1) * MB * 16 + 16 * b + (tid >> 4)] = __builtin_ldexpf(1.f, -e2);
+                if ((tid & 15) == 0) backs[(s & 1) * MB * 16 + 4 * NW * b + xrow] = __builtin_ldexpf(1.f, -e2);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const int unit = 2 * (tid & 15) + u;  // of 8 columns
-                char *at = to + ((b * 8 + unit / 4) * 64 + x_slot(unit / 4, unit % 4, tid >> 4)) * 16;
+                char *at = to + (((4 * NW * b + xrow) / 16 * 8 + unit / 4) * 64 + x_slot(unit / 4, unit % 4, xrow & 15)) * 16;
                 if constexpr (!SCALED) {
                     i32x4 o;
 #pragma unroll
@@ -499,7 +506,7 @@ __global__ __launch_bounds__(256, MB == 1 && sizeof(T) == 2 ? 2 : 1) void w4_til
             }
         }
 #pragma unroll
-        for (int b = 0; b < MB; ++b)
+        for (int b = 0; b < XB; ++b)
 #pragma unroll
             for (int i = 0; i < kXLoads; ++i) xa[b][i] = xb[b][i];
         sa = sb;
@@ -599,6 +606,235 @@ __global__ __launch_bounds__(256, MB == 1 && sizeof(T) == 2 ? 2 : 1) void w4_til
     }
 }
 
+// ---- up to 16 rows of 16 bits: W as a stream -------------------------------------------
+
+// Eight codes of one row as the B operand of a 16x16x32 product, in their order.
+// f16: 0x6400 | c and 0x6400 | c << 4 from one byte, then one packed operation takes
+// 1024 + z or 16 (64 + z) off: c - z.  bf16: the byte c is the fp8 (e4m3) number
+// c 2^-9 (0 .. 7 the subnormal ones, 8 .. 15 the first binade), so the conversion
+// from fp8 gives c itself; z is taken off the sums.
+__device__ __forceinline__ f16x8 codes_f16(uint32_t w, f16x2 zero) {
+    i32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t two = __builtin_amdgcn_perm(0, w, 0x0c000c00u | i << 16 | i);
+        const f16x2 v = __builtin_bit_cast(f16x2, (two & 0x00f0000fu) | 0x64006400u);
+        o[i] = __builtin_bit_cast(int, __builtin_elementwise_fma(v, f16x2{(_Float16)1.f, (_Float16)0.0625f}, zero));
+    }
+    return __builtin_bit_cast(f16x8, o);
+}
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t w) {
+    const uint32_t even = w & 0x0f0f0f0fu, odd = (w >> 4) & 0x0f0f0f0fu;
+    const uint32_t lo = __builtin_amdgcn_perm(odd, even, 0x05010400u), hi = __builtin_amdgcn_perm(odd, even, 0x07030602u);
+    i32x4 o;
+    o[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, false));
+    o[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 512.f, true));
+    o[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, false));
+    o[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 512.f, true));
+    return __builtin_bit_cast(bf16x8, o);
+}
+// (c - z as bf16, for x that is not finite)
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t w, float z) {
+    bf16x8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (__bf16)((float)((w >> 4 * i) & 15) - z);
+    return o;
+}
+
+constexpr int kStreamWaves = 8;
+constexpr int kStreamTable = 32 << 10;  // bytes of LDS for scales and zero points
+
+// A workgroup takes 16 rows of W, its waves a share of the columns each and no
+// barrier between its first and last: K is split inside the workgroup, so there
+// are no parts to join and no second launch.  Slices of 128 columns, four on
+// their way in registers, asked for two at a time (W's lines hold two):
+//   W   lane (c = l % 16, h = l / 16) 16 bytes, columns 32 h .. of row c; four lane
+//       swaps transpose (h, dword) so that step j takes columns 32 j + 8 h ..
+//   x   four rows of 256 bytes per instruction, through 4 KB of LDS of the wave's
+//       own into operands (loaded as operands, 16 rows of 64 bytes, the same
+//       bytes take twice the time: 22.4 us against 16.8)
+// The 16 rows' scales and zero points go to LDS at once.  bf16: g = sum c x and
+// one product with ones, sx = sum x, give s (g - z sx): exact as far as fp32 sums
+// are, and 0 for a row of zeros, as g and 8 sx round alike.  Where a sum is not
+// finite the wave repeats its share with c - z, so infinities reach what they
+// should.
+//
+// Bound by requests: a CU takes 1 KB of x and W in some 30 cycles, and x, which
+// every workgroup reads whole from its L2, is four of five.  16 x 14336 x 4096:
+// 15.5 us with groups of 64 and zero points (34.5 MB, 2.2 TB/s); sixteen waves 15.4
+// there but 9.6 against 8.0 at 4096 x 4096 and 30 against 18 at 4096 x 14336.
+template <typename T, bool ZP, int PER>
+__global__ __launch_bounds__(64 * kStreamWaves, 4) void w4_stream_kernel(W4LinearParams p) {
+    constexpr int R = 4, kAt = 2;  // slices on their way or in use, asked for at once
+    constexpr int NP = ZP ? 2 : 1;
+    constexpr bool BF = !std::is_same_v<T, _Float16>;
+    constexpr int kX = 1024;  // floats
+    // a slice of x per wave and the table of scales (and zero points); in the end
+    // the waves' sums
+    __shared__ __attribute__((aligned(16))) float lds[kStreamWaves * kX + kStreamTable / 4];
+    float *const table = lds + kStreamWaves * kX;
+    const int ld = NP * p.groups | 1;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    const int n0 = blockIdx.x * 16, rows = min(16, p.n - n0);
+    const int all = (p.k + 127) / 128, per = (all + kStreamWaves - 1) / kStreamWaves;
+    const int s0 = wave * per, s1 = min(all, s0 + per);
+    const char *const xbase = static_cast<const char *>(p.x);
+    const uint8_t *const wbase = p.codes + (int64_t)n0 * (p.k / 2);
+    char *const xl = reinterpret_cast<char *>(lds + wave * kX);
+    // (rows past the last are copies of it, never stored)
+    const uint32_t wat = (uint32_t)(min(c, rows - 1) * (p.k / 2) + 16 * h);
+    uint32_t xat[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) xat[i] = ((uint32_t)min(4 * i + h, p.m - 1) * (uint32_t)p.ldx + 8 * c) * 2;
+    struct Stage {
+        i32x4 x[4], w;
+    } st[R];
+    // (past the wave's last slice: one line of the first, never used)
+    auto fetch = [&](Stage &f, int s) __attribute__((always_inline)) {
+        const uint32_t on = s < s1 ? ~0u : 0u;
+        const int col = s < s1 ? s * 128 : 0;
+        if (col + 128 <= p.k) {
+            f.w = *reinterpret_cast<const i32x4 *>(wbase + col / 2 + (wat & on));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f.x[i] = load16(xbase + (int64_t)col * 2 + (xat[i] & on));
+        } else {
+            f.w = *reinterpret_cast<const i32x4 *>(wbase + col / 2 + (col + 32 * h < p.k ? wat : wat - 16 * h));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                f.x[i] = load16(xbase + (int64_t)col * 2 + (col + 8 * c < p.k ? xat[i] : xat[i] - 16 * c));
+        }
+    };
+    if (s0 < s1) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            fetch(st[i], s0 + i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    for (int row = wave; row < rows; row += kStreamWaves) {
+        const float *const from = p.scales + (int64_t)(n0 + row) * p.groups;
+        const uint8_t *const zfrom = ZP ? p.zps + (int64_t)(n0 + row) * p.groups : nullptr;
+        for (int g = lane; g < p.groups; g += 256) {
+            float v[4];
+            uint32_t z[4];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const int e = min(g + 64 * y, p.groups - 1);
+                v[y] = from[e];
+                z[y] = ZP ? zfrom[e] : 0;
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                float *const to = table + row * ld + NP * min(g + 64 * y, p.groups - 1);
+                to[0] = v[y];
+                // (f16: -(1024 + z), -(64 + z))
+                if (ZP) to[1] = BF ? (float)z[y] : __uint_as_float(0xd400e400u + (z[y] | z[y] << 20));
+            }
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto use = [&](Stage &f, int s, auto redo) __attribute__((always_inline)) {
+        constexpr bool REDO = decltype(redo)::value;
+        constexpr bool SX = BF && !REDO;
+        if (s * 128 + 128 > p.k && s * 128 + 8 * c >= p.k) {  // no columns there
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f.x[i] = i32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<i32x4 *>(xl + (4 * i + h) * 256 + ((c ^ (4 * i + h)) << 4)) = f.x[i];
+        // scales and zero points of the slice's groups
+        float sc[4 / PER], zf[4 / PER];
+#pragma unroll
+        for (int q = 0; q < 4 / PER; ++q) {
+            const uint32_t step = 4 * s + PER * q;
+            const int g = min((int)(p.steps == 1 ? step : __umulhi(step, p.magic)), p.groups - 1);
+            const float *const of = table + min(c, rows - 1) * ld + NP * g;
+            sc[q] = of[0];
+            zf[q] = ZP ? of[1] : BF ? 8.f : __uint_as_float(0xd480e408u);
+        }
+        uint32_t d[4] = {(uint32_t)f.w[0], (uint32_t)f.w[1], (uint32_t)f.w[2], (uint32_t)f.w[3]};
+        auto swap32 = [&](uint32_t &a, uint32_t &b) {
+            const auto v = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+            a = v[0], b = v[1];
+        };
+        auto swap16 = [&](uint32_t &a, uint32_t &b) {
+            const auto v = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+            a = v[0], b = v[1];
+        };
+        swap32(d[0], d[2]), swap32(d[1], d[3]);
+        swap16(d[0], d[1]), swap16(d[2], d[3]);
+#pragma unroll
+        for (int q = 0; q < 4 / PER; ++q) {
+            f32x4 g = {0.f, 0.f, 0.f, 0.f}, sx = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = PER * q; j < PER * q + PER; ++j) {
+                const i32x4 xv = *reinterpret_cast<const i32x4 *>(xl + c * 256 + (((4 * j + h) ^ c) << 4));
+                if constexpr (BF) {
+                    const bf16x8 a = __builtin_bit_cast(bf16x8, xv);
+                    const i32x4 one = {0x3f803f80, 0x3f803f80, 0x3f803f80, 0x3f803f80};
+                    if (SX)
+                        sx = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, one), sx, 0, 0, 0);
+                    g = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, REDO ? codes_bf16(d[j], zf[q]) : codes_bf16(d[j]), g, 0,
+                                                                0, 0);
+                } else {
+                    g = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, xv),
+                                                              codes_f16(d[j], __builtin_bit_cast(f16x2, zf[q])), g, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = fmaf(SX ? fmaf(-zf[q], sx[r], g[r]) : g[r], sc[q], acc[r]);
+        }
+    };
+#pragma unroll 1
+    for (int s = s0; s < s1; s += R) {
+#pragma unroll
+        for (int i = 0; i < R; i += kAt) {
+#pragma unroll
+            for (int y = i; y < i + kAt; ++y)
+                if (s + y < s1) use(st[y], s + y, std::false_type{});
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int y = i; y < i + kAt; ++y) fetch(st[y], s + y + R);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+    if constexpr (BF) {
+        bool odd = false;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) odd |= !(fabsf(acc[r]) < INFINITY);
+        if (__any(odd)) {  // (finite sums stay what they are without the others)
+            const f32x4 was = acc;
+            acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int s = s0; s < s1; ++s) {
+                fetch(st[0], s);
+                use(st[0], s, std::true_type{});
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = fabsf(was[r]) < INFINITY ? was[r] : acc[r];
+        }
+    }
+    __syncthreads();
+    *reinterpret_cast<f32x4 *>(lds + (wave * 64 + lane) * 4) = acc;
+    __syncthreads();
+    // the waves' sums in their order; lane (c, h), register r: row 4 h + r of x, row
+    // c of W
+    const int m = threadIdx.x >> 4, n = threadIdx.x & 15;
+    if (m >= p.m || n >= rows) return;
+    float v = 0.f;
+#pragma unroll
+    for (int u = 0; u < kStreamWaves; ++u) v += lds[(u * 64 + (m >> 2) * 16 + n) * 4 + (m & 3)];
+    if (p.bias) v += (float)static_cast<const T *>(p.bias)[n0 + n];
+    static_cast<T *>(p.y)[m * p.ldy + n0 + n] = (T)v;
+}
+
 // The splits' sums in their order, and the bias.
 template <typename T>
 __global__ __launch_bounds__(256) void w4_join_kernel(W4LinearParams p) {
@@ -617,7 +853,23 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4LinearParams p) {
     static_cast<T *>(p.y)[m * p.ldy + n] = (T)t;
 }
 
-constexpr int kRowsMax = 4;  // rows of x that the VALU form takes
+// Rows of x that the VALU form takes, and whether the stream of W takes a call.
+// us of a call's kernels (bf16, groups of 128), VALU / stream / tiles:
+//   n x k           m = 1            2             4             16
+//   1024 x 4096     3.7 / 7.7        4.4 / 7.5     5.9 / 7.5     - / 7.6 / 12.9
+//   4096 x 4096     6.2 / 8.1        7.6 / 8.0     10.5 / 7.8    - / 8.0 / 14.1
+//   4096 x 14336    12.2 / 14.8      16.4 / 15.3   23.0 / 15.0   - / 16.0 / 21.6
+//   14336 x 4096    11.4 / 17.8      15.8 / 17.9   27.7 / 17.6   - / 18.2 / 20.8
+//   28672 x 8192    30.2 / 49.7      43.3 / 49.6   79.0 / 50.4   - / 59.1 / 45.7
+// so up to two rows go to the VALU, and where W has 2^27 codes or more, more than
+// two to the tiles.  The stream holds 32-bit offsets and a row block's scales in
+// LDS.  fp32 x takes three pieces per product: four rows go to the VALU.
+int64_t rows_max(const LinearW4Desc &d) { return d.dtype == GFH_F32 ? 4 : 2; }
+bool w4_streams(const LinearW4Desc &d) {
+    const int64_t groups = (d.k + d.group - 1) / d.group;
+    return d.dtype != GFH_F32 && d.m > rows_max(d) && d.m <= 16 && d.n * d.k < (int64_t)1 << 27 && d.ldx < (int64_t)1 << 26 &&
+           16 * ((d.zps ? 2 : 1) * groups + 1) * 4 <= kStreamTable;
+}
 
 struct W4Plan {
     int mb, rt, splits, kper;
@@ -668,7 +920,7 @@ int launch_dequantize_w4(const uint8_t *codes, const float *scales, const uint8_
 }
 
 size_t linear_w4_workspace_bytes(const LinearW4Desc &d) {
-    if (d.m <= kRowsMax) return 0;
+    if (d.m <= rows_max(d) || w4_streams(d)) return 0;
     const W4Plan pl = w4_plan(d);
     return pl.splits > 1 ? (size_t)pl.splits * d.m * d.n * 4 : 0;
 }
@@ -689,7 +941,33 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
         else
             go(_Float16{});
     };
-    if (d.m <= kRowsMax) {
+    if (w4_streams(d)) {
+        p.steps = d.group >= d.k ? 1 << 30 : (int)(d.group / 32);
+        p.magic = (uint32_t)(((uint64_t)1 << 32) / p.steps + 1);
+        const dim3 grid((unsigned)((d.n + 15) / 16)), block(64 * kStreamWaves);
+        auto go = [&](auto t, auto per) {
+            using T = decltype(t);
+            constexpr int PER = decltype(per)::value;
+            if (d.zps)
+                hipLaunchKernelGGL((w4_stream_kernel<T, true, PER>), grid, block, 0, s, p);
+            else
+                hipLaunchKernelGGL((w4_stream_kernel<T, false, PER>), grid, block, 0, s, p);
+        };
+        auto sized = [&](auto t) {
+            if (p.steps % 4 == 0)
+                go(t, std::integral_constant<int, 4>{});
+            else if (p.steps % 2 == 0)
+                go(t, std::integral_constant<int, 2>{});
+            else
+                go(t, std::integral_constant<int, 1>{});
+        };
+        if (d.dtype == GFH_BF16)
+            sized(__bf16{});
+        else
+            sized(_Float16{});
+        return check_launch("linear_w4");
+    }
+    if (d.m <= rows_max(d)) {
         // eight rows of W per workgroup where that leaves two for every CU
         const bool eight = d.n >= 8 * 2 * device_cu_count();
         typed([&](auto t) {
@@ -721,9 +999,9 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
         auto go = [&](auto mb, auto per) {
             constexpr int MB = decltype(mb)::value, PER = decltype(per)::value;
             if (d.zps)
-                hipLaunchKernelGGL((w4_tiles_kernel<T, MB, true, PER>), grid, dim3(256), 0, s, p);
+                hipLaunchKernelGGL((w4_tiles_kernel<T, MB, true, PER>), grid, dim3(MB == 1 ? 256 : 512), 0, s, p);
             else
-                hipLaunchKernelGGL((w4_tiles_kernel<T, MB, false, PER>), grid, dim3(256), 0, s, p);
+                hipLaunchKernelGGL((w4_tiles_kernel<T, MB, false, PER>), grid, dim3(MB == 1 ? 256 : 512), 0, s, p);
         };
         auto sized = [&](auto per) {
             if (pl.mb == 1)

@@ -102,6 +102,45 @@ def test_linear_random(torch_dev, shape, kind):
     assert (_linear(torch_dev, x, wt, group).double() - want).abs().le(bound).all()
 
 
+# up to 16 rows: ragged slices, row blocks and groups, a group longer than the
+# rows, and scales that fill the table (8192 columns in groups of 32)
+FEW = [(3, 17, 96, 32), (5, 16, 128, 128), (16, 100, 160, 96), (9, 33, 4128, 64), (16, 40, 8192, 32), (4, 24, 992, 1024),
+       (12, 48, 1280, 160), (16, 16, 544, 192), (7, 1, 32, 32), (13, 31, 2080, 256)]
+
+
+@pytest.mark.parametrize("shape", FEW, ids=lambda v: "x".join(map(str, v)))
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_few_rows(torch_dev, shape, kind, zeros):
+    """As above: exact sums of whole numbers, then random ones."""
+    m, n, k, group = shape
+    g = torch.Generator().manual_seed(m * n + k + 1)
+    wt = W.random_weight(n, k, group, zeros, seed=k + n, exact=True)
+    x = torch.randint(-3, 4, (m, k), generator=g).to(W.TYPES[kind])
+    want = x.double() @ W.weight(*wt, group).t()
+    assert torch.equal(_linear(torch_dev, x, wt, group), want.to(W.TYPES[kind]))
+    wt = W.random_weight(n, k, group, zeros, seed=k)
+    x = torch.randn(m, k, generator=g).to(W.TYPES[kind])
+    w = W.weight(*wt, group)
+    want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    if kind == "bf16":  # sums of c x and of z x, up to 15 |x| s each
+        size = size + 15 * x.double().abs() @ torch.ones_like(w).t() * w.abs().max()
+    bound = (k + 4) * 2.0 ** -24 * size + torch.finfo(W.TYPES[kind]).eps / 2 * (want.abs() * (1 + 2 ** -9))
+    assert (_linear(torch_dev, x, wt, group).double() - want).abs().le(bound).all()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_linear_rows_of_zeros_give_zeros(torch_dev, kind):
+    """A weight row whose codes are all its zero point adds nothing, not even a
+    rounding, whatever x is."""
+    k, n, group = 2048, 20, 128
+    x = (torch.randn(8, k, generator=torch.Generator().manual_seed(9)) * 1e3).to(W.TYPES[kind])
+    wt = list(W.random_weight(n, k, group, False, seed=8))
+    wt[0][3] = 0x88
+    y = _linear(torch_dev, x, wt, group)
+    assert (y[:, 3] == 0).all() and not (y == 0).all(0)[:3].any()
+
+
 @pytest.mark.parametrize("m", [1, 4, 7, 40])
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_linear_rows_of_very_different_size(torch_dev, m, kind):
