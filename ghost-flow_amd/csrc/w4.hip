@@ -862,13 +862,15 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4LinearParams p) {
 //   14336 x 4096    11.4 / 17.8      15.8 / 17.9   27.7 / 17.6   - / 18.2 / 20.8
 //   28672 x 8192    30.2 / 49.7      43.3 / 49.6   79.0 / 50.4   - / 59.1 / 45.7
 // so up to two rows go to the VALU, and where W has 2^27 codes or more, more than
-// two to the tiles.  The stream holds 32-bit offsets and a row block's scales in
-// LDS.  fp32 x takes three pieces per product: four rows go to the VALU.
+// two to the tiles.  The stream holds a row block's scales and zero points in LDS
+// (asked for whether there are zero points or not, and without the strides: the
+// size of the workspace is asked for without them).  fp32 x takes three pieces per
+// product: four rows go to the VALU.
 int64_t rows_max(const LinearW4Desc &d) { return d.dtype == GFH_F32 ? 4 : 2; }
 bool w4_streams(const LinearW4Desc &d) {
     const int64_t groups = (d.k + d.group - 1) / d.group;
-    return d.dtype != GFH_F32 && d.m > rows_max(d) && d.m <= 16 && d.n * d.k < (int64_t)1 << 27 && d.ldx < (int64_t)1 << 26 &&
-           16 * ((d.zps ? 2 : 1) * groups + 1) * 4 <= kStreamTable;
+    return d.dtype != GFH_F32 && d.m > rows_max(d) && d.m <= 16 && d.n * d.k < (int64_t)1 << 27 &&
+           16 * (2 * groups + 1) * 4 <= kStreamTable;
 }
 
 struct W4Plan {
@@ -941,7 +943,8 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
         else
             go(_Float16{});
     };
-    if (w4_streams(d)) {
+    // (its offsets into x have 32 bits; rows further apart go to the VALU below)
+    if (w4_streams(d) && d.ldx < (int64_t)1 << 26) {
         p.steps = d.group >= d.k ? 1 << 30 : (int)(d.group / 32);
         p.magic = (uint32_t)(((uint64_t)1 << 32) / p.steps + 1);
         const dim3 grid((unsigned)((d.n + 15) / 16)), block(64 * kStreamWaves);
@@ -967,7 +970,7 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
             sized(_Float16{});
         return check_launch("linear_w4");
     }
-    if (d.m <= rows_max(d)) {
+    if (d.m <= rows_max(d) || w4_streams(d)) {
         // eight rows of W per workgroup where that leaves two for every CU
         const bool eight = d.n >= 8 * 2 * device_cu_count();
         typed([&](auto t) {
@@ -979,12 +982,17 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
                 else
                     hipLaunchKernelGGL((w4_rows_kernel<T, M, 4>), dim3((unsigned)((d.n + 3) / 4)), dim3(256), 0, s, p);
             };
-            if (d.m == 1)
-                go(std::integral_constant<int, 1>{});
-            else if (d.m == 2)
-                go(std::integral_constant<int, 2>{});
-            else
-                go(std::integral_constant<int, 4>{});
+            for (int64_t m = 0; m < d.m; m += 4) {
+                p.x = static_cast<const T *>(d.x) + m * d.ldx;
+                p.y = static_cast<T *>(d.y) + m * d.ldy;
+                p.m = (int)std::min<int64_t>(4, d.m - m);
+                if (p.m == 1)
+                    go(std::integral_constant<int, 1>{});
+                else if (p.m == 2)
+                    go(std::integral_constant<int, 2>{});
+                else
+                    go(std::integral_constant<int, 4>{});
+            }
         });
         return check_launch("linear_w4");
     }

@@ -129,6 +129,38 @@ def test_linear_few_rows(torch_dev, shape, kind, zeros):
     assert (_linear(torch_dev, x, wt, group).double() - want).abs().le(bound).all()
 
 
+@pytest.mark.parametrize("m", [2, 3, 7, 17])
+def test_linear_rows_far_apart(torch_dev, m):
+    """Rows of x whose distances pass 32 bits, in elements and in bytes."""
+    gh = _gh()
+    k, n, group, ld = 288, 40, 64, 1 << 28
+    wt = [t.to(torch_dev) for t in W.random_weight(n, k, group, True, seed=2)]
+    rows = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).to(torch_dev, torch.bfloat16)
+    wide = torch.empty((m - 1) * ld + k, dtype=torch.bfloat16, device=torch_dev)
+    x = wide.as_strided((m, k), (ld, 1))
+    x.copy_(rows)
+    a, b = gh.linear_w4(x, *wt, group_size=group), gh.linear_w4(rows, *wt, group_size=group)
+    size = rows.double().cpu().abs() @ W.weight(*[t.cpu() for t in wt], group).abs().t()
+    assert ((a.double() - b.double()).abs().cpu() <= 2.0 ** -8 * b.double().abs().cpu() + 32 * (k + 4) * 2.0 ** -24 * size).all()
+
+
+@pytest.mark.parametrize("m", [1, 3, 16, 17, 64])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_workspace_of_the_asked_size(torch_dev, m, kind, zeros):
+    """The size is asked for without the zero points and the strides, and is
+    enough with and without them."""
+    gh = _gh()
+    for n, k, group in ((80, 4096, 32), (80, 16384, 32), (300, 8192, 128)):
+        wt = W.random_weight(n, k, group, zeros, seed=k)
+        x = torch.randn(m, k, generator=torch.Generator().manual_seed(m)).to(W.TYPES[kind])
+        size = gh.linear_w4_workspace_size(m, n, k, group, W.TYPES[kind])
+        ws = torch.empty(max(size, 16), dtype=torch.uint8, device=torch_dev)
+        dev = [None if t is None else t.to(torch_dev) for t in wt]
+        got = gh.linear_w4(x.to(torch_dev), *dev, group_size=group, workspace=ws)
+        assert torch.equal(got.cpu(), _linear(torch_dev, x, wt, group))
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_linear_rows_of_zeros_give_zeros(torch_dev, kind):
     """A weight row whose codes are all its zero point adds nothing, not even a
