@@ -49,13 +49,17 @@ from .ops import (  # noqa: F401
 from .nn import (  # noqa: F401
     FlashAttention,
     FlashAttentionConfig,
+    GroupQuantizedSwiGLU,
     KVCache,
     MultiHeadAttention,
+    PagedBatch,
+    PagedKVCache,
     QuantizedSwiGLU,
     SwiGLU,
 )
 from .quantization import (  # noqa: F401
     DynamicQuantization,
+    GroupQuantizedLinear,
     QuantizationAwareTraining,
     QuantizationConfig,
     QuantizationScheme,

@@ -10,11 +10,15 @@ raise, so use eval() or dropout 0.
 
 KVCache is the in-place form of the reference's past_key / past_value
 concatenation: preallocated [B, capacity, E] buffers that every step
-appends to, so a decode step costs no copy of the past.
+appends to, so a decode step costs no copy of the past.  PagedKVCache is the
+form for many sequences of different lengths: pages that sequences take as
+they grow and give back, with MultiHeadAttention.step_paged for a ragged
+batch of their new tokens.
 
 SwiGLU follows ghostflow-nn/src/llama.rs:259-287 (LLaMA / Mistral
 feed-forward); QuantizedSwiGLU is the same block with DynamicQuantization's
-int8 weights (ghostflow-nn/src/quantization.rs:251-288).
+int8 weights (ghostflow-nn/src/quantization.rs:251-288), GroupQuantizedSwiGLU
+on 4-bit weights in groups.
 """
 from __future__ import annotations
 
@@ -23,8 +27,9 @@ import math
 import torch
 
 from . import _lib
-from .ops import (GhostFlowError, flash_attention_blockwise, mha_forward_cached, mha_forward_with_cache, qswiglu,
-                  quantize_per_channel, qweight_rowsum, swiglu)
+from .ops import (GhostFlowError, flash_attention_blockwise, linear, mha_forward_cached, mha_forward_with_cache,
+                  paged_append, paged_attention, qswiglu, quantize_per_channel, qweight_rowsum, silu_mul, swiglu)
+from .quantization import GroupQuantizedLinear
 
 
 class FlashAttentionConfig:
@@ -91,6 +96,89 @@ class KVCache:
         self.length = 0
 
 
+class PagedBatch:
+    """The new tokens of some sequences of a PagedKVCache, side by side:
+    sequence i has rows q_offsets[i] .. q_offsets[i + 1], and kv_lens[i] keys
+    with them (int32 device tensors, page_table [sequences, pages] too)."""
+
+    def __init__(self, page_table, q_offsets, kv_lens, tokens, max_kv_len):
+        self.page_table, self.q_offsets, self.kv_lens = page_table, q_offsets, kv_lens
+        self.tokens, self.max_kv_len = tokens, max_kv_len
+
+
+class PagedKVCache:
+    """Keys and values of many sequences in pages of page_size positions,
+    k_pages and v_pages [num_pages, page_size, num_kv_heads, head_dim].  The
+    host keeps which pages a sequence has: add() opens one, extend() gives
+    sequences the pages for their next tokens, remove() takes them back."""
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, *, dtype=torch.float32,
+                 device="cuda"):
+        if min(num_pages, page_size, num_kv_heads, head_dim) < 1:
+            raise GhostFlowError(_lib.INVALID_SHAPE, "a paged cache needs pages, positions, heads and dimensions")
+        self.k_pages = torch.empty((num_pages, page_size, num_kv_heads, head_dim), dtype=dtype, device=device)
+        self.v_pages = torch.empty_like(self.k_pages)
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages: dict[int, list[int]] = {}
+        self._lens: dict[int, int] = {}
+        self._next = 0
+
+    @property
+    def page_size(self) -> int:
+        return self.k_pages.shape[1]
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def length(self, seq: int) -> int:
+        return self._lens[seq]
+
+    def add(self) -> int:
+        """A new sequence without positions."""
+        seq, self._next = self._next, self._next + 1
+        self._pages[seq], self._lens[seq] = [], 0
+        return seq
+
+    def remove(self, seq: int) -> None:
+        """The sequence's pages are free again (kernels that still read them
+        come before those that write them on the same stream)."""
+        if seq not in self._pages:
+            raise GhostFlowError(_lib.INVALID_DATA, f"no sequence {seq}")
+        self._free.extend(reversed(self._pages.pop(seq)))
+        del self._lens[seq]
+
+    def extend(self, seqs, counts) -> PagedBatch:
+        """counts[i] new positions for sequence seqs[i]: their pages, and the
+        batch that step_paged, paged_append and paged_attention take.  Changes
+        nothing where the pages do not suffice."""
+        seqs, counts = [int(s) for s in seqs], [int(n) for n in counts]
+        if len(seqs) != len(counts) or len(set(seqs)) != len(seqs):
+            raise GhostFlowError(_lib.INVALID_DATA, "every sequence of a batch is named once, with its count")
+        if any(n < 0 for n in counts):
+            raise GhostFlowError(_lib.INVALID_SHAPE, "a count is negative")
+        for s in seqs:
+            if s not in self._pages:
+                raise GhostFlowError(_lib.INVALID_DATA, f"no sequence {s}")
+        need = [-(-(self._lens[s] + n) // self.page_size) - len(self._pages[s]) for s, n in zip(seqs, counts)]
+        if sum(need) > len(self._free):
+            raise GhostFlowError(_lib.INVALID_SHAPE, f"KV cache is full: {sum(need)} pages needed, {len(self._free)} "
+                                 "free")
+        offsets = [0]
+        for s, n, more in zip(seqs, counts, need):
+            self._pages[s] += [self._free.pop() for _ in range(more)]
+            self._lens[s] += n
+            offsets.append(offsets[-1] + n)
+        lens = [self._lens[s] for s in seqs]
+        width = max([len(self._pages[s]) for s in seqs] + [1])
+        rows = [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in seqs]
+        # one copy to the device
+        flat = torch.tensor(offsets + lens + [p for r in rows for p in r], dtype=torch.int32).to(self.k_pages.device)
+        n = len(seqs)
+        return PagedBatch(flat[2 * n + 1:].view(n, width), flat[:n + 1], flat[n + 1:2 * n + 1], offsets[-1],
+                          max(lens + [0]))
+
+
 class MultiHeadAttention:
     """ghostflow-nn MultiHeadAttention (attention.rs:66-170) on the GPU."""
 
@@ -110,6 +198,7 @@ class MultiHeadAttention:
         self.q_weight, self.k_weight, self.v_weight, self.out_weight = (
             mk((embed_dim, embed_dim), wb) for _ in range(4))
         self.q_bias, self.k_bias, self.v_bias, self.out_bias = (mk((embed_dim,), bb) for _ in range(4))
+        self.w4 = None  # 4-bit projections, after quantize_grouped()
 
     def _weights(self):
         if self.training and self.dropout_p > 0:
@@ -137,6 +226,32 @@ class MultiHeadAttention:
                                mask=mask, causal=causal, want_weights=want_weights)
         cache.length += s
         return r
+
+    def quantize_grouped(self, group_size: int = 128, symmetric: bool = True) -> None:
+        """4-bit projections in groups for step_paged; the other calls keep the
+        fp32 ones."""
+        self.w4 = tuple(GroupQuantizedLinear(w, b, group_size=group_size, symmetric=symmetric) for w, b in
+                        ((self.q_weight, self.q_bias), (self.k_weight, self.k_bias), (self.v_weight, self.v_bias),
+                         (self.out_weight, self.out_bias)))
+
+    def step_paged(self, x, cache: PagedKVCache, batch: PagedBatch, *, cos=None, sin=None, interleaved=False, window=0):
+        """Self-attention of the batch's new tokens x [tokens, E] over their
+        sequences, causal, their keys and values appended to the pages: a
+        prompt's chunks and single tokens in one call.  cos and sin
+        [positions, rotary_dim / 2] turn queries and keys.  fp32, or after
+        quantize_grouped() any type that the cache takes."""
+        weights = self._weights()
+        if x.dim() != 2 or tuple(x.shape) != (batch.tokens, self.embed_dim):
+            raise GhostFlowError(_lib.INVALID_SHAPE, f"x must be [{batch.tokens}, {self.embed_dim}], got {list(x.shape)}")
+        if self.w4 is not None:
+            project = lambda i, t: self.w4[i](t)  # noqa: E731
+        else:
+            project = lambda i, t: linear(t, weights[2 * i], weights[2 * i + 1])  # noqa: E731
+        q, k, v = (project(i, x).view(-1, self.num_heads, self.head_dim) for i in range(3))
+        pages = (cache.k_pages, cache.v_pages, batch.page_table, batch.q_offsets, batch.kv_lens)
+        paged_append(*pages, k, v, q=q, q_out=q, cos=cos, sin=sin, interleaved=interleaved)
+        y = paged_attention(q, *pages, window=window, max_kv_len=batch.max_kv_len, out=q)
+        return project(3, y.view(-1, self.embed_dim))
 
     def parameters(self):
         return [self.q_weight, self.q_bias, self.k_weight, self.k_bias, self.v_weight, self.v_bias,
@@ -191,6 +306,10 @@ class SwiGLU:
         weights per-channel symmetric int8, biases kept in fp32."""
         return QuantizedSwiGLU(self)
 
+    def quantize_grouped(self, group_size: int = 128, symmetric: bool = True) -> "GroupQuantizedSwiGLU":
+        """The block on 4-bit weights in groups."""
+        return GroupQuantizedSwiGLU(self, group_size, symmetric)
+
 
 class QuantizedSwiGLU:
     """SwiGLU with DynamicQuantization's int8 weights: codes [out, in],
@@ -213,5 +332,23 @@ class QuantizedSwiGLU:
         lead = x.shape[:-1]
         y = qswiglu(x.reshape(-1, self.hidden_size).contiguous(), self.gate, self.up, self.down)
         return y.reshape(*lead, self.hidden_size)
+
+    __call__ = forward
+
+
+class GroupQuantizedSwiGLU:
+    """SwiGLU on 4-bit weights in groups (GroupQuantizedLinear), x in fp32."""
+
+    def __init__(self, layer: SwiGLU, group_size: int = 128, symmetric: bool = True):
+        self.hidden_size = layer.hidden_size
+        self.intermediate_size = layer.intermediate_size
+        mk = lambda w, b: GroupQuantizedLinear(w, b, group_size=group_size, symmetric=symmetric)  # noqa: E731
+        self.gate = mk(layer.gate_weight, layer.gate_bias)
+        self.up = mk(layer.up_weight, layer.up_bias)
+        self.down = mk(layer.down_weight, layer.down_bias)
+
+    def forward(self, x):
+        """x [..., hidden] -> [..., hidden]."""
+        return self.down(silu_mul(self.gate(x), self.up(x)))
 
     __call__ = forward

@@ -12,7 +12,8 @@ computed on the device by the bit-exact kernels of quant.hip:
 DynamicQuantization.quantized_linear runs the INT8 linear on its stored
 weights and a dynamically quantized activation (gfh_qlinear_dynamic_i8:
 quantize_activation then gfh_qlinear_i8, one launch at decode sizes) -- the
-layer the reference only expresses as get_weights + fp32 matmul.  FP16 raises NotImplementedError, as the reference's
+layer the reference only expresses as get_weights + fp32 matmul.
+GroupQuantizedLinear is this library's own: 4-bit codes in groups.  FP16 raises NotImplementedError, as the reference's
 unimplemented!() does (quantization.rs:155-158, :167-168).
 """
 from __future__ import annotations
@@ -23,8 +24,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .ops import (GhostFlowError, dequantize, qlinear_dynamic, quantize_per_channel, quantize_per_tensor,
-                  qweight_rowsum)
+from .ops import (GhostFlowError, dequantize, dequantize_grouped_i4, linear_w4, qlinear_dynamic, quantize_grouped_i4,
+                  quantize_per_channel, quantize_per_tensor, qweight_rowsum)
 
 
 class QuantizationScheme(enum.IntEnum):
@@ -131,3 +132,36 @@ class DynamicQuantization:
         y = qlinear_dynamic(x.reshape(-1, x.shape[-1]).contiguous(), q.data, q.scales, self._rowsums[name],
                             bias=bias)
         return y.reshape(*x.shape[:-1], q.shape[0])
+
+
+class GroupQuantizedLinear:
+    """Linear::forward (linear.rs:56-69) on a weight of 4-bit codes in groups
+    of a row (ops.quantize_grouped_i4): beside DynamicQuantization's int8, half
+    its bytes again, for steps whose time is the weights' bytes.  The
+    activations stay what they are (float32, bfloat16 or float16); the bias is
+    rounded to their type."""
+
+    def __init__(self, weight, bias=None, *, group_size=128, symmetric=True):
+        if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+            raise GhostFlowError(_lib.INVALID_SHAPE, f"bias must be [{weight.shape[0]}], got {list(bias.shape)}")
+        self.codes, self.scales, self.zero_points = quantize_grouped_i4(weight, group_size, symmetric)
+        self.out_features, self.in_features = weight.shape
+        self.group_size = group_size
+        self.bias = bias
+
+    def forward(self, x):
+        """x [..., in] -> [..., out]."""
+        y = linear_w4(x.reshape(-1, x.shape[-1]), self.codes, self.scales, self.zero_points,
+                      None if self.bias is None else self.bias.to(x.dtype), group_size=self.group_size)
+        return y.reshape(*x.shape[:-1], self.out_features)
+
+    __call__ = forward
+
+    def dequantize(self):
+        """The weight that forward multiplies by, fp32 [out, in]."""
+        return dequantize_grouped_i4(self.codes, self.scales, self.zero_points, self.group_size)
+
+    def compression_ratio(self) -> float:
+        """fp32 bytes of the weight per byte of codes, scales and zero points."""
+        held = sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zero_points) if t is not None)
+        return 4.0 * self.out_features * self.in_features / held
