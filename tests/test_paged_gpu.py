@@ -321,3 +321,51 @@ def test_captured_step_follows_lengths_and_tables(torch_dev):
         want = gh.paged_attention(qs[0], *P.args(x))
         torch.cuda.synchronize()
         assert torch.equal(got[0], want) and torch.equal(got[1], want), rep
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("q_lens", [[1, 1], [40, 1]])
+def test_pages_whose_offsets_pass_32_bits(torch_dev, types, q_lens):
+    """Pages 2^31 + 64 elements apart: append, then attention, as over pages
+    side by side."""
+    gh = _gh()
+    b = P.batch(q_lens, [45, 9], heads=4, kv_heads=2, d=16, page=16, types=types, seed=30, spare=0, stale=0.0)
+    x = P.to(b, torch_dev)
+    num, far = x["k_pages"].shape[0], 2 ** 31 + 64
+    room = torch.empty((num - 1) * far + 2 * 512, dtype=x["k_pages"].dtype, device=torch_dev)
+    k, v = (room[at:].as_strided(x["k_pages"].shape, (far, 32, 16, 1)) for at in (0, 512))
+    k.copy_(x["k_pages"])
+    v.copy_(x["v_pages"])
+    cos, sin = (t.to(torch_dev) for t in P.angles(x["page_table"].shape[1] * 16, 16))
+    out = []
+    for pages in ((x["k_pages"], x["v_pages"]), (k, v)):
+        rest = (x["page_table"], x["q_offsets"], x["kv_lens"])
+        q = gh.paged_append(*pages, *rest, x["k"], x["v"], q=x["q"], cos=cos, sin=sin)
+        out.append(gh.paged_attention(q, *pages, *rest))
+    assert torch.equal(k, x["k_pages"]) and torch.equal(v, x["v_pages"]) and torch.equal(*out)
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("count", [63, 64, 65, 300])
+def test_many_sequences(torch_dev, types, count):
+    q_lens = [(1, 0, 2, 1, 1)[i % 5] for i in range(count)]
+    kv_lens = [(3, 17, 40, 1, 0)[(i * 7) % 5] + q_lens[i] for i in range(count)]
+    for last in (1, 50):  # decode alone, and with a chunk
+        q_lens[-1], kv_lens[-1] = last, last + 30
+        b = P.batch(q_lens, kv_lens, heads=4, kv_heads=2, d=32, page=16, types=types, seed=31)
+        _check(_attend(torch_dev, b), *P.attention(b))
+
+
+def test_on_another_stream(torch_dev):
+    gh = _gh()
+    b = P.batch([1, 1, 60], [600, 33, 100], heads=8, kv_heads=2, d=64, page=16, types=("bf16", "bf16"), seed=32, stale=0.0)
+    x = P.to(b, torch_dev)
+    want = gh.paged_attention(x["q"], *P.args(x))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    out = []
+    for s in streams:  # calls at once, each with its stream's workspace
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            out.append([gh.paged_attention(x["q"], *P.args(x)) for _ in range(5)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for os in out for o in os)
