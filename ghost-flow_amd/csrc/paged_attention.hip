@@ -60,8 +60,8 @@ struct AttnParams {
     int ntiles, nsplit, chunk;
     int min_rows, max_rows;  // sequences this launch takes: rows = tokens * group
     bool direct;             // see find_rows
-    float *acc;   // [tokens * heads][nsplit][d] parts, where nsplit > 1
-    float2 *ml;   // [tokens * heads][nsplit] their maximum (scaled) and sum
+    float *acc;   // [row][nsplit][d] parts, where nsplit > 1 (see part_row)
+    float2 *ml;   // [row][nsplit] their maximum (scaled) and sum
 };
 
 // A workgroup's rows [r0, r1) and the keys [lo, hi) that any of them sees.
@@ -70,7 +70,13 @@ struct Rows {
     int q_last;         // position of the sequence's token t is t + q_last
     int kv_len;
     int lo, hi;
+    int part;           // row r has its parts at (r + part) * kv_heads + kvh
 };
+
+// Where no sequence of a few-row launch has more than kFewRows rows (p.direct), a
+// sequence has at most kFewTiles tiles and the grid counts those; else it counts
+// tile numbers.  Parts are laid out for as many rows.
+constexpr int kFewRows = 32, kFewTiles = 3;
 
 // Tile `number` of sequence s, whose tokens are [o0, o1) and length kv_len.
 __device__ __forceinline__ bool rows_at(const AttnParams &p, int number, int s, int bm, int o0, int o1, int kv_len,
@@ -82,6 +88,7 @@ __device__ __forceinline__ bool rows_at(const AttnParams &p, int number, int s, 
     t.r1 = min(o1 * c.group, t.base + bm);
     const int rows = (o1 - o0) * c.group;
     if (t.r0 >= t.r1 || rows < p.min_rows || rows > p.max_rows) return false;
+    t.part = p.direct ? s * kFewRows - o0 * c.group : 0;
     t.kv_len = kv_len;
     t.q_last = t.kv_len - o1;
     const int first = t.r0 / c.group + t.q_last, last = (t.r1 - 1) / c.group + t.q_last;
@@ -92,10 +99,7 @@ __device__ __forceinline__ bool rows_at(const AttnParams &p, int number, int s, 
 __device__ __forceinline__ bool rows_of(const AttnParams &p, int number, int s, int bm, Rows &t) {
     return rows_at(p, number, s, bm, paged::offset_at(p.c, s), paged::offset_at(p.c, s + 1), paged::length_at(p.c, s), t);
 }
-// The tile of a workgroup of the few-row launches.  Where no sequence of the
-// launch has more than kFewRows rows (p.direct), a sequence has at most
-// kFewTiles tiles and the grid counts those; else it counts tile numbers.
-constexpr int kFewRows = 32, kFewTiles = 3;
+// The tile of a workgroup and its sequence.
 __device__ __forceinline__ bool find_rows(const AttnParams &p, int number, int bm, int lane, Rows &t, int &s) {
     const View &c = p.c;
     if (p.direct) {
@@ -140,9 +144,8 @@ __device__ __forceinline__ T *out_row(const AttnParams &p, int r, int kvh) {
     const int tok = r / p.c.group, g = r - tok * p.c.group;
     return reinterpret_cast<T *>(p.out) + tok * p.ldo + (int64_t)(kvh * p.c.group + g) * p.c.d;
 }
-__device__ __forceinline__ int64_t part_row(const AttnParams &p, int r, int kvh) {
-    const int tok = r / p.c.group, g = r - tok * p.c.group;
-    return (int64_t)tok * p.c.heads + kvh * p.c.group + g;
+__device__ __forceinline__ int64_t part_row(const AttnParams &p, const Rows &t, int r, int kvh) {
+    return (int64_t)(r + t.part) * p.c.hkv + kvh;
 }
 
 // The rows of a tile one by one, a wave each, over the keys [b, e) that each
@@ -186,7 +189,7 @@ __device__ __forceinline__ void slow_rows(const AttnParams &p, const Rows &t, in
             m = m_new;
         }
         if (parts) {
-            const int64_t at = part_row(p, r, kvh) * p.nsplit + split;
+            const int64_t at = part_row(p, t, r, kvh) * p.nsplit + split;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (lane + 64 * i < c.d) p.acc[at * c.d + lane + 64 * i] = acc[i];
@@ -510,7 +513,7 @@ __device__ __forceinline__ void join_waves(const AttnParams &p, const Rows &t, i
             A += *reinterpret_cast<const f32x4 *>(accs + (w * 16 + row) * kRow + dim) * f;
         }
         if (parts) {
-            const int64_t at = part_row(p, rr, kvh) * p.nsplit + split;
+            const int64_t at = part_row(p, t, rr, kvh) * p.nsplit + split;
             *reinterpret_cast<f32x4 *>(p.acc + at * p.c.d + dim) = A;
             if (dim == 0) p.ml[at] = make_float2(M, L);
         } else {
@@ -692,7 +695,7 @@ __device__ __forceinline__ void store_rows(const AttnParams &p, const Rows &t, i
     const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
     if (r < t.r0 || r >= t.r1) return;
-    const int64_t at = parts ? part_row(p, r, kvh) * p.nsplit + split : 0;
+    const int64_t at = parts ? part_row(p, t, r, kvh) * p.nsplit + split : 0;
     const float f = parts ? 1.f : m == -INFINITY ? 0.f : 1.0f / l;
     if (parts && h == 0) p.ml[at] = make_float2(m == -INFINITY ? m : m * p.sc2, l);
     TA *const row = out_row<TA>(p, r, kvh);
@@ -1107,7 +1110,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(AttnParams p, int bm) {
     if (!rows_of(p, r / bm + s, s, bm, t)) return;
     const int nact = active_splits(p, t);
     if (nact <= 1) return;
-    const int64_t at = part_row(p, r, kvh) * p.nsplit;
+    const int64_t at = part_row(p, t, r, kvh) * p.nsplit;
     // the largest maximum: 64 splits at a time
     float M = -INFINITY;
     for (int i = lane; i < nact; i += 64) M = max_nan(M, p.ml[at + i].x);
@@ -1143,6 +1146,7 @@ struct Plan {
     bool wide;    // the few-row launch has wide workgroups
     int few_max;  // rows of the longest sequence the few-row launch takes
     int few_split, few_chunk, chunk_split, chunk_chunk;
+    int64_t few_parts, chunk_parts;  // rows of parts
     int64_t part_floats;
 };
 
@@ -1187,10 +1191,13 @@ Plan make_plan(const PagedAttnDesc &d) {
               (d.window > 0 ? std::min(d.max_kv_len, d.window + 15) : d.max_kv_len) <= wide_keys;
     if (pl.wide) pl.few_split = 1;
     cut(rows / 128 + 1, 2 * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
-    int64_t most = 1;
-    if (pl.few) most = std::max<int64_t>(most, pl.few_split);
-    if (pl.chunk) most = std::max<int64_t>(most, pl.chunk_split);
-    pl.part_floats = most > 1 ? d.tokens * d.heads * most * (d.kv.head_dim + 2) : 0;
+    auto floats = [&](bool on, int64_t nsplit, int64_t part_rows) {
+        return on && nsplit > 1 ? part_rows * nsplit * (d.kv.head_dim + 2) : 0;
+    };
+    // (one launch after the other uses them)
+    pl.few_parts = (pl.chunk ? d.kv.num_seqs * kFewRows : rows) * d.kv.kv_heads;
+    pl.chunk_parts = rows * d.kv.kv_heads;
+    pl.part_floats = std::max(floats(pl.few, pl.few_split, pl.few_parts), floats(pl.chunk, pl.chunk_split, pl.chunk_parts));
     return pl;
 }
 
@@ -1233,12 +1240,12 @@ int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t 
     p.causal = d.causal;
     p.window = d.window >= p.c.capacity ? 0 : (int)d.window;
     const int64_t rows = d.tokens * p.c.group;
-    auto run = [&](int bm, int nsplit, int chunk, int min_rows, int max_rows, auto &&kernel) -> int {
+    auto run = [&](int bm, int nsplit, int chunk, int64_t parts, int min_rows, int max_rows, auto &&kernel) -> int {
         p.direct = max_rows == kFewRows;
         p.ntiles = p.direct ? kFewTiles * (int)d.kv.num_seqs : (int)((rows - 1) / bm + d.kv.num_seqs);
         p.nsplit = nsplit, p.chunk = chunk, p.min_rows = min_rows, p.max_rows = max_rows;
         p.acc = static_cast<float *>(workspace);
-        p.ml = reinterpret_cast<float2 *>(p.acc + d.tokens * d.heads * nsplit * d.kv.head_dim);
+        p.ml = reinterpret_cast<float2 *>(p.acc + parts * nsplit * d.kv.head_dim);
         const int64_t blocks = (int64_t)p.ntiles * p.c.hkv * nsplit;
         if (blocks > (int64_t)1 << 23) return set_error(GFH_INVALID_SHAPE, "paged_attention: grid too large");
         kernel(dim3((unsigned)blocks));
@@ -1309,8 +1316,8 @@ int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t 
         else
             go(_Float16{}, _Float16{}, One{});
     };
-    if (pl.chunk) GFH_TRY(run(128, pl.chunk_split, pl.chunk_chunk, pl.few ? pl.few_max + 1 : 0, kAll, many));
-    if (pl.few) GFH_TRY(run(16, pl.few_split, pl.few_chunk, 0, pl.few_max, few));
+    if (pl.chunk) GFH_TRY(run(128, pl.chunk_split, pl.chunk_chunk, pl.chunk_parts, pl.few ? pl.few_max + 1 : 0, kAll, many));
+    if (pl.few) GFH_TRY(run(16, pl.few_split, pl.few_chunk, pl.few_parts, 0, pl.few_max, few));
     return GFH_SUCCESS;
 }
 
