@@ -39,6 +39,26 @@ def test_quantize_and_back(torch_dev, n, k, group, symmetric):
     assert (back - w).abs().le(step * (0.5 if symmetric else 1.0) * (1 + 2 ** -20)).all()
 
 
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_quantize_ties_and_their_neighbours(torch_dev, symmetric):
+    """Values at, next to and near half steps, for scales from 2^-140 to 2^120."""
+    gh = _gh()
+    g = torch.Generator().manual_seed(12)
+    rows = []
+    for e in (-140, -126, -101, -100, -99, -20, 0, 3, 60, 99, 100, 101, 120):
+        top = (torch.rand(1, generator=g) + 1) * 7 * 2.0 ** e
+        s = top * torch.tensor(1 / 7, dtype=torch.float32) if symmetric else top * torch.tensor(1 / 15, dtype=torch.float32)
+        half = (torch.arange(-7, 7) + 0.5 if symmetric else torch.arange(0, 14) + 0.5) * s
+        up, down = (torch.nextafter(half, torch.full_like(half, d)) for d in (torch.inf, -torch.inf))
+        near = half * (1 + (torch.rand(64 - 42 - 1, 14, generator=g)[0] - 0.5) * 2.0 ** -14)
+        w = torch.cat((top, half, up, down, near))
+        rows.append(torch.nn.functional.pad(w, (0, 64 - len(w))))
+    w = torch.stack(rows)
+    got = gh.quantize_grouped_i4(w.to(torch_dev), 64, symmetric=symmetric)
+    for a, b in zip(got, W.quantize(w, 64, symmetric)):
+        assert (a is None) == (b is None) and (a is None or torch.equal(a.cpu(), b))
+
+
 def test_quantize_borders_and_nan(torch_dev):
     gh = _gh()
     w = torch.zeros(4, 32)
