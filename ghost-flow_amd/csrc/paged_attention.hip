@@ -924,17 +924,22 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(AttnParams p) {
 
 // ---- fp32 cache -------------------------------------------------------------------
 //
-// A tile of 16 rows, four waves that take 16-key tiles in turn, K and V straight
-// into registers (the next tile's while this one is computed) and both products
-// on f32 MFMA (16x16x4).  K: lane (c, h) loads dims 16 u + 4 h .. + 3 of key c,
-// and product e of step u takes dim 16 u + 4 h + e of quarter h on both sides.
-// V: lane (c, h) loads dims 64 v + 4 c .. + 3 of key 4 h + x; product (v, e, x)
-// takes dim 64 v + 4 i + e as its row i.
+// A tile of 16 rows, four waves that take 16-key tiles in turn and both products
+// on f32 MFMA (16x16x4).  K: whole rows straight to LDS, a ring of two tiles per
+// wave; product e of step u takes dim 16 u + 4 h + e of quarter h on both sides.
+// V straight into registers, 256 bytes of a row at once: lane (c, h) loads dims 64 v
+// + 4 c .. + 3 of key 4 h + x, and product (v, e, x) takes dim 64 v + 4 i + e as its
+// row i.  The next tile is on its way while this one is computed.
+//
+// Bound by bytes: 4 sequences of 1314 .. 2047 keys, 32 heads of 128, 213 MB: 50 us
+// (4.3 TB/s) and 4.7 to join.  K in registers as well was 53.
 template <int DP>
 __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
     constexpr int NU = DP / 16, NV = DP / 64, kRow = DP + 4;
-    constexpr int kStates = 4 * 16 * kRow * 4;
-    __shared__ __attribute__((aligned(16))) char lds[kStates + 4 * 16 * 8 + kMaxPages * 8 + 64];
+    constexpr int kTile = 16 * DP * 4, kStates = 4 * 2 * kTile;  // K of four waves, two tiles each; then the states
+    static_assert(kStates >= 4 * 16 * kRow * 4, "the states fit");
+    constexpr int kPer = 256 / DP, kInstr = 16 / kPer;  // rows per request, requests per tile
+    __shared__ __attribute__((aligned(1024))) char lds[kStates + 4 * 16 * 8 + kMaxPages * 8 + 64];
     float *const accs = reinterpret_cast<float *>(lds);
     float2 *const mls = reinterpret_cast<float2 *>(lds + kStates);
     int64_t *const pages = reinterpret_cast<int64_t *>(lds + kStates + 4 * 16 * 8);
@@ -979,8 +984,9 @@ __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
     bool odd = false;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     struct Tile {
-        f32x4 k[NU], v[4][NV];
+        f32x4 v[4][NV];
     };
+    char *const ring = lds + wave * 2 * kTile;
     for (int pb = b; pb < e;) {
         const int p0 = paged::page_of(cc, pb);
         __syncthreads();
@@ -995,13 +1001,14 @@ __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
                        : -1;
         };
         const f32x4 *const zeros = reinterpret_cast<const f32x4 *>(g_zero_chunk);
-        auto load = [&](int k0, Tile &f) __attribute__((always_inline)) {
-            const int64_t ka = row_at(k0 + c);
+        auto load = [&](int k0, Tile &f, char *to) __attribute__((always_inline)) {
 #pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                const int dim = 16 * u + 4 * h;
-                f.k[u] = __builtin_nontemporal_load(
-                    ka >= 0 && dim < cc.d ? reinterpret_cast<const f32x4 *>(cc.k + ka + 4 * dim) : zeros);
+            for (int i = 0; i < kInstr; ++i) {
+                const int row = i * kPer + lane / (DP / 4), ch = lane % (DP / 4) ^ row;
+                const int64_t ka = row_at(k0 + row);
+                const char *const from = ka >= 0 && 4 * ch < cc.d ? cc.k + ka + 16 * ch
+                                                                  : reinterpret_cast<const char *>(g_zero_chunk);
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)from, (lds_ptr_t)(to + i * 1024), 16, 0, kNtHint);
             }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -1014,20 +1021,22 @@ __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
                 }
             }
         };
-        Tile now, next;
         int k0 = pb + 16 * wave;
-        if (k0 < pe) load(k0, next);
-#pragma unroll 1
-        for (; k0 < pe; k0 += 64) {
-            now = next;
+        // (two tiles in turn, without a copy that would wait for the next one)
+        auto step = [&](const Tile &now, Tile &next, int st) __attribute__((always_inline)) {
             __builtin_amdgcn_sched_barrier(0);
-            load(k0 + 64, next);
+            load(k0 + 64, next, ring + (st ^ 1) * kTile);
             __builtin_amdgcn_sched_barrier(0);
+            wait_vm<kInstr + 4 * NV>();
+            __builtin_amdgcn_sched_barrier(0);
+            const char *const kt = ring + st * kTile + c * DP * 4;
             f32x4 s = zero;
 #pragma unroll
-            for (int u = 0; u < NU; ++u)
+            for (int u = 0; u < NU; ++u) {
+                const f32x4 kf = *reinterpret_cast<const f32x4 *>(kt + (((4 * u + h) ^ c) << 4));
 #pragma unroll
-                for (int x = 0; x < 4; ++x) s = __builtin_amdgcn_mfma_f32_16x16x4f32(now.k[u][x], qv[u][x], s, 0, 0, 0);
+                for (int x = 0; x < 4; ++x) s = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[x], qv[u][x], s, 0, 0, 0);
+            }
             if (k0 < all_lo || k0 + 16 > min(all_hi, pe)) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
@@ -1061,7 +1070,17 @@ __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
 #pragma unroll
                     for (int y = 0; y < 4; ++y)
                         o[v][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(now.v[x][v][y], s[x], o[v][y], 0, 0, 0);
+            k0 += 64;
+        };
+        Tile even, odds;
+        if (k0 < pe) load(k0, even, ring);
+#pragma unroll 1
+        while (k0 < pe) {
+            step(even, odds, 0);
+            if (k0 >= pe) break;
+            step(odds, even, 1);
         }
+        wait_vm<0>();  // nothing is on its way into the ring
         pb = pe;
     }
     l = quarter_sum(l);
