@@ -532,6 +532,10 @@ __device__ __forceinline__ void join_waves(const AttnParams &p, const Rows &t, i
 // on 16x16x32: lane (c = l % 16, h = l / 16) holds keys 16 kb + 4 h + r of row
 // c, which are its B operand of O^T = V^T . P^T when V^T takes the keys in the
 // same order (two transposing reads: keys 4 h .., 16 + 4 h ..).
+//
+// Bound by bytes: 64 sequences of 1024 .. 4096 keys, 32 heads over 8 of 128, bf16,
+// 659 MB: 126 us (5.2 TB/s) and 4.9 to join; the matrix units have 16 rows for the
+// group's 4 and are busy 4% of the cycles.
 template <typename TA, typename T, int DP, int NP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) {
     using H = Half<T>;
@@ -730,9 +734,9 @@ __device__ __forceinline__ void store_rows(const AttnParams &p, const Rows &t, i
 //   the maximum followed at every tile, weights added singly    564 us
 //   the maximum followed late                                   560
 //   16-bit weights added in pairs (l sums what the product sees) 544
-//   products at the higher issue priority                       525, 980 TFLOP/s
+//   products at the higher issue priority              514 .. 525, 1 PFLOP/s at best
 //   f32: one workgroup per CU, fragments two ahead              168
-//   f32: two per CU (q's pieces in 96 registers, one ahead)     131
+//   f32: two per CU (q's pieces in 96 registers, one ahead)     119
 // Eight waves in two groups that alternate between products and softmax by
 // barriers were no faster (559 against 564).
 template <typename TA, typename T, int DP, int ND, int NP>
@@ -931,8 +935,8 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(AttnParams p) {
 // + 4 c .. + 3 of key 4 h + x, and product (v, e, x) takes dim 64 v + 4 i + e as its
 // row i.  The next tile is on its way while this one is computed.
 //
-// Bound by bytes: 4 sequences of 1314 .. 2047 keys, 32 heads of 128, 213 MB: 50 us
-// (4.3 TB/s) and 4.7 to join.  K in registers as well was 53.
+// Bound by bytes: 4 sequences of 1314 .. 2047 keys, 32 heads of 128, 213 MB: 49 us
+// (4.4 TB/s) and 4.7 to join.  K in registers as well was 53.
 template <int DP>
 __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
     constexpr int NU = DP / 16, NV = DP / 64, kRow = DP + 4;
@@ -1172,7 +1176,7 @@ struct Plan {
 // Waves of a few-row workgroup: two, so that two or more workgroups share a CU;
 // as many as the LDS takes where there are too few tiles to fill the CUs and a
 // length that such a workgroup walks in a few steps: no split and no second launch
-// (12 heads of 64 over 517 keys, f16: 8.6 us and 3.9 to join -> 9.2).
+// (12 heads of 64 over 517 keys, f16: 8.6 us and 3.9 to join -> 9.4).
 constexpr int kDecodeWaves = 2, kWideWaves64 = 8, kWideWaves128 = 4;
 constexpr int kWideKeys = 96;  // per wave
 constexpr int kAll = INT32_MAX;
@@ -1200,8 +1204,8 @@ Plan make_plan(const PagedAttnDesc &d) {
     };
     const int64_t few_tiles = std::min(d.kv.num_seqs, d.tokens) + (pl.chunk ? 0 : rows / 16);
     // Workgroups of the few-row launch.  fp32: at least 384 keys each, four waves
-    // (4 sequences of up to 2047 keys, 32 heads of 128, us of the kernel by keys:
-    // 256 64.7, 384 53.2, 512 58.1).  16 bits: at least 128 keys each, six times as
+    // (4 sequences of up to 2047 keys, 32 heads of 128, us of a call by keys:
+    // 256 64, 384 54, 512 58, 768 75).  16 bits: at least 128 keys each, six times as
     // many as fit at once, for even ends (64 sequences of up to 4096 keys, 8 heads of
     // 128: twice as many 148, four times 132, six times 125, eight times 131).
     cut(few_tiles, (f32 ? 4 : 12) * cus, f32 ? 384 : 128, 64, pl.few_split, pl.few_chunk);
