@@ -222,13 +222,15 @@ GFH_API int gfh_dequantize_i4_grouped(const uint8_t *codes, const float *scales,
 /* Linear on such a weight: y[m, n] = x[m, k] . w'^T + bias[n], the codes taken
  * apart in registers.  x, bias (nullable) and y are of type dtype, rows of x
  * ldx and of y ldy elements apart.  Products of x with (c - z) in fp32, a
- * group's sum times its scale, sums in fp32, y rounded once.  fp32 x is carried
- * with all its bits for m <= 4 and above with at least 33 bits below the largest
- * magnitude of its row in each 256 columns; bf16 likewise (8 bits down to 2^-29
- * of that).  An infinite or NaN x gives inf / NaN.  Meant for few rows (decode);
- * any m is served.  y overlaps no input.
+ * group's sum times its scale, sums in fp32, y rounded once (3 .. 16 rows of bf16:
+ * a group's sum of c x less z times its sum of x).  fp32 x is carried with all
+ * its bits for m <= 4 and above with at least 33 bits below the largest magnitude
+ * of its row in each 256 columns; bf16 above 16 rows likewise (8 bits down to
+ * 2^-29 of that).  An infinite or NaN x gives inf / NaN.  Meant for few rows
+ * (decode); any m is served.  y overlaps no input.
  * workspace (nullable, 16-byte aligned) of at least
- * gfh_linear_w4_workspace_size(...) bytes; any contents. */
+ * gfh_linear_w4_workspace_size(...) bytes, with or without zero points and for
+ * any strides; any contents. */
 GFH_API size_t gfh_linear_w4_workspace_size(int dtype, int64_t m, int64_t n, int64_t k, int64_t group);
 GFH_API int gfh_linear_w4(int dtype, const void *x, int64_t ldx, const uint8_t *codes,
                           const float *scales, const uint8_t *zero_points, const void *bias,
