@@ -863,7 +863,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(AttnParams p) {
             // The maximum moves on only when some row's is 2^kLate behind: weights then
             // reach 2^(kBias + kLate), within fp16's range too, and most tiles leave
             // the sums unscaled.
-            if (__any(!((m_new - m) * p.sc2 <= kLate))) {
+            if (__any(!((m_new - m) * p.sc2 <= kLate) && m_new != -INFINITY)) {
                 const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * p.sc2);
                 l *= alpha;
 #pragma unroll

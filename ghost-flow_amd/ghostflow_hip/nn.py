@@ -238,8 +238,9 @@ class MultiHeadAttention:
         """Self-attention of the batch's new tokens x [tokens, E] over their
         sequences, causal, their keys and values appended to the pages: a
         prompt's chunks and single tokens in one call.  cos and sin
-        [positions, rotary_dim / 2] turn queries and keys.  fp32, or after
-        quantize_grouped() any type that the cache takes."""
+        [positions, rotary_dim / 2] turn queries and keys; they cover whole
+        pages of the longest sequence.  fp32, or after quantize_grouped() any
+        type that the cache takes."""
         weights = self._weights()
         if x.dim() != 2 or tuple(x.shape) != (batch.tokens, self.embed_dim):
             raise GhostFlowError(_lib.INVALID_SHAPE, f"x must be [{batch.tokens}, {self.embed_dim}], got {list(x.shape)}")
