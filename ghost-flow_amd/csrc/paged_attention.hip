@@ -1214,6 +1214,13 @@ Plan make_plan(const PagedAttnDesc &d) {
               (d.window > 0 ? std::min(d.max_kv_len, d.window + 15) : d.max_kv_len) <= wide_keys;
     if (pl.wide) pl.few_split = 1;
     cut(rows / 128 + 1, 2 * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
+    // Sequences of few rows go along in the chunk launch where they are few beside
+    // its tiles and have few keys to walk (f32 over bf16 / bf16, us of a call, two
+    // launches and one): 2048 tokens and 7 single ones of 2048 keys 148 / 90 -> 123 /
+    // 63, 1024 and 63 of 1000 keys 153 / 129 -> 136 / 101, 512 and 3 of 2000 keys 60 /
+    // 47 -> 59 / 40; but 2000 and one of 8000 keys 148 / 88 -> 337 / 172.
+    const int64_t sees = d.window > 0 ? std::min(d.max_kv_len, d.window + 127) : d.max_kv_len;
+    if (pl.chunk && 64 * d.kv.num_seqs <= rows && std::min<int64_t>(sees, pl.chunk_chunk) <= 2048) pl.few = false;
     auto floats = [&](bool on, int64_t nsplit, int64_t part_rows) {
         return on && nsplit > 1 ? part_rows * nsplit * (d.kv.head_dim + 2) : 0;
     };

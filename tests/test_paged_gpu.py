@@ -43,6 +43,7 @@ LENS = [
     ([5, 0, 1, 3], [5, 40, 65, 300]),
     ([70, 1, 33], [70, 260, 100]),
     ([200], [1000]),
+    ([300, 1, 2, 0, 130], [900, 700, 40, 5, 130]),
     ([0, 0, 2, 0], [10, 0, 9, 0]),
     ([4, 9], [2, 0]),
 ]
