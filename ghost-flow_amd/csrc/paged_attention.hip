@@ -926,6 +926,19 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(AttnParams p) {
     store_rows<TA, NB>(p, t, kvh, r, h, split, nact > 1, m, l, o);
 }
 
+// Row r of q, dims 16 u + 4 h .. + 3 per step u; zeros for rows outside the tile.
+template <int NU>
+__device__ __forceinline__ void load_q_f32(const AttnParams &p, const Rows &t, int r, int kvh, int h, f32x4 (&qv)[NU]) {
+    const bool ok = r >= t.r0 && r < t.r1;
+    const float *q = q_row<float>(p, ok ? r : t.r0, kvh);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+        const int dim = 16 * u + 4 * h;
+        const f32x4 x = *reinterpret_cast<const f32x4 *>(q + (dim < p.c.d ? dim : 0));
+        qv[u] = ok && dim < p.c.d ? (p.negate ? -x : x) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+}
+
 // ---- fp32 cache -------------------------------------------------------------------
 //
 // A tile of 16 rows, four waves that take 16-key tiles in turn and both products
@@ -963,17 +976,8 @@ __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
     const int r = t.base + c;
     int jmin, jmax;
     row_keys(p, t, r, jmin, jmax);
-    const bool row_ok = r >= t.r0 && r < t.r1;
     f32x4 qv[NU];
-    {
-        const float *q = q_row<float>(p, row_ok ? r : t.r0, kvh);
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const int dim = 16 * u + 4 * h;
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(q + (dim < cc.d ? dim : 0));
-            qv[u] = row_ok && dim < cc.d ? (p.negate ? -x : x) : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-    }
+    load_q_f32<NU>(p, t, r, kvh, h, qv);
     int x0, x1, y0, y1;
     row_keys(p, t, t.r0, x0, x1);
     row_keys(p, t, t.r1 - 1, y0, y1);
@@ -1104,6 +1108,169 @@ __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
     join_waves<float, DP, 4>(p, t, kvh, split, nact > 1, accs, mls, tid);
 }
 
+// Prompts: a tile of 64 rows, four waves of 16, K and V tiles of 32 keys in two
+// stages that all waves read, the same products as above.  Bound by the f32 matrix
+// units: 2048 tokens of 32 heads over 8 of 128, causal, 34 GFLOP 365 us (94 TFLOP/s);
+// with 16 rows per workgroup 741, bound by the keys' way from L2.
+template <int DP>
+__global__ __launch_bounds__(256, 2) void paged_f32_chunk_kernel(AttnParams p) {
+    constexpr int NU = DP / 16, NV = DP / 64, kTile = 32 * DP * 4;
+    constexpr int kPer = 256 / DP, kInstr = 32 / kPer / 4;  // rows per request, requests per tile and wave
+    __shared__ __attribute__((aligned(1024))) char lds[4 * kTile + kMaxPages * 8 + 64];  // stage, K / V; pages; flags
+    int64_t *const pages = reinterpret_cast<int64_t *>(lds + 4 * kTile);
+    int *const flags = reinterpret_cast<int *>(lds + 4 * kTile + kMaxPages * 8);
+    const View &cc = p.c;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 15, h = lane >> 4;
+    const int id = xcd_chunked(blockIdx.x, gridDim.x);
+    const int number = p.ntiles - 1 - id % p.ntiles, rest = id / p.ntiles;
+    const int split = rest % p.nsplit, kvh = rest / p.nsplit;
+    Rows t;
+    int seq;
+    if (!find_rows(p, number, 64, lane, t, seq)) return;
+    const int nact = active_splits(p, t);
+    if (split >= nact) return;
+    const int b = t.lo + split * p.chunk, e = split == nact - 1 ? t.hi : b + p.chunk;
+    const int r = t.base + 16 * wave + c;
+    int jmin, jmax;
+    row_keys(p, t, r, jmin, jmax);
+    f32x4 qv[NU];
+    load_q_f32<NU>(p, t, r, kvh, h, qv);
+    // this wave's rows, the keys that any and that all of them see
+    const int w0 = max(t.r0, t.base + 16 * wave), w1 = min(t.r1, t.base + 16 * wave + 16);
+    const bool live = w0 < w1;
+    int any_lo, any_hi, all_lo, all_hi;
+    row_keys(p, t, live ? w0 : t.r0, any_lo, all_hi);
+    row_keys(p, t, live ? w1 - 1 : t.r0, all_lo, any_hi);
+    ++all_hi, ++any_hi;
+
+    f32x4 o[NV][4];
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[v][x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    bool odd = false;
+    for (int pb = b; pb < e;) {
+        const int p0 = paged::page_of(cc, pb);
+        __syncthreads();
+        const int pe = stage_pages(cc, seq, pb, e, 4, pages, tid, 256);
+        __syncthreads();
+        const int n = (pe - pb + 31) / 32;
+        auto ask = [&](int k0, char *to) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < kInstr; ++i) {
+                const int ins = wave * kInstr + i;
+                const int row = ins * kPer + lane / (DP / 4), ch = (lane % (DP / 4)) ^ (row & 15);
+                const int key = min(k0 + row, pe - 1), pg = paged::page_of(cc, key);
+                const int64_t off = pages[pg - p0];
+                const int64_t at = off + 4 * ((int64_t)(key - pg * cc.page_size) * cc.row_stride + kvh * cc.head_stride);
+                const bool ok = k0 + row < pe && off >= 0 && 4 * ch < cc.d;
+                const char *const zero = reinterpret_cast<const char *>(g_zero_chunk);
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)(ok ? cc.k + at + 16 * ch : zero), (lds_ptr_t)(to + ins * 1024),
+                                                 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((glb_ptr_t)(ok ? cc.v + at + 16 * ch : zero),
+                                                 (lds_ptr_t)(to + kTile + ins * 1024), 16, 0, 0);
+            }
+        };
+        ask(pb, lds);
+        for (int i = 0; i < n; ++i) {
+            const int k0 = pb + 32 * i, st = i & 1;
+            // the tile is there, and every wave is done with the one before
+            wait_vm<0>();
+            __syncthreads();
+            if (i + 1 < n) ask(k0 + 32, lds + (st ^ 1) * 2 * kTile);
+            if (!live || k0 >= any_hi || k0 + 32 <= any_lo) continue;
+            const char *const kt = lds + st * 2 * kTile, *const vt = kt + kTile;
+            f32x4 s[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                f32x4 kf[2];
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    kf[kb] = *reinterpret_cast<const f32x4 *>(kt + (16 * kb + c) * DP * 4 + (((4 * u + h) ^ c) << 4));
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+                        s[kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[kb][x], qv[u][x], s[kb], 0, 0, 0);
+            }
+            if (k0 < all_lo || k0 + 32 > min(all_hi, pe)) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int j = k0 + 16 * kb + 4 * h + x;
+                        s[kb][x] = j >= jmin && j <= jmax && j < pe ? s[kb][x] : -INFINITY;
+                    }
+#pragma unroll 4
+                for (int x = 0; x < kTile / 1024; ++x) {
+                    const f32x4 w = *reinterpret_cast<const f32x4 *>(vt + (x * 64 + lane) * 16);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) odd |= !(fabsf(w[y]) < INFINITY);
+                }
+            }
+            const float m_new =
+                max_nan(m, quarter_max_nan(max_nan(max_nan(max_nan(s[0][0], s[0][1]), max_nan(s[0][2], s[0][3])),
+                                                   max_nan(max_nan(s[1][0], s[1][1]), max_nan(s[1][2], s[1][3])))));
+            // (late, as in the 16-bit chunk kernel)
+            if (__any(!((m_new - m) * p.sc2 <= 8.f) && m_new != -INFINITY)) {
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((m - m_new) * p.sc2);
+                l *= alpha;
+#pragma unroll
+                for (int v = 0; v < NV; ++v)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) o[v][y] *= alpha;
+                m = m_new;
+            }
+            const float mc = m == -INFINITY ? 0.f : m * p.sc2;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    s[kb][x] = __builtin_amdgcn_exp2f(fmaf(s[kb][x], p.sc2, -mc));
+                    l += s[kb][x];
+                }
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int v = 0; v < NV; ++v) {
+                        const int key = 4 * h + x;
+                        const f32x4 vf = *reinterpret_cast<const f32x4 *>(vt + (16 * kb + key) * DP * 4 +
+                                                                          (((16 * v + c) ^ key) << 4));
+#pragma unroll
+                        for (int y = 0; y < 4; ++y)
+                            o[v][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[y], s[kb][x], o[v][y], 0, 0, 0);
+                    }
+        }
+        pb = pe;
+    }
+    l = quarter_sum(l);
+    if (any_wave<4>(odd, flags, wave, lane)) {
+        slow_rows<float, float>(p, t, seq, kvh, b, e, split, nact > 1, 0.f, wave, 4, lane);
+        return;
+    }
+    if (r < t.r0 || r >= t.r1) return;
+    const bool parts = nact > 1;
+    const int64_t at = parts ? part_row(p, t, r, kvh) * p.nsplit + split : 0;
+    const float f = parts ? 1.f : m == -INFINITY ? 0.f : 1.0f / l;
+    if (parts && h == 0) p.ml[at] = make_float2(m == -INFINITY ? m : m * p.sc2, l);
+    float *const row = parts ? p.acc + at * cc.d : out_row<float>(p, r, kvh);
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int dim = 64 * v + 16 * h + 4 * x;
+            if (dim < cc.d)
+                *reinterpret_cast<f32x4 *>(row + dim) = f32x4{o[v][0][x], o[v][1][x], o[v][2][x], o[v][3][x]} * f;
+        }
+}
+
 // ---- the parts of split rows, in their order ------------------------------------------
 
 // A wave per (token, head), or per row that a sequence of a direct launch can
@@ -1168,6 +1335,7 @@ struct Plan {
     bool few, chunk;
     bool wide;    // the few-row launch has wide workgroups
     int few_max;  // rows of the longest sequence the few-row launch takes
+    int chunk_rows;  // of a tile
     int few_split, few_chunk, chunk_split, chunk_chunk;
     int64_t few_parts, chunk_parts;  // rows of parts
     int64_t part_floats;
@@ -1187,10 +1355,14 @@ Plan make_plan(const PagedAttnDesc &d) {
     const int64_t rows = d.tokens * group;
     const bool f32 = d.kv.dtype == GFH_F32;
     pl.few_max = kFewRows;
-    pl.few = f32 || d.kv.num_seqs > 1 || rows <= pl.few_max;
-    pl.chunk = !f32 && rows > pl.few_max && d.tokens > d.kv.num_seqs;
-    if (!pl.chunk) pl.few_max = kAll;
     const int64_t cus = device_cu_count();
+    // fp32: tiles of 64 rows where they fill the CUs (us of a call, 16 rows / 64: 32
+    // heads over 8 of 128, a prompt of 128 tokens over 500 keys 34 / 56, 512 64 / 57,
+    // 2048 741 / 365, eight of 300 over 600 keys 420 / 238).
+    pl.chunk_rows = f32 ? 64 : 128;
+    pl.chunk = rows > pl.few_max && d.tokens > d.kv.num_seqs && (!f32 || rows * d.kv.kv_heads >= pl.chunk_rows * cus);
+    pl.few = !pl.chunk || d.kv.num_seqs > 1;
+    if (!pl.chunk) pl.few_max = kAll;
     auto cut = [&](int64_t tiles, int64_t target, int64_t least, int64_t unit, int &nsplit, int &chunk) {
         const int64_t items = std::max<int64_t>(1, tiles * d.kv.kv_heads);
         // keys that a tile sees at most
@@ -1213,7 +1385,7 @@ Plan make_plan(const PagedAttnDesc &d) {
     pl.wide = !f32 && pl.few_split > 1 && few_tiles * d.kv.kv_heads <= cus &&
               (d.window > 0 ? std::min(d.max_kv_len, d.window + 15) : d.max_kv_len) <= wide_keys;
     if (pl.wide) pl.few_split = 1;
-    cut(rows / 128 + 1, 2 * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
+    cut(rows / pl.chunk_rows + 1, (f32 ? 4 : 2) * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
     // Sequences of few rows go along in the chunk launch where they are few beside
     // its tiles and have few keys to walk (f32 over bf16 / bf16, us of a call, two
     // launches and one): 2048 tokens and 7 single ones of 2048 keys 148 / 90 -> 123 /
@@ -1339,14 +1511,20 @@ int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t 
         };
         using One = std::integral_constant<int, 1>;
         using Three = std::integral_constant<int, 3>;
-        if (d.dtype == GFH_F32)
+        if (d.kv.dtype == GFH_F32) {
+            if (hd <= 64)
+                hipLaunchKernelGGL(paged_f32_chunk_kernel<64>, grid, dim3(256), 0, s, p);
+            else
+                hipLaunchKernelGGL(paged_f32_chunk_kernel<128>, grid, dim3(256), 0, s, p);
+        } else if (d.dtype == GFH_F32)
             go(float{}, __bf16{}, Three{});
         else if (d.dtype == GFH_BF16)
             go(__bf16{}, __bf16{}, One{});
         else
             go(_Float16{}, _Float16{}, One{});
     };
-    if (pl.chunk) GFH_TRY(run(128, pl.chunk_split, pl.chunk_chunk, pl.chunk_parts, pl.few ? pl.few_max + 1 : 0, kAll, many));
+    if (pl.chunk)
+        GFH_TRY(run(pl.chunk_rows, pl.chunk_split, pl.chunk_chunk, pl.chunk_parts, pl.few ? pl.few_max + 1 : 0, kAll, many));
     if (pl.few) GFH_TRY(run(16, pl.few_split, pl.few_chunk, pl.few_parts, 0, pl.few_max, few));
     return GFH_SUCCESS;
 }

@@ -47,7 +47,7 @@ LENS = [
     ([0, 0, 2, 0], [10, 0, 9, 0]),
     ([4, 9], [2, 0]),
 ]
-HEADS = [(4, 4, 64), (8, 2, 128), (6, 1, 80), (3, 3, 8), (40, 2, 32), (7, 1, 128), (2, 2, 96)]
+HEADS = [(4, 4, 64), (8, 2, 128), (6, 1, 80), (3, 3, 8), (40, 2, 32), (7, 1, 128), (2, 2, 96), (40, 1, 64)]
 
 
 @pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
@@ -64,6 +64,38 @@ def test_attention_heads(torch_dev, types, heads):
     h, hkv, d = heads
     b = P.batch([1, 40, 3], [300, 90, 77], heads=h, kv_heads=hkv, d=d, page=16, types=types, seed=2)
     _check(_attend(torch_dev, b), *P.attention(b))
+
+
+# prompts of many heads, which fill the GPU with the tiles of fp32 prompts too
+MANY = dict(heads=32, kv_heads=32, page=24, pad=2)
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("d,causal,window", [(8, True, 90), (64, True, 0), (104, False, 0), (128, True, 0), (128, True, 90)])
+def test_attention_of_prompts_of_many_heads(torch_dev, types, d, causal, window):
+    b = P.batch([300, 1, 40, 180, 0], [1100, 50, 300, 180, 9], d=d, types=types, seed=d, **MANY)
+    _check(_attend(torch_dev, b, causal=causal, window=window), *P.attention(b, causal=causal, window=window))
+
+
+@pytest.mark.parametrize("types,value", [(("f32", "f32"), float("nan")), (("f32", "f32"), float("inf")),
+                                         (("bf16", "bf16"), float("nan"))])
+@pytest.mark.parametrize("which", ["k_pages", "v_pages"])
+def test_prompts_of_many_heads_do_not_see_later_tokens(torch_dev, types, value, which):
+    b = P.batch([520], [700], d=32, types=types, seed=40, **MANY)
+    at = 500  # its token is row 320: the rows before see nothing of it
+    b[which][b["page_table"][0, at // 24].long(), at % 24] = value
+    got = _attend(torch_dev, b)
+    want, bound = P.attention(b)
+    _check(got[:320], want[:320], bound[:320])
+    assert torch.isnan(got[320:520]).all() if value != value else not torch.isfinite(got[320:520]).all()
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("heads", [(33, 1), (64, 1), (40, 1), (96, 2)], ids=lambda v: "-".join(map(str, v)))
+def test_one_token_of_more_heads_than_a_few_rows(torch_dev, types, heads):
+    for n in (1, 70, 900):
+        b = P.batch([1], [n], heads=heads[0], kv_heads=heads[1], d=64, page=16, types=types, seed=n)
+        _check(_attend(torch_dev, b), *P.attention(b))
 
 
 @pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
