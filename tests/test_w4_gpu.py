@@ -164,6 +164,30 @@ def test_linear_rows_far_apart(torch_dev, m):
     assert ((a.double() - b.double()).abs().cpu() <= 2.0 ** -8 * b.double().abs().cpu() + 32 * (k + 4) * 2.0 ** -24 * size).all()
 
 
+@pytest.mark.parametrize("m", [2, 5, 16])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("group,zeros", [(128, False), (96, True)])
+def test_linear_few_rows_of_a_large_weight(torch_dev, m, kind, group, zeros):
+    """Of 2^27 codes and more, checked at some of its rows."""
+    gh = _gh()
+    n, k = 32769, 4096
+    g = torch.Generator().manual_seed(m)
+    codes, scales, zps = W.random_weight(64, k, group, zeros, seed=m)
+    rows = torch.cat((torch.arange(16), torch.randint(0, n, (32,), generator=g), torch.arange(n - 16, n)))
+    dev = [None if t is None else torch.zeros((n, t.shape[1]), dtype=t.dtype, device=torch_dev)
+           for t in (codes, scales, zps)]
+    for t, part in zip(dev, (codes, scales, zps)):
+        if t is not None:
+            t[rows.to(torch_dev)] = part.to(torch_dev)
+    part = [None if t is None else t[rows.to(torch_dev)].cpu() for t in dev]  # (a row may be drawn twice)
+    x = torch.randn(m, k, generator=g).to(W.TYPES[kind])
+    got = gh.linear_w4(x.to(torch_dev), *dev, group_size=group).double().cpu()[:, rows]
+    w = W.weight(*part, group)
+    want, size = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    bound = (k + 2) * 2.0 ** -24 * size + torch.finfo(W.TYPES[kind]).eps / 2 * (want.abs() * (1 + 2 ** -9))
+    assert (got - want).abs().le(bound).all()
+
+
 @pytest.mark.parametrize("m", [1, 3, 16, 17, 64])
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("zeros", [False, True])
