@@ -75,8 +75,11 @@ struct Rows {
 
 // Where no sequence of a few-row launch has more than kFewRows rows (p.direct), a
 // sequence has at most kFewTiles tiles and the grid counts those; else it counts
-// tile numbers.  Parts are laid out for as many rows.
-constexpr int kFewRows = 32, kFewTiles = 3;
+// tile numbers.  Parts are laid out for as many rows.  (16 sequences of 24 rows over
+// 2000 keys, bf16: 57 us in 128-row tiles, 94 in 16-row ones; of 16 rows 44 and 58 there,
+// but 4 of them 31 and 22, and chunks of prompts in one batch with single tokens would
+// put those into 128-row tiles.)
+constexpr int kFewRows = 16, kFewTiles = 2;
 
 // Tile `number` of sequence s, whose tokens are [o0, o1) and length kv_len.
 __device__ __forceinline__ bool rows_at(const AttnParams &p, int number, int s, int bm, int o0, int o1, int kv_len,
@@ -1356,31 +1359,44 @@ Plan make_plan(const PagedAttnDesc &d) {
     const bool f32 = d.kv.dtype == GFH_F32;
     pl.few_max = kFewRows;
     const int64_t cus = device_cu_count();
+    // the keys that a row of a tile sees at most
+    const int64_t sees = std::max<int64_t>(1, d.window > 0 ? std::min(d.max_kv_len, d.window + 127) : d.max_kv_len);
+    // Tiles of 16 rows alone where the batch has few and their keys are few too, for
+    // they read them once each (us of a call, 16-row tiles / 128-row ones beside them,
+    // bf16, 32 heads over 8 of 128: 32 tokens over 500 keys 16 / 22, over 2000 21 / 30,
+    // over 8000 64 / 26; 8 times 4 tokens over 2000 24 / 30).
     // fp32: tiles of 64 rows where they fill the CUs (us of a call, 16 rows / 64: 32
     // heads over 8 of 128, a prompt of 128 tokens over 500 keys 34 / 56, 512 64 / 57,
     // 2048 741 / 365, eight of 300 over 600 keys 420 / 238).
     pl.chunk_rows = f32 ? 64 : 128;
-    pl.chunk = rows > pl.few_max && d.tokens > d.kv.num_seqs && (!f32 || rows * d.kv.kv_heads >= pl.chunk_rows * cus);
+    pl.chunk = rows > (sees <= 2048 ? 128 : kFewRows) && d.tokens > d.kv.num_seqs &&
+               (!f32 || rows * d.kv.kv_heads >= pl.chunk_rows * cus);
     pl.few = !pl.chunk || d.kv.num_seqs > 1;
     if (!pl.chunk) pl.few_max = kAll;
     auto cut = [&](int64_t tiles, int64_t target, int64_t least, int64_t unit, int &nsplit, int &chunk) {
         const int64_t items = std::max<int64_t>(1, tiles * d.kv.kv_heads);
-        // keys that a tile sees at most
-        const int64_t kv = std::max<int64_t>(1, d.window > 0 ? std::min(d.max_kv_len, d.window + 127) : d.max_kv_len);
-        int64_t ch = std::max(least, (items * kv + target - 1) / target);
+        int64_t ch = std::max(least, (items * sees + target - 1) / target);
         ch = (ch + unit - 1) / unit * unit;
-        nsplit = (int)std::min<int64_t>((kv + ch / 2) / ch, 256);
+        nsplit = (int)std::min<int64_t>((sees + ch / 2) / ch, 256);
         nsplit = std::max(nsplit, 1);
-        ch = std::max(ch, (kv + nsplit - 1) / nsplit);
+        ch = std::max(ch, (sees + nsplit - 1) / nsplit);
         chunk = (int)std::min<int64_t>((ch + unit - 1) / unit * unit, (int64_t)1 << 30);
     };
     const int64_t few_tiles = std::min(d.kv.num_seqs, d.tokens) + (pl.chunk ? 0 : rows / 16);
-    // Workgroups of the few-row launch.  fp32: at least 384 keys each, four waves
-    // (4 sequences of up to 2047 keys, 32 heads of 128, us of a call by keys:
-    // 256 64, 384 54, 512 58, 768 75).  16 bits: at least 128 keys each, six times as
-    // many as fit at once, for even ends (64 sequences of up to 4096 keys, 8 heads of
-    // 128: twice as many 148, four times 132, six times 125, eight times 131).
-    cut(few_tiles, (f32 ? 4 : 12) * cus, f32 ? 384 : 128, 64, pl.few_split, pl.few_chunk);
+    // Keys per workgroup of the few-row launch: one round of those that the CUs hold
+    // where that is at most 1024 keys, else about 704, for even ends; a row's parts
+    // are joined one after the other, so there are no more than a round needs (us of a
+    // call, six rounds of at least 128 keys, fp32 384 / this; bf16 and fp32, 32 heads
+    // over 8 of 128, lengths between a quarter and all of: one sequence of 16000 37 and
+    // 52 / 25 and 45, 8 of 4000 39 and 72 / 27 and 58, 16 of 2000 39 and 55 / 25 and 57,
+    // 64 of 2000 85 and 227 / 79 and 180).  (3/4: few_tiles counts tiles that there may
+    // be, and lengths are not all the longest.)
+    {
+        const int64_t items = std::max<int64_t>(1, few_tiles * d.kv.kv_heads);
+        int64_t keys = items * sees * 3 / 4 / (2 * cus);
+        if (keys > 1024) keys /= (keys + 703) / 704;
+        cut(few_tiles, kAll, std::max<int64_t>(128, keys), 64, pl.few_split, pl.few_chunk);
+    }
     const int64_t wide_keys = kWideKeys * (d.kv.head_dim <= 64 ? kWideWaves64 : kWideWaves128);
     pl.wide = !f32 && pl.few_split > 1 && few_tiles * d.kv.kv_heads <= cus &&
               (d.window > 0 ? std::min(d.max_kv_len, d.window + 15) : d.max_kv_len) <= wide_keys;
@@ -1391,7 +1407,6 @@ Plan make_plan(const PagedAttnDesc &d) {
     // launches and one): 2048 tokens and 7 single ones of 2048 keys 148 / 90 -> 123 /
     // 63, 1024 and 63 of 1000 keys 153 / 129 -> 136 / 101, 512 and 3 of 2000 keys 60 /
     // 47 -> 59 / 40; but 2000 and one of 8000 keys 148 / 88 -> 337 / 172.
-    const int64_t sees = d.window > 0 ? std::min(d.max_kv_len, d.window + 127) : d.max_kv_len;
     if (pl.chunk && 64 * d.kv.num_seqs <= rows && std::min<int64_t>(sees, pl.chunk_chunk) <= 2048) pl.few = false;
     auto floats = [&](bool on, int64_t nsplit, int64_t part_rows) {
         return on && nsplit > 1 ? part_rows * nsplit * (d.kv.head_dim + 2) : 0;

@@ -217,15 +217,18 @@ __device__ __forceinline__ void load_x(const T *p, float (&v)[16]) {
     }
 }
 
-// M rows of x (up to 4) on the VALU.  A workgroup takes R rows of W, its waves
+// M rows of x (up to 4) on the VALU.  A workgroup takes R = 4 rows of W, its waves
 // the 1024-column slices in turn: lane l holds 16 columns of x in registers for
 // R loads of 8 bytes of codes, so x passes through no LDS and a wave reads 512
 // consecutive bytes of a row.  fp32 products of the exact codes and x
 // (v_fma_mix); lanes and waves are summed at the end.  Bound by requests for few
 // columns and by the VALU for more rows: fp32, 1 x 4096 x 4096 5.7 us (9.0 MB), bf16,
-// 1 x 8192 x 28672 30 us (3.9 TB/s), 4 rows of it 79.
-template <typename T, int M, int R>
+// 1 x 8192 x 28672 31 us (3.9 TB/s), 2 rows of it 46.  (Eight rows of W: 1 x 4096 x
+// 4096 6.3 for 5.9, fp32 4 x 4096 x 14336 30 for 26; 2 x 8192 x 28672 44 for 50.)
+constexpr int kRowsR = 4;
+template <typename T, int M>
 __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
+    constexpr int R = kRowsR;
     __shared__ float red[4][M * R];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n0 = blockIdx.x * R;
@@ -1004,16 +1007,11 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
         return check_launch("linear_w4");
     }
     if (d.m <= rows_max(d) || w4_streams(d)) {
-        // eight rows of W per workgroup where that leaves two for every CU
-        const bool eight = d.n >= 8 * 2 * device_cu_count();
         typed([&](auto t) {
             using T = decltype(t);
             auto go = [&](auto mc) {
-                constexpr int M = decltype(mc)::value;
-                if (eight)
-                    hipLaunchKernelGGL((w4_rows_kernel<T, M, 8>), dim3((unsigned)((d.n + 7) / 8)), dim3(256), 0, s, p);
-                else
-                    hipLaunchKernelGGL((w4_rows_kernel<T, M, 4>), dim3((unsigned)((d.n + 3) / 4)), dim3(256), 0, s, p);
+                hipLaunchKernelGGL((w4_rows_kernel<T, decltype(mc)::value>), dim3((unsigned)((d.n + kRowsR - 1) / kRowsR)),
+                                   dim3(256), 0, s, p);
             };
             for (int64_t m = 0; m < d.m; m += 4) {
                 p.x = static_cast<const T *>(d.x) + m * d.ldx;

@@ -44,6 +44,7 @@ LENS = [
     ([70, 1, 33], [70, 260, 100]),
     ([200], [1000]),
     ([300, 1, 2, 0, 130], [900, 700, 40, 5, 130]),
+    ([140, 1, 2, 1, 0, 1], [200, 500, 300, 700, 4, 1000]),
     ([0, 0, 2, 0], [10, 0, 9, 0]),
     ([4, 9], [2, 0]),
 ]
