@@ -1384,7 +1384,8 @@ Plan make_plan(const PagedAttnDesc &d) {
     };
     const int64_t few_tiles = std::min(d.kv.num_seqs, d.tokens) + (pl.chunk ? 0 : rows / 16);
     // Keys per workgroup of the few-row launch: one round of those that the CUs hold
-    // where that is at most 1024 keys, else about 704, for even ends; a row's parts
+    // where that is at most 1024 keys, else about 704, for even ends (up to twelve
+    // rounds); a row's parts
     // are joined one after the other, so there are no more than a round needs (us of a
     // call, six rounds of at least 128 keys, fp32 384 / this; bf16 and fp32, 32 heads
     // over 8 of 128, lengths between a quarter and all of: one sequence of 16000 37 and
@@ -1395,6 +1396,7 @@ Plan make_plan(const PagedAttnDesc &d) {
         const int64_t items = std::max<int64_t>(1, few_tiles * d.kv.kv_heads);
         int64_t keys = items * sees * 3 / 4 / (2 * cus);
         if (keys > 1024) keys /= (keys + 703) / 704;
+        keys = std::max(keys, items * sees / (24 * cus));  // (parts stay some tens of MB at most)
         cut(few_tiles, kAll, std::max<int64_t>(128, keys), 64, pl.few_split, pl.few_chunk);
     }
     const int64_t wide_keys = kWideKeys * (d.kv.head_dim <= 64 ? kWideWaves64 : kWideWaves128);

@@ -390,6 +390,19 @@ def test_many_sequences(torch_dev, types, count):
         _check(_attend(torch_dev, b), *P.attention(b))
 
 
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("count", [1, 64])
+def test_a_wide_table_without_a_hint(torch_dev, types, count):
+    """A table for a million positions and more of every sequence: the parts stay
+    within what a stream keeps, the result the same."""
+    gh = _gh()
+    b = P.batch([1] * count, [40 + 13 * s for s in range(count)], heads=8, kv_heads=2, d=128, page=16, types=types, seed=33,
+                width=1 << 17)
+    x = P.to(b, torch_dev)
+    assert gh.paged_attention_workspace_size(x["q"], *P.args(x)) <= 64 << 20
+    _check(_attend(torch_dev, b), *P.attention(b))
+
+
 def test_on_another_stream(torch_dev):
     gh = _gh()
     b = P.batch([1, 1, 60], [600, 33, 100], heads=8, kv_heads=2, d=64, page=16, types=("bf16", "bf16"), seed=32, stale=0.0)
