@@ -16,9 +16,15 @@
 //
 // Softmax online in base 2, statistics and sums in fp32: the running maximum
 // is of the raw dot products, a probability is exp2(s c - m c + bias) with c =
-// |scale| log2 e (the sign of the scale is on q).  The bias (14 or 9 for f16, 16
-// where P is split) keeps small probabilities normal in their 16-bit form and
-// cancels in O / l.  Long axes are split over workgroups; a second kernel joins
+// |scale| log2 e (the sign of the scale is on q).  Where q has 16 bits P is rounded
+// to its type for the second product, so that this is one matrix instruction and not
+// the three of an fp32 q: O is then off by up to half a step of the type relative to P
+// |V|, beside its own rounding (against 64 bits, root mean square of normal
+// inputs: bf16 2.1e-3 .. 2.3e-3 where O's rounding alone has 1.7e-3, f16 2.6e-4 and
+// 2.2e-4).  l sums the rounded P, so the
+// weights that V is taken with add up to one.  The bias (14 or 9 for f16, 16 where P is
+// split) keeps small probabilities normal in their 16-bit form and cancels in O / l.
+// Long axes are split over workgroups; a second kernel joins
 // the parts in their order, so results do not depend on timing.
 //
 // Rows of the cache past the last key and pages outside the cache read as
@@ -636,9 +642,8 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 pv[x] = __builtin_amdgcn_exp2f(fmaf(s[x >> 2][x & 3], p.sc2, kBias - mc));
-                sum += pv[x];
+                if (NP > 1) sum += pv[x];
             }
-            l = fmaf(l, alpha, sum);
             m = m_new;
 #pragma unroll
             for (int i2 = 0; i2 < NB; ++i2) o[i2] *= alpha;
@@ -647,9 +652,11 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
             for (int x = 0; x < 4; ++x) {
                 uint32_t two[NP];
                 pieces2<T, NP>(pv[2 * x], pv[2 * x + 1], two);
+                if (NP == 1) sum = H::add2(two[0], sum);  // what the product sees
 #pragma unroll
                 for (int q = 0; q < NP; ++q) pw[q][x] = two[q];
             }
+            l = fmaf(l, alpha, sum);
             v8 pf[NP];
 #pragma unroll
             for (int q = 0; q < NP; ++q) {

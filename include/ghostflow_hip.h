@@ -459,8 +459,10 @@ GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, 
  * for the token at position p: j <= p if causal, j > p - window if window > 0.
  * A token that sees no key gets zeros.  q [tokens, heads, head_dim], rows ldq
  * apart, out the same, rows ldo apart (out may be q with ldo = ldq), of type
- * dtype as in gfh_paged_append.  Sums and softmax in fp32; out is rounded once
- * (fp32 q over a bf16 cache: fp32 products of the stored values).
+ * dtype as in gfh_paged_append.  Scores, softmax and sums in fp32; with q of 16 bits
+ * the probabilities are rounded to its type before P . V and in their sum (half a
+ * step each, relative to P |V|), with fp32 q they are not (over a bf16 cache: fp32
+ * products of the stored values); out is rounded once.
  * max_kv_len: the longest length of the batch as far as the caller knows (0:
  * max_pages * page_size); the work is split by it, the results hold for any
  * length.  workspace (nullable, 16-byte aligned) of at least

@@ -2,6 +2,8 @@
 the plain form in 64 bits (_paged.py): types, head layouts, page sizes and
 layouts, ragged and empty sequences, windows, masked rows.  Rows of the pages
 that hold no position are NaN, so any use of them shows."""
+import math
+
 import pytest
 import torch
 
@@ -416,3 +418,32 @@ def test_on_another_stream(torch_dev):
             out.append([gh.paged_attention(x["q"], *P.args(x)) for _ in range(5)])
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for os in out for o in os)
+
+
+# a value of the type next below 2, and a weight of about 1/2 that lies just under the
+# middle between two of its values
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("lens", [([1], [30]), ([1], [900]), ([1] * 40, [4000] * 40), ([40], [900]), ([1, 300], [70, 1100])],
+                         ids=lambda v: "-".join(map(str, (len(v[0]), v[0][-1]))))
+def test_weights_add_up_to_what_the_product_sees(torch_dev, types, lens):
+    """Where V is one value the result is that value: the weights, rounded for the
+    product, are rounded in their sum too.  Every 32nd key has weight 1, the others
+    w.  Sums of n fp32 terms and a few more operations are off by (n + 16) 2^-24
+    relatively, which is less than half a step of 16 bits, so those give the value
+    itself."""
+    h = P.half_step(P.TYPES[types[1]]) if types[1] != "f32" else 2.0 ** -8
+    b = P.batch(*lens, heads=4, kv_heads=2, d=64, page=16, types=types, seed=50)
+    value = 2 * (1 - h)
+    b["q"].zero_()[..., 0] = 1
+    for s, n in enumerate(lens[1]):
+        at = torch.arange(n)
+        page, row = b["page_table"][s, at // 16].long(), at % 16
+        k = torch.zeros(n, 2, 64)
+        k[..., 0] = -(at % 32 != 0).float()[:, None]
+        b["k_pages"][page, row] = k.to(b["k_pages"].dtype)
+        b["v_pages"][page, row] = value
+    got = _attend(torch_dev, b, scale=-math.log(0.5 * (1 + h * (1 - 2 ** -4)))).double().cpu()
+    if types[0] == "f32":
+        assert (got - value).abs().max() <= (max(lens[1]) + 16) * 2.0 ** -24 * value
+    else:
+        assert (got == value).all(), (got - value).abs().max()
