@@ -19,19 +19,20 @@
 // |scale| log2 e (the sign of the scale is on q).  Where q has 16 bits P is rounded
 // to its type for the second product, so that this is one matrix instruction and not
 // the three of an fp32 q: O is then off by up to half a step of the type relative to P
-// |V|, beside its own rounding (against 64 bits, root mean square of normal
-// inputs: bf16 2.1e-3 .. 2.3e-3 where O's rounding alone has 1.7e-3, f16 2.6e-4 and
-// 2.2e-4).  l sums the rounded P, so the
-// weights that V is taken with add up to one.  The bias (14 or 9 for f16, 16 where P is
-// split) keeps small probabilities normal in their 16-bit form and cancels in O / l.
-// Long axes are split over workgroups; a second kernel joins
-// the parts in their order, so results do not depend on timing.
+// |V|, beside its own rounding (against 64 bits, root mean square of normal inputs:
+// bf16 2.1e-3 .. 2.3e-3 where O's rounding alone has 1.7e-3, f16 2.6e-4 and 2.2e-4).
+// l sums the rounded P, so the weights that V is taken with add up to one.  The bias
+// (14 or 9 for f16, 16 where P is split) keeps small probabilities normal in their
+// 16-bit form and cancels in O / l.  Long axes are split over workgroups; a second
+// kernel joins the parts in their order, so results do not depend on timing.
 //
 // Rows of the cache past the last key and pages outside the cache read as
 // zeros.  A masked key must not reach a row even when its value is not
 // finite (0 * inf): a tile that holds keys which some of its rows do not see
 // is searched for such values, and its workgroup then redoes its rows one by
-// one over the keys they see (slow_rows).
+// one over the keys they see (slow_rows).  So it does where a sum of its own is not
+// finite: an infinite V meets pieces of P of either sign and weights that 16 bits
+// round to nothing, and V near the largest fp32 weights above 1.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -158,7 +159,8 @@ __device__ __forceinline__ int64_t part_row(const AttnParams &p, const Rows &t, 
 }
 
 // The rows of a tile one by one, a wave each, over the keys [b, e) that each
-// sees, in fp32: for the inputs named above.
+// sees, in fp32 and without a bias: for the inputs named above.  (Other parts of a
+// row are 2^bias larger: the maximum says so.)
 template <typename TA, typename TC>
 __device__ __forceinline__ void slow_rows(const AttnParams &p, const Rows &t, int seq, int kvh, int b, int e,
                                                     int split, bool parts, float bias, int wave, int nwaves,
@@ -191,18 +193,19 @@ __device__ __forceinline__ void slow_rows(const AttnParams &p, const Rows &t, in
                 m = l = acc[0] = acc[1] = m_new;
                 break;
             }
-            const float alpha = exp2f(m - m_new), w = exp2f(s - m_new + bias);
+            const float alpha = exp2f(m - m_new), w = exp2f(s - m_new);
             l = fmaf(l, alpha, w);
 #pragma unroll
             for (int i = 0; i < 2; ++i) acc[i] = fmaf(acc[i], alpha, w * vv[i]);
             m = m_new;
+            if (__all((lane >= c.d || acc[0] != acc[0]) && (lane + 64 >= c.d || acc[1] != acc[1]))) break;
         }
         if (parts) {
             const int64_t at = part_row(p, t, r, kvh) * p.nsplit + split;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
                 if (lane + 64 * i < c.d) p.acc[at * c.d + lane + 64 * i] = acc[i];
-            if (lane == 0) p.ml[at] = make_float2(m, l);
+            if (lane == 0) p.ml[at] = make_float2(m + bias, l);
         } else {
             const float inv = m == -INFINITY ? 0.f : 1.0f / l;
             TA *o = out_row<TA>(p, r, kvh);
@@ -686,6 +689,12 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     // 4 dims of a row.
     l = quarter_sum(l);
     const float mt = m == -INFINITY ? m : m * p.sc2;
+    if (kBias != 0.f) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) odd |= jmax >= 0 && !(fabsf(o[i][x]) < INFINITY);
+    }
     constexpr int kRow = DP + 4;
     static_assert(WAVES * 16 * (kRow + 2) * 4 <= kRing, "states over the rings");
     float *const accs = reinterpret_cast<float *>(lds);
@@ -929,6 +938,10 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(AttnParams p) {
         pb = pe;
     }
 
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int x = 0; x < 16; ++x) odd |= jmax >= 0 && !(fabsf(o[i][x]) < INFINITY);
     if (any_wave<4>(odd, flags, wave, lane)) {
         slow_rows<TA, T>(p, t, seq, kvh, b, e, split, nact > 1, kBias, wave, 4, lane);
         return;
@@ -1261,6 +1274,12 @@ __global__ __launch_bounds__(256, 2) void paged_f32_chunk_kernel(AttnParams p) {
         pb = pe;
     }
     l = quarter_sum(l);
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) odd |= jmax >= 0 && !(fabsf(o[v][y][x]) < INFINITY);
     if (any_wave<4>(odd, flags, wave, lane)) {
         slow_rows<float, float>(p, t, seq, kvh, b, e, split, nact > 1, 0.f, wave, 4, lane);
         return;

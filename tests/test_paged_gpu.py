@@ -447,3 +447,65 @@ def test_weights_add_up_to_what_the_product_sees(torch_dev, types, lens):
         assert (got - value).abs().max() <= (max(lens[1]) + 16) * 2.0 ** -24 * value
     else:
         assert (got == value).all(), (got - value).abs().max()
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("lens", [([1], [300]), ([1, 1], [5000, 40]), ([60], [300]), ([300, 1], [2000, 900])],
+                         ids=lambda v: "-".join(map(str, v[0])))
+@pytest.mark.parametrize("value", [float("inf"), float("-inf")])
+def test_an_infinite_value_that_every_row_sees(torch_dev, types, lens, value):
+    """It gives the rows what the formula has there, infinity of its sign, wherever
+    its key lies; two of both signs give NaN."""
+    b = P.batch(*lens, heads=4, kv_heads=2, d=64, page=16, types=types, seed=51)
+    for at in (10, 129, 200):
+        b["v_pages"][b["page_table"][0, at // 16].long(), at % 16, 1, at % 64] = value
+    b["v_pages"][b["page_table"][0, 3].long(), 5, 0, 7] = value
+    b["v_pages"][b["page_table"][0, 9].long(), 6, 0, 7] = -value
+    want, bound = P.attention(b)
+    got = _attend(torch_dev, b).double().cpu()
+    for test in (torch.isposinf, torch.isneginf, torch.isnan):
+        assert torch.equal(test(got), test(want)), test.__name__
+    fine = torch.isfinite(want)
+    assert (got - want).abs()[fine].le(bound[fine]).all()
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("lens", [([1], [300]), ([200], [300])], ids=lambda v: "-".join(map(str, v[0])))
+def test_an_infinite_value_of_little_weight(torch_dev, types, lens):
+    """2^-45 of the largest weight: nothing in f16, but not nothing."""
+    b = P.batch(*lens, heads=4, kv_heads=2, d=64, page=16, types=types, seed=52)
+    b["q"].zero_()[..., 0] = 1
+    b["k_pages"][..., 0] = 0  # (rows without a position too)
+    page = b["page_table"][0, 2].long()
+    b["k_pages"][page, 3, :, 0] = -45
+    b["v_pages"][page, 3, 0, 9] = float("inf")
+    got = _attend(torch_dev, b, scale=math.log(2)).double().cpu()
+    assert (got[:, :2, 9] == float("inf")).all()
+    got[:, :2, 9] = 0
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("types", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32")], ids="/".join)
+@pytest.mark.parametrize("lens", [([1], [300]), ([1], [9000]), ([200], [300])], ids=lambda v: "-".join(map(str, v)))
+def test_values_near_the_largest(torch_dev, types, lens):
+    """V of 2^112 and more: sums of weights up to 1 times V stay finite, whatever
+    constant the weights carry on the way."""
+    b = P.batch(*lens, heads=4, kv_heads=2, d=64, page=16, types=types, seed=53)
+    b["v_pages"] *= 2.0 ** 112
+    _check(_attend(torch_dev, b), *P.attention(b))
+
+
+@pytest.mark.parametrize("types", [("bf16", "bf16"), ("f32", "bf16"), ("f32", "f32")], ids="/".join)
+def test_values_near_the_largest_under_a_late_maximum(torch_dev, types):
+    """Scores that rise by less than what the running maximum may lag: weights of up
+    to 2^7.5 before V of 2^118."""
+    b = P.batch([520], [700], d=32, types=types, seed=56, **MANY)
+    b["q"].zero_()[..., 0] = 1
+    at = torch.arange(700)
+    page, row = b["page_table"][0, at // 24].long(), at % 24
+    k = torch.zeros(700, 32, 32)
+    k[64:, :, 0] = 7.5
+    b["k_pages"][page, row] = k.to(b["k_pages"].dtype)
+    b["v_pages"][page, row] = 2.0 ** 118
+    want, bound = P.attention(b, scale=math.log(2))
+    _check(_attend(torch_dev, b, scale=math.log(2))[:520], want[:520], bound[:520])
