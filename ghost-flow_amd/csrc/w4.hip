@@ -166,7 +166,7 @@ struct W4LinearParams {
     int kper;   // columns per split
     int splits;
     int steps;       // 32-column steps per group (more than there are: one group)
-    uint32_t magic;  // 2^32 / steps, rounded up
+    uint32_t magic;  // 2^32 / steps + 1 (see w4_streams)
 };
 
 // Eight codes as f16 pairs (0, 4), (1, 5), (2, 6), (3, 7), z taken off.
@@ -901,11 +901,16 @@ __global__ __launch_bounds__(256) void w4_join_kernel(W4LinearParams p) {
 // (asked for whether there are zero points or not, and without the strides: the
 // size of the workspace is asked for without them).  fp32 x takes three pieces per
 // product: four rows go to the VALU.
+//
+// The stream finds a step's group as the high word of step * magic, where magic =
+// 2^32 / steps + 1 (steps per group) is at most `steps` too large after the product
+// with steps: the quotient while step * steps < 2^32, so longer groups go elsewhere.
 int64_t rows_max(const LinearW4Desc &d) { return d.dtype == GFH_F32 ? 4 : 2; }
 bool w4_streams(const LinearW4Desc &d) {
     const int64_t groups = (d.k + d.group - 1) / d.group;
+    const bool found = groups == 1 || (d.k / 128 * 4 + 4) * (d.group / 32) < (int64_t)1 << 32;
     return d.dtype != GFH_F32 && d.m > rows_max(d) && d.m <= 16 && d.n * d.k < (int64_t)1 << 27 &&
-           16 * (2 * groups + 1) * 4 <= kStreamTable;
+           16 * (2 * groups + 1) * 4 <= kStreamTable && found;
 }
 
 struct W4Plan {

@@ -307,3 +307,26 @@ def test_captured_linear_replays(torch_dev):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want), rep
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("k,group,n", [(2100384, 2097184, 32), (8388608, 786336, 5), (4194304, 1301664, 7)])
+def test_linear_few_rows_in_very_long_groups(torch_dev, kind, k, group, n):
+    """x is not zero at the ends of the groups only, whole there, and scales are
+    powers of two: exact."""
+    gh = _gh()
+    m = 4
+    g = torch.Generator().manual_seed(k)
+    at = torch.arange(k)
+    at = at[(at % group >= group - 96) | (at % group < 64) | (at >= k - 64)]
+    codes = torch.randint(0, 256, (n, k // 2), dtype=torch.uint8, generator=g)
+    groups = -(-k // group)
+    scales = 2.0 ** (torch.arange(groups) % 8 - 4).float()[None] * 2.0 ** torch.randint(0, 2, (n, 1), generator=g)
+    zps = torch.randint(0, 16, (n, groups), dtype=torch.uint8, generator=g)
+    x = torch.zeros(m, k)
+    x[:, at] = torch.randint(-1, 2, (m, len(at)), generator=g).float()
+    c = (codes[:, at // 2] >> (at % 2 * 4).to(torch.uint8)) & 15
+    w = (c.double() - zps[:, at // group].double()) * scales[:, at // group].double()
+    got = gh.linear_w4(x.to(W.TYPES[kind]).to(torch_dev), codes.to(torch_dev), scales.to(torch_dev), zps.to(torch_dev),
+                       group_size=group)
+    assert torch.equal(got.cpu(), (x[:, at].double() @ w.t()).to(W.TYPES[kind]))
