@@ -288,15 +288,16 @@ __device__ __attribute__((aligned(16))) uint32_t g_zero_chunk[4];
 constexpr int kMaxPages = 1024;  // page offsets held in LDS: keys per pass >= kMaxPages
 
 // Byte offsets of the pages of keys [b, e) into LDS, -1 for a page outside
-// the cache; returns the end of the keys they cover.
-__device__ __forceinline__ int stage_pages(const View &c, int seq, int b, int e, int elem, int64_t *lds, int tid,
+// the cache (reported from key lo on: those before are asked for only to begin at a
+// whole tile); returns the end of the keys they cover.
+__device__ __forceinline__ int stage_pages(const View &c, int seq, int b, int e, int lo, int elem, int64_t *lds, int tid,
                                            int nthreads) {
     const int p0 = paged::page_of(c, b);
     const int n = min(kMaxPages, paged::page_of(c, e - 1) - p0 + 1);
     for (int i = tid; i < n; i += nthreads) {
         const int page = c.table[seq * c.table_stride + p0 + i];
         const bool ok = page >= 0 && page < c.num_pages;
-        if (!ok) paged::raise(c, paged::kBadPage);
+        if (!ok && p0 + i >= paged::page_of(c, lo)) paged::raise(c, paged::kBadPage);
         lds[i] = ok ? page * c.page_stride * elem : -1;
     }
     return (int)min((int64_t)e, (int64_t)(p0 + n) * c.page_size);
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     for (int pb = b; pb < e;) {
         const int p0 = paged::page_of(p.c, pb);
         __syncthreads();  // every wave is done with the pages before
-        const int pe = stage_pages(p.c, seq, pb, e, 2, pages, tid, 64 * WAVES);
+        const int pe = stage_pages(p.c, seq, pb, e, t.lo, 2, pages, tid, 64 * WAVES);
         __syncthreads();
         const int n = (pe - pb + 31) / 32;  // tiles of this pass; this wave's: wave, wave + WAVES, ..
         char *const ring = lds + wave * 4 * kTile;
@@ -810,7 +811,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(AttnParams p) {
     for (int pb = b; pb < e;) {
         const int p0 = paged::page_of(p.c, pb);
         __syncthreads();
-        const int pe = stage_pages(p.c, seq, pb, e, 2, pages, tid, 256);
+        const int pe = stage_pages(p.c, seq, pb, e, t.lo, 2, pages, tid, 256);
         __syncthreads();
         const int n = (pe - pb + 63) / 64;
         auto ask = [&](int k0, int st) __attribute__((always_inline)) {
@@ -1021,7 +1022,7 @@ __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
     for (int pb = b; pb < e;) {
         const int p0 = paged::page_of(cc, pb);
         __syncthreads();
-        const int pe = stage_pages(cc, seq, pb, e, 4, pages, tid, 256);
+        const int pe = stage_pages(cc, seq, pb, e, t.lo, 4, pages, tid, 256);
         __syncthreads();
         // byte offset of key j's row and head, -1 past the keys or outside the cache
         auto row_at = [&](int j) __attribute__((always_inline)) -> int64_t {
@@ -1178,7 +1179,7 @@ __global__ __launch_bounds__(256, 2) void paged_f32_chunk_kernel(AttnParams p) {
     for (int pb = b; pb < e;) {
         const int p0 = paged::page_of(cc, pb);
         __syncthreads();
-        const int pe = stage_pages(cc, seq, pb, e, 4, pages, tid, 256);
+        const int pe = stage_pages(cc, seq, pb, e, t.lo, 4, pages, tid, 256);
         __syncthreads();
         const int n = (pe - pb + 31) / 32;
         auto ask = [&](int k0, char *to) __attribute__((always_inline)) {

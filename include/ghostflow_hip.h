@@ -418,7 +418,8 @@ GFH_API int gfh_mha_forward_with_cache_f32(
  * page_table, q_offsets and kv_lens are read by the kernels only, so a captured
  * call can be replayed after they change.  What the host cannot check the
  * kernels do: a length outside [0, max_pages * page_size], or a token whose
- * position is, sets bit 0 of *status, a page outside [0, num_pages) bit 1.
+ * position is, sets bit 0 of *status, a page outside [0, num_pages) bit 1 where a
+ * new token goes to it or sees a key of it (so pages before a window may be gone).
  * Such tokens and pages are not written; such a page reads as zeros; a length
  * is clamped.  The caller clears *status.
  * head_dim is a multiple of 8 in [8, 128]; max_pages * page_size is at most

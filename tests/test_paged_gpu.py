@@ -509,3 +509,21 @@ def test_values_near_the_largest_under_a_late_maximum(torch_dev, types):
     b["v_pages"][page, row] = 2.0 ** 118
     want, bound = P.attention(b, scale=math.log(2))
     _check(_attend(torch_dev, b, scale=math.log(2))[:520], want[:520], bound[:520])
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("lens", [([1], [1000]), ([30], [1000]), ([200], [1000])], ids=lambda v: "-".join(map(str, v[0])))
+@pytest.mark.parametrize("page", [8, 16, 24])
+def test_pages_before_the_window_may_be_gone(torch_dev, types, lens, page):
+    """Pages none of whose keys any new token sees are not asked for: status stays."""
+    gh = _gh()
+    window = 100
+    b = P.batch(*lens, heads=4, kv_heads=2, d=64, page=page, types=types, seed=54)
+    want = P.attention(b, window=window)
+    first = lens[1][0] - lens[0][0] + 1 - window
+    b["page_table"][0, :first // page] = -1
+    x = P.to(b, torch_dev)
+    st = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+    got = gh.paged_attention(x["q"], *P.args(x), window=window, status=st)
+    _check(got, *want)
+    assert int(st) == 0
