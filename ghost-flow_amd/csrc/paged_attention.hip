@@ -101,6 +101,7 @@ __device__ __forceinline__ bool rows_at(const AttnParams &p, int number, int s, 
     t.part = p.direct ? s * kFewRows - o0 * c.group : 0;
     t.kv_len = kv_len;
     t.q_last = t.kv_len - o1;
+    if (t.q_last + o0 < 0) paged::raise(c, paged::kBadLength);  // tokens before position 0
     const int first = t.r0 / c.group + t.q_last, last = (t.r1 - 1) / c.group + t.q_last;
     t.hi = max(0, p.causal ? min(t.kv_len, last + 1) : t.kv_len);
     t.lo = p.window ? min(t.hi, max(0, first - p.window + 1)) : 0;

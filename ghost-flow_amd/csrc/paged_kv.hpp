@@ -12,7 +12,8 @@
 // read, so a captured graph can be replayed while they change.  What the host
 // cannot check, the kernels do: offsets are clamped to the rows there are,
 // lengths to what the table can hold, and a page outside the cache is neither
-// read nor written.  Each of these sets a bit of *status.
+// read nor written.  Such lengths and pages, and tokens whose position the table
+// does not hold, set a bit of *status.
 #pragma once
 
 #include "common.hpp"

@@ -527,3 +527,19 @@ def test_pages_before_the_window_may_be_gone(torch_dev, types, lens, page):
     got = gh.paged_attention(x["q"], *P.args(x), window=window, status=st)
     _check(got, *want)
     assert int(st) == 0
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("lens", [([2], [1]), ([1, 3, 1], [4, 2, 9]), ([1, 200, 1], [5, 199, 70])],
+                         ids=lambda v: "-".join(map(str, v[0])))
+def test_tokens_before_position_0_are_reported(torch_dev, types, lens):
+    """More new tokens than positions: the attention says so as the append does."""
+    gh = _gh()
+    b = P.batch(*lens, heads=4, kv_heads=2, d=64, page=16, types=types, seed=55)
+    x = P.to(b, torch_dev)
+    st = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+    _check(gh.paged_attention(x["q"], *P.args(x), status=st), *P.attention(b))
+    assert int(st) == 1
+    st.zero_()
+    gh.paged_append(*P.args(x), x["k"], x["v"], status=st)
+    assert int(st) == 1
