@@ -990,6 +990,20 @@ GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, 
             return set_error(GFH_INVALID_SHAPE, "%s: angles of %lld positions, the page table holds %lld", who,
                              (long long)rope_rows, (long long)capacity);
         if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
+        PagedAppendDesc d;
+        d.kv = *kv;
+        d.dtype = dtype;
+        d.tokens = tokens;
+        d.heads = heads;
+        d.q = q, d.k = k, d.v = v;
+        d.q_out = q_out;
+        d.ldq = ldq, d.ldqo = ldqo, d.ldk = ldk, d.ldv = ldv;
+        d.cos = rope_cos, d.sin = rope_sin;
+        d.rotary_dim = rotary_dim;
+        d.interleaved = interleaved != 0;
+        if (paged_append_blocks(d) > kMaxBlocks256)
+            return set_error(GFH_INVALID_SHAPE, "%s: %lld tokens of %lld heads are more than one launch can have", who,
+                             (long long)tokens, (long long)heads);
         GFH_TRY(check_paged_memory(who, kv));
         if (q) {
             GFH_TRY(check_rows(who, q, "q", dtype, tokens, heads, kv->head_dim, ldq));
@@ -1006,17 +1020,6 @@ GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, 
                 return set_error(GFH_INVALID_DATA, "%s: rope_cos and rope_sin must be 16-byte aligned", who);
         }
         GFH_TRY(ensure_init());
-        PagedAppendDesc d;
-        d.kv = *kv;
-        d.dtype = dtype;
-        d.tokens = tokens;
-        d.heads = heads;
-        d.q = q, d.k = k, d.v = v;
-        d.q_out = q_out;
-        d.ldq = ldq, d.ldqo = ldqo, d.ldk = ldk, d.ldv = ldv;
-        d.cos = rope_cos, d.sin = rope_sin;
-        d.rotary_dim = rotary_dim;
-        d.interleaved = interleaved != 0;
         return launch_paged_append(d, as_stream(stream));
     });
 }
@@ -1117,14 +1120,6 @@ GFH_API int gfh_linear_w4(int dtype, const void *x, int64_t ldx, const uint8_t *
         int64_t ex, ey;
         if (!extent2d(m, k, ldx, &ex) || !extent2d(m, n, ldy, &ey))
             return set_error(GFH_INVALID_SHAPE, "%s: operand extent overflows", who);
-        const size_t eb = (size_t)elem_bytes(dtype);
-        GFH_TRY(require_range(x, (size_t)ex * eb, "x"));
-        GFH_TRY(check_w4_memory(who, codes, scales, zero_points, n, k, group));
-        GFH_TRY(optional_range(bias, (size_t)n * eb, "bias"));
-        GFH_TRY(require_range(y, (size_t)ey * eb, "y"));
-        if (workspace && !aligned16(workspace))
-            return set_error(GFH_INVALID_DATA, "%s: the workspace must be 16-byte aligned", who);
-        GFH_TRY(ensure_init());
         LinearW4Desc d;
         d.dtype = dtype;
         d.x = x;
@@ -1136,6 +1131,17 @@ GFH_API int gfh_linear_w4(int dtype, const void *x, int64_t ldx, const uint8_t *
         d.y = y;
         d.ldy = ldy;
         d.m = m, d.n = n, d.k = k, d.group = group;
+        if (!linear_w4_fits(d))
+            return set_error(GFH_INVALID_SHAPE, "%s: n=%lld m=%lld are more than one launch can have", who, (long long)n,
+                             (long long)m);
+        const size_t eb = (size_t)elem_bytes(dtype);
+        GFH_TRY(require_range(x, (size_t)ex * eb, "x"));
+        GFH_TRY(check_w4_memory(who, codes, scales, zero_points, n, k, group));
+        GFH_TRY(optional_range(bias, (size_t)n * eb, "bias"));
+        GFH_TRY(require_range(y, (size_t)ey * eb, "y"));
+        if (workspace && !aligned16(workspace))
+            return set_error(GFH_INVALID_DATA, "%s: the workspace must be 16-byte aligned", who);
+        GFH_TRY(ensure_init());
         hipStream_t s = as_stream(stream);
         Scratch ws;
         const size_t need = linear_w4_workspace_bytes(d);

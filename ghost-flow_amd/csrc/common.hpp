@@ -16,6 +16,8 @@ int set_error(int code, const char *fmt, ...) __attribute__((format(printf, 2, 3
 void clear_error();
 // hipGetLastError after a launch -> GFH_COMPUTATION_FAILED with its text.
 int check_launch(const char *what);
+// Workgroups of 256 threads that a launch can have (its work-items have 32 bits).
+constexpr int64_t kMaxBlocks256 = ((int64_t)1 << 24) - 1;
 // Lazily initializes the device table; returns GFH_SUCCESS or an error code.
 int ensure_init();
 

@@ -194,6 +194,7 @@ struct PagedAppendDesc {
     int64_t rotary_dim = 0;
     bool interleaved = false;
 };
+int64_t paged_append_blocks(const PagedAppendDesc &d);  // of its grid
 int launch_paged_append(const PagedAppendDesc &d, hipStream_t s);
 // paged_attention.hip: max_kv_len in [0, capacity] is what the work is split
 // by; any length is served.  window 0: none.
@@ -230,6 +231,7 @@ struct LinearW4Desc {
     int64_t ldy = 0;
     int64_t m = 0, n = 0, k = 0, group = 0;
 };
+bool linear_w4_fits(const LinearW4Desc &d);  // the launch's grid
 size_t linear_w4_workspace_bytes(const LinearW4Desc &d);
 int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s);
 

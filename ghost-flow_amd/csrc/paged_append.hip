@@ -113,7 +113,16 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendParams p) {
     }
 }
 
+// 8 pairs per thread (16-byte loads of 16-bit types) where the head allows
+bool wide_units(const PagedAppendDesc &d) { return d.kv.head_dim % 16 == 0 && (!d.cos || d.rotary_dim % 16 == 0); }
+int units_of(const PagedAppendDesc &d) { return (int)d.kv.head_dim / (wide_units(d) ? 16 : 8); }
+int64_t waves_of(const PagedAppendDesc &d) {
+    return (((d.q ? d.heads : 0) + 2 * d.kv.kv_heads) * units_of(d) + 63) / 64;
+}
+
 }  // namespace
+
+int64_t paged_append_blocks(const PagedAppendDesc &d) { return (d.tokens * waves_of(d) + 3) / 4; }
 
 int launch_paged_append(const PagedAppendDesc &d, hipStream_t s) {
     AppendParams p{};
@@ -126,15 +135,10 @@ int launch_paged_append(const PagedAppendDesc &d, hipStream_t s) {
     p.cos = d.cos, p.sin = d.sin;
     p.rot = d.cos ? (int)d.rotary_dim : 0;
     p.interleaved = d.interleaved;
-    const int hd = (int)d.kv.head_dim;
-    // 8 pairs per thread (16-byte loads of 16-bit types) where the head allows
-    const bool wide = hd % 16 == 0 && p.rot % 16 == 0;
-    p.units = hd / (wide ? 16 : 8);
-    const int64_t heads = (d.q ? d.heads : 0) + 2 * d.kv.kv_heads;
-    p.waves = (int)((heads * p.units + 63) / 64);
-    const int64_t blocks = (d.tokens * p.waves + 3) / 4;
-    if (blocks > (int64_t)1 << 29) return set_error(GFH_INVALID_SHAPE, "paged_append: grid too large");
-    const dim3 grid((unsigned)blocks);
+    const bool wide = wide_units(d);
+    p.units = units_of(d);
+    p.waves = (int)waves_of(d);
+    const dim3 grid((unsigned)paged_append_blocks(d));
     auto go = [&](auto ta, auto tc) {
         using TA = decltype(ta);
         using TC = decltype(tc);

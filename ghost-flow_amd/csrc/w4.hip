@@ -962,6 +962,11 @@ int launch_dequantize_w4(const uint8_t *codes, const float *scales, const uint8_
     return check_launch("dequantize_i4_grouped");
 }
 
+bool linear_w4_fits(const LinearW4Desc &d) {
+    if (d.m <= rows_max(d) || w4_streams(d)) return (d.n + kRowsR - 1) / kRowsR <= kMaxBlocks256;
+    return (d.n + 127) / 128 * w4_plan(d).splits <= kMaxBlocks256 / 2;  // (of up to 512 threads)
+}
+
 size_t linear_w4_workspace_bytes(const LinearW4Desc &d) {
     if (d.m <= rows_max(d) || w4_streams(d)) return 0;
     const W4Plan pl = w4_plan(d);
@@ -1036,7 +1041,6 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
     p.splits = pl.splits;
     p.kper = pl.kper;
     const int64_t gx = (d.n + 64 * pl.rt - 1) / (64 * pl.rt) * pl.splits, gy = (d.m + 16 * pl.mb - 1) / (16 * pl.mb);
-    if (gx > (1 << 23) || gy > 65535) return set_error(GFH_INVALID_SHAPE, "linear_w4: grid too large");
     const dim3 grid((unsigned)gx, (unsigned)gy);
     typed([&](auto t) {
         using T = decltype(t);

@@ -104,3 +104,17 @@ def test_python_checks():
         gh.paged_attention(q, pages, pages, i[None], torch.zeros(2, dtype=torch.int32), i)
     with pytest.raises(gh.GhostFlowError):
         gh.paged_append(pages, pages, i[None], torch.zeros(2, dtype=torch.int32), i, q[:, :2], q[:, :2])
+
+
+def test_more_tokens_than_a_launch_can_have():
+    L, lib = _lib()
+    kv = _kv(L, head_dim=8, kv_heads=1, page_stride=16 * 8, row_stride=8, head_stride=8)
+    # a wave of 64 per token: fewer than 2^32 work-items in all
+    most = 4 * (2 ** 24 - 1)
+    word = b"more than one launch"
+    for tokens in (most, most + 1, 2 ** 30):
+        rc = lib.gfh_paged_append(C.byref(kv), L.BF16, tokens, 1, 16, 8, 16, 8, 16, 8, 16, 8, None, None, 0, 0, 0, None)
+        if tokens <= most:  # goes on to the memory, which is none
+            assert rc in (L.INVALID_DATA, L.COMPUTATION_FAILED) and word not in lib.gfh_last_error()
+        else:
+            assert rc == L.INVALID_SHAPE and word in lib.gfh_last_error(), lib.gfh_last_error()

@@ -60,3 +60,17 @@ def test_python_checks():
         gh.quantize_grouped_i4(torch.zeros(4, 64))
     with pytest.raises(gh.GhostFlowError):
         gh.linear_w4(torch.zeros(1, 64), torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 1))
+
+
+@pytest.mark.parametrize("dtype,m,most", [(0, 1, 4 * (2 ** 24 - 1)), (2, 4, 4 * (2 ** 24 - 1)), (1, 5, 128 * (2 ** 23 - 1)),
+                                          (2, 5, 128 * (2 ** 23 - 1))])
+def test_more_rows_of_the_weight_than_a_launch_can_have(dtype, m, most):
+    """Four rows of W per workgroup of 256 threads, or 128 per one of up to 512:
+    fewer than 2^32 work-items."""
+    L, lib = _lib()
+    for n in (most, most + 1):
+        rc = _linear(lib, dtype=dtype, m=m, n=n, ldy=n, k=64)
+        if n == most:  # goes on to the memory, which is none
+            assert rc in (L.INVALID_DATA, L.COMPUTATION_FAILED) and b"launch" not in lib.gfh_last_error()
+        else:
+            assert rc == L.INVALID_SHAPE and b"more than one launch" in lib.gfh_last_error(), lib.gfh_last_error()
