@@ -330,3 +330,55 @@ def test_linear_few_rows_in_very_long_groups(torch_dev, kind, k, group, n):
     got = gh.linear_w4(x.to(W.TYPES[kind]).to(torch_dev), codes.to(torch_dev), scales.to(torch_dev), zps.to(torch_dev),
                        group_size=group)
     assert torch.equal(got.cpu(), (x[:, at].double() @ w.t()).to(W.TYPES[kind]))
+
+
+@pytest.mark.parametrize("m", [3, 5, 16, 40])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_many_groups_and_values_far_below_the_largest(torch_dev, m, kind, zeros):
+    """448 groups to a row, 3 to 16 rows among them.  Every 256th column of x is 1
+    and meets a weight of 0, the others are some 2^-20 (f16: 2^-12) of it: the result
+    is theirs alone.  Each may lose 2^-39 of the 1 (half the last bit of an f16
+    subnormal after the scaling, which f16 itself has not); then sums."""
+    n, k, group = 40, 14336, 32
+    g = torch.Generator().manual_seed(m)
+    wt = W.random_weight(n, k, group, zeros, seed=m + 60)
+    z = 8 if wt[2] is None else wt[2][:, ::256 // group]
+    wt[0][:, ::128] = wt[0][:, ::128] & 0xf0 | z
+    x = (torch.randn(m, k, generator=g) * (2.0 ** -12 if kind == "f16" else 2.0 ** -20)).to(W.TYPES[kind])
+    x[:, ::256] = 1
+    w = W.weight(*wt, group)
+    assert (w[:, ::256] == 0).all()
+    want, small = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    lost = 0.0 if kind == "f16" else 2.0 ** -39 * w.abs().sum(1)
+    bound = (k + 4) * 2.0 ** -24 * small + lost + torch.finfo(W.TYPES[kind]).eps / 2 * want.abs() * (1 + 2 ** -9)
+    if kind == "f16":
+        bound = bound + 2.0 ** -25  # (the result may be subnormal)
+    assert (_linear(torch_dev, x, wt, group).double() - want).abs().le(bound).all()
+
+
+@pytest.mark.parametrize("shape", FEW, ids=lambda v: "x".join(map(str, v)))
+@pytest.mark.parametrize("zeros", [False, True])
+def test_linear_few_rows_of_bf16_by_group(torch_dev, shape, zeros):
+    """x in one group at a time, so that a lost group or another's scale shows: sums
+    of c x and of z x are off by (terms + 4) 2^-24 of the sum of (c + z) |x| s at most,
+    then one rounding to the type."""
+    m, n, k, group = shape
+    g = torch.Generator().manual_seed(m * n + k + 2)
+    wt = W.random_weight(n, k, group, zeros, seed=k + 70)
+    x = torch.randn(m, k, generator=g).to(torch.bfloat16)
+    w = W.weight(*wt, group)
+    z = 8.0 if wt[2] is None else W.spread(wt[2], k, group).double()
+    both = (W.unpack(wt[0]).double() + z) * W.spread(wt[1], k, group).double()
+    groups = -(-k // group)
+    for at in sorted({0, groups // 2, groups - 1, int(torch.randint(0, groups, (1,), generator=g))}):
+        cut = slice(at * group, min(k, at * group + group))
+        part = torch.zeros_like(x)
+        part[:, cut] = x[:, cut]
+        want = part.double() @ w.t()
+        size = part.double().abs() @ both.t()
+        bound = (cut.stop - cut.start + 4) * 2.0 ** -24 * size + 2.0 ** -8 * want.abs() * (1 + 2 ** -9)
+        assert (_linear(torch_dev, part, wt, group).double() - want).abs().le(bound).all(), at
+    want, size = x.double() @ w.t(), x.double().abs() @ both.t()
+    bound = (k + 4) * 2.0 ** -24 * size + 2.0 ** -8 * want.abs() * (1 + 2 ** -9)
+    assert (_linear(torch_dev, x, wt, group).double() - want).abs().le(bound).all()
