@@ -543,3 +543,38 @@ def test_tokens_before_position_0_are_reported(torch_dev, types, lens):
     st.zero_()
     gh.paged_append(*P.args(x), x["k"], x["v"], status=st)
     assert int(st) == 1
+
+
+# more than 1024 pages in one workgroup's keys, which takes those in turn (a small
+# hint keeps the axis whole): pages of 1 and 3 positions, pages of 16 past 16384 keys.
+# A window begins inside a page, so that such a turn ends inside a tile.
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("q_lens,kv_lens,page,window", [
+    ([1], [3000], 1, 0), ([1, 1], [5000, 1030], 3, 0), ([1], [5000], 3, 4001), ([2], [3500], 1, 2777),
+    ([1], [17500], 16, 0), ([1], [18000], 16, 16999), ([150], [3300], 1, 0), ([200, 1], [5000, 3200], 3, 0),
+    ([200], [5000], 3, 3333), ([140], [17001], 16, 0), ([140], [17001], 16, 16500),
+], ids=str)
+def test_more_pages_than_are_looked_up_at_once(torch_dev, types, q_lens, kv_lens, page, window):
+    b = P.batch(q_lens, kv_lens, heads=4, kv_heads=2, d=64, page=page, types=types, seed=57)
+    _check(_attend(torch_dev, b, window=window, max_kv_len=100), *P.attention(b, window=window))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("page,kv,window", [(1, 2500, 0), (3, 4000, 0), (3, 4000, 3301)])
+def test_more_pages_than_are_looked_up_at_once_of_many_heads(torch_dev, types, page, kv, window):
+    b = P.batch([520], [kv], d=32, heads=32, kv_heads=32, page=page, types=types, seed=58)
+    _check(_attend(torch_dev, b, window=window, max_kv_len=100), *P.attention(b, window=window))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("q_len,page,kv", [(1, 1, 3000), (4, 3, 4000), (150, 1, 3300), (200, 3, 5000)])
+def test_infinite_values_past_the_pages_looked_up_first(torch_dev, types, q_len, page, kv):
+    """One that every token sees, one that only the last does."""
+    b = P.batch([q_len], [kv], heads=4, kv_heads=2, d=64, page=page, types=types, seed=59)
+    for at, dim in ((kv - 400, 3), (kv - 1, 5)):
+        b["v_pages"][b["page_table"][0, at // page].long(), at % page, 1, dim] = float("inf")
+    want, bound = P.attention(b)
+    got = _attend(torch_dev, b, max_kv_len=100).double().cpu()
+    assert torch.equal(torch.isposinf(got), torch.isposinf(want)) and not torch.isnan(got).any()
+    fine = torch.isfinite(want)
+    assert (got - want).abs()[fine].le(bound[fine]).all()
