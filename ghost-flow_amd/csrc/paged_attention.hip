@@ -567,7 +567,9 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, h = lane >> 4;
     // Workgroups share no keys here, so they go round the XCDs as they come: a
-    // long sequence's then lie on all of them.
+    // long sequence's then lie on all of them.  (Only a sequence whose rows cross a
+    // multiple of 16 has two tiles that walk the same keys: with 7 heads to a group
+    // three of eight single tokens.)
     const int id = blockIdx.x;
     const int kvh = id % p.c.hkv, split = (id / p.c.hkv) % p.nsplit, number = id / p.c.hkv / p.nsplit;
     Rows t;

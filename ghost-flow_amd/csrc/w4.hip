@@ -324,10 +324,11 @@ __global__ __launch_bounds__(256) void w4_rows_kernel(W4LinearParams p) {
 // they join.  Scales and zero points are looked up per 32 columns, two of a row's
 // eight per lane, and go round through LDS.
 //
-// Bound by waits: a workgroup needs 4 us to its first slice and 1.5 us or more for
-// each (LDS reads, then the barrier), so two or more blocks of x take eight waves
-// of one tile each rather than four of two (f16, 50 x 4096 x 11008: 27.3 us against
-// 32.5 with the join).  K is split as far as the workgroups that fit the CUs go.
+// Bound by waits, which are this tiling's own: a workgroup needs 4 us to its first
+// slice and 1.5 us or more for each (LDS reads, then the barrier), so two or more
+// blocks of x take eight waves of one tile each rather than four of two (f16, 50 x
+// 4096 x 11008: 27.3 us against 32.5 with the join, where its bytes take 5).  K is
+// split as far as the workgroups that fit the CUs go.
 constexpr int kSlice = 256;
 typedef __attribute__((address_space(3))) void *lds_ptr_t;
 typedef __attribute__((address_space(1))) void *glb_ptr_t;
@@ -695,9 +696,10 @@ constexpr int kStreamTable = 32 << 10;  // bytes of LDS for scales and zero poin
 // should.
 //
 // Bound by requests: a CU takes 1 KB of x and W in some 30 cycles, and x, which
-// every workgroup reads whole from its L2, is four of five.  16 x 14336 x 4096:
-// 15.5 us with groups of 64 and zero points (34.5 MB, 2.2 TB/s); sixteen waves 15.4
-// there but 9.6 against 8.0 at 4096 x 4096 and 30 against 18 at 4096 x 14336.
+// every workgroup reads whole from its L2, is four of five (of 16 rows of W to a
+// workgroup; more rows to one would read less of x).  16 x 14336 x 4096: 15.5 us with
+// groups of 64 and zero points (34.5 MB, 2.2 TB/s); sixteen waves 15.4 there but 9.6
+// against 8.0 at 4096 x 4096 and 30 against 18 at 4096 x 14336.
 template <typename T, bool ZP, int PER>
 __global__ __launch_bounds__(64 * kStreamWaves, 4) void w4_stream_kernel(W4LinearParams p) {
     constexpr int R = 4, kAt = 2;  // slices on their way or in use, asked for at once
@@ -914,15 +916,14 @@ bool w4_streams(const LinearW4Desc &d) {
 }
 
 struct W4Plan {
-    int mb, rt, splits, kper;
+    int mb, splits, kper;
 };
 W4Plan w4_plan(const LinearW4Desc &d) {
     W4Plan pl{};
     const int64_t blocks = (d.m + 15) / 16;
     pl.mb = (int)std::min<int64_t>(blocks, d.dtype == GFH_F32 ? 2 : 4);
     if (pl.mb == 3) pl.mb = 4;
-    pl.rt = 2;
-    const int64_t tiles = (d.n + 64 * pl.rt - 1) / (64 * pl.rt) * ((d.m + 16 * pl.mb - 1) / (16 * pl.mb));
+    const int64_t tiles = (d.n + 127) / 128 * ((d.m + 16 * pl.mb - 1) / (16 * pl.mb));
     const int64_t slices = (d.k + kSlice - 1) / kSlice;
     // K is split as far as the workgroups that fit the CUs at once go
     const int64_t slots = (pl.mb > 1 || d.dtype == GFH_F32 ? 1 : 2) * device_cu_count();
@@ -1040,7 +1041,7 @@ int launch_linear_w4(const LinearW4Desc &d, void *workspace, hipStream_t s) {
     const W4Plan pl = w4_plan(d);
     p.splits = pl.splits;
     p.kper = pl.kper;
-    const int64_t gx = (d.n + 64 * pl.rt - 1) / (64 * pl.rt) * pl.splits, gy = (d.m + 16 * pl.mb - 1) / (16 * pl.mb);
+    const int64_t gx = (d.n + 127) / 128 * pl.splits, gy = (d.m + 16 * pl.mb - 1) / (16 * pl.mb);
     const dim3 grid((unsigned)gx, (unsigned)gy);
     typed([&](auto t) {
         using T = decltype(t);
