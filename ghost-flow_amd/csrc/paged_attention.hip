@@ -16,15 +16,17 @@
 //
 // Softmax online in base 2, statistics and sums in fp32: the running maximum
 // is of the raw dot products, a probability is exp2(s c - m c + bias) with c =
-// |scale| log2 e (the sign of the scale is on q).  Where q has 16 bits P is rounded
-// to its type for the second product, so that this is one matrix instruction and not
-// the three of an fp32 q: O is then off by up to half a step of the type relative to P
-// |V|, beside its own rounding (against 64 bits, root mean square of normal inputs:
-// bf16 2.1e-3 .. 2.3e-3 where O's rounding alone has 1.7e-3, f16 2.6e-4 and 2.2e-4).
-// l sums the rounded P, so the weights that V is taken with add up to one.  The bias
-// (14 or 9 for f16, 16 where P is split) keeps small probabilities normal in their
-// 16-bit form and cancels in O / l.  Long axes are split over workgroups; a second
-// kernel joins the parts in their order, so results do not depend on timing.
+// |scale| log2 e (the sign of the scale is on q).  fp32 q: P is carried as three bf16
+// pieces, or in fp32.  q of 16 bits: as two pieces of its type in tiles of 16 rows,
+// whose matrix units wait for bytes anyway (64 sequences of up to 4096 keys 134.2 us
+// with one, 136.3 with two; then O has its own rounding alone), and rounded to the type
+// in tiles of 128 rows, where a second piece would be a third more products: O is then
+// off by up to half a step of the type relative to P |V| as well (against 64 bits, root
+// mean square of normal inputs: bf16 2.3e-3 where O's rounding alone has 1.7e-3).
+// There l sums the rounded P, so the weights that V is taken with add up to one.  The
+// bias (14 or 9 for f16, 16 for three pieces) keeps small probabilities normal in
+// their 16-bit form and cancels in O / l.  Long axes are split over workgroups; a
+// second kernel joins the parts in their order, so results do not depend on timing.
 //
 // Rows of the cache past the last key and pages outside the cache read as
 // zeros.  A masked key must not reach a row even when its value is not
@@ -257,13 +259,19 @@ struct Half<_Float16> {
     }
 };
 
-// (x, y) as 16-bit pairs: one rounded to nearest (NP = 1), or their three
-// bf16 pieces (split_bf16.hpp).
+// (x, y) as 16-bit pairs: one rounded to nearest (NP = 1), that and what it leaves,
+// rounded (2), or their three bf16 pieces (split_bf16.hpp).
 template <typename T, int NP>
 __device__ __forceinline__ void pieces2(float x, float y, uint32_t (&w)[NP]) {
     if constexpr (NP == 1) {
         const f32x2 v = {x, y};
         w[0] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, typename Half<T>::v2));
+    } else if constexpr (NP == 2) {
+        const f32x2 v = {x, y};
+        const auto a = __builtin_convertvector(v, typename Half<T>::v2);
+        const f32x2 r = {x - (float)a[0], y - (float)a[1]};
+        w[0] = __builtin_bit_cast(uint32_t, a);
+        w[1] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, typename Half<T>::v2));
     } else {
         split2(x, y, w[0], w[1], w[2]);
     }
@@ -446,6 +454,18 @@ __device__ __forceinline__ bool not_finite(uint32_t w) {
     return (w & e) == e || ((w >> 16) & e) == e;
 }
 
+// Whether some element is infinite or NaN: 0 times it is NaN, and so is the sum of all.
+template <typename V, int N>
+__device__ __forceinline__ bool any_not_finite(const V (&o)[N]) {
+    V zero = o[0] * 0.f;
+#pragma unroll
+    for (int i = 1; i < N; ++i) zero += o[i] * 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int x = 0; x < (int)(sizeof(V) / 4); ++x) sum += zero[x];
+    return sum != sum;
+}
+
 // Whether x holds in any lane of the workgroup (a barrier on either side: the
 // caller may reuse its LDS).
 template <int WAVES>
@@ -556,6 +576,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     using v8 = typename H::v8;
     constexpr int NU = DP / 32, NB = DP / 16, kTile = 32 * DP * 2;
     constexpr int kOps = 2 * 32 * DP / 512;  // requests per tile and wave
+    constexpr int PP = NP > 1 ? NP : 2;      // pieces of P
     constexpr float kBias = NP > 1 ? 16.f : H::kBias;
     // wave, stage, K / V.  (One array for all: with several the compiler tells
     // them apart and waits for every request before any read of the rings.)
@@ -649,24 +670,23 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 pv[x] = __builtin_amdgcn_exp2f(fmaf(s[x >> 2][x & 3], p.sc2, kBias - mc));
-                if (NP > 1) sum += pv[x];
+                sum += pv[x];
             }
             m = m_new;
 #pragma unroll
             for (int i2 = 0; i2 < NB; ++i2) o[i2] *= alpha;
-            uint32_t pw[NP][4];
+            uint32_t pw[PP][4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                uint32_t two[NP];
-                pieces2<T, NP>(pv[2 * x], pv[2 * x + 1], two);
-                if (NP == 1) sum = H::add2(two[0], sum);  // what the product sees
+                uint32_t two[PP];
+                pieces2<T, PP>(pv[2 * x], pv[2 * x + 1], two);
 #pragma unroll
-                for (int q = 0; q < NP; ++q) pw[q][x] = two[q];
+                for (int q = 0; q < PP; ++q) pw[q][x] = two[q];
             }
             l = fmaf(l, alpha, sum);
-            v8 pf[NP];
+            v8 pf[PP];
 #pragma unroll
-            for (int q = 0; q < NP; ++q) {
+            for (int q = 0; q < PP; ++q) {
                 const i32x4 v = {(int)pw[q][0], (int)pw[q][1], (int)pw[q][2], (int)pw[q][3]};
                 pf[q] = __builtin_bit_cast(v8, v);
             }
@@ -680,7 +700,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
                     at[x] = key * DP * 2 + (((2 * (i4 + x) + ((c & 3) >> 1)) ^ swz_v<DP>(key)) << 4) + (c & 1) * 8;
                 read_tr4<16 * DP * 2>(vt, at, vf);
 #pragma unroll
-                for (int q = NP - 1; q >= 0; --q)
+                for (int q = PP - 1; q >= 0; --q)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) o[i4 + x] = H::mfma16(vf[x], pf[q], o[i4 + x]);
             }
@@ -693,12 +713,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     // 4 dims of a row.
     l = quarter_sum(l);
     const float mt = m == -INFINITY ? m : m * p.sc2;
-    if (kBias != 0.f) {
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) odd |= jmax >= 0 && !(fabsf(o[i][x]) < INFINITY);
-    }
+    odd |= jmax >= 0 && any_not_finite(o);
     constexpr int kRow = DP + 4;
     static_assert(WAVES * 16 * (kRow + 2) * 4 <= kRing, "states over the rings");
     float *const accs = reinterpret_cast<float *>(lds);
@@ -942,10 +957,7 @@ __global__ __launch_bounds__(256, 2) void paged_chunk_kernel(AttnParams p) {
         pb = pe;
     }
 
-#pragma unroll
-    for (int i = 0; i < NB; ++i)
-#pragma unroll
-        for (int x = 0; x < 16; ++x) odd |= jmax >= 0 && !(fabsf(o[i][x]) < INFINITY);
+    odd |= jmax >= 0 && any_not_finite(o);
     if (any_wave<4>(odd, flags, wave, lane)) {
         slow_rows<TA, T>(p, t, seq, kvh, b, e, split, nact > 1, kBias, wave, 4, lane);
         return;
@@ -1279,11 +1291,7 @@ __global__ __launch_bounds__(256, 2) void paged_f32_chunk_kernel(AttnParams p) {
     }
     l = quarter_sum(l);
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int y = 0; y < 4; ++y)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) odd |= jmax >= 0 && !(fabsf(o[v][y][x]) < INFINITY);
+    for (int v = 0; v < NV; ++v) odd |= jmax >= 0 && any_not_finite(o[v]);
     if (any_wave<4>(odd, flags, wave, lane)) {
         slow_rows<float, float>(p, t, seq, kvh, b, e, split, nact > 1, 0.f, wave, 4, lane);
         return;

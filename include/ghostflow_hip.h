@@ -462,10 +462,12 @@ GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, 
  * for the token at position p: j <= p if causal, j > p - window if window > 0.
  * A token that sees no key gets zeros.  q [tokens, heads, head_dim], rows ldq
  * apart, out the same, rows ldo apart (out may be q with ldo = ldq), of type
- * dtype as in gfh_paged_append.  Scores, softmax and sums in fp32; with q of 16 bits
- * the probabilities are rounded to its type before P . V and in their sum (half a
- * step each, relative to P |V|), with fp32 q they are not (over a bf16 cache: fp32
- * products of the stored values); out is rounded once.
+ * dtype as in gfh_paged_append.  Scores, softmax and sums in fp32, out rounded once;
+ * with fp32 q fp32 products of the stored values.  With q of 16 bits the probabilities
+ * meet V as two values of its type (16 bits in all for bf16, 22 for f16) where the
+ * call takes a sequence in tiles of 16 rows (single tokens, short chunks), and rounded
+ * to one, in their sum too (half a step, relative to P |V|), where in tiles of 128
+ * (prompts, and a few single tokens in one batch with them).
  * max_kv_len: the longest length of the batch as far as the caller knows (0:
  * max_pages * page_size); the work is split by it, the results hold for any
  * length.  workspace (nullable, 16-byte aligned) of at least

@@ -426,8 +426,8 @@ def test_on_another_stream(torch_dev):
 @pytest.mark.parametrize("lens", [([1], [30]), ([1], [900]), ([1] * 40, [4000] * 40), ([40], [900]), ([1, 300], [70, 1100])],
                          ids=lambda v: "-".join(map(str, (len(v[0]), v[0][-1]))))
 def test_weights_add_up_to_what_the_product_sees(torch_dev, types, lens):
-    """Where V is one value the result is that value: the weights, rounded for the
-    product, are rounded in their sum too.  Every 32nd key has weight 1, the others
+    """Where V is one value the result is that value: weights that are rounded for the
+    product are rounded in their sum too.  Every 32nd key has weight 1, the others
     w.  Sums of n fp32 terms and a few more operations are off by (n + 16) 2^-24
     relatively, which is less than half a step of 16 bits, so those give the value
     itself."""
@@ -578,3 +578,17 @@ def test_infinite_values_past_the_pages_looked_up_first(torch_dev, types, q_len,
     assert torch.equal(torch.isposinf(got), torch.isposinf(want)) and not torch.isnan(got).any()
     fine = torch.isfinite(want)
     assert (got - want).abs()[fine].le(bound[fine]).all()
+
+
+@pytest.mark.parametrize("types", [("bf16", "bf16"), ("f16", "f16")], ids="/".join)
+@pytest.mark.parametrize("lens", [([1], [300]), ([1], [5000]), ([1] * 6, [33, 1, 700, 64, 129, 2000]), ([3, 0, 1, 4], [50, 40, 65, 300])],
+                         ids=lambda v: "-".join(map(str, v[0])))
+def test_single_tokens_lose_nothing_to_the_weights(torch_dev, types, lens):
+    """As _paged's bound, but for the weights' rounding: two pieces leave half a step
+    of half a step."""
+    h = P.half_step(P.TYPES[types[0]])
+    for heads, kv_heads, d in ((8, 2, 128), (4, 4, 64)):
+        b = P.batch(*lens, heads=heads, kv_heads=kv_heads, d=d, page=16, types=types, seed=61)
+        want, bound = P.attention(b)
+        size = P.attention(dict(b, v_pages=b["v_pages"].abs()))[0]
+        _check(_attend(torch_dev, b), want, bound - size * (h - h * h))
