@@ -20,8 +20,8 @@
 // pieces, or in fp32.  q of 16 bits: as two pieces of its type in tiles of 16 rows,
 // whose matrix units wait for bytes anyway (64 sequences of up to 4096 keys 134.2 us
 // with one, 136.3 with two; then O has its own rounding alone), and rounded to the type
-// in tiles of 128 rows, where a second piece would be a third more products: O is then
-// off by up to half a step of the type relative to P |V| as well (against 64 bits, root
+// in tiles of 128 rows, where a second piece would be half as many products more: O is
+// then off by up to half a step of the type relative to P |V| as well (against 64 bits, root
 // mean square of normal inputs: bf16 2.3e-3 where O's rounding alone has 1.7e-3).
 // There l sums the rounded P, so the weights that V is taken with add up to one.  The
 // bias (14 or 9 for f16, 16 for three pieces) keeps small probabilities normal in
@@ -568,8 +568,8 @@ __device__ __forceinline__ void join_waves(const AttnParams &p, const Rows &t, i
 // same order (two transposing reads: keys 4 h .., 16 + 4 h ..).
 //
 // Bound by bytes: 64 sequences of 1024 .. 4096 keys, 32 heads over 8 of 128, bf16,
-// 659 MB: 126 us (5.2 TB/s) and 4.9 to join; the matrix units have 16 rows for the
-// group's 4 and are busy 4% of the cycles.
+// 659 MB: 131 us (5.0 TB/s) and 4.8 to join; the matrix units have 16 rows for the
+// group's 4 and are busy 4.5% of the cycles.
 template <typename TA, typename T, int DP, int NP, int WAVES>
 __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) {
     using H = Half<T>;
@@ -1385,7 +1385,7 @@ struct Plan {
 // Waves of a few-row workgroup: two, so that two or more workgroups share a CU;
 // as many as the LDS takes where there are too few tiles to fill the CUs and a
 // length that such a workgroup walks in a few steps: no split and no second launch
-// (12 heads of 64 over 517 keys, f16: 8.6 us and 3.9 to join -> 9.4).
+// (12 heads of 64 over 517 keys, f16: 8.6 us and 3.9 to join -> 9.7).
 constexpr int kDecodeWaves = 2, kWideWaves64 = 8, kWideWaves128 = 4;
 constexpr int kWideKeys = 96;  // per wave
 constexpr int kAll = INT32_MAX;
