@@ -592,3 +592,30 @@ def test_single_tokens_lose_nothing_to_the_weights(torch_dev, types, lens):
         want, bound = P.attention(b)
         size = P.attention(dict(b, v_pages=b["v_pages"].abs()))[0]
         _check(_attend(torch_dev, b), want, bound - size * (h - h * h))
+
+
+@pytest.mark.parametrize("types", P.PAIRS, ids="/".join)
+@pytest.mark.parametrize("lens", [([1], [300]), ([3], [4000]), ([60], [300]), ([300], [500])],
+                         ids=lambda v: "-".join(map(str, v)))
+@pytest.mark.parametrize("d", [24, 64, 128])
+def test_rows_one_by_one_over_a_page_outside_the_cache(torch_dev, types, lens, d):
+    """A NaN that only the last token sees sends its workgroup's rows through their
+    keys one by one; the pages outside the cache read as zeros there too."""
+    gh = _gh()
+    b = P.batch(*lens, heads=4, kv_heads=2, d=d, page=16, types=types, seed=62, spare=5)
+    n = lens[1][0]
+    where = b["page_table"][0, (n - 1) // 16].long(), (n - 1) % 16, 1, 2
+    b["v_pages"][where] = float("nan")
+    unused = sorted(set(range(b["k_pages"].shape[0])) - set(b["page_table"].flatten().tolist()))[0]
+    for pages in ("k_pages", "v_pages"):
+        b[pages][unused] = 0
+    bad = dict(b, page_table=b["page_table"].clone())
+    for at in (0, 7, 8, 9, 10, 16):
+        b["page_table"][0, at] = unused
+        bad["page_table"][0, at] = -1 if at % 2 else 10 ** 6
+    want, bound = P.attention(b)
+    x = P.to(bad, torch_dev)
+    got = gh.paged_attention(x["q"], *P.args(x)).double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.isnan(got[-1, 2:, 2]).all()
+    fine = torch.isfinite(want)
+    assert (got - want).abs()[fine].le(bound[fine]).all()
