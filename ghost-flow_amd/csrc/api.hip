@@ -1039,7 +1039,8 @@ GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t token
         const char *who = "paged_attention";
         GFH_TRY(check_paged(who, kv, dtype, tokens, heads));
         if (window < 0) return set_error(GFH_INVALID_SHAPE, "%s: window %lld", who, (long long)window);
-        if (!std::isfinite(scale)) return set_error(GFH_INVALID_DATA, "%s: scale is not finite", who);
+        if (!std::isfinite(scale * 1.5f))  // (times log2 e)
+            return set_error(GFH_INVALID_DATA, "%s: scale %g is out of range", who, (double)scale);
         if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
         GFH_TRY(check_paged_memory(who, kv));
         GFH_TRY(check_rows(who, q, "q", dtype, tokens, heads, kv->head_dim, ldq));

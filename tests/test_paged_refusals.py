@@ -118,3 +118,13 @@ def test_more_tokens_than_a_launch_can_have():
             assert rc in (L.INVALID_DATA, L.COMPUTATION_FAILED) and word not in lib.gfh_last_error()
         else:
             assert rc == L.INVALID_SHAPE and word in lib.gfh_last_error(), lib.gfh_last_error()
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("-inf"), 3e38, -3e38])
+def test_scales_out_of_range(scale):
+    """Times log2 e they have to be finite: 0 times them is 0 then."""
+    L, lib = _lib()
+    assert _attend(lib, _kv(L), L.BF16, scale=scale) == L.INVALID_DATA
+    assert b"scale" in lib.gfh_last_error()
+    assert _attend(lib, _kv(L), L.BF16, scale=2e38) in (L.INVALID_DATA, L.COMPUTATION_FAILED)
+    assert b"scale" not in lib.gfh_last_error()
