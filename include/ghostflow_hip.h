@@ -224,8 +224,8 @@ GFH_API int gfh_dequantize_i4_grouped(const uint8_t *codes, const float *scales,
  * ldx and of y ldy elements apart.  Products of x with (c - z) in fp32, a
  * group's sum times its scale, sums in fp32, y rounded once.  x is carried
  *   m <= 2 (fp32: m <= 4), and f16: with all its bits;
- *   bf16, 3 .. 16 rows, n k < 2^27, at most 255 groups to a row and (k / 32) (group /
- *   32) < 2^32: with all its bits, as a group's sum of c x less z times its sum of x;
+ *   bf16, 3 .. 16 rows, n k < 2^27, at most 255 groups to a row and one group or (k /
+ *   32 + 4) (group / 32) < 2^32: with all its bits, as a group's sum of c x less z times its sum of x;
  *   otherwise relative to the largest magnitude of its row in each 256 columns:
  *   fp32 with at least 33 bits below it, bf16 with 8 bits down to 2^-29 of it.
  * An infinite or NaN x gives inf / NaN.  Meant for few rows
