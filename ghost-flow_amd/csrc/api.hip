@@ -130,7 +130,7 @@ int sgemm_common(int trans_a, int trans_b, int64_t m, int64_t n, int64_t k, floa
 
 namespace {
 
-int elem_bytes(int dtype) { return dtype == GFH_F32 ? 4 : 2; }
+int elem_bytes(int dtype) { return dtype == GFH_F32 ? 4 : dtype == GFH_U8 ? 1 : 2; }
 
 // A 4-bit weight's sizes: [n, k] in groups of `group` columns.
 int check_w4(const char *who, int64_t n, int64_t k, int64_t group) {
@@ -153,14 +153,28 @@ int check_w4_memory(const char *who, const uint8_t *codes, const float *scales, 
     return GFH_SUCCESS;
 }
 
-// The checks that both calls over a paged cache make of it and of the batch.
-int check_paged(const char *who, const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads) {
+// The checks that the calls over a paged cache make of it and of the batch.  scales:
+// of a cache of 8 bits, NULL for the others; any_types: activations of any type over
+// these too.
+int check_paged(const char *who, const gfh_paged_kv *kv, int dtype, int64_t tokens, int64_t heads,
+                const gfh_paged_scales *scales = nullptr, bool any_types = false) {
     if (!kv) return set_error(GFH_NULL_POINTER, "%s: kv is NULL", who);
-    const bool types = kv->dtype == GFH_F16 || kv->dtype == GFH_BF16 || kv->dtype == GFH_F32;
-    if (!types || !(dtype == kv->dtype || (dtype == GFH_F32 && kv->dtype == GFH_BF16)))
+    auto floating = [](int t) { return t == GFH_F16 || t == GFH_BF16 || t == GFH_F32; };
+    if (scales) {
+        if (kv->dtype != GFH_U8 || !floating(dtype))
+            return set_error(GFH_INVALID_DATA, "%s: dtype %d over a cache of dtype %d with scales (f16, bf16 or f32 over u8)",
+                             who, dtype, kv->dtype);
+        if (kv->head_dim % 16 != 0)
+            return set_error(GFH_INVALID_SHAPE, "%s: head_dim %lld of a cache of 8 bits must be a multiple of 16", who,
+                             (long long)kv->head_dim);
+        if (scales->page_stride < 0 || scales->head_stride < 0)
+            return set_error(GFH_INVALID_SHAPE, "%s: negative stride of the scales", who);
+    } else if (!floating(kv->dtype) || !(any_types ? floating(dtype)
+                                                   : dtype == kv->dtype || (dtype == GFH_F32 && kv->dtype == GFH_BF16))) {
         return set_error(GFH_INVALID_DATA,
                          "%s: activations of dtype %d over a cache of dtype %d (the same, or f32 over bf16)", who,
                          dtype, kv->dtype);
+    }
     if (kv->head_dim < 8 || kv->head_dim > 128 || kv->head_dim % 8 != 0)
         return set_error(GFH_INVALID_SHAPE, "%s: head_dim %lld must be a multiple of 8 in [8, 128]", who,
                          (long long)kv->head_dim);
@@ -185,7 +199,7 @@ int check_paged(const char *who, const gfh_paged_kv *kv, int dtype, int64_t toke
     return GFH_SUCCESS;
 }
 
-int check_paged_memory(const char *who, const gfh_paged_kv *kv) {
+int check_paged_memory(const char *who, const gfh_paged_kv *kv, const gfh_paged_scales *scales = nullptr) {
     int64_t e = 0, a, b, c;
     if (kv->num_pages > 0) {
         if (!mul_ok(kv->num_pages - 1, kv->page_stride, &a) || !mul_ok(kv->page_size - 1, kv->row_stride, &b) ||
@@ -205,6 +219,17 @@ int check_paged_memory(const char *who, const gfh_paged_kv *kv) {
     GFH_TRY(optional_range(kv->status, 4, "status"));
     if (!aligned16(kv->k_pages) || !aligned16(kv->v_pages))
         return set_error(GFH_INVALID_DATA, "%s: k_pages and v_pages must be 16-byte aligned", who);
+    if (scales) {
+        e = 0;
+        if (kv->num_pages > 0) {
+            if (!mul_ok(kv->num_pages - 1, scales->page_stride, &a) || !mul_ok(kv->kv_heads - 1, scales->head_stride, &b) ||
+                !count_ok({a, 4}) || !count_ok({b, 4}))
+                return set_error(GFH_INVALID_SHAPE, "%s: extent of the scales overflows", who);
+            e = a + b + kv->page_size;
+        }
+        GFH_TRY(require_range(scales->k, (size_t)e, "k_scales"));
+        GFH_TRY(require_range(scales->v, (size_t)e, "v_scales"));
+    }
     return GFH_SUCCESS;
 }
 
@@ -232,6 +257,90 @@ PagedAttnDesc paged_attn_desc(const gfh_paged_kv &kv, int64_t tokens, int64_t he
     d.max_kv_len = max_kv_len <= 0 || max_kv_len > capacity ? capacity : max_kv_len;
     d.window = window >= capacity ? 0 : window;
     return d;
+}
+
+// gfh_paged_append's and gfh_paged_append_norm's arguments: what does not need the memory.
+int append_desc(const char *who, const gfh_paged_kv *kv, const gfh_paged_scales *scales, int dtype, int64_t tokens,
+                int64_t heads, const void *q, int64_t ldq, void *q_out, int64_t ldqo, const void *k, int64_t ldk,
+                const void *v, int64_t ldv, const float *rope_cos, const float *rope_sin, int64_t rope_rows,
+                int64_t rotary_dim, int interleaved, PagedAppendDesc &d) {
+    GFH_TRY(check_paged(who, kv, dtype, tokens, heads, scales));
+    if (!q != !q_out) return set_error(GFH_NULL_POINTER, "%s: q and q_out are given together", who);
+    if (!rope_cos != !rope_sin)
+        return set_error(GFH_NULL_POINTER, "%s: rope_cos and rope_sin are given together", who);
+    const int64_t capacity = kv->max_pages * kv->page_size;
+    if (rope_cos && (rotary_dim < 8 || rotary_dim % 8 != 0 || rotary_dim > kv->head_dim))
+        return set_error(GFH_INVALID_SHAPE, "%s: rotary_dim %lld must be a multiple of 8 in [8, head_dim]", who,
+                         (long long)rotary_dim);
+    if (rope_cos && (rope_rows < capacity || rope_rows > ((int64_t)1 << 40)))
+        return set_error(GFH_INVALID_SHAPE, "%s: angles of %lld positions, the page table holds %lld", who,
+                         (long long)rope_rows, (long long)capacity);
+    d.kv = *kv;
+    d.dtype = dtype;
+    d.tokens = tokens;
+    d.heads = heads;
+    d.q = q, d.k = k, d.v = v;
+    d.q_out = q_out;
+    d.ldq = ldq, d.ldqo = ldqo, d.ldk = ldk, d.ldv = ldv;
+    d.cos = rope_cos, d.sin = rope_sin;
+    d.rotary_dim = rotary_dim;
+    d.interleaved = interleaved != 0;
+    return GFH_SUCCESS;
+}
+
+// The launch and the memory of an append.
+int check_append(const char *who, const PagedAppendDesc &d, const gfh_paged_scales *scales, int64_t rope_rows,
+                 int64_t blocks) {
+    if (blocks > kMaxBlocks256)
+        return set_error(GFH_INVALID_SHAPE, "%s: %lld tokens of %lld heads are more than one launch can have", who,
+                         (long long)d.tokens, (long long)d.heads);
+    GFH_TRY(check_paged_memory(who, &d.kv, scales));
+    if (d.q) {
+        GFH_TRY(check_rows(who, d.q, "q", d.dtype, d.tokens, d.heads, d.kv.head_dim, d.ldq));
+        GFH_TRY(check_rows(who, d.q_out, "q_out", d.dtype, d.tokens, d.heads, d.kv.head_dim, d.ldqo));
+        if (d.q == d.q_out && d.ldq != d.ldqo)
+            return set_error(GFH_INVALID_SHAPE, "%s: q_out on q needs the same rows", who);
+    }
+    GFH_TRY(check_rows(who, d.k, "k", d.dtype, d.tokens, d.kv.kv_heads, d.kv.head_dim, d.ldk));
+    GFH_TRY(check_rows(who, d.v, "v", d.dtype, d.tokens, d.kv.kv_heads, d.kv.head_dim, d.ldv));
+    if (d.cos) {
+        GFH_TRY(require_range(d.cos, (size_t)rope_rows * (d.rotary_dim / 2) * 4, "rope_cos"));
+        GFH_TRY(require_range(d.sin, (size_t)rope_rows * (d.rotary_dim / 2) * 4, "rope_sin"));
+        if (!aligned16(d.cos) || !aligned16(d.sin))
+            return set_error(GFH_INVALID_DATA, "%s: rope_cos and rope_sin must be 16-byte aligned", who);
+    }
+    return GFH_SUCCESS;
+}
+
+// gfh_paged_attention, or with scales gfh_paged_attention_q8.
+int attend(const char *who, const gfh_paged_kv *kv, const gfh_paged_scales *scales, int dtype, int64_t tokens,
+           int64_t heads, const void *q, int64_t ldq, void *out, int64_t ldo, float scale, int causal, int64_t window,
+           int64_t max_kv_len, void *workspace, size_t workspace_bytes, gfh_stream_t stream) {
+    GFH_TRY(check_paged(who, kv, dtype, tokens, heads, scales));
+    if (window < 0) return set_error(GFH_INVALID_SHAPE, "%s: window %lld", who, (long long)window);
+    if (!std::isfinite(scale * 1.5f))  // (times log2 e)
+        return set_error(GFH_INVALID_DATA, "%s: scale %g is out of range", who, (double)scale);
+    if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
+    GFH_TRY(check_paged_memory(who, kv, scales));
+    GFH_TRY(check_rows(who, q, "q", dtype, tokens, heads, kv->head_dim, ldq));
+    GFH_TRY(check_rows(who, out, "out", dtype, tokens, heads, kv->head_dim, ldo));
+    if (q == out && ldq != ldo) return set_error(GFH_INVALID_SHAPE, "%s: out on q needs the same rows", who);
+    if (workspace && !aligned16(workspace))
+        return set_error(GFH_INVALID_DATA, "%s: the workspace must be 16-byte aligned", who);
+    GFH_TRY(ensure_init());
+    PagedAttnDesc d = paged_attn_desc(*kv, tokens, heads, max_kv_len, window);
+    d.dtype = dtype;
+    d.q = q;
+    d.ldq = ldq;
+    d.out = out;
+    d.ldo = ldo;
+    d.scale = scale;
+    d.causal = causal != 0;
+    hipStream_t s = as_stream(stream);
+    Scratch ws;
+    const size_t need = scales ? paged_attention_q8_workspace_bytes(d) : paged_attention_workspace_bytes(d);
+    if (need) GFH_TRY(ws.acquire(workspace, workspace_bytes, need, s));
+    return scales ? launch_paged_attention_q8(d, *scales, ws.ptr(), s) : launch_paged_attention(d, ws.ptr(), s);
 }
 
 }  // namespace
@@ -978,49 +1087,65 @@ GFH_API int gfh_paged_append(const gfh_paged_kv *kv, int dtype, int64_t tokens, 
                              int64_t rotary_dim, int interleaved, gfh_stream_t stream) {
     return guarded([&]() -> int {
         const char *who = "paged_append";
-        GFH_TRY(check_paged(who, kv, dtype, tokens, heads));
-        if (!q != !q_out) return set_error(GFH_NULL_POINTER, "%s: q and q_out are given together", who);
-        if (!rope_cos != !rope_sin)
-            return set_error(GFH_NULL_POINTER, "%s: rope_cos and rope_sin are given together", who);
-        const int64_t capacity = kv->max_pages * kv->page_size;
-        if (rope_cos && (rotary_dim < 8 || rotary_dim % 8 != 0 || rotary_dim > kv->head_dim))
-            return set_error(GFH_INVALID_SHAPE, "%s: rotary_dim %lld must be a multiple of 8 in [8, head_dim]", who,
-                             (long long)rotary_dim);
-        if (rope_cos && (rope_rows < capacity || rope_rows > ((int64_t)1 << 40)))
-            return set_error(GFH_INVALID_SHAPE, "%s: angles of %lld positions, the page table holds %lld", who,
-                             (long long)rope_rows, (long long)capacity);
-        if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
         PagedAppendDesc d;
-        d.kv = *kv;
-        d.dtype = dtype;
-        d.tokens = tokens;
-        d.heads = heads;
-        d.q = q, d.k = k, d.v = v;
-        d.q_out = q_out;
-        d.ldq = ldq, d.ldqo = ldqo, d.ldk = ldk, d.ldv = ldv;
-        d.cos = rope_cos, d.sin = rope_sin;
-        d.rotary_dim = rotary_dim;
-        d.interleaved = interleaved != 0;
-        if (paged_append_blocks(d) > kMaxBlocks256)
-            return set_error(GFH_INVALID_SHAPE, "%s: %lld tokens of %lld heads are more than one launch can have", who,
-                             (long long)tokens, (long long)heads);
-        GFH_TRY(check_paged_memory(who, kv));
-        if (q) {
-            GFH_TRY(check_rows(who, q, "q", dtype, tokens, heads, kv->head_dim, ldq));
-            GFH_TRY(check_rows(who, q_out, "q_out", dtype, tokens, heads, kv->head_dim, ldqo));
-            if (q == q_out && ldq != ldqo)
-                return set_error(GFH_INVALID_SHAPE, "%s: q_out on q needs the same rows", who);
-        }
-        GFH_TRY(check_rows(who, k, "k", dtype, tokens, kv->kv_heads, kv->head_dim, ldk));
-        GFH_TRY(check_rows(who, v, "v", dtype, tokens, kv->kv_heads, kv->head_dim, ldv));
-        if (rope_cos) {
-            GFH_TRY(require_range(rope_cos, (size_t)rope_rows * (rotary_dim / 2) * 4, "rope_cos"));
-            GFH_TRY(require_range(rope_sin, (size_t)rope_rows * (rotary_dim / 2) * 4, "rope_sin"));
-            if (!aligned16(rope_cos) || !aligned16(rope_sin))
-                return set_error(GFH_INVALID_DATA, "%s: rope_cos and rope_sin must be 16-byte aligned", who);
-        }
+        GFH_TRY(append_desc(who, kv, nullptr, dtype, tokens, heads, q, ldq, q_out, ldqo, k, ldk, v, ldv, rope_cos, rope_sin,
+                            rope_rows, rotary_dim, interleaved, d));
+        if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
+        GFH_TRY(check_append(who, d, nullptr, rope_rows, paged_append_blocks(d)));
         GFH_TRY(ensure_init());
         return launch_paged_append(d, as_stream(stream));
+    });
+}
+
+GFH_API int gfh_paged_append_norm(const gfh_paged_kv *kv, const gfh_paged_scales *scales, int dtype, int64_t tokens,
+                                  int64_t heads, const void *q, int64_t ldq, void *q_out, int64_t ldqo, const void *k,
+                                  int64_t ldk, const void *v, int64_t ldv, const float *rope_cos, const float *rope_sin,
+                                  int64_t rope_rows, int64_t rotary_dim, int interleaved, const float *q_norm,
+                                  const float *k_norm, double norm_eps, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "paged_append_norm";
+        PagedAppendDesc d;
+        GFH_TRY(append_desc(who, kv, scales, dtype, tokens, heads, q, ldq, q_out, ldqo, k, ldk, v, ldv, rope_cos, rope_sin,
+                            rope_rows, rotary_dim, interleaved, d));
+        if ((q_norm || k_norm) && !(norm_eps >= 0.0 && std::isfinite(norm_eps)))
+            return set_error(GFH_INVALID_DATA, "%s: norm_eps %g must be finite and at least 0", who, norm_eps);
+        if (q_norm && !q) return set_error(GFH_NULL_POINTER, "%s: q_norm without q", who);
+        if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
+        GFH_TRY(check_append(who, d, scales, rope_rows, paged_append_norm_blocks(d)));
+        GFH_TRY(optional_range(q_norm, (size_t)kv->head_dim * 4, "q_norm"));
+        GFH_TRY(optional_range(k_norm, (size_t)kv->head_dim * 4, "k_norm"));
+        if (!aligned16(q_norm) || !aligned16(k_norm))
+            return set_error(GFH_INVALID_DATA, "%s: q_norm and k_norm must be 16-byte aligned", who);
+        GFH_TRY(ensure_init());
+        PagedNormDesc n;
+        if (scales) n.scales = *scales;
+        n.q_norm = q_norm, n.k_norm = k_norm;
+        n.eps = norm_eps;
+        return launch_paged_append_norm(d, n, as_stream(stream));
+    });
+}
+
+GFH_API int gfh_paged_read(const gfh_paged_kv *kv, const gfh_paged_scales *scales, int dtype, int64_t tokens, void *k_out,
+                           int64_t ldk, void *v_out, int64_t ldv, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "paged_read";
+        GFH_TRY(check_paged(who, kv, dtype, tokens, kv ? kv->kv_heads : 0, scales, true));
+        if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
+        PagedReadDesc d;
+        d.kv = *kv;
+        if (scales) d.scales = *scales;
+        d.dtype = dtype;
+        d.tokens = tokens;
+        d.k_out = k_out, d.v_out = v_out;
+        d.ldk = ldk, d.ldv = ldv;
+        if (paged_read_blocks(d) > kMaxBlocks256)
+            return set_error(GFH_INVALID_SHAPE, "%s: %lld tokens are more than one launch can have", who,
+                             (long long)tokens);
+        GFH_TRY(check_paged_memory(who, kv, scales));
+        GFH_TRY(check_rows(who, k_out, "k_out", dtype, tokens, kv->kv_heads, kv->head_dim, ldk));
+        GFH_TRY(check_rows(who, v_out, "v_out", dtype, tokens, kv->kv_heads, kv->head_dim, ldv));
+        GFH_TRY(ensure_init());
+        return launch_paged_read(d, as_stream(stream));
     });
 }
 
@@ -1036,32 +1161,29 @@ GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t token
                                 int64_t ldq, void *out, int64_t ldo, float scale, int causal, int64_t window,
                                 int64_t max_kv_len, void *workspace, size_t workspace_bytes, gfh_stream_t stream) {
     return guarded([&]() -> int {
-        const char *who = "paged_attention";
-        GFH_TRY(check_paged(who, kv, dtype, tokens, heads));
-        if (window < 0) return set_error(GFH_INVALID_SHAPE, "%s: window %lld", who, (long long)window);
-        if (!std::isfinite(scale * 1.5f))  // (times log2 e)
-            return set_error(GFH_INVALID_DATA, "%s: scale %g is out of range", who, (double)scale);
-        if (tokens == 0 || kv->num_seqs == 0) return GFH_SUCCESS;
-        GFH_TRY(check_paged_memory(who, kv));
-        GFH_TRY(check_rows(who, q, "q", dtype, tokens, heads, kv->head_dim, ldq));
-        GFH_TRY(check_rows(who, out, "out", dtype, tokens, heads, kv->head_dim, ldo));
-        if (q == out && ldq != ldo) return set_error(GFH_INVALID_SHAPE, "%s: out on q needs the same rows", who);
-        if (workspace && !aligned16(workspace))
-            return set_error(GFH_INVALID_DATA, "%s: the workspace must be 16-byte aligned", who);
-        GFH_TRY(ensure_init());
-        PagedAttnDesc d = paged_attn_desc(*kv, tokens, heads, max_kv_len, window);
-        d.dtype = dtype;
-        d.q = q;
-        d.ldq = ldq;
-        d.out = out;
-        d.ldo = ldo;
-        d.scale = scale;
-        d.causal = causal != 0;
-        hipStream_t s = as_stream(stream);
-        Scratch ws;
-        const size_t need = paged_attention_workspace_bytes(d);
-        if (need) GFH_TRY(ws.acquire(workspace, workspace_bytes, need, s));
-        return launch_paged_attention(d, ws.ptr(), s);
+        return attend("paged_attention", kv, nullptr, dtype, tokens, heads, q, ldq, out, ldo, scale, causal, window,
+                      max_kv_len, workspace, workspace_bytes, stream);
+    });
+}
+
+GFH_API size_t gfh_paged_attention_q8_workspace_size(const gfh_paged_kv *kv, int64_t tokens, int64_t heads,
+                                                     int64_t window, int64_t max_kv_len) {
+    const gfh_paged_scales none{};
+    if (!kv || window < 0 || check_paged("paged_attention_q8", kv, GFH_F32, tokens, heads, &none) != GFH_SUCCESS ||
+        tokens == 0 || kv->num_seqs == 0)
+        return 0;
+    return paged_attention_q8_workspace_bytes(paged_attn_desc(*kv, tokens, heads, max_kv_len, window));
+}
+
+GFH_API int gfh_paged_attention_q8(const gfh_paged_kv *kv, const gfh_paged_scales *scales, int dtype, int64_t tokens,
+                                   int64_t heads, const void *q, int64_t ldq, void *out, int64_t ldo, float scale,
+                                   int causal, int64_t window, int64_t max_kv_len, void *workspace,
+                                   size_t workspace_bytes, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "paged_attention_q8";
+        if (!scales) return set_error(GFH_NULL_POINTER, "%s: scales is NULL", who);
+        return attend(who, kv, scales, dtype, tokens, heads, q, ldq, out, ldo, scale, causal, window, max_kv_len, workspace,
+                      workspace_bytes, stream);
     });
 }
 

@@ -196,6 +196,25 @@ struct PagedAppendDesc {
 };
 int64_t paged_append_blocks(const PagedAppendDesc &d);  // of its grid
 int launch_paged_append(const PagedAppendDesc &d, hipStream_t s);
+// paged_append_norm.hip: kv.dtype GFH_U8 goes with scales; the norms nullable.
+struct PagedNormDesc {
+    gfh_paged_scales scales{};
+    const float *q_norm = nullptr, *k_norm = nullptr;
+    double eps = 0.0;
+};
+int64_t paged_append_norm_blocks(const PagedAppendDesc &d);
+int launch_paged_append_norm(const PagedAppendDesc &d, const PagedNormDesc &n, hipStream_t s);
+// paged_read.hip: dtype of the output.
+struct PagedReadDesc {
+    gfh_paged_kv kv{};
+    gfh_paged_scales scales{};
+    int dtype = 0;
+    int64_t tokens = 0;
+    void *k_out = nullptr, *v_out = nullptr;
+    int64_t ldk = 0, ldv = 0;
+};
+inline int64_t paged_read_blocks(const PagedReadDesc &d) { return (d.tokens + 3) / 4; }
+int launch_paged_read(const PagedReadDesc &d, hipStream_t s);
 // paged_attention.hip: max_kv_len in [0, capacity] is what the work is split
 // by; any length is served.  window 0: none.
 struct PagedAttnDesc {
@@ -212,6 +231,9 @@ struct PagedAttnDesc {
 };
 size_t paged_attention_workspace_bytes(const PagedAttnDesc &d);
 int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t s);
+// paged_attention_q8.hip: the same over a cache of 8 bits.
+size_t paged_attention_q8_workspace_bytes(const PagedAttnDesc &d);
+int launch_paged_attention_q8(const PagedAttnDesc &d, const gfh_paged_scales &scales, void *workspace, hipStream_t s);
 
 // w4.hip: 4-bit weights in groups of columns (codes [n, k / 2], scales and
 // zero points [n, ceil(k / group)], zps nullable), k and group multiples of 32.

@@ -21,7 +21,7 @@
 namespace gfh {
 namespace paged {
 
-enum Status : int { kBadLength = 1, kBadPage = 2 };
+enum Status : int { kBadLength = 1, kBadPage = 2, kBadValue = 4 };
 
 struct View {
     char *k, *v;

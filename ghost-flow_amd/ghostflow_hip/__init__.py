@@ -30,6 +30,7 @@ from .ops import (  # noqa: F401
     paged_append,
     paged_attention,
     paged_attention_workspace_size,
+    paged_read,
     qlinear,
     qlinear_dynamic,
     qswiglu,

@@ -32,7 +32,7 @@ STATUS_NAMES = {
 }
 
 # Element types (gfh_dtype): the dtype bytes of a state dict.
-F16, BF16, F32 = 0, 1, 2
+F16, BF16, F32, U8 = 0, 1, 2, 8
 
 _p = C.c_void_p
 _i = C.c_int
@@ -79,6 +79,11 @@ SIGNATURES = {
                               _p]),
     "gfh_paged_attention_workspace_size": (_sz, [_p, _i64, _i64, _i64, _i64]),
     "gfh_paged_attention": (_i, [_p, _i, _i64, _i64, _p, _i64, _p, _i64, _f, _i, _i64, _i64, _p, _sz, _p]),
+    "gfh_paged_append_norm": (_i, [_p, _p, _i, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _p, _i64,
+                                   _i64, _i, _p, _p, C.c_double, _p]),
+    "gfh_paged_read": (_i, [_p, _p, _i, _i64, _p, _i64, _p, _i64, _p]),
+    "gfh_paged_attention_q8_workspace_size": (_sz, [_p, _i64, _i64, _i64, _i64]),
+    "gfh_paged_attention_q8": (_i, [_p, _p, _i, _i64, _i64, _p, _i64, _p, _i64, _f, _i, _i64, _i64, _p, _sz, _p]),
     "gfh_silu_mul_f32": (_i, [_p, _p, _p, _i64, _p]),
     "gfh_state_dict_open": (_i, [C.c_char_p, C.POINTER(C.c_void_p)]),
     "gfh_state_dict_close": (None, [_p]),
@@ -134,6 +139,11 @@ class PagedKv(C.Structure):
                 ("page_table", C.c_void_p), ("max_pages", C.c_int64), ("table_stride", C.c_int64),
                 ("num_seqs", C.c_int64), ("kv_lens", C.c_void_p), ("q_offsets", C.c_void_p),
                 ("status", C.c_void_p)]
+
+
+class PagedScales(C.Structure):
+    """gfh_paged_scales (include/ghostflow_hip.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64)]
 
 
 def load():

@@ -28,7 +28,7 @@ import torch
 
 from . import _lib
 from .ops import (GhostFlowError, flash_attention_blockwise, linear, mha_forward_cached, mha_forward_with_cache,
-                  paged_append, paged_attention, qswiglu, quantize_per_channel, qweight_rowsum, silu_mul, swiglu)
+                  paged_append, paged_attention, paged_read, qswiglu, quantize_per_channel, qweight_rowsum, silu_mul, swiglu)
 from .quantization import GroupQuantizedLinear
 
 
@@ -110,7 +110,12 @@ class PagedKVCache:
     """Keys and values of many sequences in pages of page_size positions,
     k_pages and v_pages [num_pages, page_size, num_kv_heads, head_dim].  The
     host keeps which pages a sequence has: add() opens one, extend() gives
-    sequences the pages for their next tokens, remove() takes them back."""
+    sequences the pages for their next tokens, remove() takes them back.
+
+    dtype uint8: 8 bits to a value, with k_scales and v_scales [num_pages,
+    num_kv_heads, page_size] for the steps (gfh_paged_scales in
+    ghostflow_hip.h); half the memory of a 16-bit cache, for activations of any
+    type."""
 
     def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, *, dtype=torch.float32,
                  device="cuda"):
@@ -118,6 +123,10 @@ class PagedKVCache:
             raise GhostFlowError(_lib.INVALID_SHAPE, "a paged cache needs pages, positions, heads and dimensions")
         self.k_pages = torch.empty((num_pages, page_size, num_kv_heads, head_dim), dtype=dtype, device=device)
         self.v_pages = torch.empty_like(self.k_pages)
+        self.k_scales = self.v_scales = None
+        if dtype == torch.uint8:
+            self.k_scales = torch.empty((num_pages, num_kv_heads, page_size), dtype=dtype, device=device)
+            self.v_scales = torch.empty_like(self.k_scales)
         self._free = list(range(num_pages - 1, -1, -1))
         self._pages: dict[int, list[int]] = {}
         self._lens: dict[int, int] = {}
@@ -139,6 +148,17 @@ class PagedKVCache:
         seq, self._next = self._next, self._next + 1
         self._pages[seq], self._lens[seq] = [], 0
         return seq
+
+    def read(self, seq: int, dtype=torch.float32):
+        """The sequence's keys and values, [length, num_kv_heads, head_dim]
+        each."""
+        if seq not in self._pages:
+            raise GhostFlowError(_lib.INVALID_DATA, f"no sequence {seq}")
+        n, dev = self._lens[seq], self.k_pages.device
+        pages = self._pages[seq] or [-1]
+        flat = torch.tensor([0, n, n] + pages, dtype=torch.int32).to(dev)
+        return paged_read(self.k_pages, self.v_pages, flat[None, 3:], flat[:2], flat[2:3], tokens=n, dtype=dtype,
+                          k_scales=self.k_scales, v_scales=self.v_scales)
 
     def remove(self, seq: int) -> None:
         """The sequence's pages are free again (kernels that still read them
@@ -199,8 +219,20 @@ class MultiHeadAttention:
             mk((embed_dim, embed_dim), wb) for _ in range(4))
         self.q_bias, self.k_bias, self.v_bias, self.out_bias = (mk((embed_dim,), bb) for _ in range(4))
         self.w4 = None  # 4-bit projections, after quantize_grouped()
+        self.q_norm = self.k_norm = None  # weights [head_dim] of norms per head, after enable_qk_norm()
+        self.norm_eps = 1e-6
 
-    def _weights(self):
+    def enable_qk_norm(self, eps: float = 1e-6) -> None:
+        """Queries and keys are normed per head in front of the rotation:
+        weights q_norm and k_norm [head_dim], one at first.  Of step_paged
+        alone; the other calls refuse such a layer."""
+        self.q_norm = torch.ones(self.head_dim, dtype=torch.float32, device=self.q_weight.device)
+        self.k_norm = torch.ones_like(self.q_norm)
+        self.norm_eps = eps
+
+    def _weights(self, norms=False):
+        if self.q_norm is not None and not norms:
+            raise GhostFlowError(_lib.INVALID_DATA, "norms of queries and keys are of step_paged alone")
         if self.training and self.dropout_p > 0:
             raise GhostFlowError(_lib.INVALID_DATA, "attention dropout is not implemented on this path; "
                                  "call eval() or use dropout 0")
@@ -240,8 +272,9 @@ class MultiHeadAttention:
         prompt's chunks and single tokens in one call.  cos and sin
         [positions, rotary_dim / 2] turn queries and keys; they cover whole
         pages of the longest sequence.  fp32, or after quantize_grouped() any
-        type that the cache takes."""
-        weights = self._weights()
+        type that the cache takes.  After enable_qk_norm() queries and keys are
+        normed first."""
+        weights = self._weights(norms=True)
         if x.dim() != 2 or tuple(x.shape) != (batch.tokens, self.embed_dim):
             raise GhostFlowError(_lib.INVALID_SHAPE, f"x must be [{batch.tokens}, {self.embed_dim}], got {list(x.shape)}")
         if self.w4 is not None:
@@ -250,13 +283,16 @@ class MultiHeadAttention:
             project = lambda i, t: linear(t, weights[2 * i], weights[2 * i + 1])  # noqa: E731
         q, k, v = (project(i, x).view(-1, self.num_heads, self.head_dim) for i in range(3))
         pages = (cache.k_pages, cache.v_pages, batch.page_table, batch.q_offsets, batch.kv_lens)
-        paged_append(*pages, k, v, q=q, q_out=q, cos=cos, sin=sin, interleaved=interleaved)
-        y = paged_attention(q, *pages, window=window, max_kv_len=batch.max_kv_len, out=q)
+        scales = {"k_scales": cache.k_scales, "v_scales": cache.v_scales}
+        paged_append(*pages, k, v, q=q, q_out=q, cos=cos, sin=sin, interleaved=interleaved, q_norm=self.q_norm,
+                     k_norm=self.k_norm, norm_eps=self.norm_eps, **scales)
+        y = paged_attention(q, *pages, window=window, max_kv_len=batch.max_kv_len, out=q, **scales)
         return project(3, y.view(-1, self.embed_dim))
 
     def parameters(self):
+        norms = [] if self.q_norm is None else [self.q_norm, self.k_norm]
         return [self.q_weight, self.q_bias, self.k_weight, self.k_bias, self.v_weight, self.v_bias,
-                self.out_weight, self.out_bias]
+                self.out_weight, self.out_bias] + norms
 
     def train(self):
         self.training = True

@@ -552,6 +552,7 @@ def _rows(t, name, like, tokens, heads, d):
 
 
 _PAGED_KV = struct.Struct("@PPi7qP3qPPP")  # gfh_paged_kv; packed by hand, a ctypes Structure costs 3 us more
+_PAGED_SCALES = struct.Struct("@PP2q")  # gfh_paged_scales
 
 
 def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
@@ -560,7 +561,7 @@ def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
     if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype != k_pages.dtype:
         raise GhostFlowError(_lib.INVALID_SHAPE, "k_pages and v_pages must be [pages, page_size, kv_heads, head_dim], of "
                              "one type and with one layout")
-    dt = _dtype(k_pages, "k_pages")
+    dt = _lib.U8 if k_pages.dtype == torch.uint8 else _dtype(k_pages, "k_pages")
     pages, page_size, hkv, d = shape
     sp, sr, sh, sd = stride
     if sd != 1 and d > 1:
@@ -587,17 +588,43 @@ def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
     return kv, hkv, d
 
 
+def _paged_scales(k_scales, v_scales, k_pages):
+    """gfh_paged_scales of the step bytes [pages, kv_heads, page_size] that go
+    with pages of 8 bits, None for others."""
+    if (k_scales is None) != (v_scales is None) or (k_scales is None) == (k_pages.dtype == torch.uint8):
+        raise GhostFlowError(_lib.INVALID_DATA, "k_scales and v_scales go with pages of uint8, and those with both")
+    if k_scales is None:
+        return None
+    pages, page_size, hkv, _ = k_pages.shape
+    shape, stride = k_scales.shape, k_scales.stride()
+    if shape != (pages, hkv, page_size) or v_scales.shape != shape or v_scales.stride() != stride:
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"k_scales and v_scales must be [{pages}, {hkv}, {page_size}] with one "
+                             f"layout, got {list(shape)} and {list(v_scales.shape)}")
+    if k_scales.dtype != torch.uint8 or v_scales.dtype != torch.uint8 or (page_size > 1 and stride[2] != 1):
+        raise GhostFlowError(_lib.INVALID_DATA, "k_scales and v_scales must be uint8, the rows of a page contiguous")
+    if k_scales.device != k_pages.device or v_scales.device != k_pages.device:
+        raise GhostFlowError(_lib.INVALID_DATA, f"k_scales and v_scales must be on {k_pages.device}")
+    return _PAGED_SCALES.pack(k_scales.data_ptr(), v_scales.data_ptr(), stride[0] if pages > 1 else 0,
+                              stride[1] if hkv > 1 else 0)
+
+
 def paged_append(k_pages, v_pages, page_table, q_offsets, kv_lens, k, v, *, q=None, q_out=None, cos=None, sin=None,
-                 interleaved=False, status=None):
+                 interleaved=False, status=None, k_scales=None, v_scales=None, q_norm=None, k_norm=None, norm_eps=1e-6):
     """Writes the new tokens' k and v [tokens, kv_heads, head_dim] into their
     sequences' pages [pages, page_size, kv_heads, head_dim], k turned by the
     rotary tables cos / sin [positions, rotary_dim / 2] (fp32) at the tokens'
     positions, and returns q [tokens, heads, head_dim] turned the same way
     (into q_out, which may be q; None without q).  gfh_paged_kv in
     ghostflow_hip.h says what page_table [seqs, pages], q_offsets [seqs + 1],
-    kv_lens [seqs] (the new tokens included) and status (all int32) are."""
+    kv_lens [seqs] (the new tokens included) and status (all int32) are.
+
+    q_norm and k_norm [head_dim] (fp32): queries and keys are first normed per
+    head, x / sqrt(mean(x^2) + norm_eps) * weight.  k_scales and v_scales
+    [pages, kv_heads, page_size] with pages, all uint8: rows are written in 8
+    bits, with the byte of their step (gfh_paged_scales)."""
     dev = k.device
     kv, hkv, d = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev)
+    scales = _paged_scales(k_scales, v_scales, k_pages)
     dt = _dtype(k, "k")
     tokens = k.shape[0] if k.dim() else 0
     ldk = _rows(k, "k", k, tokens, hkv, d)
@@ -623,21 +650,63 @@ def paged_append(k_pages, v_pages, page_table, q_offsets, kv_lens, k, v, *, q=No
         _same_device(dev, cos, sin)
         rows, half = cos.shape
         cp, sp = cos.data_ptr(), sin.data_ptr()
-    _call(dev, lib().gfh_paged_append, kv, dt, tokens, heads, qp, ldq, qop, ldqo, k.data_ptr(), ldk, v.data_ptr(), ldv,
-          cp, sp, rows, 2 * half, 1 if interleaved else 0)
+    if scales is None and q_norm is None and k_norm is None:
+        _call(dev, lib().gfh_paged_append, kv, dt, tokens, heads, qp, ldq, qop, ldqo, k.data_ptr(), ldk, v.data_ptr(),
+              ldv, cp, sp, rows, 2 * half, 1 if interleaved else 0)
+        return q_out
+    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is None:
+            continue
+        _need(w, torch.float32, name)
+        _same_device(dev, w)
+        if w.shape != (d,):
+            raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be [{d}], got {list(w.shape)}")
+    _call(dev, lib().gfh_paged_append_norm, kv, scales, dt, tokens, heads, qp, ldq, qop, ldqo, k.data_ptr(), ldk,
+          v.data_ptr(), ldv, cp, sp, rows, 2 * half, 1 if interleaved else 0, _ptr(q_norm), _ptr(k_norm),
+          float(norm_eps))
     return q_out
 
 
+def paged_read(k_pages, v_pages, page_table, q_offsets, kv_lens, *, tokens=None, dtype=torch.float32, k_out=None,
+               v_out=None, status=None, k_scales=None, v_scales=None):
+    """What the pages hold at the batch's new positions, as dense k and v
+    [tokens, kv_heads, head_dim] (into k_out and v_out, else of dtype): the
+    inverse of paged_append.  A batch with as many new tokens as positions
+    reads its sequences whole.  Arguments as paged_append's; without k_out and
+    v_out, tokens is the last of q_offsets where the caller does not give it
+    (which waits for the device).  Rows behind the last sequence are left as
+    they are, and zero in tensors made here."""
+    dev = k_pages.device
+    kv, hkv, d = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev)
+    scales = _paged_scales(k_scales, v_scales, k_pages)
+    if (k_out is None) != (v_out is None):
+        raise GhostFlowError(_lib.INVALID_DATA, "k_out and v_out are given together")
+    if k_out is None:
+        if tokens is None:
+            tokens = int(q_offsets[-1])
+        k_out = torch.zeros((tokens, hkv, d), dtype=dtype, device=dev)
+        v_out = torch.zeros_like(k_out)
+    dt = _dtype(k_out, "k_out")
+    tokens = k_out.shape[0] if k_out.dim() else 0
+    _same_device(dev, k_out)
+    ldk = _rows(k_out, "k_out", k_out, tokens, hkv, d)
+    ldv = _rows(v_out, "v_out", k_out, tokens, hkv, d)
+    _call(dev, lib().gfh_paged_read, kv, scales, dt, tokens, k_out.data_ptr(), ldk, v_out.data_ptr(), ldv)
+    return k_out, v_out
+
+
 def paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, *, scale=None, causal=True, window=0,
-                    max_kv_len=None, out=None, workspace=None, status=None):
+                    max_kv_len=None, out=None, workspace=None, status=None, k_scales=None, v_scales=None):
     """Attention of the new tokens q [tokens, heads, head_dim] over their
     sequences' pages (arguments as paged_append's): token at position p sees
     the keys j < kv_len, j <= p if causal, j > p - window if window.  Returns
     out like q (which may be q); rows behind the last sequence are left as
     they are, and zero in an out made here.  max_kv_len: the batch's longest
-    length where the caller knows it."""
+    length where the caller knows it.  k_scales and v_scales go with pages of
+    uint8; q is then of any type."""
     dev = q.device
     kv, _, d = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev)
+    scales = _paged_scales(k_scales, v_scales, k_pages)
     dt = _dtype(q, "q")
     if q.dim() != 3:
         raise GhostFlowError(_lib.INVALID_SHAPE, "q must be [tokens, heads, head_dim]")
@@ -652,8 +721,12 @@ def paged_attention(q, k_pages, v_pages, page_table, q_offsets, kv_lens, *, scal
     if workspace is not None:
         _same_device(dev, workspace)
         ws, ws_bytes = _workspace(workspace)
-    _call(dev, lib().gfh_paged_attention, kv, dt, tokens, heads, q.data_ptr(), ldq, out.data_ptr(), ldo, float(scale),
-          1 if causal else 0, int(window), int(max_kv_len or 0), ws, ws_bytes)
+    rest = (dt, tokens, heads, q.data_ptr(), ldq, out.data_ptr(), ldo, float(scale), 1 if causal else 0, int(window),
+            int(max_kv_len or 0), ws, ws_bytes)
+    if scales is None:
+        _call(dev, lib().gfh_paged_attention, kv, *rest)
+    else:
+        _call(dev, lib().gfh_paged_attention_q8, kv, scales, *rest)
     return out
 
 
@@ -661,8 +734,9 @@ def paged_attention_workspace_size(q, k_pages, v_pages, page_table, q_offsets, k
                                    max_kv_len=None) -> int:
     """Bytes of paged_attention's workspace for these arguments."""
     kv, _, _ = _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, None, q.device)
-    return int(lib().gfh_paged_attention_workspace_size(kv, q.shape[0], q.shape[1], int(window),
-                                                          int(max_kv_len or 0)))
+    size = (lib().gfh_paged_attention_q8_workspace_size if k_pages.dtype == torch.uint8
+            else lib().gfh_paged_attention_workspace_size)
+    return int(size(kv, q.shape[0], q.shape[1], int(window), int(max_kv_len or 0)))
 
 
 # ---- SwiGLU feed-forward block (ghostflow-nn/src/llama.rs:259-287) -------------

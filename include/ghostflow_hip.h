@@ -68,7 +68,7 @@ typedef void *gfh_stream_t;
 
 /* Element types of activations and caches where a call takes several: the
  * dtype bytes of the state dict (ghostflow-core/src/serialize.rs:188-215). */
-typedef enum gfh_dtype { GFH_F16 = 0, GFH_BF16 = 1, GFH_F32 = 2 } gfh_dtype;
+typedef enum gfh_dtype { GFH_F16 = 0, GFH_BF16 = 1, GFH_F32 = 2, GFH_U8 = 8 } gfh_dtype;
 
 /* ---- library ----------------------------------------------------------- */
 
@@ -480,6 +480,60 @@ GFH_API int gfh_paged_attention(const gfh_paged_kv *kv, int dtype, int64_t token
                                 const void *q, int64_t ldq, void *out, int64_t ldo, float scale,
                                 int causal, int64_t window, int64_t max_kv_len, void *workspace,
                                 size_t workspace_bytes, gfh_stream_t stream);
+
+/* ---- key/value cache of 8 bits, norms of queries and keys ------------------ */
+
+/* A cache whose pages hold codes: gfh_paged_kv with dtype GFH_U8 (strides in bytes)
+ * and a byte for the step of every row, a row being the head_dim dims of a
+ * key/value head at a position (its key or its value):
+ *   k, v   the byte of row r of page p, key/value head hh, at p * page_stride +
+ *          hh * head_stride + r
+ *   step   s(b) = (8 + b % 8) 2^(b / 8 - 22) of a byte b in [0, 207] (larger ones
+ *          count as 207); code c stands for (c - 128) s
+ *   written: b = the smallest with 127 s(b) >= max|x|, c = clamp(round(x / s), -127,
+ *          127) + 128, x in fp32, round half away from zero.  A NaN counts as 0, and
+ *          magnitudes above 15240 as that; either sets bit 2 of *status.
+ * head_dim is a multiple of 16.  Rows need head_dim + 1 bytes.  Attention is fastest
+ * where page_size, both strides and both pointers are multiples of 8. */
+typedef struct gfh_paged_scales {
+    uint8_t *k, *v;
+    int64_t page_stride, head_stride;
+} gfh_paged_scales;
+
+/* gfh_paged_append with norms of queries and keys in front of the rotation, into any
+ * cache: scales with a GFH_U8 cache (dtype is any), else NULL (dtype as there).
+ *   q_norm, k_norm [head_dim] fp32 weights, 16-byte aligned, nullable each:
+ *   y = (x r) w,  r = 1 / sqrt(mean(x^2) + norm_eps)  per head and token
+ * the mean in fp64, r and every later operation rounded to fp32, then to the output's
+ * type once.  v is not normed. */
+GFH_API int gfh_paged_append_norm(const gfh_paged_kv *kv, const gfh_paged_scales *scales, int dtype, int64_t tokens,
+                                  int64_t heads, const void *q, int64_t ldq, void *q_out, int64_t ldqo, const void *k,
+                                  int64_t ldk, const void *v, int64_t ldv, const float *rope_cos, const float *rope_sin,
+                                  int64_t rope_rows, int64_t rotary_dim, int interleaved, const float *q_norm,
+                                  const float *k_norm, double norm_eps, gfh_stream_t stream);
+
+/* The cached rows at the new tokens' positions as dense values of type dtype:
+ * k_out, v_out [tokens, kv_heads, head_dim], rows ldk / ldv elements apart.  A batch
+ * with as many tokens as positions (q_len = kv_lens[s]) reads its sequences whole.
+ * scales as in gfh_paged_append_norm; any dtype over any cache, rounded once.  Rows
+ * behind the last sequence, and of positions that the table cannot hold, are left as
+ * they are; a page outside the cache reads as zeros. */
+GFH_API int gfh_paged_read(const gfh_paged_kv *kv, const gfh_paged_scales *scales, int dtype, int64_t tokens, void *k_out,
+                           int64_t ldk, void *v_out, int64_t ldv, gfh_stream_t stream);
+
+/* gfh_paged_attention over a GFH_U8 cache, q and out of any dtype.  Keys and values
+ * meet q and P as the exact values that the codes stand for; fp32 q as two f16 pieces
+ * of its row's range (22 bits, and 2^-39 of the row's largest magnitude), 16-bit q
+ * with all its bits down to that.  P meets V as two f16 pieces, and for q of 16 bits in
+ * tiles of 128 rows (prompts) rounded to f16, in its sum too.  The cache holds nothing
+ * infinite or NaN; a row of q that does gets NaN (zeros where all its scores are
+ * -inf).  Scores, softmax and sums in fp32, out rounded once. */
+GFH_API size_t gfh_paged_attention_q8_workspace_size(const gfh_paged_kv *kv, int64_t tokens, int64_t heads,
+                                                     int64_t window, int64_t max_kv_len);
+GFH_API int gfh_paged_attention_q8(const gfh_paged_kv *kv, const gfh_paged_scales *scales, int dtype, int64_t tokens,
+                                   int64_t heads, const void *q, int64_t ldq, void *out, int64_t ldo, float scale,
+                                   int causal, int64_t window, int64_t max_kv_len, void *workspace,
+                                   size_t workspace_bytes, gfh_stream_t stream);
 
 /* ---- SwiGLU feed-forward block ------------------------------------------ */
 

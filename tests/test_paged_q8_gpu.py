@@ -1,0 +1,500 @@
+"""A paged cache of 8 bits on the GPU: codes and steps as the rule has them,
+values read back, and attention over them against 64 bits."""
+import math
+
+import pytest
+import torch
+
+import _paged as P
+import _q8 as Q
+
+pytestmark = pytest.mark.gpu
+
+
+def _gh():
+    import ghostflow_hip as gh
+
+    return gh
+
+
+# ---- append and read ---------------------------------------------------------------
+
+def _append(b, dev, *, cos=None, sin=None, interleaved=False, q_norm=None, k_norm=None, eps=1e-6, status=None):
+    gh = _gh()
+    x = Q.to(b, dev)
+    move = lambda t: None if t is None else t.to(dev)  # noqa: E731
+    extra = Q.scales(x) if "k_scales" in b else {}
+    q = gh.paged_append(*P.args(x), x["k"], x["v"], q=x["q"], cos=move(cos), sin=move(sin), interleaved=interleaved,
+                        q_norm=move(q_norm), k_norm=move(k_norm), norm_eps=eps, status=status, **extra)
+    return q, x
+
+
+def _expected(b, *, cos=None, sin=None, interleaved=False, k_norm=None, eps=1e-6):
+    """Pages and step bytes after the append."""
+    pages = {n: b[n].clone() for n in ("k_pages", "v_pages", "k_scales", "v_scales")}
+    for s in range(len(b["kv_lens"])):
+        a, e = int(b["q_offsets"][s]), int(b["q_offsets"][s + 1])
+        for t in range(a, e):
+            p = int(b["kv_lens"][s]) - (e - t)
+            at, row = int(b["page_table"][s, p // b["page"]]), p % b["page"]
+            k = Q.turned(Q.normed(b["k"][t], k_norm, eps), p, cos, sin, interleaved)
+            for n, x in (("k", k), ("v", b["v"][t].float())):
+                pages[n + "_pages"][at, row], pages[n + "_scales"][at, :, row] = Q.quantise(x)
+    return pages
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,d,rot,interleaved,norm", [
+    (4, 2, 64, 64, False, True), (8, 8, 128, 64, True, True), (5, 1, 80, 80, False, False), (6, 3, 48, 8, False, True),
+    (3, 1, 16, 16, True, False), (7, 1, 112, 0, False, True), (2, 2, 96, 24, True, True), (32, 8, 128, 128, False, False),
+])
+def test_codes_and_steps(torch_dev, kind, heads, kv_heads, d, rot, interleaved, norm):
+    """Every byte of the cache, written or not, is the rule's: the norm's sum is in
+    64 bits and every later operation is one fp32 rounding, so there is nothing
+    to allow for.  The queries are within their one rounding, and the norm's and
+    the rotation's few in fp32."""
+    g = torch.Generator().manual_seed(d)
+    b = Q.batch([3, 1, 0, 20], [19, 1, 4, 20], kind=kind, heads=heads, kv_heads=kv_heads, d=d, page=7, pad=2, seed=d)
+    b["k"] *= 1.5
+    cos, sin = P.angles(28, rot) if rot else (None, None)
+    w = [1 + 0.3 * torch.randn(d, generator=g) if norm else None for _ in range(2)]
+    q, x = _append(b, torch_dev, cos=cos, sin=sin, interleaved=interleaved, q_norm=w[0], k_norm=w[1])
+    want = _expected(b, cos=cos, sin=sin, interleaved=interleaved, k_norm=w[1])
+    for n, t in want.items():
+        assert torch.equal(x[n].cpu(), t), n
+    off = b["q_offsets"].tolist()
+    for s, n in enumerate(b["kv_lens"].tolist()):
+        for t in range(off[s], off[s + 1]):
+            y = b["q"][t].double()
+            if norm:
+                y = y / (y.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w[0].double()
+            size = y.abs().amax()
+            y = P.turned(y, n - (off[s + 1] - t), cos, sin, interleaved)
+            assert ((q[t].cpu().double() - y).abs() <= P.half_step(b["q"].dtype) * y.abs() + 8 * 2.0 ** -24 * size).all()
+    # read back: the cached values rounded once
+    pages = (x["k_pages"], x["v_pages"], x["page_table"], x["kv_lens"].new_tensor([0, 19, 20, 24, 44]), x["kv_lens"])
+    for dt in P.TYPES.values():
+        got = _gh().paged_read(*pages, dtype=dt, **Q.scales(x))
+        for y, n in zip(got, ("k", "v")):
+            rows = torch.cat([P.rows_of({**b, n + "_pages": Q.values(want[n + "_pages"], want[n + "_scales"].transpose(1, 2))},
+                                        s)[0 if n == "k" else 1] for s in range(4)])
+            assert torch.equal(y.cpu(), rows.to(dt))
+
+
+@pytest.mark.parametrize("types", P.PAIRS)
+@pytest.mark.parametrize("d,rot,interleaved,which", [(64, 64, False, "qk"), (80, 40, True, "k"), (24, 8, False, "q"),
+                                                     (128, 0, False, "qk"), (8, 8, True, "qk")])
+def test_norms_into_other_caches(torch_dev, types, d, rot, interleaved, which):
+    """Norms and rotation against 64 bits: one rounding to the type, and three
+    operations for the norm and three for the rotation in fp32 on values that the
+    pair's length bounds."""
+    g = torch.Generator().manual_seed(d + 1)
+    b = P.batch([2, 0, 9], [30, 5, 9], heads=6, kv_heads=2, d=d, page=5, types=types, pad=1, seed=d)
+    cos, sin = P.angles(30, rot) if rot else (None, None)
+    w = {x: 1 + 0.3 * torch.randn(d, generator=g) for x in which}
+    x = P.to(b, torch_dev)
+    move = lambda t: None if t is None else t.to(torch_dev)  # noqa: E731
+    q = _gh().paged_append(*P.args(x), x["k"], x["v"], q=x["q"], cos=move(cos), sin=move(sin), interleaved=interleaved,
+                           q_norm=move(w.get("q")), k_norm=move(w.get("k")), norm_eps=1e-5)
+    off = b["q_offsets"].tolist()
+    written = torch.zeros(b["k_pages"].shape[:2], dtype=torch.bool)
+    for s, n in enumerate(b["kv_lens"].tolist()):
+        for t in range(off[s], off[s + 1]):
+            p = n - (off[s + 1] - t)
+            at, row = int(b["page_table"][s, p // b["page"]]), p % b["page"]
+            written[at, row] = True
+            for name, got in (("q", q[t]), ("k", x["k_pages"][at, row])):
+                y = b[name][t].double()
+                if name in w:
+                    y = y / (y.square().mean(-1, keepdim=True) + 1e-5).sqrt() * w[name].double()
+                size = y.abs().amax()
+                y = P.turned(y, p, cos, sin, interleaved)
+                h = P.half_step(got.dtype)
+                assert ((got.cpu().double() - y).abs() <= h * y.abs() + 8 * 2.0 ** -24 * size).all(), (name, t)
+            assert torch.equal(x["v_pages"][at, row].cpu(), b["v"][t].to(b["v_pages"].dtype))
+    for n in ("k_pages", "v_pages"):  # nothing else is touched
+        assert torch.equal(x[n].cpu()[~written].nan_to_num(7.0), b[n][~written].nan_to_num(7.0))
+    got = _gh().paged_read(x["k_pages"], x["v_pages"], x["page_table"], x["q_offsets"], x["kv_lens"], tokens=12,
+                           dtype=torch.float32)
+    for t in range(11):
+        s = 0 if t < 2 else 2
+        p = int(b["kv_lens"][s]) - (off[s + 1] - t)
+        at, row = int(b["page_table"][s, p // 5]), p % 5
+        assert torch.equal(got[0][t], x["k_pages"][at, row].float()) and torch.equal(got[1][t], x["v_pages"][at, row].float())
+    assert (got[0][11] == 0).all()
+
+
+def test_values_at_the_ends(torch_dev):
+    """Zeros, the smallest and largest steps, halves between two codes, values
+    that no step holds: their codes, and the bit of status."""
+    d, inf, nan = 16, float("inf"), float("nan")
+    rows = torch.zeros(12, 1, d)
+    rows[1] = torch.arange(d) * 2.0 ** -22 * 4  # halves of the smallest step
+    rows[2, 0, 0], rows[2, 0, 1] = 127 * 9 * 2.0 ** -10, 4.5 * 9 * 2.0 ** -10
+    rows[3] = -(torch.arange(d) + 0.5) * 2.0 ** -5
+    rows[4] = 15240.0
+    rows[5] = torch.linspace(-15240, 15240, d)
+    rows[6, 0, 3] = 1e-40
+    rows[7] = torch.tensor([127.0, 126.5] * 8) * (1 + 2.0 ** -23)
+    b = Q.batch([12], [12], kind="f32", heads=1, kv_heads=1, d=d, page=16, seed=1)
+    b["k"], b["v"] = rows, rows.flip(0)
+    status = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+    _, x = _append(b, torch_dev, status=status)
+    for n, t in _expected(b).items():
+        assert torch.equal(x[n].cpu(), t), n
+    assert int(status) == 0
+    for bad in (inf, -inf, nan, 15240.0 * (1 + 2.0 ** -22), -3e38):
+        rows[2, 0, 5] = bad
+        b["k"], b["v"] = rows, torch.zeros_like(rows)
+        status.zero_()
+        _, x = _append(b, torch_dev, status=status)
+        for n, t in _expected(b).items():
+            assert torch.equal(x[n].cpu(), t), (bad, n)
+        assert int(status) == 4, bad
+
+
+def test_what_cannot_be_written(torch_dev):
+    """Bad pages and lengths: nothing is written for them, their bits are set,
+    reading gives zeros or leaves the row."""
+    b = Q.batch([4, 4], [8, 8], kind="bf16", heads=2, kv_heads=2, d=32, page=4, seed=2)
+    b["page_table"][0, 1] = -1
+    b["page_table"][1, 1] = 10 ** 6
+    status = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+    _, x = _append(b, torch_dev, status=status)
+    for n in ("k_pages", "v_pages", "k_scales", "v_scales"):
+        assert torch.equal(x[n].cpu(), b[n])
+    assert int(status) == 2
+    status.zero_()
+    k, v = (torch.full((8, 2, 32), 5.0, device=torch_dev) for _ in range(2))
+    _gh().paged_read(*P.args(x), k_out=k, v_out=v, status=status, **Q.scales(x))
+    assert int(status) == 2 and (k == 0).all() and (v == 0).all()
+    x["kv_lens"][0] = 2  # two of its four tokens lie before position 0
+    x["kv_lens"][1] = 11  # the table holds 8
+    x["page_table"].zero_()
+    status.zero_()
+    k.fill_(5.0)
+    _gh().paged_read(*P.args(x), k_out=k, v_out=v, status=status, **Q.scales(x))
+    assert int(status) == 1 and (k[:2] == 5).all() and (k[2:4] != 5).any() and (k[5:] == 5).all()
+
+
+@pytest.mark.parametrize("layout,steps_like", [("heads", "rows"), ("rows", "pages"), ("heads", "pages")])
+def test_layouts(torch_dev, layout, steps_like):
+    b = Q.batch([5, 1], [21, 9], kind="f16", heads=4, kv_heads=2, d=64, page=8, seed=3, layout=layout, steps_like=steps_like)
+    _, x = _append(b, torch_dev)
+    after = {**b, **_expected(b)}
+    for n in ("k_pages", "v_pages", "k_scales", "v_scales"):
+        assert torch.equal(x[n].cpu(), after[n]), n
+    _check(after, torch_dev, x=x)
+
+
+# ---- attention ----------------------------------------------------------------------
+
+def _check(b, dev, *, x=None, scale=None, causal=True, window=0, max_kv=None, **kw):
+    """The bound of _paged.attention covers this form too: q has its bits to 2^-23 (two
+    pieces; 16-bit q all of them), P as two pieces to 2^-23, and as one to 2^-11, which
+    is at most half a step of a 16-bit type.  Results of f16 below 2^-14 lie 2^-24
+    apart: their rounding is off by up to 2^-25 whatever their size."""
+    want, bound = P.attention(Q.plain(b), scale=scale, causal=causal, window=window)
+    bound = bound + (2.0 ** -25 if b["q"].dtype == torch.float16 else 0.0)
+    x = Q.to(b, dev) if x is None else x
+    out = torch.full_like(x["q"], 3.0)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+    _gh().paged_attention(x["q"], *P.args(x), scale=scale, causal=causal, window=window, max_kv_len=max_kv, out=out,
+                          status=status, **Q.scales(x), **kw)
+    got = out.cpu().double()
+    live = ~want.isnan()
+    assert ((got - want).abs() <= bound)[live].all(), float(((got - want).abs() / bound)[live].max())
+    assert (got[~live] == 3.0).all() and int(status) == 0
+    return out
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (8, 2, 128), (5, 1, 80), (7, 1, 32), (6, 2, 96), (16, 1, 16),
+                                              (3, 3, 48), (20, 1, 112)])
+@pytest.mark.parametrize("page", [16, 5])
+def test_single_tokens(torch_dev, kind, heads, kv_heads, d, page):
+    kv = [1, 2, 31, 33, 300, 65, 127, 1030]
+    b = Q.batch([1] * len(kv), kv, kind=kind, heads=heads, kv_heads=kv_heads, d=d, page=page, pad=1, seed=d + page)
+    _check(b, torch_dev)
+    _check(b, torch_dev, window=40, scale=-0.3)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(32, 8, 128), (28, 4, 128), (48, 2, 64), (20, 5, 80)])
+def test_single_tokens_alone(torch_dev, kind, heads, kv_heads, d):
+    """Many rows, one token to a sequence: tiles of 16 rows whatever their number,
+    groups that cross them, more rows than a tile."""
+    kv = [1, 40, 700, 2100, 129, 64]
+    b = Q.batch([1] * len(kv), kv, kind=kind, heads=heads, kv_heads=kv_heads, d=d, page=24, seed=d + heads)
+    _check(b, torch_dev)
+    _check(b, torch_dev, window=100, max_kv=2100)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (8, 2, 128), (5, 1, 80), (6, 2, 96), (4, 1, 16)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 70), (False, 0), (False, 100)])
+def test_chunks(torch_dev, kind, heads, kv_heads, d, causal, window):
+    q, kv = [150, 1, 70, 0, 200, 33], [150, 90, 333, 7, 260, 33]
+    for page in (32, 12):
+        b = Q.batch(q, kv, kind=kind, heads=heads, kv_heads=kv_heads, d=d, page=page, seed=d + page)
+        _check(b, torch_dev, causal=causal, window=window)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("q,kv", [([1], [9000]), ([3, 1], [5000, 40]), ([600], [3000]), ([300, 1, 1], [2500, 2600, 8])])
+def test_long_axes_in_parts(torch_dev, kind, q, kv):
+    b = Q.batch(q, kv, kind=kind, heads=4, kv_heads=1, d=64, page=16, seed=5)
+    a = _check(b, torch_dev)
+    assert torch.equal(a, _check(b, torch_dev))  # and again the same
+    _check(b, torch_dev, max_kv=max(kv))
+    _check(b, torch_dev, max_kv=64)  # a wrong length: split otherwise
+    gh = _gh()
+    x = Q.to(b, torch_dev)
+    n = gh.paged_attention_workspace_size(x["q"], *P.args(x))
+    ws = torch.full((max(n, 16),), 255, dtype=torch.uint8, device=torch_dev)
+    assert torch.equal(_check(b, torch_dev, workspace=ws), a)
+
+
+def test_pages_of_one_row(torch_dev):
+    """More pages than a workgroup looks up at once."""
+    for kv, q in ((1500, 1), (2300, 40)):
+        b = Q.batch([q], [kv], kind="bf16", heads=4, kv_heads=1, d=32, page=1, seed=6)
+        _check(b, torch_dev)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("size", [2.0 ** -14, 2.0 ** -20, 300.0, 3e3])
+def test_rows_of_any_size(torch_dev, kind, size):
+    """Steps at the ends of their range; values whose f16 is subnormal.  (The bound goes
+    with |q||k| and |V|.)"""
+    b = Q.batch([1, 140], [200, 300], kind=kind, heads=2, kv_heads=1, d=64, page=16, seed=8, size=size)
+    _check(b, torch_dev, scale=0.125 / size)
+
+
+@pytest.mark.parametrize("kind,size", [("f32", 1e-30), ("f32", 1e25), ("bf16", 1e-30), ("bf16", 1e25), ("f16", 3e-6),
+                                       ("f16", 1e4)])
+def test_queries_of_any_size(torch_dev, kind, size):
+    """Tiny f16 queries are subnormal as they come, with the bits that they have."""
+    b = Q.batch([1, 140], [200, 300], kind=kind, heads=2, kv_heads=1, d=64, page=16, seed=9)
+    b["q"] = (b["q"].float() * size).to(b["q"].dtype)
+    _check(b, torch_dev, scale=0.125 / size)
+
+
+@pytest.mark.parametrize("q_len", [1, 150])
+def test_queries_that_are_not_finite(torch_dev, q_len):
+    """Such a row is NaN; the others are not touched by it."""
+    b = Q.batch([q_len, 1], [200, 50], kind="bf16", heads=4, kv_heads=2, d=64, page=16, seed=10)
+    want, bound = P.attention(Q.plain(b))
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        x = Q.to(b, torch_dev)
+        x["q"][0, 1, 5] = bad
+        got = _gh().paged_attention(x["q"], *P.args(x), **Q.scales(x)).cpu().double()
+        assert got[0, 1].isnan().all()
+        got[0, 1] = want[0, 1]
+        assert ((got - want).abs() <= bound).all()
+
+
+def test_bad_pages_and_lengths(torch_dev):
+    """A page outside the cache reads as zeros, a length beyond the table is cut;
+    both are reported."""
+    gh = _gh()
+    for q_len, page in ((1, 16), (1, 6), (130, 16)):
+        b = Q.batch([q_len], [160], kind="f32", heads=2, kv_heads=1, d=32, page=page, seed=11)
+        flat = Q.plain(b)
+        for bad in (-1, 10 ** 7):
+            x = Q.to(b, torch_dev)
+            x["page_table"][0, 1] = bad
+            zero = {**flat, "k_pages": flat["k_pages"].clone(), "v_pages": flat["v_pages"].clone()}
+            for n in ("k_pages", "v_pages"):
+                zero[n][int(b["page_table"][0, 1])] = 0
+            want, bound = P.attention(zero)
+            status = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+            got = gh.paged_attention(x["q"], *P.args(x), status=status, **Q.scales(x)).cpu().double()
+            assert int(status) == 2 and ((got - want).abs() <= bound).all()
+        x = Q.to(b, torch_dev)
+        x["kv_lens"][0] = 10 ** 6
+        status.zero_()
+        gh.paged_attention(x["q"], *P.args(x), status=status, **Q.scales(x))
+        assert int(status) & 1
+    # pages before a window may be gone
+    b = Q.batch([1], [160], kind="bf16", heads=2, kv_heads=1, d=32, page=16, seed=12)
+    gone = {**b, "page_table": b["page_table"].clone()}
+    gone["page_table"][0, :7] = -1
+    want, bound = P.attention(Q.plain(b), window=32)
+    x = Q.to(gone, torch_dev)
+    status.zero_()
+    got = gh.paged_attention(x["q"], *P.args(x), window=32, status=status, **Q.scales(x)).cpu().double()
+    assert int(status) == 0 and ((got - want).abs() <= bound).all()
+
+
+def test_many_sequences(torch_dev):
+    """More than a wave's round of the search, empty ones among them."""
+    g = torch.Generator().manual_seed(13)
+    kv = torch.randint(1, 90, (150,), generator=g).tolist()
+    q = [min(n, int(x)) for n, x in zip(kv, torch.randint(0, 4, (150,), generator=g))]
+    b = Q.batch(q, kv, kind="f16", heads=4, kv_heads=2, d=64, page=16, pad=3, seed=13)
+    _check(b, torch_dev)
+    _append_and_check = _expected(b)
+    _, x = _append(b, torch_dev)
+    for n, t in _append_and_check.items():
+        assert torch.equal(x[n].cpu(), t), n
+
+
+def test_nothing_to_do(torch_dev):
+    gh = _gh()
+    b = Q.batch([0, 0], [0, 4], kind="bf16", heads=2, kv_heads=2, d=32, page=4, seed=14)
+    x = Q.to(b, torch_dev)
+    assert gh.paged_attention(x["q"], *P.args(x), **Q.scales(x)).shape == (0, 2, 32)
+    gh.paged_append(*P.args(x), x["k"], x["v"], q=x["q"], **Q.scales(x))
+    assert gh.paged_read(*P.args(x), **Q.scales(x))[0].shape == (0, 2, 32)
+
+
+def test_out_on_q(torch_dev):
+    b = Q.batch([1, 140], [200, 300], kind="bf16", heads=4, kv_heads=2, d=64, page=16, seed=15)
+    x = Q.to(b, torch_dev)
+    want = _gh().paged_attention(x["q"], *P.args(x), **Q.scales(x))
+    _gh().paged_attention(x["q"], *P.args(x), out=x["q"], **Q.scales(x))
+    assert torch.equal(x["q"], want)
+
+
+# ---- steps ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_steps_of_a_layer(torch_dev, kind):
+    """step_paged over an 8-bit cache with norms, prompt and single tokens, against the
+    same formulas on the same projections: the cached rows are the rule's on the layer's
+    own projections, and the attention is that of the rows that the cache returns."""
+    gh = _gh()
+    torch.manual_seed(16)
+    e, heads, dt = 128, 4, P.TYPES[kind]
+    m = gh.MultiHeadAttention(e, heads)
+    m.eval()
+    m.quantize_grouped(32)
+    m.enable_qk_norm(1e-5)
+    m.q_norm += 0.2 * torch.randn_like(m.q_norm)
+    m.k_norm += 0.2 * torch.randn_like(m.k_norm)
+    assert len(m.parameters()) == 10
+    cos, sin = (t.to(torch_dev) for t in P.angles(64, e // heads))
+    c = gh.PagedKVCache(20, 8, heads, e // heads, dtype=torch.uint8)
+    ids = [c.add(), c.add()]
+    past = {i: torch.empty(0, e, dtype=dt) for i in ids}
+    for counts in ([30, 5], [1, 1], [2, 20], [1, 1]):
+        new = [(torch.randn(n, e) * 0.4).to(dt) for n in counts]
+        x = torch.cat(new).to(torch_dev)
+        got = m.step_paged(x, c, c.extend(ids, counts), cos=cos, sin=sin)
+        q, k, v = (m.w4[i](x).view(-1, heads, e // heads).cpu() for i in range(3))
+        y, bounds, at = [], [], 0
+        for i, n in zip(ids, counts):
+            first = len(past[i])
+            past[i] = torch.cat((past[i], x[at:at + n].cpu()))
+            kk, vv = (t.cpu() for t in c.read(i))
+            assert kk.shape == (first + n, heads, e // heads)
+            rows = torch.stack([Q.turned(Q.normed(k[at + j], m.k_norm.cpu(), 1e-5), first + j, cos.cpu(), sin.cpu(), False)
+                                for j in range(n)])
+            assert torch.equal(kk[first:], Q.values(*Q.quantise(rows)))
+            assert torch.equal(vv[first:], Q.values(*Q.quantise(v[at:at + n])))
+            qq = torch.stack([Q.turned(Q.normed(q[at + j], m.q_norm.cpu(), 1e-5), first + j, cos.cpu(), sin.cpu(), False)
+                              for j in range(n)]).to(dt)
+            one = {"q": qq, "q_offsets": torch.tensor([0, n]), "kv_lens": torch.tensor([first + n]), "page": first + n,
+                   "page_table": torch.zeros(1, 1, dtype=torch.int32), "k_pages": kk[None], "v_pages": vv[None]}
+            o, bound = P.attention(one)
+            y.append(o.flatten(1))
+            bounds.append(bound.flatten(1))
+            at += n
+        w, bias = m.w4[3].dequantize().double().cpu(), m.w4[3].bias.double().cpu()
+        y, bounds = torch.cat(y), torch.cat(bounds)
+        want = y @ w.t() + bias
+        # attention's own bound through the projection, whose sums of 128 terms are in
+        # fp32 and which rounds once
+        room = (bounds + 2 * P.half_step(dt) * y.abs() + 136 * 2.0 ** -24 * y.abs()) @ w.abs().t()
+        assert ((got.cpu().double() - want).abs() <= room + P.half_step(dt) * want.abs() + 2.0 ** -22).all()
+    for call in (lambda: m.step(torch.zeros(1, 1, e, device=torch_dev), gh.KVCache(1, 4, e)),
+                 lambda: m.forward(torch.zeros(1, 1, e, device=torch_dev))):
+        with pytest.raises(gh.GhostFlowError, match="step_paged"):
+            call()
+
+
+def test_a_captured_step(torch_dev):
+    """Append, read and attention in one graph, replayed after lengths, tables and
+    values changed, with eager work between: every replay is the eager result."""
+    gh = _gh()
+    b = Q.batch([1, 1, 1], [700, 20, 333], kind="bf16", heads=8, kv_heads=2, d=64, page=16, seed=17, spare=8)
+    x = Q.to(b, torch_dev)
+    w = (1 + 0.1 * torch.randn(64)).to(torch_dev)
+    out, back = torch.zeros_like(x["q"]), [torch.zeros_like(x["k"]) for _ in range(2)]
+    size = gh.paged_attention_workspace_size(x["q"], *P.args(x))
+    ws = torch.empty(max(size, 16), dtype=torch.uint8, device=torch_dev)
+    q_out = torch.zeros_like(x["q"])
+
+    def step():
+        gh.paged_append(*P.args(x), x["k"], x["v"], q=x["q"], q_out=q_out, q_norm=w, k_norm=w, **Q.scales(x))
+        gh.paged_attention(q_out, *P.args(x), out=out, workspace=ws, **Q.scales(x))
+        gh.paged_read(*P.args(x), k_out=back[0], v_out=back[1], **Q.scales(x))
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        step()
+    for n in range(4):
+        x["k"].copy_(torch.randn(x["k"].shape))
+        x["q"].copy_(torch.randn(x["q"].shape))
+        x["kv_lens"].copy_(torch.tensor([700 - 90 * n, 20 + n, 333], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in (out, *back, q_out, x["k_pages"], x["k_scales"])]
+        for t in (out, *back, q_out):
+            t.zero_()
+        step()
+        torch.cuda.synchronize()
+        for a, t in zip(got, (out, *back, q_out, x["k_pages"], x["k_scales"])):
+            assert torch.equal(a, t)
+
+
+def test_two_streams_at_once(torch_dev):
+    """Calls without a workspace on two streams, each over its own cache."""
+    gh = _gh()
+    work = []
+    for seed in (18, 19):
+        b = Q.batch([1, 1], [3000, 900], kind="bf16", heads=8, kv_heads=2, d=128, page=16, seed=seed)
+        x = Q.to(b, torch_dev)
+        work.append((x, gh.paged_attention(x["q"], *P.args(x), **Q.scales(x)), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, (x, _, s) in enumerate(work):
+            with torch.cuda.stream(s):
+                outs[i].append(gh.paged_attention(x["q"], *P.args(x), **Q.scales(x)))
+    torch.cuda.synchronize()
+    for i, (_, want, _) in enumerate(work):
+        assert all(torch.equal(o, want) for o in outs[i])
+
+
+def test_offsets_beyond_32_bits(torch_dev):
+    """Pages whose bytes lie beyond 2^32 from the cache's first."""
+    gh = _gh()
+    pages, page, hkv, d = 70000, 64, 8, 128  # 4.6 GB each
+    k = torch.empty(pages, page, hkv, d, dtype=torch.uint8, device=torch_dev)
+    v = torch.empty_like(k)
+    ks = torch.empty(pages, hkv, page, dtype=torch.uint8, device=torch_dev)
+    vs = torch.empty_like(ks)
+    table = torch.tensor([[pages - 1, 3, pages - 2]], dtype=torch.int32, device=torch_dev)
+    g = torch.Generator(device=torch_dev).manual_seed(20)
+    new = [torch.randn(150, hkv, d, generator=g, device=torch_dev) for _ in range(2)]
+    off, lens = (torch.tensor(t, dtype=torch.int32, device=torch_dev) for t in ([0, 150], [150]))
+    gh.paged_append(k, v, table, off, lens, *new, k_scales=ks, v_scales=vs)
+    got = gh.paged_read(k, v, table, off, lens, tokens=150, k_scales=ks, v_scales=vs)
+    want = [Q.values(*Q.quantise(t.cpu())) for t in new]
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(got, want))
+    for n in (1, 150):
+        q = torch.randn(n, hkv, d, generator=g, device=torch_dev)
+        o = gh.paged_attention(q, k, v, table, off.new_tensor([0, n]), lens, k_scales=ks, v_scales=vs).cpu().double()
+        score = torch.einsum("qhd,khd->hqk", q.cpu().double(), want[0].double()) / math.sqrt(d)
+        hidden = torch.arange(150)[None] > torch.arange(150 - n, 150)[:, None]
+        p = torch.softmax(score.masked_fill(hidden, -math.inf), -1)
+        ref = torch.einsum("hqk,khd->qhd", p, want[1].double())
+        # scores: sums of 128 terms of at most some 4 x 4 in fp32, over sqrt(128)
+        assert (o - ref).abs().max() <= 2 * 136 * 2.0 ** -24 * 16 * 128 / math.sqrt(d)
