@@ -20,6 +20,7 @@ using namespace gfh;
 namespace {
 
 constexpr int64_t kMaxDim = INT32_MAX;
+constexpr int64_t kMaxSampleRows = (int64_t)1 << 20;
 
 bool mul_ok(int64_t a, int64_t b, int64_t *out) {
     __int128 r = (__int128)a * (__int128)b;
@@ -1184,6 +1185,57 @@ GFH_API int gfh_paged_attention_q8(const gfh_paged_kv *kv, const gfh_paged_scale
         if (!scales) return set_error(GFH_NULL_POINTER, "%s: scales is NULL", who);
         return attend(who, kv, scales, dtype, tokens, heads, q, ldq, out, ldo, scale, causal, window, max_kv_len, workspace,
                       workspace_bytes, stream);
+    });
+}
+
+GFH_API size_t gfh_sample_workspace_size(int64_t rows, int64_t vocab) {
+    if (rows <= 0 || rows > kMaxSampleRows || vocab <= 0 || vocab > sample_max_vocab()) return 0;
+    return sample_workspace_bytes(rows, vocab);
+}
+
+GFH_API int gfh_sample(int dtype, const void *logits, int64_t ld, int64_t rows, int64_t vocab, const float *u,
+                       const gfh_sampling *settings, int32_t *tokens, float *logprobs, void *workspace,
+                       size_t workspace_bytes, gfh_stream_t stream) {
+    return guarded([&]() -> int {
+        const char *who = "sample";
+        if (dtype != GFH_F16 && dtype != GFH_BF16 && dtype != GFH_F32)
+            return set_error(GFH_INVALID_DATA, "%s: logits of dtype %d", who, dtype);
+        if (rows < 0 || rows > kMaxSampleRows || vocab < 1 || vocab > sample_max_vocab() || ld < vocab)
+            return set_error(GFH_INVALID_SHAPE, "%s: rows=%lld vocab=%lld ld=%lld out of range (vocab at most %lld)", who,
+                             (long long)rows, (long long)vocab, (long long)ld, (long long)sample_max_vocab());
+        if (!settings) return set_error(GFH_NULL_POINTER, "%s: settings is NULL", who);
+        const gfh_sampling &g = *settings;
+        if ((!g.temperatures && std::isnan(g.temperature)) || (!g.top_ps && std::isnan(g.top_p)) ||
+            (!g.min_ps && std::isnan(g.min_p)))
+            return set_error(GFH_INVALID_DATA, "%s: a setting is NaN", who);
+        if (rows == 0) return GFH_SUCCESS;
+        SampleDesc d;
+        d.dtype = dtype;
+        d.logits = logits;
+        d.ld = ld, d.rows = rows, d.vocab = vocab;
+        d.u = u;
+        d.set = g;
+        d.tokens = tokens;
+        d.logprobs = logprobs;
+        int64_t e;
+        if (sample_blocks(d) > kMaxBlocks256 || !extent2d(rows, vocab, ld, &e))
+            return set_error(GFH_INVALID_SHAPE, "%s: %lld rows of %lld logits are more than one launch can have", who,
+                             (long long)rows, (long long)vocab);
+        GFH_TRY(require_range(logits, (size_t)e * elem_bytes(dtype), "logits"));
+        GFH_TRY(require_range(u, (size_t)rows * 4, "u"));
+        GFH_TRY(optional_range(g.temperatures, (size_t)rows * 4, "temperatures"));
+        GFH_TRY(optional_range(g.top_ks, (size_t)rows * 4, "top_ks"));
+        GFH_TRY(optional_range(g.top_ps, (size_t)rows * 4, "top_ps"));
+        GFH_TRY(optional_range(g.min_ps, (size_t)rows * 4, "min_ps"));
+        GFH_TRY(require_range(tokens, (size_t)rows * 4, "tokens"));
+        GFH_TRY(optional_range(logprobs, (size_t)rows * 4, "logprobs"));
+        if (reinterpret_cast<uintptr_t>(logits) % elem_bytes(dtype) != 0 || (workspace && !aligned16(workspace)))
+            return set_error(GFH_INVALID_DATA, "%s: logits must be aligned to their type, the workspace to 16 bytes", who);
+        GFH_TRY(ensure_init());
+        hipStream_t s = as_stream(stream);
+        Scratch ws;
+        GFH_TRY(ws.acquire(workspace, workspace_bytes, sample_workspace_bytes(rows, vocab), s));
+        return launch_sample(d, ws.ptr(), s);
     });
 }
 

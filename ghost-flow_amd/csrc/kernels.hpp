@@ -235,6 +235,21 @@ int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t 
 size_t paged_attention_q8_workspace_bytes(const PagedAttnDesc &d);
 int launch_paged_attention_q8(const PagedAttnDesc &d, const gfh_paged_scales &scales, void *workspace, hipStream_t s);
 
+// sample.hip: at most sample_max_vocab() logits to a row.
+struct SampleDesc {
+    int dtype = 0;
+    const void *logits = nullptr;
+    int64_t ld = 0, rows = 0, vocab = 0;
+    const float *u = nullptr;
+    gfh_sampling set{};
+    int32_t *tokens = nullptr;
+    float *logprobs = nullptr;
+};
+int64_t sample_max_vocab();
+int64_t sample_blocks(const SampleDesc &d);  // of the first launch
+size_t sample_workspace_bytes(int64_t rows, int64_t vocab);
+int launch_sample(const SampleDesc &d, void *workspace, hipStream_t s);
+
 // w4.hip: 4-bit weights in groups of columns (codes [n, k / 2], scales and
 // zero points [n, ceil(k / group)], zps nullable), k and group multiples of 32.
 int launch_quantize_w4(const float *w, int64_t n, int64_t k, int64_t group, uint8_t *codes, float *scales, uint8_t *zps,

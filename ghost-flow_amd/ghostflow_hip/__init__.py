@@ -39,6 +39,8 @@ from .ops import (  # noqa: F401
     quantize_per_tensor,
     quantize_per_tensor_workspace_size,
     qweight_rowsum,
+    sample,
+    sample_workspace_size,
     save_state_dict,
     sdpa,
     set_pointer_checks,

@@ -67,6 +67,8 @@ SIGNATURES = {
     "gfh_gemv_w8": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _p]),
     "gfh_gemv_w8_noalloc": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _p]),
     "gfh_softmax_lastdim_f32": (_i, [_p, _p, _i64, _i64, _p]),
+    "gfh_sample_workspace_size": (_sz, [_i64, _i64]),
+    "gfh_sample": (_i, [_i, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _sz, _p]),
     "gfh_flash_attention_workspace_size": (_sz, [_i64, _i64, _i64]),
     "gfh_flash_attention_f32": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _f, _p, _sz, _p]),
     "gfh_sdpa_f32": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _f, _i, _p, _i64, _p]),
@@ -144,6 +146,12 @@ class PagedKv(C.Structure):
 class PagedScales(C.Structure):
     """gfh_paged_scales (include/ghostflow_hip.h)."""
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Sampling(C.Structure):
+    """gfh_sampling (include/ghostflow_hip.h)."""
+    _fields_ = [("temperatures", C.c_void_p), ("top_ks", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p),
+                ("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float), ("min_p", C.c_float)]
 
 
 def load():

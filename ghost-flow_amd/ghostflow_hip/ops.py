@@ -398,6 +398,62 @@ def softmax_lastdim(x, out=None):
     return y
 
 
+_SAMPLING = struct.Struct("@PPPPfiff")  # gfh_sampling
+
+
+def sample_workspace_size(rows: int, vocab: int) -> int:
+    """Bytes of sample's workspace for logits [rows, vocab]."""
+    return int(lib().gfh_sample_workspace_size(rows, vocab))
+
+
+def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, want_logprobs=False, out=None, workspace=None):
+    """A token (int32) per row of logits [rows, vocab] (rows may be strided), of
+    float32, bfloat16 or float16, drawn with the uniform numbers u [rows] in
+    [0, 1): temperature (0: the largest logit), then top_k (0: all), top_p (1:
+    all) and min_p (0: all), each a number or a tensor [rows] (float32, top_k
+    int32).  With want_logprobs also the logarithm of the token's probability
+    among those that were left.  gfh_sample in ghostflow_hip.h has the rules;
+    a row of which nothing can be drawn gets -1."""
+    if not logits.is_cuda:
+        raise GhostFlowError(_lib.INVALID_DATA, "logits must be a device tensor")
+    dt, dev = _dtype(logits, "logits"), logits.device
+    if logits.dim() != 2:
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"logits must be [rows, vocab], got {list(logits.shape)}")
+    rows, vocab = logits.shape
+    if vocab > 1 and logits.stride(1) != 1:
+        raise GhostFlowError(_lib.INVALID_DATA, "the entries of a row of logits must be contiguous")
+    ptrs, values = [], []
+    for name, x, dtype, kind in (("temperature", temperature, torch.float32, float), ("top_k", top_k, torch.int32, int),
+                                 ("top_p", top_p, torch.float32, float), ("min_p", min_p, torch.float32, float)):
+        if torch.is_tensor(x):
+            _need_rows(x, dtype, name, rows, dev)
+            ptrs.append(x.data_ptr())
+            values.append(0)
+        else:
+            ptrs.append(0)
+            values.append(kind(x))
+    if not -2 ** 31 <= values[1] < 2 ** 31:
+        values[1] = 0  # more than there are
+    _need_rows(u, torch.float32, "u", rows, dev)
+    tokens = torch.empty(rows, dtype=torch.int32, device=dev) if out is None else out
+    _need_rows(tokens, torch.int32, "out", rows, dev)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=dev) if want_logprobs else None
+    ws, ws_bytes = None, 0
+    if workspace is not None:
+        _same_device(dev, workspace)
+        ws, ws_bytes = _workspace(workspace)
+    _call(dev, lib().gfh_sample, dt, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, u.data_ptr(),
+          _SAMPLING.pack(*ptrs, *values), tokens.data_ptr(), _ptr(logprobs), ws, ws_bytes)
+    return (tokens, logprobs) if want_logprobs else tokens
+
+
+def _need_rows(t, dtype, name, rows, dev):
+    _need(t, dtype, name)
+    _same_device(dev, t)
+    if t.shape != (rows,):
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be [{rows}], got {list(t.shape)}")
+
+
 def sdpa(q, k, v, *, scale=None, causal=False, mask=None, want_weights=False, out=None):
     """Fused scaled_dot_product_attention on [B, H, S, D] tensors."""
     for t, nm in ((q, "q"), (k, "k"), (v, "v")):

@@ -291,6 +291,37 @@ GFH_API int gfh_gemv_w8_noalloc(const float *x, const int8_t *qw,
 GFH_API int gfh_softmax_lastdim_f32(const float *x, float *y, int64_t rows,
                                     int64_t cols, gfh_stream_t stream);
 
+/* How tokens are drawn (host struct): a device array of one value per row, or, where
+ * that is NULL, the value for all rows.
+ *   temperature  T > 0; else the row takes its largest logit
+ *   top_k        of the larger ones, in [1, vocab); else all
+ *   top_p        below 1, else all; at 0 and below the largest alone
+ *   min_p        above 0, else all */
+typedef struct gfh_sampling {
+    const float *temperatures;
+    const int32_t *top_ks;
+    const float *top_ps, *min_ps;
+    float temperature;
+    int32_t top_k;
+    float top_p, min_p;
+} gfh_sampling;
+
+/* A token per row of logits [rows, vocab] (type dtype, rows ld elements apart), from
+ * numbers u [rows] in [0, 1) that the caller draws.  With w_i = exp((l_i - max l) / T)
+ * and a row ordered by larger logit, then lower index: the first top_k; of those the
+ * ones with less than top_p times their sum of w before them (the first in any case);
+ * of those the ones with w >= min_p.  tokens[row] is the first of them, by index, whose
+ * running sum of w exceeds u times their total; logprobs (nullable) gets the logarithm of
+ * its w over that total.  Weights are held to 2^-45 of the largest and summed exactly,
+ * so results do not depend on the order of sums.  A logit of -inf or NaN is never
+ * drawn; of infinite ones all are alike and the others have w = 0; a row with none to draw
+ * gets -1 (and NaN).  vocab <= 2^19.  workspace (nullable, 16-byte aligned) of at least
+ * gfh_sample_workspace_size(rows, vocab) bytes, any contents. */
+GFH_API size_t gfh_sample_workspace_size(int64_t rows, int64_t vocab);
+GFH_API int gfh_sample(int dtype, const void *logits, int64_t ld, int64_t rows, int64_t vocab, const float *u,
+                       const gfh_sampling *settings, int32_t *tokens, float *logprobs, void *workspace,
+                       size_t workspace_bytes, gfh_stream_t stream);
+
 /* Fused scaled-dot-product attention, Q [b,h,sq,d], K/V [b,h,skv,d],
  * out [b,h,sq,d]:  softmax(mask(Q.K^T * scale)) . V
  *   - scale multiplies the finished dot product (mul_scalar after the
