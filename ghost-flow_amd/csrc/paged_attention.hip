@@ -505,7 +505,7 @@ __global__ __launch_bounds__(64 * WAVES) void paged_decode_kernel(AttnParams p) 
     for (int i = 0; i < NB; ++i) *reinterpret_cast<f32x4 *>(accs + (wave * 16 + c) * kRow + 16 * i + 4 * h) = o[i];
     if (h == 0) mls[wave * 16 + c] = make_float2(mt, l);
     __syncthreads();
-    join_waves<TA, DP, WAVES>(p, t, kvh, split, nact > 1, accs, mls, tid);
+    join_waves<TA, DP>(p, t, kvh, split, nact > 1, accs, mls, WAVES, tid);
 }
 
 // ---- many rows: chunks of prompts ---------------------------------------------------
@@ -897,7 +897,7 @@ __global__ __launch_bounds__(256, 2) void paged_f32_kernel(AttnParams p) {
                 f32x4{o[v][0][x], o[v][1][x], o[v][2][x], o[v][3][x]};
     if (h == 0) mls[wave * 16 + c] = make_float2(m == -INFINITY ? m : m * p.sc2, l);
     __syncthreads();
-    join_waves<float, DP, 4>(p, t, kvh, split, nact > 1, accs, mls, tid);
+    join_waves<float, DP>(p, t, kvh, split, nact > 1, accs, mls, 4, tid);
 }
 
 // Prompts: a tile of 64 rows, four waves of 16, K and V tiles of 32 keys in two

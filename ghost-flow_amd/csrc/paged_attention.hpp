@@ -229,22 +229,22 @@ __device__ __forceinline__ void wait_vm() {
     __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14));
 }
 
-// The waves' states of a 16-row tile from LDS (rows of DP + 4 floats, their
-// maximum and sum) to the tile's rows: thread i takes 4 dims of a row.
-template <typename TA, int DP, int WAVES>
+// The states that `waves` waves have of a 16-row tile from LDS (rows of DP + 4 floats, their
+// maximum and sum) to the tile's rows: their thread i takes 4 dims of a row.
+template <typename TA, int DP>
 __device__ __forceinline__ void join_waves(const AttnParams &p, const Rows &t, int kvh, int split, bool parts,
-                                           const float *accs, const float2 *mls, int tid) {
+                                           const float *accs, const float2 *mls, int waves, int tid) {
     constexpr int kRow = DP + 4;
-    for (int i = tid; i < 16 * DP / 4; i += 64 * WAVES) {
+    for (int i = tid; i < 16 * DP / 4; i += 64 * waves) {
         const int row = i / (DP / 4), dim = 4 * (i % (DP / 4));
         const int rr = t.base + row;
         if (rr < t.r0 || rr >= t.r1 || dim >= p.c.d) continue;
         float M = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) M = max_nan(M, mls[w * 16 + row].x);
+        for (int w = 0; w < waves; ++w) M = max_nan(M, mls[w * 16 + row].x);
         f32x4 A = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
+        for (int w = 0; w < waves; ++w) {
             const float2 x = mls[w * 16 + row];
             const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - M);
             L = fmaf(x.y, f, L);

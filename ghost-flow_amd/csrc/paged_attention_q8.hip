@@ -26,6 +26,7 @@ struct Q8Params {
     AttnParams a;
     const uint8_t *ks, *vs;
     int64_t scale_page, scale_head;  // bytes
+    int side;     // heads of a few-row workgroup, a divisor of its waves
     bool eights;  // 8 keys from a multiple of 8 lie in one page, their step bytes aligned
 };
 
@@ -70,18 +71,18 @@ __device__ __forceinline__ uint32_t values(uint32_t w, const Step &s) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, s.f, s.g));
 }
 
-// The rows of q as B operands: dims first + u step .. + 7 per step u, as NQ f16 pieces of
+// The rows of q as B operands: dims dim_of(u) .. + 7 per step u, as NQ f16 pieces of
 // q 2^k; `over` takes the maximum over the lanes of a row.  Returns 2^-k, NaN for a
 // row that is not finite.
-template <typename TA, int NU, int NQ, typename F>
-__device__ __forceinline__ float load_q8(const AttnParams &p, const Rows &t, int r, int kvh, int first, int step,
+template <typename TA, int NU, int NQ, typename D, typename F>
+__device__ __forceinline__ float load_q8(const AttnParams &p, const Rows &t, int r, int kvh, D &&dim_of,
                                          f16x8 (&qf)[NU][NQ], F &&over) {
     const bool ok = r >= t.r0 && r < t.r1;
     const TA *q = q_row<TA>(p, ok ? r : t.r0, kvh);
     float x[NU][8], most = 0.f;
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
-        const int dim = first + u * step;
+        const int dim = dim_of(u);
         load_vec<8>(q + (dim < p.c.d ? dim : 0), x[u]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -127,18 +128,20 @@ __device__ __forceinline__ f16x8 as_operand(uint32_t a, uint32_t b, uint32_t c, 
 
 // ---- few rows: decode --------------------------------------------------------------
 //
-// A tile of 16 rows, WAVES waves that take 32-key tiles in turn, each with its own
-// softmax state; the states are joined in LDS at the end.  Codes go from memory
-// straight into the registers of the lane that multiplies them: lane (c = l % 16, h =
-// l / 16) has
-//   K: dims DP / 4 h .. of keys 8 (c / 4) + c % 4 and + 4 (rows c of two blocks), so row
-//      4 h + x of block kb is key 8 h + 4 kb + x, and lane h has keys 8 h .. + 7 of S^T;
+// A tile of 16 rows of pp.side neighbouring key/value heads, whose rows of the cache
+// lie side by side; WAVES / side waves of a head take 32-key tiles in turn, each with
+// its own softmax state, and the states of a head are joined in LDS at the end.  Codes go from
+// memory straight into the registers of the lane that multiplies them: lane (c = l %
+// 16, h = l / 16) has
+//   K: dims 64 i + 16 h .. + 15 of keys 8 (c / 4) + c % 4 and + 4 (rows c of two blocks), so
+//      row 4 h + x of block kb is key 8 h + 4 kb + x, and lane h has keys 8 h .. + 7 of S^T;
 //   V: dims DP / 16 c .. of those keys 8 h .. + 7: the byte permutes that make f16 of
 //      codes also bring the same dim of two keys side by side, so V needs no
 //      transposition elsewhere.  Row i of block b of O^T is dim DP / 16 i + b.
-// The next tile's loads are on their way while a tile is computed.
+// The next tile's K is asked for when this one's has been multiplied, V likewise: half
+// a tile per wave is on its way at any time, in registers that are free anyway.
 template <typename TA, int DP, int NQ, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_decode_kernel(Q8Params pp) {
+__global__ __launch_bounds__(64 * WAVES, NQ > 1 ? 2 : 3) void paged_q8_decode_kernel(Q8Params pp) {
     using H = Half<_Float16>;
     constexpr int NU = DP / 32, NB = DP / 16, KP = DP / 64, NV = DP / 64;  // NV: dwords of V per key
     constexpr float kBias = H::kBias;
@@ -152,9 +155,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_decode_kernel(Q8Params
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 15, h = lane >> 4;
-    // (round the XCDs as they come, as in paged_attention.hip)
-    const int id = blockIdx.x;
-    const int kvh = id % cc.hkv, split = (id / cc.hkv) % p.nsplit, number = id / cc.hkv / p.nsplit;
+    // The workgroups of a tile's heads go to one XCD, as their rows share lines of memory.
+    const int groups = cc.hkv / pp.side, units = gridDim.x / groups, even = units & ~7;
+    int id = blockIdx.x, first, unit;
+    if (id < even * groups) {
+        first = (id >> 3) % groups, unit = (id & 7) + 8 * ((id >> 3) / groups);
+    } else {
+        id -= even * groups;
+        first = id % groups, unit = even + id / groups;
+    }
+    // (parts of one number later: whether a part has keys then does not go by the XCD)
+    const int number = unit % p.ntiles, split = unit / p.ntiles;
+    const int kvh = first * pp.side + wave % pp.side, sub = wave / pp.side, subs = WAVES / pp.side;
     Rows t;
     int seq;
     if (!find_rows(p, number, 16, lane, t, seq)) return;
@@ -167,8 +179,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_decode_kernel(Q8Params
     int jmin, jmax;
     row_keys(p, t, r, jmin, jmax);
     f16x8 qf[NU][NQ];
-    const float down = load_q8<TA, NU, NQ>(p, t, r, kvh, DP / 4 * h, 8, qf, [](float x) { return quarter_max_nan(x); });
-    const float scl = row_scale(p, down);
+    float scl = 0.f;
     // keys that every row sees: [all_lo, all_hi)
     int x0, x1, y0, y1;
     row_keys(p, t, t.r0, x0, x1);
@@ -182,16 +193,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_decode_kernel(Q8Params
 
     typedef uint32_t vrow __attribute__((ext_vector_type(NV)));
     typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    struct Tile {
-        i32x4 k[2][KP];
-        vrow v[8];
-        u32x2 ks, vs;  // step bytes: of the lane's two keys at byte c % 4 of either word; of keys 8 h ..
-    };
+    i32x4 kw[2][KP];
+    vrow vw[8];
+    u32x2 ks, vs;  // step bytes: of the lane's two keys at byte c % 4 of either word; of keys 8 h ..
     const int64_t head = kvh * cc.head_stride, scale_head = kvh * pp.scale_head;
     // dims past the head's: its first ones, which q's zeros or nobody takes
     int kdim[KP];
 #pragma unroll
-    for (int i = 0; i < KP; ++i) kdim[i] = DP / 4 * h + 16 * i < cc.d ? DP / 4 * h + 16 * i : 0;
+    for (int i = 0; i < KP; ++i) kdim[i] = 64 * i + 16 * h < cc.d ? 64 * i + 16 * h : 0;
     const int vdim = DP / 16 * c < cc.d ? DP / 16 * c : 0;
     const char *const mid = reinterpret_cast<const char *>(g_mid_row);
 
@@ -200,82 +209,84 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_decode_kernel(Q8Params
         __syncthreads();  // every wave is done with the pages before
         const int pe = stage_page_numbers(cc, seq, pb, e, t.lo, pages, tid, 64 * WAVES);
         __syncthreads();
-        auto load = [&](int k0, Tile &f) __attribute__((always_inline)) {
-            if (pp.eights) {
-                // groups of 8 keys, from multiples of 8: one of K and one of V per lane
-                // (past the end: the last)
-                auto group = [&](int g, const char *pages_at, const uint8_t *bytes, const char *&rows, int64_t &stride,
-                                 const char *&steps) __attribute__((always_inline)) {
-                    const int key = min(k0 + 8 * g, (pe - 1) & ~7), pg = paged::page_of(cc, key);
-                    const int page = pages[pg - p0], prow = key - pg * cc.page_size;
-                    const bool ok = page >= 0;
-                    rows = ok ? pages_at + page * cc.page_stride + prow * cc.row_stride + head : mid;
-                    stride = ok ? cc.row_stride : 0;
-                    steps = ok ? reinterpret_cast<const char *>(bytes) + page * pp.scale_page + scale_head + prow : mid;
-                };
-                const char *rows, *steps;
-                int64_t stride;
-                group(c >> 2, cc.k, pp.ks, rows, stride, steps);
+        // Where a key's row begins, how far the next one is, and its step byte.
+        auto at = [&](int key, const char *cache, const uint8_t *bytes, const char *&rows, int64_t &stride,
+                      const uint8_t *&steps) __attribute__((always_inline)) {
+            const int pg = paged::page_of(cc, key), page = pages[pg - p0], prow = key - pg * cc.page_size;
+            const bool ok = page >= 0;
+            rows = ok ? cache + page * cc.page_stride + prow * cc.row_stride + head : mid;
+            stride = ok ? cc.row_stride : 0;
+            steps = ok ? bytes + page * pp.scale_page + scale_head + prow : reinterpret_cast<const uint8_t *>(mid);
+        };
+        const char *rows;
+        const uint8_t *steps;
+        int64_t stride;
+        auto load_k = [&](int k0) __attribute__((always_inline)) {
+            if (pp.eights) {  // a group of 8 keys, from a multiple of 8 (past the end: the last)
+                at(min(k0 + 8 * (c >> 2), (pe - 1) & ~7), cc.k, pp.ks, rows, stride, steps);
                 rows += (c & 3) * stride;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
                     for (int i = 0; i < KP; ++i)
-                        f.k[kb][i] = __builtin_nontemporal_load(
+                        kw[kb][i] = __builtin_nontemporal_load(
                             reinterpret_cast<const i32x4 *>(rows + 4 * kb * stride + kdim[i]));
-                f.ks = *reinterpret_cast<const u32x2 *>(steps);
-                group(h, cc.v, pp.vs, rows, stride, steps);
+                ks = *reinterpret_cast<const u32x2 *>(steps);
+            } else {
 #pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    f.v[x] = __builtin_nontemporal_load(reinterpret_cast<const vrow *>(rows + x * stride + vdim));
-                f.vs = *reinterpret_cast<const u32x2 *>(steps);
-                return;
-            }
-            // pages of other sizes: every key by itself
-            auto at = [&](int key, const char *pages_at, const uint8_t *bytes, const char *&row, uint32_t &step)
-                          __attribute__((always_inline)) {
-                key = min(key, pe - 1);
-                const int pg = paged::page_of(cc, key), page = pages[pg - p0], prow = key - pg * cc.page_size;
-                const bool ok = page >= 0;
-                row = ok ? pages_at + page * cc.page_stride + prow * cc.row_stride + head : mid;
-                step = *(ok ? bytes + page * pp.scale_page + scale_head + prow : reinterpret_cast<const uint8_t *>(mid));
-            };
-            const char *row;
-            uint32_t step;
+                for (int kb = 0; kb < 2; ++kb) {
+                    at(min(k0 + 8 * (c >> 2) + (c & 3) + 4 * kb, pe - 1), cc.k, pp.ks, rows, stride, steps);
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                at(k0 + 8 * (c >> 2) + (c & 3) + 4 * kb, cc.k, pp.ks, row, step);
-#pragma unroll
-                for (int i = 0; i < KP; ++i) f.k[kb][i] = *reinterpret_cast<const i32x4 *>(row + kdim[i]);
-                f.ks[kb] = step << (8 * (c & 3));
-            }
-            f.vs = u32x2{0u, 0u};
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                at(k0 + 8 * h + x, cc.v, pp.vs, row, step);
-                f.v[x] = *reinterpret_cast<const vrow *>(row + vdim);
-                f.vs[x >> 2] |= step << (8 * (x & 3));
+                    for (int i = 0; i < KP; ++i) kw[kb][i] = *reinterpret_cast<const i32x4 *>(rows + kdim[i]);
+                    ks[kb] = (uint32_t)*steps << (8 * (c & 3));
+                }
             }
         };
-        int k0 = pb + 32 * wave;
-        // (two tiles in turn, without a copy that would wait for the next one)
-        auto step = [&](const Tile &now, Tile &next) __attribute__((always_inline)) {
-            if (k0 + 32 * WAVES < pe) load(k0 + 32 * WAVES, next);
-            __builtin_amdgcn_sched_barrier(0);
+        auto load_v = [&](int k0) __attribute__((always_inline)) {
+            if (pp.eights) {
+                at(min(k0 + 8 * h, (pe - 1) & ~7), cc.v, pp.vs, rows, stride, steps);
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    vw[x] = __builtin_nontemporal_load(reinterpret_cast<const vrow *>(rows + x * stride + vdim));
+                vs = *reinterpret_cast<const u32x2 *>(steps);
+            } else {
+                vs = u32x2{0u, 0u};
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    at(min(k0 + 8 * h + x, pe - 1), cc.v, pp.vs, rows, stride, steps);
+                    vw[x] = *reinterpret_cast<const vrow *>(rows + vdim);
+                    vs[x >> 2] |= (uint32_t)*steps << (8 * (x & 3));
+                }
+            }
+        };
+        int k0 = pb + 32 * sub;
+        if (k0 < pe) load_k(k0), load_v(k0);
+        if (pb == b) {  // (while the first tile is on its way)
+            const float down = load_q8<TA, NU, NQ>(
+                p, t, r, kvh, [&](int u) { return 64 * (u / 2) + 16 * h + 8 * (u % 2); }, qf,
+                [](float x) { return quarter_max_nan(x); });
+            scl = row_scale(p, down);
+        }
+#pragma unroll 1
+        for (; k0 < pe; k0 += 32 * subs) {
             f32x4 s[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                const float sk = quarter_step(now.ks[kb] >> (8 * (c & 3)) & 0xff);
+                const float sk = quarter_step(ks[kb] >> (8 * (c & 3)) & 0xff);
                 const Step st = step_pair(sk, sk);
 #pragma unroll
                 for (int u = 0; u < NU; ++u) {
-                    const uint32_t w0 = (uint32_t)now.k[kb][u / 2][2 * (u % 2)], w1 = (uint32_t)now.k[kb][u / 2][2 * (u % 2) + 1];
+                    const uint32_t w0 = (uint32_t)kw[kb][u / 2][2 * (u % 2)], w1 = (uint32_t)kw[kb][u / 2][2 * (u % 2) + 1];
                     const f16x8 kf = as_operand(values<false>(w0, st), values<true>(w0, st), values<false>(w1, st),
                                                 values<true>(w1, st));
 #pragma unroll
                     for (int q = NQ - 1; q >= 0; --q) s[kb] = H::mfma16(kf, qf[u][q], s[kb]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            const bool more = k0 + 32 * subs < pe;
+            if (more) load_k(k0 + 32 * subs);
+            __builtin_amdgcn_sched_barrier(0);
             if (k0 < all_lo || k0 + 32 > min(all_hi, pe)) {
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
@@ -315,7 +326,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_decode_kernel(Q8Params
             Step vst[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const uint32_t w = now.vs[x >> 1] >> (16 * (x & 1));
+                const uint32_t w = vs[x >> 1] >> (16 * (x & 1));
                 vst[x] = step_pair(quarter_step(w & 0xff), quarter_step(w >> 8 & 0xff));
             }
 #pragma unroll
@@ -326,7 +337,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_decode_kernel(Q8Params
                     uint32_t two[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
-                        two[x] = __builtin_amdgcn_perm(now.v[2 * x + 1][w], now.v[2 * x][w], half ? 0x07030602u : 0x05010400u);
+                        two[x] = __builtin_amdgcn_perm(vw[2 * x + 1][w], vw[2 * x][w], half ? 0x07030602u : 0x05010400u);
                     const f16x8 va = as_operand(values<false>(two[0], vst[0]), values<false>(two[1], vst[1]),
                                                 values<false>(two[2], vst[2]), values<false>(two[3], vst[3]));
                     const f16x8 vb = as_operand(values<true>(two[0], vst[0]), values<true>(two[1], vst[1]),
@@ -338,31 +349,28 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_decode_kernel(Q8Params
                         o[i + 1] = H::mfma16(vb, pf[q], o[i + 1]);
                     }
                 }
-            k0 += 32 * WAVES;
-        };
-        Tile even, odds;
-        if (k0 < pe) load(k0, even);
-#pragma unroll 1
-        while (k0 < pe) {
-            step(even, odds);
-            if (k0 >= pe) break;
-            step(odds, even);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_v(k0 + 32 * subs);
+            __builtin_amdgcn_sched_barrier(0);
         }
         pb = pe;
     }
 
-    // Join the waves: o[b], register x is dim DP / 16 (4 h + x) + b of row c.
+    // Join the waves of a head: o[b], register x is dim DP / 16 (4 h + x) + b of row c.
     l = 0.25f * quarter_sum(l);
     const float mt = m == -INFINITY ? m : m * scl;
+    const int state = wave % pp.side * subs + sub;
 #pragma unroll
     for (int x = 0; x < 4; ++x)
 #pragma unroll
         for (int i = 0; i < NB; i += 4)
-            *reinterpret_cast<f32x4 *>(accs + (wave * 16 + c) * kRow + NB * (4 * h + x) + i) =
+            *reinterpret_cast<f32x4 *>(accs + (state * 16 + c) * kRow + NB * (4 * h + x) + i) =
                 f32x4{o[i][x], o[i + 1][x], o[i + 2][x], o[i + 3][x]};
-    if (h == 0) mls[wave * 16 + c] = make_float2(mt, l);
+    if (h == 0) mls[state * 16 + c] = make_float2(mt, l);
     __syncthreads();
-    join_waves<TA, DP, WAVES>(p, t, kvh, split, nact > 1, accs, mls, tid);
+    const int place = wave % pp.side;
+    join_waves<TA, DP>(p, t, kvh, split, nact > 1, accs + place * subs * 16 * kRow, mls + place * subs * 16, subs,
+                       sub * 64 + lane);
 }
 
 // ---- many rows: chunks of prompts ---------------------------------------------------
@@ -401,7 +409,7 @@ __global__ __launch_bounds__(256, 2) void paged_q8_chunk_kernel(Q8Params pp) {
     int jmin, jmax;
     row_keys(p, t, r, jmin, jmax);
     f16x8 qf[NU][NQ];
-    const float down = load_q8<TA, NU, NQ>(p, t, r, kvh, 8 * h, 16, qf, [](float x) {
+    const float down = load_q8<TA, NU, NQ>(p, t, r, kvh, [&](int u) { return 8 * h + 16 * u; }, qf, [](float x) {
         const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
         return max_nan(__uint_as_float(a[0]), __uint_as_float(a[1]));
     });
@@ -588,6 +596,7 @@ struct Plan {
     bool few, chunk;
     bool wide;    // the few-row launch has wide workgroups
     int few_max;  // rows of the longest sequence the few-row launch takes
+    int side;     // heads of a few-row workgroup
     int few_split, few_chunk, chunk_split, chunk_chunk;
     int64_t few_parts, chunk_parts;  // rows of parts
     int64_t part_floats;
@@ -618,16 +627,26 @@ Plan make_plan(const PagedAttnDesc &d) {
         chunk = (int)std::min<int64_t>((ch + unit - 1) / unit * unit, (int64_t)1 << 30);
     };
     const int64_t few_tiles = std::min(d.kv.num_seqs, d.tokens) + (pl.chunk ? 0 : rows / 16);
+    // Keys per workgroup of the few-row launch.  One round of the workgroups that fit the
+    // CUs (three; two with fp32 q, whose workspace is as large; lengths are not all the longest: 3/4), where a row's parts, which are joined one
+    // after the other, are then at most 32 of at least 256 keys.  Four heads to a
+    // workgroup (us of a call, bf16, 32 heads over 8 of 128: 64 sequences of 1024 .. 4096
+    // keys 77 / one head 88, all of 4096 120 / 124), unless their waves then have few tiles
+    // each (16 of 500 .. 2000 keys 29 / 24, one of 16384 32 / 22) or one head needs no
+    // second part (256 of 175 .. 700 keys 70 / 64).
     {
-        const int64_t items = std::max<int64_t>(1, few_tiles * d.kv.kv_heads);
-        int64_t keys = items * sees * 3 / 4 / (2 * cus);
-        if (keys > 1024) keys /= (keys + 703) / 704;
-        keys = std::max(keys, items * sees / (24 * cus));  // (parts stay some tens of MB at most)
-        cut(few_tiles, kAll, std::max<int64_t>(128, keys), 64, pl.few_split, pl.few_chunk);
+        const bool apart = d.tokens == d.kv.num_seqs && 16 % group == 0;  // no row beyond a sequence's first tile
+        const int64_t tiles = apart ? d.kv.num_seqs : few_tiles, slots = 3 * cus;
+        int64_t keys = tiles * d.kv.kv_heads * sees * 3 / 4 / slots;
+        pl.side = 1;
+        if (keys >= 1024 && keys * 3 / 2 < sees)
+            while (pl.side < kDecodeWaves && d.kv.kv_heads % (2 * pl.side) == 0) pl.side *= 2;
+        keys = std::max<int64_t>({256, keys / pl.side, sees / 32});
+        cut(few_tiles, kAll, keys, 64, pl.few_split, pl.few_chunk);
     }
     pl.wide = pl.few_split > 1 && few_tiles * d.kv.kv_heads <= cus &&
               (d.window > 0 ? std::min(d.max_kv_len, d.window + 15) : d.max_kv_len) <= kWideKeys * kWideWaves;
-    if (pl.wide) pl.few_split = 1;
+    if (pl.wide) pl.few_split = pl.side = 1;
     cut(rows / 128 + 1, 2 * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
     if (pl.chunk && 64 * d.kv.num_seqs <= rows && std::min<int64_t>(sees, pl.chunk_chunk) <= 2048) pl.few = false;
     auto floats = [&](bool on, int64_t nsplit, int64_t part_rows) {
@@ -661,6 +680,7 @@ int launch_paged_attention_q8(const PagedAttnDesc &d, const gfh_paged_scales &sc
     pp.scale_page = scales.page_stride, pp.scale_head = scales.head_stride;
     pp.eights = d.kv.page_size % 8 == 0 &&
                 ((scales.page_stride | scales.head_stride | (int64_t)(uintptr_t)scales.k | (int64_t)(uintptr_t)scales.v) & 7) == 0;
+    pp.side = pl.side;
     const int64_t rows = d.tokens * p.c.group;
     auto run = [&](int bm, int nsplit, int chunk, int64_t parts, int min_rows, int max_rows, auto &&kernel) -> int {
         p.direct = max_rows == kFewRows;
@@ -668,7 +688,7 @@ int launch_paged_attention_q8(const PagedAttnDesc &d, const gfh_paged_scales &sc
         p.nsplit = nsplit, p.chunk = chunk, p.min_rows = min_rows, p.max_rows = max_rows;
         p.acc = static_cast<float *>(workspace);
         p.ml = reinterpret_cast<float2 *>(p.acc + parts * nsplit * d.kv.head_dim);
-        const int64_t blocks = (int64_t)p.ntiles * p.c.hkv * nsplit;
+        const int64_t blocks = (int64_t)p.ntiles * (p.c.hkv / (bm == 16 ? pp.side : 1)) * nsplit;
         if (blocks > (int64_t)1 << 23) return set_error(GFH_INVALID_SHAPE, "paged_attention_q8: grid too large");
         kernel(dim3((unsigned)blocks));
         GFH_TRY(check_launch("paged_attention_q8"));
