@@ -10,17 +10,22 @@
 // Weights are integers, round(w 2^44): sums are exact in 64 bits (up to 2^19 entries),
 // the same in any order, and a border between two tokens lies within 2^-35 of its
 // place whatever the vocabulary, so no u meets another token than in a longer format
-// but for one in 10^10.  An exponential is a table of 2^(j / 32), a polynomial of five
-// terms beyond (2e-15) and the exponent: some 20 operations, two thirds of them fp64,
+// but for one in 10^10.  An exponential is a table of 2^(j / 128), a polynomial of four
+// terms beyond (2e-15) and the exponent: 17 operations without a branch, 9 of them fp64,
 // which this card issues at the rate of fp32.
 //
 // Two launches.  The first (a workgroup per 4096 logits, read once) leaves the largest of
-// every 16, of its 4096 and where it is, and the sum of their weights where the row's
-// settings need one.  The second has a workgroup per row, which rarely reads the row
-// again: the k-th largest of the 16s' maxima bounds the k-th largest logit from below,
-// so a few groups hold all candidates; those are sorted.  With no filter the sums find
-// the 4096 that hold the token.  A row whose filter keeps more than kCandidates (a
-// flat one under top-p) is searched whole: bins, then radix.
+// every 16, of its 4096 and where it is, and, where the row's settings need the sum of all
+// weights, that of its own, under top-p in bins of a 16th of z as well.  The second has a
+// workgroup per row:
+//  * no filter: the sums find the 4096 that hold the token;
+//  * top-k, min_p (pick_from_few): the k-th largest of the 16s' maxima bounds the k-th
+//    largest logit from below, so a few groups, found without reading the row, hold all
+//    candidates, which are then put in order;
+//  * top-p (pick_by_bins): the bins say which one is cut, one pass over the row collects
+//    its logits, and their bits say the cut;
+//  * anything else, such as a large k or one bin of equal logits (pick_from_row): the row
+//    is searched whole, by bins, then the cut's 32 bits by eleven, eleven and ten.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -33,7 +38,12 @@ namespace {
 
 constexpr int kGroup = 16, kSlice = 4096, kGroups = kSlice / kGroup;  // logits; groups of a slice
 constexpr int kMaxSlices = 128;
-constexpr int kBins = 2048, kCandidates = 2048, kGuess = 1024, kPickThreads = 1024;
+constexpr int kBins = 512;       // of a 16th of z
+constexpr int kDigits = 2048;    // a radix step
+constexpr int kCandidates = 2048, kGuess = 1024, kPickThreads = 1024;
+constexpr int kPerPick = kSlice / kPickThreads;  // logits of a slice per thread
+constexpr int kListed = 7168;   // logits of a bin
+constexpr int kTable = 128;
 constexpr double kOne = 0x1p44;
 static_assert((int64_t)kMaxSlices * kSlice == (int64_t)1 << 19, "sums of that many weights in 64 bits");
 
@@ -51,6 +61,7 @@ struct SampleParams {
     gfh_sampling set;
     float *maxima;  // [row][slices kGroups], -inf past the vocabulary
     Slice *slice;   // [row][slices]
+    uint64_t *bins; // [row][slices][kBins] sums of weights relative to the slice's most, where Settings::bins
     int32_t *tokens;
     float *logprobs;  // nullable
 };
@@ -63,6 +74,8 @@ struct Settings {
     __device__ __forceinline__ bool greedy() const { return !(temperature > 0.f); }
     // whether the sum of all weights is needed
     __device__ __forceinline__ bool all() const { return !greedy() && !k && (p < 1.0 || !(min_p > 0.0)); }
+    __device__ __forceinline__ bool bins(int slices) const { return all() && p < 1.0 && slices > 1; }
+    __device__ __forceinline__ float per() const { return 16.f / temperature; }
 };
 __device__ __forceinline__ Settings settings(const SampleParams &s, int row) {
     Settings r;
@@ -76,27 +89,46 @@ __device__ __forceinline__ Settings settings(const SampleParams &s, int row) {
     return r;
 }
 
-// exp((l - most) / T) 2^44, rounded; scale = 32 log2 e / T, table[j] = 2^(j / 32).
-__device__ __forceinline__ uint64_t weight(float l, float most, double scale, const double *table) {
-    if (l == most) return (uint64_t)1 << 44;  // (infinite ones too)
-    const double y = ((double)l - (double)most) * scale;
-    if (!(y > -32.0 * 46)) return 0;  // NaN and -inf too
-    const double t = y + 0x1.8p52;
+// exp((l - most) / T) 2^44, rounded, plus 2^52 in the bits of a double, for finite most and
+// l below infinity; scale = 128 log2 e / T, table[j] = 2^(j / 128 + 44).
+__device__ __forceinline__ uint64_t weight_bits(float l, double most, double scale, const double *table) {
+    // (-inf goes to what rounds to 0, and so does NaN, which 0 times it is)
+    const double y = fmax(((double)l - most) * scale, -128.0 * 47);
+    const double t = y + 0x1.8p52;  // its low bits: y rounded
     const int n = (int)(uint32_t)__double_as_longlong(t);
-    const double r = (y - (t - 0x1.8p52)) * 0x1.62e42fefa39efp-6;  // ln 2 / 32
-    double e = fma(r, 1.0 / 120, 1.0 / 24);
-    e = fma(r, e, 1.0 / 6);
-    e = fma(r, e, 0.5);
+    const double r = y - (t - 0x1.8p52);  // in 128ths of an octave
+    constexpr double c = 0x1.62e42fefa39efp-8;  // ln 2 / 128
+    double e = fma(r, c * c * c * c / 24, c * c * c / 6);
+    e = fma(r, e, c * c / 2);
+    e = fma(r, e, c);
     e = fma(r, e, 1.0);
-    e = fma(r, e, 1.0);
-    // 2^(n / 32 + 44), then the integer in the low bits of 2^52 + it
-    const double f = __longlong_as_double(__double_as_longlong(table[n & 31]) + ((int64_t)((n >> 5) + 44) << 52));
-    return (uint64_t)__double_as_longlong(fma(e, f, 0x1p52)) & 0xfffffffffffffull;
+    // times 2^(n / 128 + 44), the integer part of n / 128 straight into the exponent
+    const uint64_t f = __double_as_longlong(table[n & (kTable - 1)]);
+    const uint32_t hi = (uint32_t)(f >> 32) + ((uint32_t)(n & -kTable) << 13);
+    return __double_as_longlong(fma(e, __longlong_as_double((uint64_t)hi << 32 | (uint32_t)f), 0x1p52));
+}
+constexpr uint64_t kBitsOfZero = 0x4330000000000000ull;  // of 2^52
+__device__ __forceinline__ uint64_t weight(float l, float most, double scale, const double *table) {
+    if (most == INFINITY) return l == most ? (uint64_t)1 << 44 : 0;
+    return weight_bits(l, (double)most, scale, table) - kBitsOfZero;
 }
 __device__ __forceinline__ void fill_table(double *table, int tid) {
-    if (tid < 32) table[tid] = exp2(tid / 32.0);
+    if (tid < kTable) table[tid] = exp2(tid * (1.0 / kTable)) * kOne;
 }
-__device__ __forceinline__ double weight_scale(float temperature) { return 32.0 * 1.4426950408889634 / (double)temperature; }
+constexpr double kLog2e = 1.4426950408889634;
+__device__ __forceinline__ double weight_scale(float temperature) { return kTable * kLog2e / (double)temperature; }
+// exp2 of (a - b) in units of scale, for a <= b; 0 where b alone is infinite
+__device__ __forceinline__ double relative(float a, float b, double scale) {
+    return a == b ? 1.0 : b == INFINITY || a == -INFINITY ? 0.0 : exp2(((double)a - (double)b) * scale * (1.0 / kTable));
+}
+
+// The bin of a logit: 16ths of z on a grid that does not depend on the row, counted from
+// the largest's down; not rising with l.  (Where the grid's numbers leave their range all
+// have the last.)
+__device__ __forceinline__ float grid_of(float l, float per) { return floorf(l * per); }
+__device__ __forceinline__ int bin_of(float l, float top, float per) {
+    return (int)fmaxf(fminf(top - grid_of(l, per), (float)(kBins - 1)), 0.f);
+}
 
 // The logits of a group: -inf for NaN and from `end` on.
 template <typename T>
@@ -121,7 +153,8 @@ __device__ __forceinline__ void load_group(const T *row, int first, int end, flo
 
 template <typename T>
 __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) {
-    __shared__ double table[32];
+    __shared__ double table[kTable];
+    __shared__ uint64_t hist[kBins];
     __shared__ float mosts[4];
     __shared__ int ats[4];
     __shared__ uint64_t sums[4];
@@ -132,6 +165,7 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
     float x[kGroup];
     load_group(reinterpret_cast<const T *>(s.logits) + row * s.ld, first, s.vocab, x);
     fill_table(table, tid);
+    for (int i = tid; i < kBins; i += kGroups) hist[i] = 0;
     float most = x[0];
 #pragma unroll
     for (int e = 1; e < kGroup; ++e) most = fmaxf(most, x[e]);
@@ -153,8 +187,21 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
         if (mosts[w] > most) most = mosts[w], at = ats[w];
     uint64_t sum = 0;
     if (set.all()) {
+        const bool bins = set.bins(s.slices);
         const double scale = weight_scale(set.temperature);
-        if (most > -INFINITY) {
+        const float per = set.per(), top = grid_of(most, per);
+        if (most < INFINITY && most > -INFINITY) {
+            uint64_t w[kGroup];
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) w[e] = weight_bits(x[e], (double)most, scale, table) - kBitsOfZero;
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) sum += w[e];
+            if (bins) {
+#pragma unroll
+                for (int e = 0; e < kGroup; ++e)
+                    if (w[e]) atomicAdd((unsigned long long *)&hist[bin_of(x[e], top, per)], (unsigned long long)w[e]);
+            }
+        } else if (most == INFINITY) {
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) sum += weight(x[e], most, scale, table);
         }
@@ -163,6 +210,10 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
         sum = sums[0] + sums[1] + sums[2] + sums[3];
+        if (bins) {
+            uint64_t *const to = s.bins + ((int64_t)row * s.slices + slice) * kBins;
+            for (int i = tid; i < kBins; i += kGroups) to[i] = hist[i];
+        }
     }
     if (tid == 0) s.slice[(int64_t)row * s.slices + slice] = {most, at, sum};
 }
@@ -170,19 +221,38 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
 // ---- the second launch ------------------------------------------------------------
 
 struct PickShared {
-    double table[32];
+    double table[kTable];
     uint64_t wave_sums[2][kPickThreads / 64];
-    double slice_sums[kMaxSlices];
-    uint64_t chunk_sums[kMaxSlices];
-    uint32_t count[kBins];
-    uint64_t sum[kBins];
-    uint64_t key[kCandidates];
+    double slice_sums[kMaxSlices];   // running sums of all weights
+    double slice_scale[kMaxSlices];  // of a slice's weights in the row's
+    double kept[kMaxSlices];
+    uint64_t tied[kMaxSlices];
+    float slice_top[kMaxSlices];
+    uint32_t count[kDigits];
+    uint64_t sum[kDigits];  // (or doubles)
+    __attribute__((aligned(16))) uint64_t key[kCandidates];
     uint64_t weight[kCandidates];
     int index[kCandidates];
-    int hot[kCandidates];
-    int found;
+    int rank[kCandidates];
+    int order[kCandidates];
+    int found, n;
+    uint32_t edge[2];
     uint64_t found_count, found_sum;
+    double above;
 };
+
+// A bin's logits, over the candidates' arrays.
+struct List {
+    uint32_t key[kListed];
+    int at[kListed];
+};
+static_assert(sizeof(List) <= kCandidates * (2 * sizeof(uint64_t) + 3 * sizeof(int)), "the list fits");
+
+// The low bits of a key that are the same for all values of a type of one sign.
+template <typename T>
+constexpr int kZeroBits = std::is_same_v<T, float> ? 0 : std::is_same_v<T, _Float16> ? 13 : 16;
+
+__device__ __forceinline__ void sh_max(int &to, int x) { atomicMax(&to, x); }
 
 // Inclusive sum over the workgroup's threads, and the total; call after call takes
 // the other half of wave_sums, so one barrier does.
@@ -207,19 +277,20 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t x, PickShared &sh, int &
     return before + x;
 }
 
-// The bin of a logit: a 64th of z below the largest; not rising with l.
-__device__ __forceinline__ int bin_of(float l, float most, float per) {
-    if (l == most) return 0;
-    return (int)fminf((most - l) * per, (float)(kBins - 1));  // (NaN: the last)
-}
 // Larger logits have larger keys; all that cannot be drawn the lowest.
 __device__ __forceinline__ uint32_t order_key(float l) {
     const uint32_t u = __float_as_uint(l == 0.f ? 0.f : l);
     return u >> 31 ? ~u : u | 0x80000000u;
 }
 
+// The logit of a complemented key.
+__device__ __forceinline__ float logit_of(uint32_t inverse) {
+    const uint32_t key = ~inverse;
+    return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key);
+}
+
 struct Row {
-    float most, per;  // largest logit; bins to a unit of it
+    float most, top, per;  // largest logit, its bin of the grid, bins to a unit of it
     double scale;
     int k;
     double p, min_p;
@@ -230,7 +301,7 @@ struct Row {
 __device__ __forceinline__ void answer(const SampleParams &s, int row, int token, float l, const Row &r, double total) {
     s.tokens[row] = token;
     if (!s.logprobs) return;
-    const double z = l == r.most ? 0.0 : ((double)l - (double)r.most) * (r.scale * (1.0 / (32.0 * 1.4426950408889634)));
+    const double z = l == r.most ? 0.0 : ((double)l - (double)r.most) * (r.scale * (1.0 / (kTable * kLog2e)));
     s.logprobs[row] = (float)(z - log(total / kOne));
 }
 // floor(u total), below total.
@@ -240,18 +311,18 @@ __device__ __forceinline__ uint64_t target_of(double u, uint64_t total) {
     return n < total ? n : total - 1;
 }
 
-// No filter: the slice by the sums, then the token in it.
-template <typename T>
-__device__ __forceinline__ void pick_from_all(const SampleParams &s, int row, const Row &r, PickShared &sh, int tid,
-                                              double total) {
-    // sh.slice_sums: running sums
+// The slice that holds the token, by the slices' running sums of what stays, then the token
+// in it; stays(l, first, b) says which of a thread's logits do.
+template <typename T, typename F>
+__device__ __forceinline__ void pick_in_slice(const SampleParams &s, int row, const Row &r, PickShared &sh, int &turn,
+                                              int tid, const double *sums, F &&stays) {
+    const double total = sums[s.slices - 1], aim = fmin(fmax(r.u, 0.0), 1.0) * total;
     if (tid < 64) {
-        const double target = fmin(fmax(r.u, 0.0), 1.0) * total;
         int n = 0, last = -1;
         for (int i = tid; i < s.slices; i += 64) {
-            const double before = i ? sh.slice_sums[i - 1] : 0.0;
-            n += sh.slice_sums[i] <= target;
-            last = sh.slice_sums[i] > before ? i : last;
+            const double before = i ? sums[i - 1] : 0.0;
+            n += sums[i] <= aim;
+            last = sums[i] > before ? i : last;
         }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o), last = max(last, __shfl_xor(last, o));
@@ -259,35 +330,66 @@ __device__ __forceinline__ void pick_from_all(const SampleParams &s, int row, co
     }
     __syncthreads();
     const int slice = sh.found;
-    const double target = fmin(fmax(r.u, 0.0), 1.0) * total - (slice ? sh.slice_sums[slice - 1] : 0.0);
+    const double target = aim - (slice ? sums[slice - 1] : 0.0);
     const T *const x = reinterpret_cast<const T *>(s.logits) + row * s.ld;
-    constexpr int kPer = kSlice / kPickThreads;
+    constexpr int kPer = kPerPick;
     const int first = slice * kSlice + tid * kPer;
     float l[kPer];
+    bool in[kPer];
     uint64_t w[kPer], sum = 0;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        l[e] = first + e < s.vocab ? (float)x[first + e] : -INFINITY;
-        w[e] = weight(l[e], r.most, r.scale, sh.table);
+        const float v = first + e < s.vocab ? (float)x[first + e] : -INFINITY;
+        l[e] = v == v ? v : -INFINITY;
+    }
+    stays(l, first, in);
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+        w[e] = in[e] ? weight(l[e], r.most, r.scale, sh.table) : 0;
         sum += w[e];
     }
-    int turn = 0;
     uint64_t all;
-    uint64_t upto = block_scan(sum, sh, turn, tid, all);
-    // (weights so small that all are 0 here: the slice's largest)
-    const Slice sl = s.slice[(int64_t)row * s.slices + slice];
-    if (all == 0) {
+    uint64_t before = block_scan(sum, sh, turn, tid, all) - sum;
+    if (all == 0) {  // weights so small that all are 0 here: the slice's largest
+        const Slice sl = s.slice[(int64_t)row * s.slices + slice];
         if (tid == 0) answer(s, row, sl.at, sl.most, r, total);
         return;
     }
     uint64_t n = target > 0.0 ? (uint64_t)target : 0;
     n = n < all ? n : all - 1;
-    upto -= sum;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-        if (upto <= n && n < upto + w[e]) answer(s, row, first + e, l[e], r, total);
-        upto += w[e];
+        if (before <= n && n < before + w[e]) answer(s, row, first + e, l[e], r, total);
+        before += w[e];
     }
+}
+
+// The places of n keys (all different, ~0 never) in rising order: sh.order.  Every
+// key counts the smaller ones.
+__device__ __forceinline__ void put_in_order(PickShared &sh, int n, int tid) {
+    int size = 64;
+    while (size < n) size <<= 1;
+    for (int i = tid; i < size; i += kPickThreads) {
+        sh.rank[i] = 0;
+        if (i >= n) sh.key[i] = ~(uint64_t)0;
+    }
+    __syncthreads();
+    const int parts = max(1, kPickThreads / size), per = size / parts;
+    typedef unsigned long long pair __attribute__((ext_vector_type(2)));
+    for (int i = tid % size; i < n; i += kPickThreads) {
+        const uint64_t mine = sh.key[i];
+        const int first = parts > 1 ? tid / size * per : 0;
+        int smaller = 0;
+#pragma unroll 8
+        for (int j = first; j < first + per; j += 2) {
+            const pair k = *reinterpret_cast<const pair *>(&sh.key[j]);
+            smaller += (k[0] < mine) + (k[1] < mine);
+        }
+        atomicAdd(&sh.rank[i], smaller);
+    }
+    __syncthreads();
+    for (int i = tid; i < n; i += kPickThreads) sh.order[sh.rank[i]] = i;
+    __syncthreads();
 }
 
 // Candidates, if they are few enough: the logits in bins up to the one that holds
@@ -303,36 +405,63 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
     uint64_t total;
     int last = kBins - 1;  // bin of the last candidates
     bool guess = false;
-    if (!r.k && r.min_p > 0.0) {
-        const double b = -log(r.min_p) * 64.0 + 2.0;  // (2: the bins' own rounding)
+    if (!r.k && r.min_p > 0.0 && fabsf(r.top) < 0x1p22f) {
+        const double b = -log(r.min_p) * 16.0 + 3.0;  // (the grid's cell of the largest, and roundings)
         last = (int)fmin(fmax(b, 0.0), (double)(kBins - 1));
     }
+    // this thread's groups: neighbours, the first kHeld kept in registers
+    constexpr int kHeld = 8;
+    const int per = (groups + kPickThreads - 1) / kPickThreads, g0 = tid * per, g1 = min(groups, g0 + per);
+    int bin[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) bin[i] = i < per && g0 + i < g1 ? bin_of(maxima[g0 + i], r.top, r.per) : kBins;
+    auto each_group = [&](auto &&f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i)
+            if (bin[i] < kBins) f(g0 + i, bin[i]);
+        for (int i = g0 + kHeld; i < g1; ++i) f(i, bin_of(maxima[i], r.top, r.per));
+    };
     if (r.k || r.p < 1.0) {
         const int want = r.k ? r.k : min(kGuess, groups / 4 + 1);
         if (want > kCandidates) return false;
-        for (int i = tid; i < kBins; i += kPickThreads) sh.count[i] = 0;
+        if (tid < kBins) sh.count[tid] = 0;
         __syncthreads();
-        for (int i = tid; i < groups; i += kPickThreads) atomicAdd(&sh.count[bin_of(maxima[i], r.most, r.per)], 1u);
-        if (tid == 0) sh.found = kBins - 1;
+        each_group([&](int, int b) { atomicAdd(&sh.count[b], 1u); });
         __syncthreads();
-        const uint32_t a = sh.count[2 * tid], b = sh.count[2 * tid + 1];
-        const uint64_t upto = block_scan(a + b, sh, turn, tid, total);
-        const int before = (int)(upto - a - b);
-        if (before < want && before + (int)a >= want) sh.found = 2 * tid;
-        if (before + (int)a < want && (int)upto >= want) sh.found = 2 * tid + 1;
+        if (tid < 64) {
+            constexpr int kEach = kBins / 64;
+            int c[kEach], n = 0, at = kBins - 1;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) n += c[e] = (int)sh.count[kEach * tid + e];
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(upto, o);
+                upto += tid >= o ? y : 0;
+            }
+            upto -= n;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) {
+                at = upto < want && upto + c[e] >= want ? kEach * tid + e : at;
+                upto += c[e];
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
+            if (tid == 0) sh.found = at;
+        }
         __syncthreads();
         guess = !r.k && sh.found < last;
         last = min(last, sh.found);
     }
     // the groups that have candidates, in their order
-    const int per = (groups + kPickThreads - 1) / kPickThreads;
     uint64_t mine = 0;
-    for (int i = tid * per; i < min(groups, (tid + 1) * per); ++i) mine += bin_of(maxima[i], r.most, r.per) <= last;
-    uint64_t at = block_scan(mine, sh, turn, tid, total) - mine;
+    each_group([&](int, int b) { mine += b <= last; });
+    int at = (int)(block_scan(mine, sh, turn, tid, total) - mine);
     if (total > kCandidates) return false;
     const int hot = (int)total;
-    for (int i = tid * per; mine && i < min(groups, (tid + 1) * per); ++i)
-        if (bin_of(maxima[i], r.most, r.per) <= last) sh.hot[at++] = i;
+    if (mine) each_group([&](int g, int b) {
+        if (b <= last) sh.order[at++] = g;
+    });
     __syncthreads();
     // the candidates, in their order
     int n = 0;
@@ -341,13 +470,13 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
         int first = 0;
         uint32_t in = 0;
         if (h0 + tid < hot) {
-            first = sh.hot[h0 + tid] * kGroup;
+            first = sh.order[h0 + tid] * kGroup;
             load_group(x, first, s.vocab, l);
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e) in |= (uint32_t)(bin_of(l[e], r.most, r.per) <= last && first + e < s.vocab) << e;
+            for (int e = 0; e < kGroup; ++e) in |= (uint32_t)(bin_of(l[e], r.top, r.per) <= last && first + e < s.vocab) << e;
         }
         const uint64_t c = __popc(in);
-        at = n + block_scan(c, sh, turn, tid, total) - c;
+        at = n + (int)(block_scan(c, sh, turn, tid, total) - c);
         n += (int)total;
         if (n > kCandidates) return false;
 #pragma unroll
@@ -355,24 +484,13 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
             if (in >> e & 1) {
                 sh.key[at] = (uint64_t)~order_key(l[e]) << 32 | (uint32_t)at;
                 sh.index[at] = first + e;
-                sh.weight[at] = weight(l[e], r.most, r.scale, sh.table);
                 ++at;
             }
     }
-    // sorted: larger logits first, equal ones as they came
-    int size = 2;
-    while (size < n) size <<= 1;
-    for (int i = n + tid; i < size; i += kPickThreads) sh.key[i] = ~(uint64_t)0;
-    for (int b = 2; b <= size; b <<= 1)
-        for (int d = b >> 1; d > 0; d >>= 1) {
-            __syncthreads();
-            const int i = (tid & ~(d - 1)) * 2 + (tid & (d - 1));
-            if (i + d < size) {
-                const uint64_t p = sh.key[i], q = sh.key[i + d];
-                if ((p > q) == !(i & b)) sh.key[i] = q, sh.key[i + d] = p;
-            }
-        }
     __syncthreads();
+    for (int i = tid; i < n; i += kPickThreads)
+        sh.weight[i] = weight(logit_of((uint32_t)(sh.key[i] >> 32)), r.most, r.scale, sh.table);
+    put_in_order(sh, n, tid);
     // how many stay
     static_assert(kCandidates == 2 * kPickThreads, "two places per thread");
     int pos[2];
@@ -380,21 +498,20 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int j = 2 * tid + e;
-        pos[e] = j < n ? (int)(uint32_t)sh.key[j] : 0;
+        pos[e] = j < n ? sh.order[j] : 0;
         w[e] = j < n ? sh.weight[pos[e]] : 0;
     }
     uint64_t limit = ~(uint64_t)0;
     const int k = r.k ? min(r.k, n) : n;
-    uint64_t upto = block_scan((2 * tid < k ? w[0] : 0) + (2 * tid + 1 < k ? w[1] : 0), sh, turn, tid, total);
+    const uint64_t inside = (2 * tid < k ? w[0] : 0) + (2 * tid + 1 < k ? w[1] : 0);
+    uint64_t before = block_scan(inside, sh, turn, tid, total) - inside;
     if (r.p < 1.0) {
         const double most = r.p * (r.k ? (double)total : all);
         limit = most > 0.0 ? (uint64_t)ceil(most) : 0;
         if (guess && total < limit) return false;  // the next ones would stay too
     }
     // (a thread's sum without the places from k on, which do not stay anyway)
-    uint64_t before = upto - (2 * tid < k ? w[0] : 0) - (2 * tid + 1 < k ? w[1] : 0);
     const double least = r.min_p * kOne;
-    __syncthreads();
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         const int j = 2 * tid + e;
@@ -405,9 +522,8 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
     __syncthreads();
     w[0] = 2 * tid < n ? sh.weight[2 * tid] : 0;
     w[1] = 2 * tid + 1 < n ? sh.weight[2 * tid + 1] : 0;
-    upto = block_scan(w[0] + w[1], sh, turn, tid, total);
+    before = block_scan(w[0] + w[1], sh, turn, tid, total) - w[0] - w[1];
     const uint64_t target = target_of(r.u, total);
-    before = upto - w[0] - w[1];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         if (before <= target && target < before + w[e]) {
@@ -416,6 +532,234 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
         }
         before += w[e];
     }
+    return true;
+}
+
+// top-p without top-k: the bins of the first launch say which bin the cut lies in; one
+// pass over the row collects that bin's logits.  False: too many in it, or min_p may cut
+// before.  (The last bin holds what lies more than 32 below the largest of its slice: 2^19
+// e^-32 of the weights at most, less than the 2^-24 that p leaves.)
+template <typename T>
+__device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, const Row &r, PickShared &sh, int tid,
+                                             double all) {
+    const T *const x = reinterpret_cast<const T *>(s.logits) + row * s.ld;
+    const uint64_t *const bins = s.bins + (int64_t)row * s.slices * kBins;
+    const Slice *const slices = s.slice + (int64_t)row * s.slices;
+    if (!(fabsf(r.top) < 0x1p22f)) return false;
+    int turn = 0;
+    double *const sums = reinterpret_cast<double *>(sh.sum);
+    __syncthreads();
+    if (tid < s.slices) {
+        const float most = slices[tid].most;
+        sh.slice_top[tid] = most > -INFINITY ? grid_of(most, r.per) : r.top - kBins;
+        sh.slice_scale[tid] = relative(most, r.most, r.scale);
+    }
+    __syncthreads();
+    // the row's bins, two threads to each with half of the slices
+    {
+        const int b = tid % kBins, part = tid / kBins, half = (s.slices + 1) / 2;
+        static_assert(kPickThreads == 2 * kBins, "two threads per bin");
+        double sum = 0.0;
+        for (int i = part * half; i < min(s.slices, (part + 1) * half); ++i) {
+            const int at = b - (int)fminf(r.top - sh.slice_top[i], (float)kBins);
+            if (at >= 0 && at < kBins - 1) sum += (double)bins[i * kBins + at] * sh.slice_scale[i];
+        }
+        sums[tid] = sum;
+    }
+    __syncthreads();
+    const double limit = r.p * all;
+    if (tid < 64) {
+        constexpr int kEach = kBins / 64;
+        double c[kEach], n = 0.0;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) n += c[e] = sums[kEach * tid + e] + sums[kBins + kEach * tid + e];
+        double upto = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double y = __shfl_up(upto, o);
+            upto += tid >= o ? y : 0.0;
+        }
+        upto -= n;
+        // (the first bin that reaches the limit; lane by lane from the first)
+        int at = kBins;
+        double above = 0.0;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const bool here = at == kBins && c[e] > 0.0 && upto + c[e] >= limit;
+            at = here ? kEach * tid + e : at;
+            above = here ? upto : above;
+            upto += c[e];
+        }
+        int first = at;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o));
+        if (tid == 0) sh.n = 0;
+        if (at == first && at < kBins) sh.above = above;
+        if (tid == 0) sh.found = first;
+    }
+    __syncthreads();
+    const int cut = sh.found;
+    if (cut >= kBins - 1) return false;
+    // min_p may take something of the bins up to this one
+    if (r.min_p > 0.0 && !(exp(-(cut + 2) * (1.0 / 16)) >= r.min_p)) return false;
+    const double above = sh.above;
+    // what stays of every slice in the bins before
+    for (int i = tid >> 6; i < s.slices; i += kPickThreads / 64) {
+        const int end = cut - (int)fminf(r.top - sh.slice_top[i], (float)kBins);
+        double sum = 0.0;
+        for (int b = tid & 63; b < end; b += 64) sum += (double)bins[i * kBins + b];
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        if ((tid & 63) == 0) sh.kept[i] = sum * sh.slice_scale[i];
+    }
+    // The bin's keys are neighbours, from the lowest whose grid number is the bin's to the
+    // highest: a wave each looks for where it and the next one begin.
+    if (tid < 128) {
+        const float from = r.top - (float)cut + (float)(tid >> 6);
+        uint32_t key = 0;  // all less than it are below
+        for (int bit = 31; bit >= 0; --bit) {
+            const uint32_t up = key | 1u << bit;
+            const float l = logit_of(~(up - 1));
+            key = l != l ? (up >> 31 ? key : up) : grid_of(l, r.per) < from ? up : key;
+        }
+        if ((tid & 63) == 0) sh.edge[tid >> 6] = key;
+    }
+    __syncthreads();
+    uint32_t lo = sh.edge[0], hi = sh.edge[1] - 1;
+    // its logits and places, in any order
+    List &list = *reinterpret_cast<List *>(sh.key);
+    const int lane = tid & 63;
+    for (int i0 = 0; i0 < s.vocab; i0 += kPickThreads * kGroup) {
+        const int first = i0 + tid * kGroup;
+        float l[kGroup];
+        uint32_t in = 0;
+        if (first < s.vocab) {
+            load_group(x, first, s.vocab, l);
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) in |= (uint32_t)(order_key(l[e]) - lo <= hi - lo) << e;
+        }
+        if (!__any(in != 0)) continue;
+        int upto = __popc(in);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(upto, o);
+            upto += lane >= o ? y : 0;
+        }
+        int at = 0;
+        if (lane == 63) at = atomicAdd(&sh.n, upto);
+        at = __shfl(at, 63) + upto - (int)__popc(in);
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e)
+            if (in >> e & 1) {
+                if (at < kListed) list.key[at] = order_key(l[e]), list.at[at] = first + e;
+                ++at;
+            }
+    }
+    __syncthreads();
+    const int n = sh.n;
+    if (n > kListed) return false;
+    // the cut's key, eleven bits of what is open at a time
+    double before = above;
+    uint64_t ties = 0;
+    for (;;) {
+        const int shift = max(0, 32 - __builtin_clz((hi - lo) | 1) - 11);
+        __syncthreads();
+        for (int i = tid; i < kDigits; i += kPickThreads) sh.count[i] = 0, sh.sum[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kPickThreads) {
+            const uint32_t key = list.key[i];
+            if (key - lo > hi - lo) continue;
+            const int digit = (int)((hi - key) >> shift);
+            atomicAdd(&sh.count[digit], 1u);
+            atomicAdd((unsigned long long *)&sh.sum[digit],
+                      (unsigned long long)weight(logit_of(~key), r.most, r.scale, sh.table));
+        }
+        __syncthreads();
+        const uint64_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1], s0 = sh.sum[2 * tid], s1 = sh.sum[2 * tid + 1];
+        if (tid == 0) sh.found = -1;
+        uint64_t total;
+        double ahead = before + (double)(block_scan(s0 + s1, sh, turn, tid, total) - s0 - s1);
+        // the last digit that something of stays: its first logit has less than the limit before
+        // it (or none at all); where the sums' last bits let none stay, the first
+        int mine = -1;
+        if (c0 && (ahead < limit || ahead == 0.0)) mine = 2 * tid, sh_max(sh.found, mine);
+        if (c1 && (ahead + (double)s0 < limit || ahead + (double)s0 == 0.0)) mine = 2 * tid + 1, sh_max(sh.found, mine);
+        __syncthreads();
+        const int found = sh.found;
+        if (found < 0) return false;
+        if (found >> 1 == tid) {
+            sh.above = found & 1 ? ahead + (double)s0 : ahead;
+            sh.found_count = found & 1 ? c1 : c0;
+            sh.found_sum = found & 1 ? s1 : s0;
+        }
+        __syncthreads();
+        before = sh.above;
+        const uint32_t top = hi - ((uint32_t)found << shift);
+        lo = max(lo, top - ((1u << shift) - 1));
+        hi = top;
+        if (shift == 0 || shift <= kZeroBits<T>) {
+            // one value: equal logits, equal weights
+            const uint64_t w = sh.found_sum / sh.found_count;
+            ties = sh.found_count;
+            if (w) ties = min(ties, before < limit ? (uint64_t)ceil(fmin((limit - before) / (double)w, 0x1p40)) : (uint64_t)0);
+            ties = max(ties, (uint64_t)1);
+            break;
+        }
+    }
+    // what stays of it, slice by slice; of equal ones the first by their index
+    if (tid < s.slices) sh.tied[tid] = 0, sh.count[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kPickThreads) {
+        const uint32_t key = list.key[i];
+        const int slice = list.at[i] / kSlice;
+        if (key > hi)
+            atomicAdd((unsigned long long *)&sh.tied[slice], (unsigned long long)weight(logit_of(~key), r.most, r.scale, sh.table));
+        else if (key >= lo)
+            atomicAdd(&sh.count[slice], 1u);
+    }
+    __syncthreads();
+    const uint64_t equal = sh.found_sum / sh.found_count;
+    if (tid < 64) {
+        double upto = 0.0;
+        uint32_t ranks = 0;
+        for (int i0 = 0; i0 < s.slices; i0 += 64) {
+            const bool in = i0 + tid < s.slices;
+            uint32_t c = in ? sh.count[i0 + tid] : 0, rank = c;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(rank, o);
+                rank += tid >= o ? y : 0;
+            }
+            rank += ranks - c;  // equal ones in the slices before
+            const uint64_t stay = rank < ties ? min((uint64_t)c, ties - rank) : 0;
+            double v = in ? sh.kept[i0 + tid] + (double)(sh.tied[i0 + tid] + stay * equal) : 0.0;
+            ranks = __shfl(rank + c, 63);
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const double y = __shfl_up(v, o);
+                v += tid >= o ? y : 0.0;
+            }
+            if (in) sh.kept[i0 + tid] = upto + v, sh.count[i0 + tid] = rank;
+            upto += __shfl(v, 63);
+        }
+    }
+    __syncthreads();
+    // (a thread's logits are neighbours, and so are the threads: a scan counts the equal ones)
+    pick_in_slice<T>(s, row, r, sh, turn, tid, sh.kept, [&](const float (&l)[kPerPick], int first, bool (&stays)[kPerPick]) {
+        uint64_t c = 0, total;
+#pragma unroll
+        for (int e = 0; e < kPerPick; ++e) {
+            const uint32_t key = order_key(l[e]);
+            stays[e] = key > hi;
+            c += key >= lo && key <= hi;
+        }
+        uint64_t rank = sh.count[first / kSlice] + block_scan(c, sh, turn, tid, total) - c;
+#pragma unroll
+        for (int e = 0; e < kPerPick; ++e) {
+            const uint32_t key = order_key(l[e]);
+            if (key >= lo && key <= hi) stays[e] = rank++ < ties;
+        }
+    });
     return true;
 }
 
@@ -440,7 +784,7 @@ __device__ __forceinline__ Cut cut_row(const SampleParams &s, int row, const Row
         const int shift = round == 1 ? 21 : round == 2 ? 10 : 0;
         const uint32_t known = round <= 1 ? 0u : round == 2 ? ~0u << 21 : ~0u << 10;
         __syncthreads();
-        for (int i = tid; i < kBins; i += kPickThreads) sh.count[i] = 0, sh.sum[i] = 0;
+        for (int i = tid; i < kDigits; i += kPickThreads) sh.count[i] = 0, sh.sum[i] = 0;
         if (tid == 0) sh.found = -1;
         __syncthreads();
         for (int i0 = tid * kGroup; i0 < s.vocab; i0 += kPickThreads * kGroup) {
@@ -449,7 +793,7 @@ __device__ __forceinline__ Cut cut_row(const SampleParams &s, int row, const Row
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) {
                 if (i0 + e >= s.vocab) continue;
-                const int b = bin_of(l[e], r.most, r.per);
+                const int b = bin_of(l[e], r.top, r.per);
                 const uint32_t key = order_key(l[e]);
                 int at;
                 if (round == 0)
@@ -463,6 +807,7 @@ __device__ __forceinline__ Cut cut_row(const SampleParams &s, int row, const Row
             }
         }
         __syncthreads();
+        static_assert(kDigits == 2 * kPickThreads && kBins <= kDigits, "two places per thread");
         uint64_t total;
         const uint64_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1], s0 = sh.sum[2 * tid], s1 = sh.sum[2 * tid + 1];
         uint64_t cn = count + block_scan(c0 + c1, sh, turn, tid, total) - c0 - c1;
@@ -549,17 +894,17 @@ __device__ __forceinline__ void pick_from_row(const SampleParams &s, int row, co
     uint64_t w[kPer];
     for (int i = 0; i < s.slices; ++i) {
         uint64_t part;
-        if (tid == 0) sh.key[i] = tied;
+        if (tid == 0) sh.kept[i] = (double)tied;
         block_scan(slice_weights(i, tied, l, w), sh, turn, tid, part);
         upto += part;
-        if (tid == 0) sh.chunk_sums[i] = upto;
+        if (tid == 0) sh.tied[i] = upto;
     }
     __syncthreads();
     const uint64_t target = target_of(r.u, upto);
     int slice = 0;
-    while (sh.chunk_sums[slice] <= target) ++slice;  // (ends: target < the last)
-    const uint64_t start = slice ? sh.chunk_sums[slice - 1] : 0;
-    tied = sh.key[slice];
+    while (sh.tied[slice] <= target) ++slice;  // (ends: target < the last)
+    const uint64_t start = slice ? sh.tied[slice - 1] : 0;
+    tied = (uint64_t)sh.kept[slice];
     sum = slice_weights(slice, tied, l, w);
     uint64_t part;
     uint64_t before = start + block_scan(sum, sh, turn, tid, part) - sum;
@@ -599,12 +944,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
             double before = 0.0;
             for (int i0 = 0; i0 < s.slices; i0 += 64) {
                 double w = 0.0;
-                if (i0 + tid < s.slices) {
-                    const Slice x = sl[i0 + tid];
-                    w = x.most == most ? (double)x.sum
-                                       : (double)x.sum * exp2(((double)x.most - (double)most) * scale * (1.0 / 32));
-                    w = x.most == most || (most < INFINITY && x.most > -INFINITY) ? w : 0.0;
-                }
+                if (i0 + tid < s.slices) w = (double)sl[i0 + tid].sum * relative(sl[i0 + tid].most, most, scale);
 #pragma unroll
                 for (int o = 1; o < 64; o <<= 1) {
                     const double y = __shfl_up(w, o);
@@ -625,12 +965,23 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
         }
         return;
     }
-    const Row r{most, 64.f / set.temperature, scale, set.k, set.p, set.min_p, (double)s.u[row]};
+    const float per = set.per();
+    const Row r{most, grid_of(most, per), per, scale, set.k, set.p, set.min_p, (double)s.u[row]};
     const double all = set.all() ? sh.slice_sums[s.slices - 1] : 0.0;
-    if (!r.k && !(r.p < 1.0) && !(r.min_p > 0.0))
-        pick_from_all<T>(s, row, r, sh, tid, all);
-    else if (!pick_from_few<T>(s, row, r, sh, tid, all))
-        pick_from_row<T>(s, row, r, sh, tid, all);
+    if (!r.k && !(r.p < 1.0) && !(r.min_p > 0.0)) {
+        int turn = 0;
+        pick_in_slice<T>(s, row, r, sh, turn, tid, sh.slice_sums, [](const float (&)[kPerPick], int, bool (&b)[kPerPick]) {
+#pragma unroll
+            for (int e = 0; e < kPerPick; ++e) b[e] = true;
+        });
+        return;
+    }
+    if (set.bins(s.slices)) {
+        if (pick_by_bins<T>(s, row, r, sh, tid, all)) return;
+        __syncthreads();
+    }
+    if (pick_from_few<T>(s, row, r, sh, tid, all)) return;
+    pick_from_row<T>(s, row, r, sh, tid, all);
 }
 
 int64_t slices_of(int64_t vocab) { return (vocab + kSlice - 1) / kSlice; }
@@ -640,7 +991,8 @@ int64_t slices_of(int64_t vocab) { return (vocab + kSlice - 1) / kSlice; }
 int64_t sample_max_vocab() { return (int64_t)kMaxSlices * kSlice; }
 int64_t sample_blocks(const SampleDesc &d) { return d.rows * slices_of(d.vocab); }
 size_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
-    return (size_t)(rows * slices_of(vocab)) * (kGroups * sizeof(float) + sizeof(Slice));
+    const int64_t slices = slices_of(vocab);
+    return (size_t)(rows * slices) * (kGroups * sizeof(float) + sizeof(Slice) + (slices > 1 ? kBins * sizeof(uint64_t) : 0));
 }
 
 int launch_sample(const SampleDesc &d, void *workspace, hipStream_t st) {
@@ -653,6 +1005,7 @@ int launch_sample(const SampleDesc &d, void *workspace, hipStream_t st) {
     s.set = d.set;
     s.slice = static_cast<Slice *>(workspace);
     s.maxima = reinterpret_cast<float *>(s.slice + d.rows * s.slices);
+    s.bins = reinterpret_cast<uint64_t *>(s.maxima + d.rows * s.slices * kGroups);
     s.tokens = d.tokens;
     s.logprobs = d.logprobs;
     auto go = [&](auto t) -> int {
