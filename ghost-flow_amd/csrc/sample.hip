@@ -130,25 +130,36 @@ __device__ __forceinline__ int bin_of(float l, float top, float per) {
     return (int)fmaxf(fminf(top - grid_of(l, per), (float)(kBins - 1)), 0.f);
 }
 
-// The logits of a group: -inf for NaN and from `end` on.
+// A group of logits as it lies in memory (rows begin anywhere that their type allows),
+// and in fp32: -inf for NaN and from `end` on.  Apart, so that loads can be on their way.
+template <typename T>
+struct Group {
+    static constexpr int E = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+    vec v[kGroup / E];
+
+    __device__ __forceinline__ void load(const T *row, int first, int end) {
+        if (first + kGroup <= end) {
+#pragma unroll
+            for (int i = 0; i < kGroup / E; ++i) v[i] = *reinterpret_cast<const vec *>(row + first + i * E);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kGroup; ++e) v[e / E][e % E] = first + e < end ? row[first + e] : (T)-INFINITY;
+        }
+    }
+    __device__ __forceinline__ void values(float (&x)[kGroup]) const {
+#pragma unroll
+        for (int e = 0; e < kGroup; ++e) {
+            x[e] = (float)v[e / E][e % E];
+            x[e] = x[e] == x[e] ? x[e] : -INFINITY;
+        }
+    }
+};
 template <typename T>
 __device__ __forceinline__ void load_group(const T *row, int first, int end, float (&x)[kGroup]) {
-    constexpr int E = 16 / sizeof(T);
-    // (rows begin anywhere that their type allows)
-    typedef T vec __attribute__((ext_vector_type(E), aligned(sizeof(T))));
-    if (first + kGroup <= end) {
-#pragma unroll
-        for (int i = 0; i < kGroup / E; ++i) {
-            const vec v = *reinterpret_cast<const vec *>(row + first + i * E);
-#pragma unroll
-            for (int e = 0; e < E; ++e) x[i * E + e] = (float)v[e];
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < kGroup; ++e) x[e] = first + e < end ? (float)row[first + e] : -INFINITY;
-    }
-#pragma unroll
-    for (int e = 0; e < kGroup; ++e) x[e] = x[e] == x[e] ? x[e] : -INFINITY;
+    Group<T> g;
+    g.load(row, first, end);
+    g.values(x);
 }
 
 template <typename T>
@@ -409,12 +420,18 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
         const double b = -log(r.min_p) * 16.0 + 3.0;  // (the grid's cell of the largest, and roundings)
         last = (int)fmin(fmax(b, 0.0), (double)(kBins - 1));
     }
-    // this thread's groups: neighbours, the first kHeld kept in registers
+    // this thread's groups: whole fours, neighbours, the first kHeld kept in registers
     constexpr int kHeld = 8;
-    const int per = (groups + kPickThreads - 1) / kPickThreads, g0 = tid * per, g1 = min(groups, g0 + per);
+    const int per = ((groups + kPickThreads - 1) / kPickThreads + 3) & ~3, g0 = tid * per, g1 = min(groups, g0 + per);
     int bin[kHeld];
+    {
+        f32x4 held[kHeld / 4];
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) bin[i] = i < per && g0 + i < g1 ? bin_of(maxima[g0 + i], r.top, r.per) : kBins;
+        for (int i = 0; i < kHeld / 4; ++i)  // (all on their way at once)
+            held[i] = *reinterpret_cast<const f32x4 *>(maxima + min(g0 + 4 * i, s.slices * kGroups - 4));
+#pragma unroll
+        for (int i = 0; i < kHeld; ++i) bin[i] = i < per && g0 + i < g1 ? bin_of(held[i / 4][i % 4], r.top, r.per) : kBins;
+    }
     auto each_group = [&](auto &&f) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kHeld; ++i)
@@ -560,9 +577,11 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
         const int b = tid % kBins, part = tid / kBins, half = (s.slices + 1) / 2;
         static_assert(kPickThreads == 2 * kBins, "two threads per bin");
         double sum = 0.0;
+#pragma unroll 8
         for (int i = part * half; i < min(s.slices, (part + 1) * half); ++i) {
             const int at = b - (int)fminf(r.top - sh.slice_top[i], (float)kBins);
-            if (at >= 0 && at < kBins - 1) sum += (double)bins[i * kBins + at] * sh.slice_scale[i];
+            const uint64_t w = bins[i * kBins + max(at, 0)];
+            sum += at >= 0 && at < kBins - 1 ? (double)w * sh.slice_scale[i] : 0.0;
         }
         sums[tid] = sum;
     }
@@ -607,7 +626,12 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
     for (int i = tid >> 6; i < s.slices; i += kPickThreads / 64) {
         const int end = cut - (int)fminf(r.top - sh.slice_top[i], (float)kBins);
         double sum = 0.0;
-        for (int b = tid & 63; b < end; b += 64) sum += (double)bins[i * kBins + b];
+#pragma unroll
+        for (int j = 0; j < kBins / 64; ++j) {
+            const int b = 64 * j + (tid & 63);
+            const uint64_t w = bins[i * kBins + b];
+            sum += b < end ? (double)w : 0.0;
+        }
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
         if ((tid & 63) == 0) sh.kept[i] = sum * sh.slice_scale[i];
@@ -626,38 +650,45 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
     }
     __syncthreads();
     uint32_t lo = sh.edge[0], hi = sh.edge[1] - 1;
-    // its logits and places, in any order
+    // the places of its logits, in any order, from the groups whose largest reaches it; a wave's
+    // next groups are on their way
     List &list = *reinterpret_cast<List *>(sh.key);
-    const int lane = tid & 63;
-    for (int i0 = 0; i0 < s.vocab; i0 += kPickThreads * kGroup) {
-        const int first = i0 + tid * kGroup;
-        float l[kGroup];
-        uint32_t in = 0;
-        if (first < s.vocab) {
-            load_group(x, first, s.vocab, l);
+    {
+        const int groups = (s.vocab + kGroup - 1) / kGroup, last = groups - 1;
+        const float *const maxima = s.maxima + (int64_t)row * s.slices * kGroups;
+        const float low = logit_of(~lo), high = logit_of(~hi);
+        Group<T> now, next;
+        bool any = __any(maxima[min(tid, last)] >= low), any2;
+        if (any) now.load(x, min(tid, last) * kGroup, s.vocab);
+        for (int g = tid; g - (tid & 63) < groups; g += kPickThreads, now = next, any = any2) {
+            any2 = __any(maxima[min(g + kPickThreads, last)] >= low) && g - (tid & 63) + kPickThreads < groups;
+            if (any2) next.load(x, min(g + kPickThreads, last) * kGroup, s.vocab);
+            if (!any) continue;
+            float l[kGroup];
+            now.values(l);
+            uint32_t in = 0;
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e) in |= (uint32_t)(order_key(l[e]) - lo <= hi - lo) << e;
-        }
-        if (!__any(in != 0)) continue;
-        int upto = __popc(in);
+            for (int e = 0; e < kGroup; ++e) in |= (uint32_t)(l[e] >= low && l[e] <= high) << e;
+            in = g < groups ? in : 0;
+            if (!__any(in != 0)) continue;
+            const int mine = __popc(in);
+            int upto = mine;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(upto, o);
-            upto += lane >= o ? y : 0;
-        }
-        int at = 0;
-        if (lane == 63) at = atomicAdd(&sh.n, upto);
-        at = __shfl(at, 63) + upto - (int)__popc(in);
-#pragma unroll
-        for (int e = 0; e < kGroup; ++e)
-            if (in >> e & 1) {
-                if (at < kListed) list.key[at] = order_key(l[e]), list.at[at] = first + e;
-                ++at;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int y = __shfl_up(upto, o);
+                upto += (tid & 63) >= o ? y : 0;
             }
+            int at = 0;
+            if ((tid & 63) == 63) at = atomicAdd(&sh.n, upto);
+            at = __builtin_amdgcn_readlane(at, 63) + upto - mine;
+            for (; in; in &= in - 1, ++at)
+                if (at < kListed) list.at[at] = g * kGroup + __builtin_ctz(in);
+        }
     }
     __syncthreads();
     const int n = sh.n;
     if (n > kListed) return false;
+    for (int i = tid; i < n; i += kPickThreads) list.key[i] = order_key((float)x[list.at[i]]);
     // the cut's key, eleven bits of what is open at a time
     double before = above;
     uint64_t ties = 0;
