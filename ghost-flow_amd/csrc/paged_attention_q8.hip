@@ -62,7 +62,8 @@ __device__ __forceinline__ float quarter_step(uint32_t b) {
     return __uint_as_float((min(b, (uint32_t)paged::kMaxStep) + (paged::kStepBits - 16)) << 20);
 }
 __device__ __forceinline__ Step step_pair(float s0, float s1) {
-    return {f16x2{(_Float16)s0, (_Float16)s1}, f16x2{(_Float16)(-1152.f * s0), (_Float16)(-1152.f * s1)}};
+    const f16x2 f = {(_Float16)s0, (_Float16)s1};
+    return {f, f * (_Float16)-1152.f};  // (exact: four bits times 9 2^7)
 }
 // Codes in bytes 0, 1 (HI: 2, 3) of w as f16 values.
 template <bool HI>
@@ -375,18 +376,25 @@ __global__ __launch_bounds__(64 * WAVES, NQ > 1 ? 2 : 3) void paged_q8_decode_ke
 
 // ---- many rows: chunks of prompts ---------------------------------------------------
 //
-// A tile of 128 rows, four waves of 32, K and V tiles of 64 keys in two stages of LDS,
-// one barrier per tile and the products as in paged_attention.hip.  Codes come into
-// registers (16 of K and of V per thread and 16 bytes of row, a tile ahead), become
-// f16 there and go to LDS as the layout of those products wants them.
-template <typename TA, int DP, int ND, int NQ>
-__global__ __launch_bounds__(256, 2) void paged_q8_chunk_kernel(Q8Params pp) {
+// A tile of 32 rows per wave, K and V tiles of 64 keys in two stages of LDS, one barrier
+// per tile and the products as in paged_attention.hip.  Codes come into registers (16 of K
+// and of V per thread and row, a tile ahead), become f16 there and go to LDS as the
+// layout of those products wants them.
+//
+// Bound by the vector ALU and the matrix units together, as the 16-bit kernel is, with some
+// 90 vector instructions per wave and tile more for the codes (of 290; half as many in tiles
+// of 256 rows): 2048 tokens over 16384 keys, 32 heads over 8 of 128, 515 GFLOP, bf16 550 us
+// (0.94 PFLOP/s; 520 over an f16 cache), fp32 in two pieces 902 (1.14 PFLOP/s of products).
+template <typename TA, int DP, int ND, int NQ, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_chunk_kernel(Q8Params pp) {
     using H = Half<_Float16>;
+    static_assert(DP % 16 == 0 && (WAVES == 4 || WAVES == 8));
     constexpr int NU = 2 * ND, NB = ND, kTile = 64 * DP * 2;  // ND: 32-dim blocks computed
     constexpr int NP = NQ;                                    // pieces of P
     constexpr float kLate = 6.f, kBias = 9.f;
     constexpr int kAheadK = NQ > 1 ? 1 : 2, kAheadV = NQ > 1 ? 1 : 3;  // steps that fragments are read ahead
-    constexpr int kRowUnits = DP / 16, kUnits = 64 * kRowUnits / 256;  // 16 codes each; per thread
+    constexpr int kRowUnits = DP / 16, kStep = 64 * WAVES / kRowUnits;
+    constexpr int kUnits = kStep < 64 ? 64 / kStep : 1;  // of 16 codes, per thread that has one
     __shared__ __attribute__((aligned(1024))) char lds[4 * kTile + kPageSlots * 4];  // stage, K / V; pages
     int *const pages = reinterpret_cast<int *>(lds + 4 * kTile);
     const AttnParams &p = pp.a;
@@ -400,7 +408,7 @@ __global__ __launch_bounds__(256, 2) void paged_q8_chunk_kernel(Q8Params pp) {
     const int split = rest % p.nsplit, kvh = rest / p.nsplit;
     Rows t;
     int seq;
-    if (!find_rows(p, number, 128, lane, t, seq)) return;
+    if (!find_rows(p, number, 32 * WAVES, lane, t, seq)) return;
     const int nact = active_splits(p, t);
     if (split >= nact) return;
     const int b0 = t.lo & ~63, b = b0 + split * p.chunk, e = split == nact - 1 ? t.hi : b + p.chunk;
@@ -430,8 +438,9 @@ __global__ __launch_bounds__(256, 2) void paged_q8_chunk_kernel(Q8Params pp) {
         for (int x = 0; x < 16; ++x) o[i][x] = 0.f;
     float m = -INFINITY, l = 0.f;
 
-    // this thread's units of a tile: 16 codes from dim 16 uch of key urow + 256 / kRowUnits i
+    // this thread's units of a tile: 16 codes from dim 16 uch of key urow + kStep i
     const int urow = tid / kRowUnits, uch = tid % kRowUnits;
+    const bool has = kStep <= 64 || urow < 64;
     const int udim = 16 * uch < cc.d ? 16 * uch : 0;  // (past the head's dims: its first, for nobody)
     const char *const mid = reinterpret_cast<const char *>(g_mid_row);
     struct {
@@ -442,13 +451,14 @@ __global__ __launch_bounds__(256, 2) void paged_q8_chunk_kernel(Q8Params pp) {
     for (int pb = b; pb < e;) {
         const int p0 = paged::page_of(cc, pb);
         __syncthreads();
-        const int pe = stage_page_numbers(cc, seq, pb, e, t.lo, pages, tid, 256);
+        const int pe = stage_page_numbers(cc, seq, pb, e, t.lo, pages, tid, 64 * WAVES);
         __syncthreads();
         const int n = (pe - pb + 63) / 64;
         auto ask = [&](int k0) __attribute__((always_inline)) {
+            if (!has) return;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                const int key = min(k0 + urow + 256 / kRowUnits * i, pe - 1), pg = paged::page_of(cc, key);
+                const int key = min(k0 + urow + kStep * i, pe - 1), pg = paged::page_of(cc, key);
                 const int page = pages[pg - p0], prow = key - pg * cc.page_size;
                 const bool ok = page >= 0;
                 const int64_t at = page * cc.page_stride + prow * cc.row_stride + kvh * cc.head_stride + udim;
@@ -460,10 +470,11 @@ __global__ __launch_bounds__(256, 2) void paged_q8_chunk_kernel(Q8Params pp) {
             }
         };
         auto put = [&](int st) __attribute__((always_inline)) {
+            if (!has) return;
             char *const to = lds + st * 2 * kTile;
 #pragma unroll
             for (int i = 0; i < kUnits; ++i) {
-                const int row = urow + 256 / kRowUnits * i;
+                const int row = urow + kStep * i;
                 auto widen = [&](const i32x4 &w, uint32_t byte, char *tile, int swz) __attribute__((always_inline)) {
                     const float s = quarter_step(byte);
                     const Step stp = step_pair(s, s);
@@ -597,6 +608,7 @@ struct Plan {
     bool wide;    // the few-row launch has wide workgroups
     int few_max;  // rows of the longest sequence the few-row launch takes
     int side;     // heads of a few-row workgroup
+    int chunk_rows;  // of a tile
     int few_split, few_chunk, chunk_split, chunk_chunk;
     int64_t few_parts, chunk_parts;  // rows of parts
     int64_t part_floats;
@@ -647,7 +659,12 @@ Plan make_plan(const PagedAttnDesc &d) {
     pl.wide = pl.few_split > 1 && few_tiles * d.kv.kv_heads <= cus &&
               (d.window > 0 ? std::min(d.max_kv_len, d.window + 15) : d.max_kv_len) <= kWideKeys * kWideWaves;
     if (pl.wide) pl.few_split = pl.side = 1;
-    cut(rows / 128 + 1, 2 * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
+    // Tiles of 256 rows, whose codes become f16 once for twice as many rows, where they fill
+    // the CUs and walk many keys (us of a call, 128 rows / 256, 32 heads over 8 of 128: 2048
+    // tokens over 16384 keys bf16 608 / 550, fp32 942 / 902; over 2048 69 / 70 and 96 / 101; six
+    // chunks of up to 700 over a window of 1024, fp32, 74 / 90).
+    pl.chunk_rows = rows * d.kv.kv_heads >= 256 * cus && sees >= 4096 ? 256 : 128;
+    cut(rows / pl.chunk_rows + 1, 256 / pl.chunk_rows * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
     if (pl.chunk && 64 * d.kv.num_seqs <= rows && std::min<int64_t>(sees, pl.chunk_chunk) <= 2048) pl.few = false;
     auto floats = [&](bool on, int64_t nsplit, int64_t part_rows) {
         return on && nsplit > 1 ? part_rows * nsplit * (d.kv.head_dim + 2) : 0;
@@ -734,16 +751,24 @@ int launch_paged_attention_q8(const PagedAttnDesc &d, const gfh_paged_scales &sc
         by_type([&](auto ta, auto nq) {
             using TA = decltype(ta);
             constexpr int NQ = decltype(nq)::value;
+            auto tile = [&](auto dp, auto nd) {
+                constexpr int DP = decltype(dp)::value, ND = decltype(nd)::value;
+                if (pl.chunk_rows == 256)
+                    hipLaunchKernelGGL((paged_q8_chunk_kernel<TA, DP, ND, NQ, 8>), grid, dim3(512), 0, s, pp);
+                else
+                    hipLaunchKernelGGL((paged_q8_chunk_kernel<TA, DP, ND, NQ, 4>), grid, dim3(256), 0, s, pp);
+            };
+            using D128 = std::integral_constant<int, 128>;
             if (hd <= 64)
-                hipLaunchKernelGGL((paged_q8_chunk_kernel<TA, 64, 2, NQ>), grid, dim3(256), 0, s, pp);
+                tile(std::integral_constant<int, 64>{}, Two{});
             else if (hd <= 96)
-                hipLaunchKernelGGL((paged_q8_chunk_kernel<TA, 128, 3, NQ>), grid, dim3(256), 0, s, pp);
+                tile(D128{}, std::integral_constant<int, 3>{});
             else
-                hipLaunchKernelGGL((paged_q8_chunk_kernel<TA, 128, 4, NQ>), grid, dim3(256), 0, s, pp);
+                tile(D128{}, std::integral_constant<int, 4>{});
         });
     };
     if (pl.chunk)
-        GFH_TRY(run(128, pl.chunk_split, pl.chunk_chunk, pl.chunk_parts, pl.few ? pl.few_max + 1 : 0, kAll, many));
+        GFH_TRY(run(pl.chunk_rows, pl.chunk_split, pl.chunk_chunk, pl.chunk_parts, pl.few ? pl.few_max + 1 : 0, kAll, many));
     if (pl.few) GFH_TRY(run(16, pl.few_split, pl.few_chunk, pl.few_parts, 0, pl.few_max, few));
     return GFH_SUCCESS;
 }

@@ -255,6 +255,34 @@ def test_long_axes_in_parts(torch_dev, kind, q, kv):
     assert torch.equal(_check(b, torch_dev, workspace=ws), a)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,kv_heads,d,window", [(32, 8, 128, 0), (64, 64, 48, 5000), (48, 6, 80, 0)])
+def test_long_prompts(torch_dev, kind, heads, kv_heads, d, window):
+    """Enough rows and keys for the largest tiles, ragged, in parts, with a single token beside
+    them; the reference and the bound of _paged.attention head by head on the GPU."""
+    q_lens, kv_lens = [2070, 1, 77], [5200, 4500, 4200]
+    b = Q.batch(q_lens, kv_lens, kind=kind, heads=heads, kv_heads=kv_heads, d=d, page=32, seed=d)
+    x = Q.to(b, torch_dev)
+    got = _gh().paged_attention(x["q"], *P.args(x), window=window, **Q.scales(x))
+    flat = Q.plain(b)
+    u, h = 2.0 ** -24, P.half_step(b["q"].dtype)
+    at = 0
+    for s, (n, kv) in enumerate(zip(q_lens, kv_lens)):
+        k, v = (t.to(torch_dev) for t in P.rows_of(flat, s))
+        pos = torch.arange(kv - n, kv, device=torch_dev)[:, None]
+        j = torch.arange(kv, device=torch_dev)[None]
+        hidden = (j > pos) | ((j <= pos - window) if window else False)
+        for i in range(0, heads, 5):
+            q = x["q"][at:at + n, i].double()
+            kk, vv = k[:, i * kv_heads // heads].t().contiguous(), v[:, i * kv_heads // heads].contiguous()
+            p = torch.softmax((q @ kk / math.sqrt(d)).masked_fill(hidden, -math.inf), -1)
+            want, size = p @ vv, p @ vv.abs()
+            delta = u * (d + 8) / math.sqrt(d) * (q.abs() @ kk.abs()).masked_fill(hidden, 0).amax(-1, keepdim=True)
+            bound = h * want.abs() + size * (h + 2 * delta + 2.0 ** -21 + kv * u)
+            assert ((got[at:at + n, i].double() - want).abs() <= bound).all(), (s, i)
+        at += n
+
+
 def test_pages_of_one_row(torch_dev):
     """More pages than a workgroup looks up at once."""
     for kv, q in ((1500, 1), (2300, 40)):
