@@ -29,7 +29,7 @@ struct AppendNormParams {
     int64_t ldq, ldqo, ldk, ldv;  // elements between tokens
     const float *cos, *sin;
     const float *q_norm, *k_norm;
-    double eps;
+    double eps, inv_d;
     uint8_t *k_scales, *v_scales;
     int64_t scale_page, scale_head;  // bytes between pages, heads; rows are adjacent
     int rot;  // rotated dims R, 0 without tables
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void paged_append_norm_kernel(AppendNormParams
         for (int e = 0; e < W; ++e) sum += (double)a[e] * a[e] + (double)b[e] * b[e];
         sum = over_group(sum, p.shift, [](double x, double y) { return x + y; });
         if (live && norm) {
-            const float r = (float)(1.0 / sqrt(sum / p.c.d + p.eps));
+            const float r = (float)rsqrt(fma(sum, p.inv_d, p.eps));
             float wa[W], wb[W];
             load_vec<W>(norm + a0, wa);
             load_vec<W>(norm + b0, wb);
@@ -226,6 +226,7 @@ int launch_paged_append_norm(const PagedAppendDesc &d, const PagedNormDesc &n, h
     p.ldq = d.ldq, p.ldqo = d.ldqo, p.ldk = d.ldk, p.ldv = d.ldv;
     p.cos = d.cos, p.sin = d.sin;
     p.q_norm = n.q_norm, p.k_norm = n.k_norm, p.eps = n.eps;
+    p.inv_d = 1.0 / (double)d.kv.head_dim;
     p.k_scales = n.scales.k, p.v_scales = n.scales.v;
     p.scale_page = n.scales.page_stride, p.scale_head = n.scales.head_stride;
     p.rot = d.cos ? (int)d.rotary_dim : 0;

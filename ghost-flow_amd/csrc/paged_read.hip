@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void paged_read_kernel(ReadParams p) {
         }
 #pragma unroll
         for (int a = 0; a < kAhead; ++a)
-            if (u0 + 64 * a < 2 * half) store_vec<E>(to[a], x[a]);
+            if (u0 + 64 * a < 2 * half) store_vec<E, true>(to[a], x[a]);
     }
 }
 

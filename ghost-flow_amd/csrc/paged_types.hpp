@@ -6,20 +6,22 @@
 
 namespace gfh {
 
-// N consecutive elements, aligned to min(16, N * sizeof(T)) bytes.
-template <int N, typename T>
+// N consecutive elements, aligned to min(16, N * sizeof(T)) bytes.  ONCE: nothing else
+// touches them (nontemporal).
+template <int N, bool ONCE = false, typename T>
 __device__ __forceinline__ void load_vec(const T *p, float (&x)[N]) {
     constexpr int kPer = N * sizeof(T) <= 16 ? N : 16 / (int)sizeof(T);
     typedef T vec __attribute__((ext_vector_type(kPer)));
     typedef float fvec __attribute__((ext_vector_type(kPer)));
 #pragma unroll
     for (int i = 0; i < N / kPer; ++i) {
-        const fvec v = __builtin_convertvector(reinterpret_cast<const vec *>(p)[i], fvec);
+        const vec *const at = reinterpret_cast<const vec *>(p) + i;
+        const fvec v = __builtin_convertvector(ONCE ? __builtin_nontemporal_load(at) : *at, fvec);
 #pragma unroll
         for (int e = 0; e < kPer; ++e) x[i * kPer + e] = v[e];
     }
 }
-template <int N, typename T>
+template <int N, bool ONCE = false, typename T>
 __device__ __forceinline__ void store_vec(T *p, const float (&x)[N]) {
     constexpr int kPer = N * sizeof(T) <= 16 ? N : 16 / (int)sizeof(T);
     typedef T vec __attribute__((ext_vector_type(kPer)));
@@ -29,7 +31,11 @@ __device__ __forceinline__ void store_vec(T *p, const float (&x)[N]) {
         fvec v;
 #pragma unroll
         for (int e = 0; e < kPer; ++e) v[e] = x[i * kPer + e];
-        reinterpret_cast<vec *>(p)[i] = __builtin_convertvector(v, vec);
+        vec *const at = reinterpret_cast<vec *>(p) + i;
+        if constexpr (ONCE)
+            __builtin_nontemporal_store(__builtin_convertvector(v, vec), at);
+        else
+            *at = __builtin_convertvector(v, vec);
     }
 }
 
