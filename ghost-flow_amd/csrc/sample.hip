@@ -577,7 +577,7 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
         const int b = tid % kBins, part = tid / kBins, half = (s.slices + 1) / 2;
         static_assert(kPickThreads == 2 * kBins, "two threads per bin");
         double sum = 0.0;
-#pragma unroll 8
+#pragma unroll 16
         for (int i = part * half; i < min(s.slices, (part + 1) * half); ++i) {
             const int at = b - (int)fminf(r.top - sh.slice_top[i], (float)kBins);
             const uint64_t w = bins[i * kBins + max(at, 0)];
@@ -657,19 +657,24 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
         const int groups = (s.vocab + kGroup - 1) / kGroup, last = groups - 1;
         const float *const maxima = s.maxima + (int64_t)row * s.slices * kGroups;
         const float low = logit_of(~lo), high = logit_of(~hi);
+        static_assert(kMaxSlices * kGroups <= 32 * kPickThreads, "a bit per group of a thread");
+        uint32_t reach = 0;  // this thread's groups, kPickThreads apart
+#pragma unroll 8
+        for (int i = 0; i < (groups + kPickThreads - 1) / kPickThreads; ++i) {
+            const int g = tid + i * kPickThreads;
+            reach |= (uint32_t)(maxima[min(g, last)] >= low && g < groups) << i;
+        }
         Group<T> now, next;
-        bool any = __any(maxima[min(tid, last)] >= low), any2;
-        if (any) now.load(x, min(tid, last) * kGroup, s.vocab);
-        for (int g = tid; g - (tid & 63) < groups; g += kPickThreads, now = next, any = any2) {
-            any2 = __any(maxima[min(g + kPickThreads, last)] >= low) && g - (tid & 63) + kPickThreads < groups;
-            if (any2) next.load(x, min(g + kPickThreads, last) * kGroup, s.vocab);
-            if (!any) continue;
+        if (__any(reach & 1)) now.load(x, min(tid, last) * kGroup, s.vocab);
+        for (int g = tid; g - (tid & 63) < groups; g += kPickThreads, now = next, reach >>= 1) {
+            if (__any(reach & 2)) next.load(x, min(g + kPickThreads, last) * kGroup, s.vocab);
+            if (!__any(reach & 1)) continue;
             float l[kGroup];
             now.values(l);
             uint32_t in = 0;
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) in |= (uint32_t)(l[e] >= low && l[e] <= high) << e;
-            in = g < groups ? in : 0;
+            in = reach & 1 ? in : 0;
             if (!__any(in != 0)) continue;
             const int mine = __popc(in);
             int upto = mine;
