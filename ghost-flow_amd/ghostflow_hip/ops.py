@@ -609,6 +609,7 @@ def _rows(t, name, like, tokens, heads, d):
 
 _PAGED_KV = struct.Struct("@PPi7qP3qPPP")  # gfh_paged_kv; packed by hand, a ctypes Structure costs 3 us more
 _PAGED_SCALES = struct.Struct("@PP2q")  # gfh_paged_scales
+_PAGE_DTYPES = {**_DTYPES, torch.uint8: _lib.U8}
 
 
 def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
@@ -617,7 +618,9 @@ def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
     if len(shape) != 4 or v_pages.shape != shape or v_pages.stride() != stride or v_pages.dtype != k_pages.dtype:
         raise GhostFlowError(_lib.INVALID_SHAPE, "k_pages and v_pages must be [pages, page_size, kv_heads, head_dim], of "
                              "one type and with one layout")
-    dt = _lib.U8 if k_pages.dtype == torch.uint8 else _dtype(k_pages, "k_pages")
+    dt = _PAGE_DTYPES.get(k_pages.dtype)
+    if dt is None:
+        raise GhostFlowError(_lib.INVALID_DATA, f"k_pages must be float32, bfloat16, float16 or uint8, got {k_pages.dtype}")
     pages, page_size, hkv, d = shape
     sp, sr, sh, sd = stride
     if sd != 1 and d > 1:
@@ -647,10 +650,11 @@ def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
 def _paged_scales(k_scales, v_scales, k_pages):
     """gfh_paged_scales of the step bytes [pages, kv_heads, page_size] that go
     with pages of 8 bits, None for others."""
-    if (k_scales is None) != (v_scales is None) or (k_scales is None) == (k_pages.dtype == torch.uint8):
-        raise GhostFlowError(_lib.INVALID_DATA, "k_scales and v_scales go with pages of uint8, and those with both")
-    if k_scales is None:
+    codes = k_pages.dtype == torch.uint8
+    if k_scales is None and v_scales is None and not codes:
         return None
+    if k_scales is None or v_scales is None or not codes:
+        raise GhostFlowError(_lib.INVALID_DATA, "k_scales and v_scales go with pages of uint8, and those with both")
     pages, page_size, hkv, _ = k_pages.shape
     shape, stride = k_scales.shape, k_scales.stride()
     if shape != (pages, hkv, page_size) or v_scales.shape != shape or v_scales.stride() != stride:
