@@ -147,10 +147,11 @@ struct Group {
             for (int e = 0; e < kGroup; ++e) v[e / E][e % E] = first + e < end ? row[first + e] : (T)-INFINITY;
         }
     }
+    __device__ __forceinline__ float value(int e) const { return (float)v[e / E][e % E]; }
     __device__ __forceinline__ void values(float (&x)[kGroup]) const {
 #pragma unroll
         for (int e = 0; e < kGroup; ++e) {
-            x[e] = (float)v[e / E][e % E];
+            x[e] = value(e);
             x[e] = x[e] == x[e] ? x[e] : -INFINITY;
         }
     }
@@ -161,6 +162,58 @@ __device__ __forceinline__ void load_group(const T *row, int first, int end, flo
     g.load(row, first, end);
     g.values(x);
 }
+
+// ---- a wave's lanes, in the VALU: the LDS path's permutes, one after the other, cost more -----
+//
+// x of the lane that a DPP pattern names; 0 where it names none, and outside the rows of 16.
+template <int PATTERN, int ROWS = 0xf, typename T>
+__device__ __forceinline__ T from_lane(T x) {
+    constexpr int N = sizeof(T) / 4;
+    typedef int words __attribute__((ext_vector_type(N)));
+    words w;
+    if constexpr (N == 1) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), PATTERN, ROWS, 0xf, false));
+    } else {
+        w = __builtin_bit_cast(words, x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = __builtin_amdgcn_update_dpp(0, w[i], PATTERN, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, w);
+    }
+}
+template <typename T>
+__device__ __forceinline__ T of_lane(T x, int lane) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+    } else {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+        return __builtin_bit_cast(T, (uint64_t)hi << 32 | lo);
+    }
+}
+// The sum of a lane's x and those of the lanes before it.
+template <typename T>
+__device__ __forceinline__ T sum_upto(T x) {
+    x += from_lane<0x111>(x);       // row_shr:1
+    x += from_lane<0x112>(x);       // row_shr:2
+    x += from_lane<0x114>(x);       // row_shr:4
+    x += from_lane<0x118>(x);       // row_shr:8
+    x += from_lane<0x142, 0xa>(x);  // row_bcast:15, to the second and fourth row
+    x += from_lane<0x143, 0xc>(x);  // row_bcast:31, to the upper two
+    return x;
+}
+// f over all lanes, in each; every lane has to be active.
+template <typename T, typename F>
+__device__ __forceinline__ T over_wave(T x, F &&f) {
+    x = f(x, from_lane<0xB1>(x));   // quad_perm [1,0,3,2]
+    x = f(x, from_lane<0x4E>(x));   // quad_perm [2,3,0,1]
+    x = f(x, from_lane<0x141>(x));  // row_half_mirror
+    x = f(x, from_lane<0x140>(x));  // row_mirror
+    return f(f(of_lane(x, 0), of_lane(x, 16)), f(of_lane(x, 32), of_lane(x, 48)));
+}
+constexpr auto add = [](auto a, auto b) { return a + b; };
+constexpr auto smaller = [](int a, int b) { return min(a, b); };
+constexpr auto larger = [](auto a, auto b) { return a > b ? a : b; };
 
 template <typename T>
 __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) {
@@ -184,13 +237,9 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
     int at = INT_MAX;
 #pragma unroll
     for (int e = kGroup - 1; e >= 0; --e) at = x[e] == most ? first + e : at;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor(most, o);
-        const int a2 = __shfl_xor(at, o);
-        if (m2 > most || (m2 == most && a2 < at)) most = m2, at = a2;
-    }
-    if (lane == 0) mosts[wave] = most, ats[wave] = at;
+    const float highest = over_wave(most, larger);
+    at = over_wave(most == highest ? at : INT_MAX, smaller);
+    if (lane == 0) mosts[wave] = highest, ats[wave] = at;
     __syncthreads();
     most = mosts[0], at = ats[0];
 #pragma unroll
@@ -216,8 +265,7 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) sum += weight(x[e], most, scale, table);
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor((unsigned long long)sum, o);
+        sum = over_wave(sum, add);
         if (lane == 0) sums[wave] = sum;
         __syncthreads();
         sum = sums[0] + sums[1] + sums[2] + sums[3];
@@ -269,11 +317,7 @@ __device__ __forceinline__ void sh_max(int &to, int x) { atomicMax(&to, x); }
 // the other half of wave_sums, so one barrier does.
 __device__ __forceinline__ uint64_t block_scan(uint64_t x, PickShared &sh, int &turn, int tid, uint64_t &total) {
     const int lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t y = __shfl_up((unsigned long long)x, o);
-        x += lane >= o ? y : 0;
-    }
+    x = sum_upto(x);
     uint64_t *const sums = sh.wave_sums[turn];
     turn ^= 1;
     if (lane == 63) sums[wave] = x;
@@ -335,8 +379,8 @@ __device__ __forceinline__ void pick_in_slice(const SampleParams &s, int row, co
             n += sums[i] <= aim;
             last = sums[i] > before ? i : last;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o), last = max(last, __shfl_xor(last, o));
+        n = over_wave(n, add);
+        last = over_wave(last, larger);
         if (tid == 0) sh.found = min(n, last);
     }
     __syncthreads();
@@ -450,20 +494,13 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
             int c[kEach], n = 0, at = kBins - 1;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) n += c[e] = (int)sh.count[kEach * tid + e];
-            int upto = n;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int y = __shfl_up(upto, o);
-                upto += tid >= o ? y : 0;
-            }
-            upto -= n;
+            int upto = sum_upto(n) - n;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) {
                 at = upto < want && upto + c[e] >= want ? kEach * tid + e : at;
                 upto += c[e];
             }
-#pragma unroll
-            for (int o = 32; o > 0; o >>= 1) at = min(at, __shfl_xor(at, o));
+            at = over_wave(at, smaller);
             if (tid == 0) sh.found = at;
         }
         __syncthreads();
@@ -592,13 +629,7 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
         double c[kEach], n = 0.0;
 #pragma unroll
         for (int e = 0; e < kEach; ++e) n += c[e] = sums[kEach * tid + e] + sums[kBins + kEach * tid + e];
-        double upto = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(upto, o);
-            upto += tid >= o ? y : 0.0;
-        }
-        upto -= n;
+        double upto = sum_upto(n) - n;
         // (the first bin that reaches the limit; lane by lane from the first)
         int at = kBins;
         double above = 0.0;
@@ -609,9 +640,7 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
             above = here ? upto : above;
             upto += c[e];
         }
-        int first = at;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) first = min(first, __shfl_xor(first, o));
+        const int first = over_wave(at, smaller);
         if (tid == 0) sh.n = 0;
         if (at == first && at < kBins) sh.above = above;
         if (tid == 0) sh.found = first;
@@ -632,8 +661,7 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
             const uint64_t w = bins[i * kBins + b];
             sum += b < end ? (double)w : 0.0;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        sum = over_wave(sum, add);
         if ((tid & 63) == 0) sh.kept[i] = sum * sh.slice_scale[i];
     }
     // The bin's keys are neighbours, from the lowest whose grid number is the bin's to the
@@ -669,23 +697,17 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
         for (int g = tid; g - (tid & 63) < groups; g += kPickThreads, now = next, reach >>= 1) {
             if (__any(reach & 2)) next.load(x, min(g + kPickThreads, last) * kGroup, s.vocab);
             if (!__any(reach & 1)) continue;
-            float l[kGroup];
-            now.values(l);
-            uint32_t in = 0;
+            uint32_t in = 0;  // (a NaN is in no range)
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e) in |= (uint32_t)(l[e] >= low && l[e] <= high) << e;
-            in = reach & 1 ? in : 0;
-            if (!__any(in != 0)) continue;
-            const int mine = __popc(in);
-            int upto = mine;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const int y = __shfl_up(upto, o);
-                upto += (tid & 63) >= o ? y : 0;
+            for (int e = kGroup - 1; e >= 0; --e) {
+                const float l = now.value(e);
+                in = in + in + (uint32_t)(l == __builtin_amdgcn_fmed3f(l, low, high));
             }
+            in = reach & 1 ? in : 0;
+            const int mine = __popc(in), upto = sum_upto(mine);
             int at = 0;
-            if ((tid & 63) == 63) at = atomicAdd(&sh.n, upto);
-            at = __builtin_amdgcn_readlane(at, 63) + upto - mine;
+            if ((tid & 63) == 63 && upto) at = atomicAdd(&sh.n, upto);
+            at = of_lane(at, 63) + upto - mine;
             for (; in; in &= in - 1, ++at)
                 if (at < kListed) list.at[at] = g * kGroup + __builtin_ctz(in);
         }
@@ -694,18 +716,24 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
     const int n = sh.n;
     if (n > kListed) return false;
     for (int i = tid; i < n; i += kPickThreads) list.key[i] = order_key((float)x[list.at[i]]);
-    // the cut's key, eleven bits of what is open at a time
+    // the cut's key: first by 2048ths of the bin, whose lowest and highest keys are what is open
+    // then (of one value mostly); eleven bits of that at a time
     double before = above;
     uint64_t ties = 0;
-    for (;;) {
+    for (bool parts = true;; parts = false) {
         const int shift = max(0, 32 - __builtin_clz((hi - lo) | 1) - 11);
+        const float end = r.top - (float)cut + 1.f;
+        const auto digit_of = [&](uint32_t key) {
+            if (!parts) return (int)((hi - key) >> shift);
+            return (int)fminf(fmaxf(fmaf(-logit_of(~key), r.per, end) * kDigits, 0.f), (float)(kDigits - 1));
+        };
         __syncthreads();
         for (int i = tid; i < kDigits; i += kPickThreads) sh.count[i] = 0, sh.sum[i] = 0;
         __syncthreads();
         for (int i = tid; i < n; i += kPickThreads) {
             const uint32_t key = list.key[i];
             if (key - lo > hi - lo) continue;
-            const int digit = (int)((hi - key) >> shift);
+            const int digit = digit_of(key);
             atomicAdd(&sh.count[digit], 1u);
             atomicAdd((unsigned long long *)&sh.sum[digit],
                       (unsigned long long)weight(logit_of(~key), r.most, r.scale, sh.table));
@@ -730,10 +758,20 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
         }
         __syncthreads();
         before = sh.above;
-        const uint32_t top = hi - ((uint32_t)found << shift);
-        lo = max(lo, top - ((1u << shift) - 1));
-        hi = top;
-        if (shift == 0 || shift <= kZeroBits<T>) {
+        if (parts) {
+            if (tid == 0) sh.edge[0] = ~0u, sh.edge[1] = 0;
+            __syncthreads();
+            for (int i = tid; i < n; i += kPickThreads) {
+                const uint32_t key = list.key[i];
+                if (digit_of(key) == found) atomicMin(&sh.edge[0], key), atomicMax(&sh.edge[1], key);
+            }
+            __syncthreads();
+            lo = sh.edge[0], hi = sh.edge[1];
+        } else {
+            hi -= (uint32_t)found << shift;
+            lo = max(lo, hi - ((1u << shift) - 1));
+        }
+        if (lo == hi || (!parts && shift <= kZeroBits<T>)) {
             // one value: equal logits, equal weights
             const uint64_t w = sh.found_sum / sh.found_count;
             ties = sh.found_count;
@@ -760,23 +798,14 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
         uint32_t ranks = 0;
         for (int i0 = 0; i0 < s.slices; i0 += 64) {
             const bool in = i0 + tid < s.slices;
-            uint32_t c = in ? sh.count[i0 + tid] : 0, rank = c;
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const uint32_t y = __shfl_up(rank, o);
-                rank += tid >= o ? y : 0;
-            }
-            rank += ranks - c;  // equal ones in the slices before
+            const uint32_t c = in ? sh.count[i0 + tid] : 0;
+            const uint32_t rank = sum_upto(c) + ranks - c;  // equal ones in the slices before
             const uint64_t stay = rank < ties ? min((uint64_t)c, ties - rank) : 0;
             double v = in ? sh.kept[i0 + tid] + (double)(sh.tied[i0 + tid] + stay * equal) : 0.0;
-            ranks = __shfl(rank + c, 63);
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(v, o);
-                v += tid >= o ? y : 0.0;
-            }
+            ranks = of_lane(rank + c, 63);
+            v = sum_upto(v);
             if (in) sh.kept[i0 + tid] = upto + v, sh.count[i0 + tid] = rank;
-            upto += __shfl(v, 63);
+            upto += of_lane(v, 63);
         }
     }
     __syncthreads();
@@ -969,25 +998,18 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleParams 
             const float m = sl[i].most;
             if (m > most) most = m, at = sl[i].at;
         }
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const float m2 = __shfl_xor(most, o);
-            const int a2 = __shfl_xor(at, o);
-            if (m2 > most || (m2 == most && a2 < at)) most = m2, at = a2;
-        }
+        const float highest = over_wave(most, larger);
+        at = over_wave(most == highest ? at : INT_MAX, smaller);
+        most = highest;
         if (tid == 0) row_most = most, row_at = at;
         if (set.all()) {
             double before = 0.0;
             for (int i0 = 0; i0 < s.slices; i0 += 64) {
                 double w = 0.0;
                 if (i0 + tid < s.slices) w = (double)sl[i0 + tid].sum * relative(sl[i0 + tid].most, most, scale);
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const double y = __shfl_up(w, o);
-                    w += tid >= o ? y : 0.0;
-                }
+                w = sum_upto(w);
                 if (i0 + tid < s.slices) sh.slice_sums[i0 + tid] = before + w;
-                before += __shfl(w, 63);
+                before += of_lane(w, 63);
             }
         }
     }
