@@ -38,7 +38,8 @@ namespace {
 
 constexpr int kGroup = 16, kSlice = 4096, kGroups = kSlice / kGroup;  // logits; groups of a slice
 constexpr int kMaxSlices = 128;
-constexpr int kBins = 512;       // of a 16th of z
+constexpr int kBins = 512, kCell = 16, kCells = kBins / kCell;  // of a 16th of z; bins summed together
+constexpr int kStored = kBins + kCells;  // of a slice
 constexpr int kDigits = 2048;    // a radix step
 constexpr int kCandidates = 2048, kGuess = 1024, kPickThreads = 1024;
 constexpr int kPerPick = kSlice / kPickThreads;  // logits of a slice per thread
@@ -61,7 +62,7 @@ struct SampleParams {
     gfh_sampling set;
     float *maxima;  // [row][slices kGroups], -inf past the vocabulary
     Slice *slice;   // [row][slices]
-    uint64_t *bins; // [row][slices][kBins] sums of weights relative to the slice's most, where Settings::bins
+    uint64_t *bins; // [row][slices][kBins and kCells] sums of weights relative to the slice's most, where Settings::bins
     int32_t *tokens;
     float *logprobs;  // nullable
 };
@@ -129,6 +130,9 @@ __device__ __forceinline__ float grid_of(float l, float per) { return floorf(l *
 __device__ __forceinline__ int bin_of(float l, float top, float per) {
     return (int)fmaxf(fminf(top - grid_of(l, per), (float)(kBins - 1)), 0.f);
 }
+// The highest bin of the grid's cell of kCell bins: where a slice's bins count from, so that
+// the cells of slices meet.
+__device__ __forceinline__ float cell_top(float bin) { return floorf(bin * (1.f / kCell)) * kCell + (kCell - 1); }
 
 // A group of logits as it lies in memory (rows begin anywhere that their type allows),
 // and in fp32: -inf for NaN and from `end` on.  Apart, so that loads can be on their way.
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
     if (set.all()) {
         const bool bins = set.bins(s.slices);
         const double scale = weight_scale(set.temperature);
-        const float per = set.per(), top = grid_of(most, per);
+        const float per = set.per(), top = cell_top(grid_of(most, per));
         if (most < INFINITY && most > -INFINITY) {
             uint64_t w[kGroup];
 #pragma unroll
@@ -270,8 +274,16 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
         __syncthreads();
         sum = sums[0] + sums[1] + sums[2] + sums[3];
         if (bins) {
-            uint64_t *const to = s.bins + ((int64_t)row * s.slices + slice) * kBins;
-            for (int i = tid; i < kBins; i += kGroups) to[i] = hist[i];
+            // (the last bin, of all that lies further down, is no use)
+            uint64_t *const to = s.bins + ((int64_t)row * s.slices + slice) * kStored;
+            static_assert(kBins == 2 * kGroups && kCell == 16, "eight threads to a cell");
+            const uint64_t a = hist[2 * tid], b = 2 * tid + 1 < kBins - 1 ? hist[2 * tid + 1] : 0;
+            to[2 * tid] = a, to[2 * tid + 1] = b;
+            uint64_t c = a + b;
+            c += from_lane<0xB1>(c);
+            c += from_lane<0x4E>(c);
+            c += from_lane<0x141>(c);
+            if (tid % 8 == 0) to[kBins + tid / 8] = c;
         }
     }
     if (tid == 0) s.slice[(int64_t)row * s.slices + slice] = {most, at, sum};
@@ -286,7 +298,7 @@ struct PickShared {
     double slice_scale[kMaxSlices];  // of a slice's weights in the row's
     double kept[kMaxSlices];
     uint64_t tied[kMaxSlices];
-    float slice_top[kMaxSlices];
+    int slice_cell[kMaxSlices];      // cells from the row's first to its own
     uint32_t count[kDigits];
     uint64_t sum[kDigits];  // (or doubles)
     __attribute__((aligned(16))) uint64_t key[kCandidates];
@@ -591,89 +603,115 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
 
 // top-p without top-k: the bins of the first launch say which bin the cut lies in; one
 // pass over the row collects that bin's logits.  False: too many in it, or min_p may cut
-// before.  (The last bin holds what lies more than 32 below the largest of its slice: 2^19
-// e^-32 of the weights at most, less than the 2^-24 that p leaves.)
+// before.  (The last bin holds what lies more than 31 below the largest of its slice: 2^19
+// e^-31 of the weights at most, less than the 2^-24 that p leaves.)
 template <typename T>
 __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, const Row &r, PickShared &sh, int tid,
                                              double all) {
     const T *const x = reinterpret_cast<const T *>(s.logits) + row * s.ld;
-    const uint64_t *const bins = s.bins + (int64_t)row * s.slices * kBins;
+    const uint64_t *const bins = s.bins + (int64_t)row * s.slices * kStored;
     const Slice *const slices = s.slice + (int64_t)row * s.slices;
     if (!(fabsf(r.top) < 0x1p22f)) return false;
+    const float top = cell_top(r.top);
     int turn = 0;
     double *const sums = reinterpret_cast<double *>(sh.sum);
     __syncthreads();
     if (tid < s.slices) {
         const float most = slices[tid].most;
-        sh.slice_top[tid] = most > -INFINITY ? grid_of(most, r.per) : r.top - kBins;
+        sh.slice_cell[tid] = most > -INFINITY ? (int)fminf(top - cell_top(grid_of(most, r.per)), (float)kBins) / kCell : kCells;
         sh.slice_scale[tid] = relative(most, r.most, r.scale);
     }
-    __syncthreads();
-    // the row's bins, two threads to each with half of the slices
-    {
-        const int b = tid % kBins, part = tid / kBins, half = (s.slices + 1) / 2;
-        static_assert(kPickThreads == 2 * kBins, "two threads per bin");
-        double sum = 0.0;
-#pragma unroll 16
-        for (int i = part * half; i < min(s.slices, (part + 1) * half); ++i) {
-            const int at = b - (int)fminf(r.top - sh.slice_top[i], (float)kBins);
-            const uint64_t w = bins[i * kBins + max(at, 0)];
-            sum += at >= 0 && at < kBins - 1 ? (double)w * sh.slice_scale[i] : 0.0;
-        }
-        sums[tid] = sum;
-    }
+    if (tid == 0) sh.n = 0;
     __syncthreads();
     const double limit = r.p * all;
-    if (tid < 64) {
-        constexpr int kEach = kBins / 64;
-        double c[kEach], n = 0.0;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) n += c[e] = sums[kEach * tid + e] + sums[kBins + kEach * tid + e];
-        double upto = sum_upto(n) - n;
-        // (the first bin that reaches the limit; lane by lane from the first)
-        int at = kBins;
-        double above = 0.0;
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            const bool here = at == kBins && c[e] > 0.0 && upto + c[e] >= limit;
-            at = here ? kEach * tid + e : at;
-            above = here ? upto : above;
-            upto += c[e];
+    // the row's cells, 32 threads to each with every 32nd slice; the first that reaches the limit
+    {
+        constexpr int kParts = kPickThreads / kCells;
+        const int c = tid % kCells;
+        double sum = 0.0;
+#pragma unroll 4
+        for (int i = tid / kCells; i < s.slices; i += kParts) {
+            const int at = c - sh.slice_cell[i];
+            const uint64_t w = bins[i * kStored + kBins + max(at, 0)];
+            sum += at >= 0 ? (double)w * sh.slice_scale[i] : 0.0;
         }
-        const int first = over_wave(at, smaller);
-        if (tid == 0) sh.n = 0;
-        if (at == first && at < kBins) sh.above = above;
-        if (tid == 0) sh.found = first;
+        sums[tid] = sum;
+        __syncthreads();
+        if (tid < 64) {
+            double v = 0.0;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) v += sums[i * kCells + c];
+            v = tid < kCells ? v : 0.0;
+            const double upto = sum_upto(v) - v;
+            const uint64_t here = __ballot(v > 0.0 && upto + v >= limit);
+            if (tid == 0) sh.found = here ? __builtin_ctzll(here) : -1;
+            if (here && tid == __builtin_ctzll(here)) sh.above = upto;
+        }
+        __syncthreads();
     }
-    __syncthreads();
+    const int cell = sh.found;
+    if (cell < 0) return false;
+    // its bins in the same way, 64 threads to each
+    {
+        constexpr int kParts = kPickThreads / kCell;
+        const double before = sh.above;
+        const int b = tid % kCell;
+        double sum = 0.0;
+#pragma unroll 2
+        for (int i = tid / kCell; i < s.slices; i += kParts) {
+            const int at = cell - sh.slice_cell[i];
+            const uint64_t w = bins[i * kStored + max(at, 0) * kCell + b];
+            sum += at >= 0 ? (double)w * sh.slice_scale[i] : 0.0;
+        }
+        sums[tid] = sum;
+        __syncthreads();
+        if (tid < 64) {
+            double v = 0.0;
+#pragma unroll
+            for (int i = 0; i < kParts / 4; ++i) v += sums[(i * 4 + tid / kCell) * kCell + b];
+            v = quarter_sum_f64(v, tid);
+            v = tid < kCell ? v : 0.0;
+            const double upto = before + (sum_upto(v) - v);
+            // (where the last bits say that none does, the last with anything)
+            const uint64_t some = __ballot(v > 0.0), here = __ballot(v > 0.0 && upto + v >= limit);
+            const int at = here ? __builtin_ctzll(here) : 63 - __builtin_clzll(some | 1);
+            if (tid == 0) sh.found = cell * kCell + at;
+            if (tid == at) sh.above = upto;
+        }
+        __syncthreads();
+    }
     const int cut = sh.found;
-    if (cut >= kBins - 1) return false;
     // min_p may take something of the bins up to this one
     if (r.min_p > 0.0 && !(exp(-(cut + 2) * (1.0 / 16)) >= r.min_p)) return false;
     const double above = sh.above;
-    // what stays of every slice in the bins before
-    for (int i = tid >> 6; i < s.slices; i += kPickThreads / 64) {
-        const int end = cut - (int)fminf(r.top - sh.slice_top[i], (float)kBins);
-        double sum = 0.0;
-#pragma unroll
-        for (int j = 0; j < kBins / 64; ++j) {
-            const int b = 64 * j + (tid & 63);
-            const uint64_t w = bins[i * kBins + b];
-            sum += b < end ? (double)w : 0.0;
-        }
-        sum = over_wave(sum, add);
-        if ((tid & 63) == 0) sh.kept[i] = sum * sh.slice_scale[i];
+    // what stays of every slice in the bins before: 32 lanes each
+    for (int i0 = 0; i0 < s.slices; i0 += kPickThreads / 32) {
+        const int i = min(i0 + tid / 32, s.slices - 1), c = tid % 32;
+        const uint64_t *const of = bins + i * kStored;
+        const int at = cell - sh.slice_cell[i];
+        static_assert(kCells == 32 && kCell <= 32, "a lane per cell");
+        const uint64_t whole = of[kBins + c], some = of[max(at, 0) * kCell + c % kCell];
+        uint64_t w = (c < at ? whole : 0) + (at >= 0 && c < cut % kCell ? some : 0);
+        w += from_lane<0xB1>(w);
+        w += from_lane<0x4E>(w);
+        w += from_lane<0x141>(w);
+        w += from_lane<0x140>(w);
+        w = tid & 32 ? of_lane(w, 32) + of_lane(w, 48) : of_lane(w, 0) + of_lane(w, 16);
+        if (c == 0) sh.kept[i] = (double)w * sh.slice_scale[i];
     }
     // The bin's keys are neighbours, from the lowest whose grid number is the bin's to the
     // highest: a wave each looks for where it and the next one begin.
     if (tid < 128) {
-        const float from = r.top - (float)cut + (float)(tid >> 6);
+        const float from = top - (float)cut + (float)(tid >> 6);
         uint32_t key = 0;  // all less than it are below
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t up = key | 1u << bit;
+        const auto step = [&](int shift, uint32_t lanes) {
+            const uint32_t lane = tid & 63, up = key | lane << shift;
             const float l = logit_of(~(up - 1));
-            key = l != l ? (up >> 31 ? key : up) : grid_of(l, r.per) < from ? up : key;
-        }
+            const bool below = l != l ? !(up >> 31) : grid_of(l, r.per) < from;
+            key |= (uint32_t)(__popcll(__ballot(lane < lanes && (lane == 0 || below))) - 1) << shift;
+        };
+        for (int shift = 26; shift > 0; shift -= 6) step(shift, 64);
+        step(0, 4);
         if ((tid & 63) == 0) sh.edge[tid >> 6] = key;
     }
     __syncthreads();
@@ -692,24 +730,34 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
             const int g = tid + i * kPickThreads;
             reach |= (uint32_t)(maxima[min(g, last)] >= low && g < groups) << i;
         }
+        const int rounds = (groups + kPickThreads - 1) / kPickThreads;
         Group<T> now, next;
         if (__any(reach & 1)) now.load(x, min(tid, last) * kGroup, s.vocab);
-        for (int g = tid; g - (tid & 63) < groups; g += kPickThreads, now = next, reach >>= 1) {
-            if (__any(reach & 2)) next.load(x, min(g + kPickThreads, last) * kGroup, s.vocab);
-            if (!__any(reach & 1)) continue;
-            uint32_t in = 0;  // (a NaN is in no range)
+        uint64_t found[2] = {};  // bits of four groups each
+        for (int i = 0; i < rounds; ++i, now = next) {
+            if (__any(reach >> i & 2)) next.load(x, min(tid + (i + 1) * kPickThreads, last) * kGroup, s.vocab);
+            if (__any(reach >> i & 1)) {
+                uint32_t in = 0;  // (a NaN is in no range)
 #pragma unroll
-            for (int e = kGroup - 1; e >= 0; --e) {
-                const float l = now.value(e);
-                in = in + in + (uint32_t)(l == __builtin_amdgcn_fmed3f(l, low, high));
+                for (int e = kGroup - 1; e >= 0; --e) {
+                    const float l = now.value(e);
+                    in = in + in + (uint32_t)(l == __builtin_amdgcn_fmed3f(l, low, high));
+                }
+                const uint64_t bits = (uint64_t)(reach >> i & 1 ? in : 0) << (i % 4 * kGroup);
+                found[0] |= i & 4 ? 0 : bits;
+                found[1] |= i & 4 ? bits : 0;
             }
-            in = reach & 1 ? in : 0;
-            const int mine = __popc(in), upto = sum_upto(mine);
+            if (i % 8 < 7 && i < rounds - 1) continue;
+            const int mine = __popcll(found[0]) + __popcll(found[1]), upto = sum_upto(mine);
             int at = 0;
             if ((tid & 63) == 63 && upto) at = atomicAdd(&sh.n, upto);
             at = of_lane(at, 63) + upto - mine;
-            for (; in; in &= in - 1, ++at)
-                if (at < kListed) list.at[at] = g * kGroup + __builtin_ctz(in);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                for (; found[h]; found[h] &= found[h] - 1, ++at) {
+                    const int bit = __builtin_ctzll(found[h]), g = tid + ((i & ~7) + 4 * h + bit / kGroup) * kPickThreads;
+                    if (at < kListed) list.at[at] = g * kGroup + bit % kGroup;
+                }
         }
     }
     __syncthreads();
@@ -722,7 +770,7 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
     uint64_t ties = 0;
     for (bool parts = true;; parts = false) {
         const int shift = max(0, 32 - __builtin_clz((hi - lo) | 1) - 11);
-        const float end = r.top - (float)cut + 1.f;
+        const float end = top - (float)cut + 1.f;
         const auto digit_of = [&](uint32_t key) {
             if (!parts) return (int)((hi - key) >> shift);
             return (int)fminf(fmaxf(fmaf(-logit_of(~key), r.per, end) * kDigits, 0.f), (float)(kDigits - 1));
@@ -1050,7 +1098,7 @@ int64_t sample_max_vocab() { return (int64_t)kMaxSlices * kSlice; }
 int64_t sample_blocks(const SampleDesc &d) { return d.rows * slices_of(d.vocab); }
 size_t sample_workspace_bytes(int64_t rows, int64_t vocab) {
     const int64_t slices = slices_of(vocab);
-    return (size_t)(rows * slices) * (kGroups * sizeof(float) + sizeof(Slice) + (slices > 1 ? kBins * sizeof(uint64_t) : 0));
+    return (size_t)(rows * slices) * (kGroups * sizeof(float) + sizeof(Slice) + (slices > 1 ? kStored * sizeof(uint64_t) : 0));
 }
 
 int launch_sample(const SampleDesc &d, void *workspace, hipStream_t st) {
