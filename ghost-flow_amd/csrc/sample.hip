@@ -144,12 +144,15 @@ struct Group {
 
     __device__ __forceinline__ void load(const T *row, int first, int end) {
         if (first + kGroup <= end) {
-#pragma unroll
-            for (int i = 0; i < kGroup / E; ++i) v[i] = *reinterpret_cast<const vec *>(row + first + i * E);
+            load_whole(row + first);
         } else {
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) v[e / E][e % E] = first + e < end ? row[first + e] : (T)-INFINITY;
         }
+    }
+    __device__ __forceinline__ void load_whole(const T *from) {
+#pragma unroll
+        for (int i = 0; i < kGroup / E; ++i) v[i] = *reinterpret_cast<const vec *>(from + i * E);
     }
     __device__ __forceinline__ float value(int e) const { return (float)v[e / E][e % E]; }
     __device__ __forceinline__ void values(float (&x)[kGroup]) const {
@@ -730,33 +733,41 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
             const int g = tid + i * kPickThreads;
             reach |= (uint32_t)(maxima[min(g, last)] >= low && g < groups) << i;
         }
+        // Several loads are on their way at once, with no branch around any: a group that is not
+        // wanted takes the row's first, one that ends past the row the row's last sixteen.
+        constexpr int kAhead = sizeof(T) == 2 ? 8 : 4;
         const int rounds = (groups + kPickThreads - 1) / kPickThreads;
-        Group<T> now, next;
-        if (__any(reach & 1)) now.load(x, min(tid, last) * kGroup, s.vocab);
-        uint64_t found[2] = {};  // bits of four groups each
-        for (int i = 0; i < rounds; ++i, now = next) {
-            if (__any(reach >> i & 2)) next.load(x, min(tid + (i + 1) * kPickThreads, last) * kGroup, s.vocab);
-            if (__any(reach >> i & 1)) {
+        for (int i0 = 0; i0 < rounds; i0 += kAhead, reach >>= kAhead) {
+            if (!__any(reach & ((1u << kAhead) - 1))) continue;
+            Group<T> g[kAhead];
+            const auto place = [&](int j) { return min((tid + (i0 + j) * kPickThreads) * kGroup, s.vocab - kGroup); };
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) g[j].load_whole(x + (reach >> j & 1 ? place(j) : 0));
+            uint64_t found[kAhead / 4] = {};  // bits of four groups each
+            int mine = 0;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                if (!__any(reach >> j & 1)) continue;
                 uint32_t in = 0;  // (a NaN is in no range)
 #pragma unroll
                 for (int e = kGroup - 1; e >= 0; --e) {
-                    const float l = now.value(e);
+                    const float l = g[j].value(e);
                     in = in + in + (uint32_t)(l == __builtin_amdgcn_fmed3f(l, low, high));
                 }
-                const uint64_t bits = (uint64_t)(reach >> i & 1 ? in : 0) << (i % 4 * kGroup);
-                found[0] |= i & 4 ? 0 : bits;
-                found[1] |= i & 4 ? bits : 0;
+                const int twice = ((tid + (i0 + j) * kPickThreads) * kGroup - place(j)) & (kGroup - 1);  // of the group before
+                in = reach >> j & 1 ? in >> twice << twice : 0;
+                found[j / 4] |= (uint64_t)in << (j % 4 * kGroup);
+                mine += __popc(in);
             }
-            if (i % 8 < 7 && i < rounds - 1) continue;
-            const int mine = __popcll(found[0]) + __popcll(found[1]), upto = sum_upto(mine);
+            const int upto = sum_upto(mine);
             int at = 0;
             if ((tid & 63) == 63 && upto) at = atomicAdd(&sh.n, upto);
             at = of_lane(at, 63) + upto - mine;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < kAhead / 4; ++h)
                 for (; found[h]; found[h] &= found[h] - 1, ++at) {
-                    const int bit = __builtin_ctzll(found[h]), g = tid + ((i & ~7) + 4 * h + bit / kGroup) * kPickThreads;
-                    if (at < kListed) list.at[at] = g * kGroup + bit % kGroup;
+                    const int bit = __builtin_ctzll(found[h]);
+                    if (at < kListed) list.at[at] = place(4 * h + bit / kGroup) + bit % kGroup;
                 }
         }
     }
