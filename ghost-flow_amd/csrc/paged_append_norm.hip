@@ -76,6 +76,23 @@ __device__ __forceinline__ void store_codes(uint8_t *p, const float (&x)[W], flo
     *reinterpret_cast<vec *>(p) = v;
 }
 
+// N elements on their way: loaded here, fp32 when they are first needed.
+template <typename T, int N>
+struct Run {
+    static constexpr int kPer = N * sizeof(T) <= 16 ? N : 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(kPer)));
+    vec v[N / kPer] = {};
+
+    __device__ __forceinline__ void load(const T *p) {
+#pragma unroll
+        for (int i = 0; i < N / kPer; ++i) v[i] = reinterpret_cast<const vec *>(p)[i];
+    }
+    __device__ __forceinline__ void values(float (&x)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = (float)v[i / kPer][i % kPer];
+    }
+};
+
 // W pairs: 2 W elements of a head.  TA: activations, TC: cache (uint8_t: codes).
 template <typename TA, typename TC, int W>
 __global__ __launch_bounds__(256) void paged_append_norm_kernel(AppendNormParams p) {
@@ -85,20 +102,6 @@ __global__ __launch_bounds__(256) void paged_append_norm_kernel(AppendNormParams
     const int wave = __builtin_amdgcn_readfirstlane((int)((int64_t)blockIdx.x * 4 + (threadIdx.x >> 6)));
     const int t = wave / p.waves, part = wave % p.waves;
     if (t >= p.c.tokens) return;
-    const int n = paged::wave_leading(p.c.num_seqs + 1, lane, [&](int s) { return p.c.q_offsets[s] <= t; });
-    if (n == 0 || n > p.c.num_seqs) return;  // before the first or behind the last sequence: left as it is
-    const int s = n - 1;
-    // position: counted from the sequence's end
-    const int64_t at = (int64_t)p.c.kv_lens[s] - ((int64_t)p.c.q_offsets[s + 1] - t);
-    if (at < 0 || at >= p.c.capacity) {
-        if (lane == 0) paged::raise(p.c, paged::kBadLength);
-        return;
-    }
-    const int pos = (int)at, pg = paged::page_of(p.c, pos);
-    const int page = p.c.table[s * p.c.table_stride + pg], prow = pos - pg * p.c.page_size;
-    const bool page_ok = page >= 0 && page < p.c.num_pages;
-    if (!page_ok && lane == 0) paged::raise(p.c, paged::kBadPage);
-
     // (lanes without a unit go along with zeros: their group's swaps need them)
     const int heads_per = 64 >> p.shift, i = lane & ((1 << p.shift) - 1);
     const int head = part * heads_per + (lane >> p.shift);  // heads of q, then k, then v
@@ -118,18 +121,42 @@ __global__ __launch_bounds__(256) void paged_append_norm_kernel(AppendNormParams
     // the unit's two runs of W elements
     const bool split = turn && !p.interleaved;
     const int a0 = split ? i * W : i * 2 * W, b0 = split ? a0 + rot / 2 : a0 + W;
-    float a[W], b[W], c[W], sn[W];
-#pragma unroll
-    for (int e = 0; e < W; ++e) a[e] = b[e] = c[e] = sn[e] = 0.f;
+    const float *const norm = is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
+    // what does not go by the position is on its way while that is found
+    Run<TA, W> raw_a, raw_b;
+    Run<float, W> weight_a, weight_b, raw_c, raw_s;
     if (live) {
-        load_vec<W>(src + a0, a);
-        load_vec<W>(src + b0, b);
-        if (turn) {
-            load_vec<W>(p.cos + (int64_t)pos * (rot / 2) + i * W, c);
-            load_vec<W>(p.sin + (int64_t)pos * (rot / 2) + i * W, sn);
+        raw_a.load(src + a0);
+        raw_b.load(src + b0);
+        if (norm) {
+            weight_a.load(norm + a0);
+            weight_b.load(norm + b0);
         }
     }
-    const float *const norm = is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
+    const int n = paged::wave_leading(p.c.num_seqs + 1, lane, [&](int s) { return p.c.q_offsets[s] <= t; });
+    if (n == 0 || n > p.c.num_seqs) return;  // before the first or behind the last sequence: left as it is
+    const int s = n - 1;
+    // position: counted from the sequence's end
+    const int64_t at = (int64_t)p.c.kv_lens[s] - ((int64_t)p.c.q_offsets[s + 1] - t);
+    if (at < 0 || at >= p.c.capacity) {
+        if (lane == 0) paged::raise(p.c, paged::kBadLength);
+        return;
+    }
+    const int pos = (int)at;
+    if (live && turn) {
+        raw_c.load(p.cos + (int64_t)pos * (rot / 2) + i * W);
+        raw_s.load(p.sin + (int64_t)pos * (rot / 2) + i * W);
+    }
+    const int pg = paged::page_of(p.c, pos);
+    const int page = p.c.table[s * p.c.table_stride + pg], prow = pos - pg * p.c.page_size;
+    const bool page_ok = page >= 0 && page < p.c.num_pages;
+    if (!page_ok && lane == 0) paged::raise(p.c, paged::kBadPage);
+
+    float a[W], b[W], c[W], sn[W];
+    raw_a.values(a);
+    raw_b.values(b);
+    raw_c.values(c);
+    raw_s.values(sn);
     if (p.q_norm || p.k_norm) {
         double sum = 0.0;
 #pragma unroll
@@ -138,8 +165,8 @@ __global__ __launch_bounds__(256) void paged_append_norm_kernel(AppendNormParams
         if (live && norm) {
             const float r = (float)rsqrt(fma(sum, p.inv_d, p.eps));
             float wa[W], wb[W];
-            load_vec<W>(norm + a0, wa);
-            load_vec<W>(norm + b0, wb);
+            weight_a.values(wa);
+            weight_b.values(wb);
 #pragma unroll
             for (int e = 0; e < W; ++e) {
                 a[e] = a[e] * r * wa[e];
