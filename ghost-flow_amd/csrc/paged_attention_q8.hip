@@ -141,6 +141,11 @@ __device__ __forceinline__ f16x8 as_operand(uint32_t a, uint32_t b, uint32_t c, 
 //      transposition elsewhere.  Row i of block b of O^T is dim DP / 16 i + b.
 // The next tile's K is asked for when this one's has been multiplied, V likewise: half
 // a tile per wave is on its way at any time, in registers that are free anyway.
+//
+// Bound by bytes: 64 sequences of up to 4096 keys, 32 heads over 8 of 128, bf16, 333 MB: 72 us
+// (4.6 TB/s) and 5 for the join.  Two tiles ahead (234 registers) gained nothing, four waves
+// per SIMD spill (134 us), loads that stay in the caches took 82.  One token over 517 keys:
+// 9.7 us, the way from offsets to length to page to codes and the waves' join.
 template <typename TA, int DP, int NQ, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, NQ > 1 ? 2 : 3) void paged_q8_decode_kernel(Q8Params pp) {
     using H = Half<_Float16>;
@@ -640,8 +645,9 @@ Plan make_plan(const PagedAttnDesc &d) {
     };
     const int64_t few_tiles = std::min(d.kv.num_seqs, d.tokens) + (pl.chunk ? 0 : rows / 16);
     // Keys per workgroup of the few-row launch.  One round of the workgroups that fit the
-    // CUs (three; two with fp32 q, whose workspace is as large; lengths are not all the longest: 3/4), where a row's parts, which are joined one
-    // after the other, are then at most 32 of at least 256 keys.  Four heads to a
+    // CUs (three; fp32 q's two make more rounds, of as much workspace; lengths are not all
+    // the longest: 3/4), where a row's parts, which are joined one after the other, are then
+    // at most 32 of at least 256 keys.  Four heads to a
     // workgroup (us of a call, bf16, 32 heads over 8 of 128: 64 sequences of 1024 .. 4096
     // keys 77 / one head 88, all of 4096 120 / 124), unless their waves then have few tiles
     // each (16 of 500 .. 2000 keys 29 / 24, one of 16384 32 / 22) or one head needs no
