@@ -1,6 +1,7 @@
 """ghostflow_hip -- Python bindings of the gfx950 backend for GhostFlow's dense
-hot path (fp32 GEMM / Linear, int8 quantized linear, decode GEMV, SDPA) and
-the layers built on it (MultiHeadAttention with a KV cache, SwiGLU).
+hot path (fp32 GEMM / Linear, int8 quantized linear, decode GEMV, SDPA), the
+layers built on it (MultiHeadAttention with a KV cache, SwiGLU), and a decode
+step of many sequences (caches in pages, 4-bit weights, sampling).
 
 All compute goes through the C ABI of libghostflow_hip.so
 (include/ghostflow_hip.h); see ops.py.  The package lives in the

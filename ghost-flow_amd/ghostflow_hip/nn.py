@@ -13,7 +13,8 @@ concatenation: preallocated [B, capacity, E] buffers that every step
 appends to, so a decode step costs no copy of the past.  PagedKVCache is the
 form for many sequences of different lengths: pages that sequences take as
 they grow and give back, with MultiHeadAttention.step_paged for a ragged
-batch of their new tokens.
+batch of their new tokens; with dtype uint8 it holds codes of 8 bits and a
+step byte per row.
 
 SwiGLU follows ghostflow-nn/src/llama.rs:259-287 (LLaMA / Mistral
 feed-forward); QuantizedSwiGLU is the same block with DynamicQuantization's
