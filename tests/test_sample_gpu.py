@@ -122,6 +122,24 @@ def test_equal_logits(torch_dev, vocab):
     assert got.tolist() == [n // 2 - 1, n // 4 - 1, n // 4 - 1 + (n // 2 % 2), 3 * n // 4 - 1]
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_parts_of_a_row_on_different_levels(torch_dev, kind):
+    """Runs of 4096 logits whose largest lie from nothing to far apart, the cut among
+    a few values or many, around 0 and away from it."""
+    g = torch.Generator().manual_seed(11)
+    n = 60
+    t = torch.tensor([0.3, 1.0, 1.7, 6.0]).repeat(n // 4)
+    p = torch.rand(n, generator=g) * 0.98 + 0.01
+    least = torch.where(torch.arange(n) % 5 == 4, 0.02, 0.0)
+    k = torch.where(torch.arange(n) % 7 == 6, 500, 0).int()
+    levels = torch.tensor([-100.0, -21.0, -5.0, -1.9, -0.5, -0.06, 0.0, 0.0])
+    for spread in (0.02, 1.0, 8.0):
+        x = torch.rand(n, 30000, generator=g) * spread
+        x += levels[torch.randint(0, 8, (n, 8), generator=g)].repeat_interleave(4096, 1)[:, :30000]
+        x += torch.tensor([0.0, -spread / 2, 40.0])[torch.arange(n) % 3, None]
+        check(x.to(TYPES[kind]), torch.rand(n, generator=g), t, k, p, least, dev=torch_dev)
+
+
 def test_infinite_and_nan_logits(torch_dev):
     for vocab in (40, 6000):
         g = torch.Generator().manual_seed(vocab)
@@ -271,3 +289,15 @@ def test_a_step_from_hidden_states_to_tokens(torch_dev):
         tokens.append(check(y, u, torch.full((3,), 0.8), torch.full((3,), 40, dtype=torch.int32), torch.full((3,), 0.9),
                             torch.zeros(3), dev=torch_dev))
     assert torch.equal(*tokens)
+
+
+def test_numbers_past_fp32(torch_dev):
+    """Numbers that fp32 does not hold count as infinite, a k past int32 as none."""
+    gh = _gh()
+    g = torch.Generator().manual_seed(2)
+    x, u = torch.randn(50, 300, generator=g).to(torch_dev), torch.rand(50, generator=g).to(torch_dev)
+    for a, b in ((dict(temperature=1e300), dict(temperature=INF)), (dict(top_p=-1e300), dict(top_p=0.0)),
+                 (dict(min_p=1e39), dict(top_k=1)), (dict(top_k=10 ** 30), dict())):
+        assert torch.equal(gh.sample(x, u, **a), gh.sample(x, u, **b)), a
+    with pytest.raises(gh.GhostFlowError):
+        gh.sample(x, u, temperature=NAN)
