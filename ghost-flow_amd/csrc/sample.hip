@@ -85,14 +85,20 @@ struct Settings {
     __device__ __forceinline__ float per() const { return 16.f / temperature; }
 };
 __device__ __forceinline__ Settings settings(const SampleParams &s, int row) {
+    // (no branch around a load, so all are on their way at once: u stands in for absent rows)
+    const auto given = [&](const float *of, float all) {
+        const float x = (of ? of : s.u)[row];
+        return of ? x : all;
+    };
+    const int32_t *const ks = s.set.top_ks ? s.set.top_ks : reinterpret_cast<const int32_t *>(s.u);
+    const float temperature = given(s.set.temperatures, s.set.temperature), p = given(s.set.top_ps, s.set.top_p),
+                min_p = given(s.set.min_ps, s.set.min_p);
+    const int32_t some = ks[row], k = s.set.top_ks ? some : s.set.top_k;
     Settings r;
-    r.temperature = s.set.temperatures ? s.set.temperatures[row] : s.set.temperature;
-    r.k = s.set.top_ks ? s.set.top_ks[row] : s.set.top_k;
-    if (r.k < 0 || r.k >= s.vocab) r.k = 0;
-    r.p = s.set.top_ps ? s.set.top_ps[row] : s.set.top_p;
-    if (!(r.p < 1.0)) r.p = 1.0;
-    r.min_p = s.set.min_ps ? s.set.min_ps[row] : s.set.min_p;
-    if (!(r.min_p > 0.0)) r.min_p = 0.0;
+    r.temperature = temperature;
+    r.k = k < 0 || k >= s.vocab ? 0 : k;
+    r.p = p < 1.f ? (double)p : 1.0;
+    r.min_p = min_p > 0.f ? (double)min_p : 0.0;
     return r;
 }
 
