@@ -88,7 +88,7 @@ def _call(dev, fn, *args):
     as a decode step's kernels take: the device is only switched where it has
     to be, and the stream comes as its handle."""
     index = dev.index
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
@@ -596,7 +596,7 @@ def mha_forward_with_cache(query, key, value, wq, bq, wk, bk, wv, bv, wo, bo, nu
 def _rows(t, name, like, tokens, heads, d):
     """Elements between the tokens of t [tokens, heads, d] (heads and dims
     contiguous), of like's type and on its device."""
-    if t.dtype != like.dtype or t.device != like.device or not t.is_cuda:
+    if t.dtype is not like.dtype or t.get_device() != like.get_device() or not t.is_cuda:
         raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be {like.dtype} on {like.device} (a GPU), got {t.dtype} on "
                              f"{t.device}")
     if t.shape != (tokens, heads, d):
@@ -625,7 +625,8 @@ def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
     sp, sr, sh, sd = stride
     if sd != 1 and d > 1:
         raise GhostFlowError(_lib.INVALID_DATA, "the dims of k_pages must be contiguous")
-    if dev.type != "cuda" or k_pages.device != dev or v_pages.device != dev:
+    index = dev.index  # (device numbers compare faster than devices; of a host tensor -1)
+    if dev.type != "cuda" or k_pages.get_device() != index or v_pages.get_device() != index:
         raise GhostFlowError(_lib.INVALID_DATA, f"k_pages and v_pages must be on {dev}, a GPU")
     tshape, tstride = page_table.shape, page_table.stride()
     seqs = kv_lens.shape[0] if kv_lens.dim() == 1 else -1
@@ -634,10 +635,12 @@ def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
                              f"got {list(tshape)}, {list(q_offsets.shape)}, {list(kv_lens.shape)}")
     width = tshape[1]
     i32 = torch.int32
-    for t, n in ((page_table, "page_table"), (q_offsets, "q_offsets"), (kv_lens, "kv_lens")):
-        if t.dtype != i32 or t.device != dev or not (t.is_contiguous() or (t is page_table and tstride[1] == 1)):
-            raise GhostFlowError(_lib.INVALID_DATA, f"{n} must be a contiguous int32 tensor on {dev}")
-    if status is not None and (status.dtype != i32 or status.device != dev or status.numel() < 1):
+    if (page_table.dtype is not i32 or q_offsets.dtype is not i32 or kv_lens.dtype is not i32
+            or page_table.get_device() != index or q_offsets.get_device() != index or kv_lens.get_device() != index
+            or not (tstride[1] == 1 or page_table.is_contiguous()) or not q_offsets.is_contiguous()
+            or not kv_lens.is_contiguous()):
+        raise GhostFlowError(_lib.INVALID_DATA, f"page_table, q_offsets and kv_lens must be contiguous int32 tensors on {dev}")
+    if status is not None and (status.dtype is not i32 or status.get_device() != index or status.numel() < 1):
         raise GhostFlowError(_lib.INVALID_DATA, f"status must be an int32 tensor on {dev}")
     # (a stride over a single element says nothing)
     kv = _PAGED_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), dt, pages, page_size, hkv, d, sp if pages > 1 else 0,
@@ -650,7 +653,7 @@ def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
 def _paged_scales(k_scales, v_scales, k_pages):
     """gfh_paged_scales of the step bytes [pages, kv_heads, page_size] that go
     with pages of 8 bits, None for others."""
-    codes = k_pages.dtype == torch.uint8
+    codes = k_pages.dtype is torch.uint8
     if k_scales is None and v_scales is None and not codes:
         return None
     if k_scales is None or v_scales is None or not codes:
@@ -660,9 +663,10 @@ def _paged_scales(k_scales, v_scales, k_pages):
     if shape != (pages, hkv, page_size) or v_scales.shape != shape or v_scales.stride() != stride:
         raise GhostFlowError(_lib.INVALID_SHAPE, f"k_scales and v_scales must be [{pages}, {hkv}, {page_size}] with one "
                              f"layout, got {list(shape)} and {list(v_scales.shape)}")
-    if k_scales.dtype != torch.uint8 or v_scales.dtype != torch.uint8 or (page_size > 1 and stride[2] != 1):
+    if k_scales.dtype is not torch.uint8 or v_scales.dtype is not torch.uint8 or (page_size > 1 and stride[2] != 1):
         raise GhostFlowError(_lib.INVALID_DATA, "k_scales and v_scales must be uint8, the rows of a page contiguous")
-    if k_scales.device != k_pages.device or v_scales.device != k_pages.device:
+    index = k_pages.get_device()
+    if k_scales.get_device() != index or v_scales.get_device() != index:
         raise GhostFlowError(_lib.INVALID_DATA, f"k_scales and v_scales must be on {k_pages.device}")
     return _PAGED_SCALES.pack(k_scales.data_ptr(), v_scales.data_ptr(), stride[0] if pages > 1 else 0,
                               stride[1] if hkv > 1 else 0)
