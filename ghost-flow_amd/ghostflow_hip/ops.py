@@ -448,8 +448,8 @@ def sample(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, want_lo
 
 
 def _need_rows(t, dtype, name, rows, dev):
-    _need(t, dtype, name)
-    _same_device(dev, t)
+    if t.dtype is not dtype or t.get_device() != dev.index or not t.is_contiguous():
+        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be a contiguous {dtype} tensor on {dev}")
     if t.shape != (rows,):
         raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be [{rows}], got {list(t.shape)}")
 
@@ -607,6 +607,11 @@ def _rows(t, name, like, tokens, heads, d):
     return ld if tokens > 1 else heads * d
 
 
+def _need_f32(t, name, dev):
+    if t.dtype is not torch.float32 or t.get_device() != dev.index or not t.is_contiguous():
+        raise GhostFlowError(_lib.INVALID_DATA, f"{name} must be a contiguous float32 tensor on {dev}")
+
+
 _PAGED_KV = struct.Struct("@PPi7qP3qPPP")  # gfh_paged_kv; packed by hand, a ctypes Structure costs 3 us more
 _PAGED_SCALES = struct.Struct("@PP2q")  # gfh_paged_scales
 _PAGE_DTYPES = {**_DTYPES, torch.uint8: _lib.U8}
@@ -707,28 +712,29 @@ def paged_append(k_pages, v_pages, page_table, q_offsets, kv_lens, k, v, *, q=No
     if (cos is None) != (sin is None):
         raise GhostFlowError(_lib.INVALID_DATA, "cos and sin are given together")
     if cos is not None:
-        _need(cos, torch.float32, "cos")
-        _need(sin, torch.float32, "sin")
-        if cos.dim() != 2 or cos.shape != sin.shape:
+        _need_f32(cos, "cos", dev)
+        _need_f32(sin, "sin", dev)
+        shape = cos.shape
+        if len(shape) != 2 or sin.shape != shape:
             raise GhostFlowError(_lib.INVALID_SHAPE, "cos and sin must be [positions, rotary_dim / 2]")
-        _same_device(dev, cos, sin)
-        rows, half = cos.shape
+        rows, half = shape
         cp, sp = cos.data_ptr(), sin.data_ptr()
     if scales is None and q_norm is None and k_norm is None:
         _call(dev, lib().gfh_paged_append, kv, dt, tokens, heads, qp, ldq, qop, ldqo, k.data_ptr(), ldk, v.data_ptr(),
               ldv, cp, sp, rows, 2 * half, 1 if interleaved else 0)
         return q_out
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is None:
-            continue
-        _need(w, torch.float32, name)
-        _same_device(dev, w)
-        if w.shape != (d,):
-            raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be [{d}], got {list(w.shape)}")
+    wq = None if q_norm is None else _norm_weights(q_norm, "q_norm", d, dev)
+    wk = None if k_norm is None else _norm_weights(k_norm, "k_norm", d, dev)
     _call(dev, lib().gfh_paged_append_norm, kv, scales, dt, tokens, heads, qp, ldq, qop, ldqo, k.data_ptr(), ldk,
-          v.data_ptr(), ldv, cp, sp, rows, 2 * half, 1 if interleaved else 0, _ptr(q_norm), _ptr(k_norm),
-          float(norm_eps))
+          v.data_ptr(), ldv, cp, sp, rows, 2 * half, 1 if interleaved else 0, wq, wk, float(norm_eps))
     return q_out
+
+
+def _norm_weights(w, name, d, dev):
+    _need_f32(w, name, dev)
+    if w.shape != (d,):
+        raise GhostFlowError(_lib.INVALID_SHAPE, f"{name} must be [{d}], got {list(w.shape)}")
+    return w.data_ptr()
 
 
 def paged_read(k_pages, v_pages, page_table, q_offsets, kv_lens, *, tokens=None, dtype=torch.float32, k_out=None,
