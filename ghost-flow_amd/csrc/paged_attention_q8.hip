@@ -388,8 +388,8 @@ __global__ __launch_bounds__(64 * WAVES, NQ > 1 ? 2 : 3) void paged_q8_decode_ke
 //
 // Bound by the vector ALU and the matrix units together, as the 16-bit kernel is, with some
 // 90 vector instructions per wave and tile more for the codes (of 290; half as many in tiles
-// of 256 rows): 2048 tokens over 16384 keys, 32 heads over 8 of 128, 515 GFLOP, bf16 550 us
-// (0.94 PFLOP/s; 520 over an f16 cache), fp32 in two pieces 902 (1.14 PFLOP/s of products).
+// of 256 rows): 2048 tokens over 16384 keys, 32 heads over 8 of 128, 515 GFLOP, bf16 532 us
+// (0.97 PFLOP/s; 515 over an f16 cache), fp32 in two pieces 902 (1.14 PFLOP/s of products).
 template <typename TA, int DP, int ND, int NQ, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_chunk_kernel(Q8Params pp) {
     using H = Half<_Float16>;

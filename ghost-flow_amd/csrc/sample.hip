@@ -29,7 +29,7 @@
 //
 // Bound by the way through a row's single workgroup, and the first launch of many rows by the
 // exponentials' operations beside the bytes.  Launches, us: one row of 32000, top-k and top-p,
-// fp32 3.5 and 12; 64 rows of 131072, settings of all kinds, bf16 11 and 26; 256 rows of 50257
+// fp32 3.3 and 12; 64 rows of 131072, settings of all kinds, bf16 11 and 26; 256 rows of 50257
 // without filters, fp32 18 (2.8 TB/s) and 7.  Per stage of top-p over 131072: 3 to the cut
 // cell and bin, 9 to list the bin, 5 to the cut's key, 4 to the token.
 #include <climits>
