@@ -21,10 +21,12 @@
 //  * no filter: the sums find the 4096 that hold the token;
 //  * top-k, min_p (pick_from_few): the k-th largest of the 16s' maxima bounds the k-th
 //    largest logit from below, so a few groups, found without reading the row, hold all
-//    candidates, which are then put in order;
+//    candidates; up to 512 are put in order, each counting those before it, of up to 7168
+//    the cut is found by radix (1000 of 131072: 32 us of a call for 64 rows; 1644 logits
+//    under all kinds of settings 26, in order by counting 114);
 //  * top-p (pick_by_bins): the bins say which one is cut, one pass over the row collects
 //    its logits, and their bits say the cut;
-//  * anything else, such as a large k or one bin of equal logits (pick_from_row): the row
+//  * anything else, such as a larger k or one bin of equal logits (pick_from_row): the row
 //    is searched whole, by bins, then the cut's 32 bits by eleven, eleven and ten.
 //
 // Bound by the way through a row's single workgroup, and the first launch of many rows by the
@@ -47,9 +49,11 @@ constexpr int kMaxSlices = 128;
 constexpr int kBins = 512, kCell = 16, kCells = kBins / kCell;  // of a 16th of z; bins summed together
 constexpr int kStored = kBins + kCells;  // of a slice
 constexpr int kDigits = 2048;    // a radix step
-constexpr int kCandidates = 2048, kGuess = 1024, kPickThreads = 1024;
+constexpr int kGuess = 1024, kPickThreads = 1024;
 constexpr int kPerPick = kSlice / kPickThreads;  // logits of a slice per thread
-constexpr int kListed = 7168;   // logits of a bin
+constexpr int kListed = 7168;  // candidates, or logits of a bin
+constexpr int kHot = 4096;     // groups that have candidates
+constexpr int kFew = 512;      // candidates that are put in order
 constexpr int kTable = 128;
 constexpr double kOne = 0x1p44;
 static_assert((int64_t)kMaxSlices * kSlice == (int64_t)1 << 19, "sums of that many weights in 64 bits");
@@ -99,6 +103,7 @@ __device__ __forceinline__ Settings settings(const SampleParams &s, int row) {
     r.k = k < 0 || k >= s.vocab ? 0 : k;
     r.p = p < 1.f ? (double)p : 1.0;
     r.min_p = min_p > 0.f ? (double)min_p : 0.0;
+    if (r.min_p > 1.0) r.k = 1;  // none but the first
     return r;
 }
 
@@ -306,6 +311,17 @@ __global__ __launch_bounds__(kGroups) void sample_slices_kernel(SampleParams s) 
 
 // ---- the second launch ------------------------------------------------------------
 
+// Logits that the cut lies among.
+struct List {
+    __attribute__((aligned(16))) uint32_t key[kListed];
+    int at[kListed];
+};
+// A few of them, in order.
+struct Few {
+    uint64_t weight[kFew];
+    int rank[kFew], order[kFew];
+};
+
 struct PickShared {
     double table[kTable];
     uint64_t wave_sums[2][kPickThreads / 64];
@@ -315,24 +331,13 @@ struct PickShared {
     uint64_t tied[kMaxSlices];
     int slice_cell[kMaxSlices];      // cells from the row's first to its own
     uint32_t count[kDigits];
-    uint64_t sum[kDigits];  // (or doubles)
-    __attribute__((aligned(16))) uint64_t key[kCandidates];
-    uint64_t weight[kCandidates];
-    int index[kCandidates];
-    int rank[kCandidates];
-    int order[kCandidates];
+    __attribute__((aligned(16))) uint64_t sum[kDigits];  // (or doubles, kHot numbers of groups, Few)
+    List list;
     int found, n;
     uint32_t edge[2];
     uint64_t found_count, found_sum;
     double above;
 };
-
-// A bin's logits, over the candidates' arrays.
-struct List {
-    uint32_t key[kListed];
-    int at[kListed];
-};
-static_assert(sizeof(List) <= kCandidates * (2 * sizeof(uint64_t) + 3 * sizeof(int)), "the list fits");
 
 // The low bits of a key that are the same for all values of a type of one sign.
 template <typename T>
@@ -444,37 +449,115 @@ __device__ __forceinline__ void pick_in_slice(const SampleParams &s, int row, co
     }
 }
 
-// The places of n keys (all different, ~0 never) in rising order: sh.order.  Every
-// key counts the smaller ones.
-__device__ __forceinline__ void put_in_order(PickShared &sh, int n, int tid) {
+// The places of n <= kFew logits in the order, list.key their complemented keys and
+// list.at rising: Few::order.  Each counts those before it.
+__device__ __forceinline__ void put_in_order(PickShared &sh, Few &few, int n, int tid) {
     int size = 64;
     while (size < n) size <<= 1;
-    for (int i = tid; i < size; i += kPickThreads) {
-        sh.rank[i] = 0;
-        if (i >= n) sh.key[i] = ~(uint64_t)0;
+    if (tid < size) {
+        few.rank[tid] = 0;
+        if (tid >= n) sh.list.key[tid] = ~0u;  // (behind all)
     }
     __syncthreads();
-    const int parts = max(1, kPickThreads / size), per = size / parts;
-    typedef unsigned long long pair __attribute__((ext_vector_type(2)));
-    for (int i = tid % size; i < n; i += kPickThreads) {
-        const uint64_t mine = sh.key[i];
-        const int first = parts > 1 ? tid / size * per : 0;
-        int smaller = 0;
-#pragma unroll 8
-        for (int j = first; j < first + per; j += 2) {
-            const pair k = *reinterpret_cast<const pair *>(&sh.key[j]);
-            smaller += (k[0] < mine) + (k[1] < mine);
+    const int per = size * size / kPickThreads, i = tid % size;
+    static_assert(64 * 64 >= 4 * kPickThreads && kFew <= kPickThreads, "four keys at a time");
+    typedef uint32_t four __attribute__((ext_vector_type(4)));
+    if (i < n) {
+        const uint32_t mine = sh.list.key[i];
+        const int first = tid / size * per;
+        int before = 0;
+#pragma unroll 4
+        for (int j = first; j < first + per; j += 4) {
+            const four k = *reinterpret_cast<const four *>(&sh.list.key[j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) before += k[e] < mine + (uint32_t)(j + e < i);
         }
-        atomicAdd(&sh.rank[i], smaller);
+        atomicAdd(&few.rank[i], before);
     }
     __syncthreads();
-    for (int i = tid; i < n; i += kPickThreads) sh.order[sh.rank[i]] = i;
+    if (tid < n) few.order[few.rank[tid]] = tid;
     __syncthreads();
+}
+
+// A cut among listed logits: those of complemented keys below lo stay, and the first
+// `ties` of those up to hi, which are equal.
+struct ListCut {
+    uint32_t lo, hi;
+    uint64_t ties, sum;  // sum of the weights that stay
+    bool open;           // nothing is cut
+};
+
+// The first k of n listed logits in the order, of those the ones with less than `limit`
+// before them (and the first).  The range of z that they lie in by 2048ths, then the keys
+// between the lowest and the highest of the part that holds the cut (mostly one value),
+// eleven bits at a time.
+template <typename T>
+__device__ __forceinline__ ListCut cut_list(const Row &r, PickShared &sh, int &turn, int tid, int n, int bins, uint64_t k,
+                                            uint64_t limit) {
+    uint64_t count = 0, sum = 0;  // before the part that is looked into
+    uint32_t lo = 0, hi = ~0u;
+    const float end = r.top + 1.f, per = (float)kDigits / (float)bins;
+    for (bool parts = fabsf(r.top) < 0x1p22f && r.per > 0.f;; parts = false) {
+        const int shift = max(0, 32 - __builtin_clz((hi - lo) | 1) - 11);
+        const auto digit_of = [&](uint32_t key) {
+            if (!parts) return (int)((key - lo) >> shift);
+            return (int)fminf(fmaxf(fmaf(-logit_of(key), r.per, end) * per, 0.f), (float)(kDigits - 1));
+        };
+        __syncthreads();
+        for (int i = tid; i < kDigits; i += kPickThreads) sh.count[i] = 0, sh.sum[i] = 0;
+        if (tid == 0) sh.found = -1, sh.edge[0] = ~0u, sh.edge[1] = 0;
+        __syncthreads();
+        for (int i = tid; i < n; i += kPickThreads) {
+            const uint32_t key = sh.list.key[i];
+            if (key - lo > hi - lo) continue;
+            const int digit = digit_of(key);
+            atomicAdd(&sh.count[digit], 1u);
+            atomicAdd((unsigned long long *)&sh.sum[digit],
+                      (unsigned long long)weight(logit_of(key), r.most, r.scale, sh.table));
+        }
+        __syncthreads();
+        uint64_t total;
+        const uint64_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1], s0 = sh.sum[2 * tid], s1 = sh.sum[2 * tid + 1];
+        uint64_t cn = count + block_scan(c0 + c1, sh, turn, tid, total) - c0 - c1;
+        uint64_t sn = sum + block_scan(s0 + s1, sh, turn, tid, total) - s0 - s1;
+        // the first digit that the cut lies in or behind (found by one thread)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint64_t c = e ? c1 : c0, w = e ? s1 : s0;
+            const bool open = cn < k && (sn < limit || cn == 0), shut = cn + c >= k || sn + w >= limit;
+            if (c && open && shut) sh.found = 2 * tid + e, sh.found_count = cn, sh.found_sum = sn;
+            cn += c, sn += w;
+        }
+        __syncthreads();
+        const int at = sh.found;
+        if (at < 0) return {~0u, ~0u, 0, sum + total, true};
+        count = sh.found_count, sum = sh.found_sum;
+        if (parts) {
+            for (int i = tid; i < n; i += kPickThreads) {
+                const uint32_t key = sh.list.key[i];
+                if (digit_of(key) == at) atomicMin(&sh.edge[0], key), atomicMax(&sh.edge[1], key);
+            }
+            __syncthreads();
+            lo = sh.edge[0], hi = sh.edge[1];
+        } else {
+            lo += (uint32_t)at << shift;
+            hi = min(hi, lo + ((1u << shift) - 1));
+        }
+        if (lo == hi || (!parts && shift <= kZeroBits<T>)) {
+            // equal logits, equal weights
+            const uint64_t have = sh.count[at], w = sh.sum[at] / have;
+            uint64_t ties = min(have, k - count);
+            if (w) ties = min(ties, sum < limit ? (limit - sum - 1) / w + 1 : 0);
+            if (count + ties == 0) ties = 1;
+            return {lo, hi, ties, sum + ties * w, false};
+        }
+    }
 }
 
 // Candidates, if they are few enough: the logits in bins up to the one that holds
 // the k-th largest maximum of a group (top-k), of a quarter of the groups or the
-// kGuess-th (top-p, which may need more), or min_p.  False: not enough, or too many.
+// kGuess-th (top-p, which may need more, so not where all can be listed), or min_p.
+// False: not enough, or too many.
 template <typename T>
 __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, const Row &r, PickShared &sh, int tid,
                                               double all) {
@@ -507,9 +590,8 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
             if (bin[i] < kBins) f(g0 + i, bin[i]);
         for (int i = g0 + kHeld; i < g1; ++i) f(i, bin_of(maxima[i], r.top, r.per));
     };
-    if (r.k || r.p < 1.0) {
+    if (r.k || (r.p < 1.0 && s.vocab > kListed)) {
         const int want = r.k ? r.k : min(kGuess, groups / 4 + 1);
-        if (want > kCandidates) return false;
         if (tid < kBins) sh.count[tid] = 0;
         __syncthreads();
         each_group([&](int, int b) { atomicAdd(&sh.count[b], 1u); });
@@ -536,10 +618,12 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
     uint64_t mine = 0;
     each_group([&](int, int b) { mine += b <= last; });
     int at = (int)(block_scan(mine, sh, turn, tid, total) - mine);
-    if (total > kCandidates) return false;
+    if (total > kHot) return false;
     const int hot = (int)total;
+    int *const hots = reinterpret_cast<int *>(sh.sum);
+    static_assert(sizeof(sh.sum) >= kHot * sizeof(int) && sizeof(sh.sum) >= sizeof(Few), "in place of the sums");
     if (mine) each_group([&](int g, int b) {
-        if (b <= last) sh.order[at++] = g;
+        if (b <= last) hots[at++] = g;
     });
     __syncthreads();
     // the candidates, in their order
@@ -549,7 +633,7 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
         int first = 0;
         uint32_t in = 0;
         if (h0 + tid < hot) {
-            first = sh.order[h0 + tid] * kGroup;
+            first = hots[h0 + tid] * kGroup;
             load_group(x, first, s.vocab, l);
 #pragma unroll
             for (int e = 0; e < kGroup; ++e) in |= (uint32_t)(bin_of(l[e], r.top, r.per) <= last && first + e < s.vocab) << e;
@@ -557,59 +641,82 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
         const uint64_t c = __popc(in);
         at = n + (int)(block_scan(c, sh, turn, tid, total) - c);
         n += (int)total;
-        if (n > kCandidates) return false;
+        if (n > kListed) return false;
 #pragma unroll
         for (int e = 0; e < kGroup; ++e)
             if (in >> e & 1) {
-                sh.key[at] = (uint64_t)~order_key(l[e]) << 32 | (uint32_t)at;
-                sh.index[at] = first + e;
+                sh.list.key[at] = ~order_key(l[e]);
+                sh.list.at[at] = first + e;
                 ++at;
             }
     }
     __syncthreads();
-    for (int i = tid; i < n; i += kPickThreads)
-        sh.weight[i] = weight(logit_of((uint32_t)(sh.key[i] >> 32)), r.most, r.scale, sh.table);
-    put_in_order(sh, n, tid);
-    // how many stay
-    static_assert(kCandidates == 2 * kPickThreads, "two places per thread");
-    int pos[2];
-    uint64_t w[2];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int j = 2 * tid + e;
-        pos[e] = j < n ? sh.order[j] : 0;
-        w[e] = j < n ? sh.weight[pos[e]] : 0;
-    }
-    uint64_t limit = ~(uint64_t)0;
-    const int k = r.k ? min(r.k, n) : n;
-    const uint64_t inside = (2 * tid < k ? w[0] : 0) + (2 * tid + 1 < k ? w[1] : 0);
-    uint64_t before = block_scan(inside, sh, turn, tid, total) - inside;
-    if (r.p < 1.0) {
-        const double most = r.p * (r.k ? (double)total : all);
-        limit = most > 0.0 ? (uint64_t)ceil(most) : 0;
-        if (guess && total < limit) return false;  // the next ones would stay too
-    }
-    // (a thread's sum without the places from k on, which do not stay anyway)
     const double least = r.min_p * kOne;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        const int j = 2 * tid + e;
-        const bool stays = j == 0 || (j < k && before < limit && (double)w[e] >= least);
-        if (j < n && !stays) sh.weight[pos[e]] = 0;
-        before += w[e];
-    }
-    __syncthreads();
-    w[0] = 2 * tid < n ? sh.weight[2 * tid] : 0;
-    w[1] = 2 * tid + 1 < n ? sh.weight[2 * tid + 1] : 0;
-    before = block_scan(w[0] + w[1], sh, turn, tid, total) - w[0] - w[1];
-    const uint64_t target = target_of(r.u, total);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-        if (before <= target && target < before + w[e]) {
-            const int i = sh.index[2 * tid + e];
-            answer(s, row, i, (float)x[i], r, (double)total);
+    const auto limit_of = [&](double sum) {
+        const double most = r.p * sum;
+        return most > 0.0 ? (uint64_t)ceil(most) : 0;
+    };
+    const uint64_t none = ~(uint64_t)0;
+    if (n <= kFew) {
+        Few &few = *reinterpret_cast<Few *>(sh.sum);
+        if (tid < n) few.weight[tid] = weight(logit_of(sh.list.key[tid]), r.most, r.scale, sh.table);
+        put_in_order(sh, few, n, tid);
+        // how many stay
+        const int pos = tid < n ? few.order[tid] : 0;
+        uint64_t w = tid < n ? few.weight[pos] : 0;
+        const int k = r.k ? min(r.k, n) : n;
+        const uint64_t inside = tid < k ? w : 0;  // (a place from k on does not stay anyway)
+        uint64_t before = block_scan(inside, sh, turn, tid, total) - inside;
+        uint64_t limit = none;
+        if (r.p < 1.0) {
+            limit = limit_of(r.k ? (double)total : all);
+            if (guess && total < limit) return false;  // the next ones would stay too
         }
-        before += w[e];
+        const bool stays = tid == 0 || (tid < k && before < limit && (double)w >= least);
+        if (tid < n && !stays) few.weight[pos] = 0;
+        __syncthreads();
+        w = tid < n ? few.weight[tid] : 0;
+        before = block_scan(w, sh, turn, tid, total) - w;
+        const uint64_t target = target_of(r.u, total);
+        if (before <= target && target < before + w)
+            answer(s, row, sh.list.at[tid], logit_of(sh.list.key[tid]), r, (double)total);
+        return true;
+    }
+    ListCut cut{~0u, ~0u, 0, 0, true};
+    // by k, then by p of what that leaves
+#pragma unroll 1
+    for (int step = r.k ? 0 : 1; step < (r.p < 1.0 ? 2 : 1); ++step) {
+        const uint64_t limit = step ? limit_of(all) : none;
+        cut = cut_list<T>(r, sh, turn, tid, n, last + 1, r.k ? (uint64_t)r.k : none, limit);
+        if (cut.open && guess && cut.sum < limit) return false;
+        all = (double)cut.sum;
+    }
+    // what stays, in the order of the indices: a thread's places are neighbours
+    const int each = (n + kPickThreads - 1) / kPickThreads, from = tid * each, to = min(from + each, n);
+    uint64_t equal = 0, sum = 0;
+    for (int j = from; j < to; ++j) equal += !cut.open && sh.list.key[j] >= cut.lo && sh.list.key[j] <= cut.hi;
+    const uint64_t ahead = block_scan(equal, sh, turn, tid, total) - equal;
+    const auto weight_of = [&](int j, uint64_t &rank) {
+        const uint32_t key = sh.list.key[j];
+        const float l = logit_of(key);
+        const bool stays = cut.open || key < cut.lo || (key <= cut.hi && rank++ < cut.ties);
+        const uint64_t w = weight(l, r.most, r.scale, sh.table);
+        return stays && (l == r.most || (double)w >= least) ? w : 0;
+    };
+    uint64_t rank = ahead;
+#pragma unroll 1
+    for (int j = from; j < to; ++j) sum += weight_of(j, rank);
+    uint64_t before = block_scan(sum, sh, turn, tid, total) - sum;
+    const uint64_t target = target_of(r.u, total);
+    if (before <= target && target < before + sum) {
+        rank = ahead;
+        int j = from;
+#pragma unroll 1
+        for (;; ++j) {
+            before += weight_of(j, rank);
+            if (target < before) break;
+        }
+        answer(s, row, sh.list.at[j], logit_of(sh.list.key[j]), r, (double)total);
     }
     return true;
 }
@@ -731,7 +838,7 @@ __device__ __forceinline__ bool pick_by_bins(const SampleParams &s, int row, con
     uint32_t lo = sh.edge[0], hi = sh.edge[1] - 1;
     // the places of its logits, in any order, from the groups whose largest reaches it; a wave's
     // next groups are on their way
-    List &list = *reinterpret_cast<List *>(sh.key);
+    List &list = sh.list;
     {
         const int groups = (s.vocab + kGroup - 1) / kGroup, last = groups - 1;
         const float *const maxima = s.maxima + (int64_t)row * s.slices * kGroups;
@@ -921,14 +1028,22 @@ __device__ __forceinline__ Cut cut_row(const SampleParams &s, int row, const Row
         for (int i = tid; i < kDigits; i += kPickThreads) sh.count[i] = 0, sh.sum[i] = 0;
         if (tid == 0) sh.found = -1;
         __syncthreads();
-        for (int i0 = tid * kGroup; i0 < s.vocab; i0 += kPickThreads * kGroup) {
-            float l[kGroup];
-            load_group(x, i0, s.vocab, l);
+        constexpr int kAtOnce = 4;
+        typedef T vec __attribute__((ext_vector_type(kAtOnce), aligned(sizeof(T))));
+        for (int i0 = tid * kAtOnce; i0 < s.vocab; i0 += kPickThreads * kAtOnce) {
+            vec v;
+            if (i0 + kAtOnce <= s.vocab) {
+                v = *reinterpret_cast<const vec *>(x + i0);
+            } else {
 #pragma unroll
-            for (int e = 0; e < kGroup; ++e) {
+                for (int e = 0; e < kAtOnce; ++e) v[e] = i0 + e < s.vocab ? x[i0 + e] : (T)-INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < kAtOnce; ++e) {
                 if (i0 + e >= s.vocab) continue;
-                const int b = bin_of(l[e], r.top, r.per);
-                const uint32_t key = order_key(l[e]);
+                const float y = (float)v[e], l = y == y ? y : -INFINITY;
+                const int b = bin_of(l, r.top, r.per);
+                const uint32_t key = order_key(l);
                 int at;
                 if (round == 0)
                     at = b;
@@ -937,7 +1052,7 @@ __device__ __forceinline__ Cut cut_row(const SampleParams &s, int row, const Row
                 else
                     continue;
                 atomicAdd(&sh.count[at], 1u);
-                atomicAdd((unsigned long long *)&sh.sum[at], (unsigned long long)weight(l[e], r.most, r.scale, sh.table));
+                atomicAdd((unsigned long long *)&sh.sum[at], (unsigned long long)weight(l, r.most, r.scale, sh.table));
             }
         }
         __syncthreads();
@@ -983,13 +1098,12 @@ __device__ __forceinline__ void pick_from_row(const SampleParams &s, int row, co
     Cut cut{0, none, 0};
     double total = all;
     __syncthreads();
-    if (r.k) {
-        cut = cut_row<T>(s, row, r, sh, turn, tid, (uint64_t)r.k, none);
-        total = (double)cut.sum;
-    }
-    if (r.p < 1.0) {
+#pragma unroll 1
+    for (int step = r.k ? 0 : 1; step < (r.p < 1.0 ? 2 : 1); ++step) {
         const double most = r.p * total;
-        cut = cut_row<T>(s, row, r, sh, turn, tid, r.k ? (uint64_t)r.k : none, most > 0.0 ? (uint64_t)ceil(most) : 0);
+        const uint64_t limit = step ? most > 0.0 ? (uint64_t)ceil(most) : 0 : none;
+        cut = cut_row<T>(s, row, r, sh, turn, tid, r.k ? (uint64_t)r.k : none, limit);
+        total = (double)cut.sum;
     }
     // weights that stay, slice by slice in the order of the indices; then the token's slice
     // again

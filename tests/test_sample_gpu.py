@@ -140,6 +140,34 @@ def test_parts_of_a_row_on_different_levels(torch_dev, kind):
         check(x.to(TYPES[kind]), torch.rand(n, generator=g), t, k, p, least, dev=torch_dev)
 
 
+def test_min_p_above_one(torch_dev):
+    """No weight reaches it, so the first of the largest alone stays, however many are equal."""
+    for vocab in (40, 3000, 9001, 70000):
+        x = torch.zeros(3, vocab)
+        x[0, 7:] = 2.0
+        x[1, 1::2] = 0.5
+        got = _gh().sample(x.to(torch_dev), torch.tensor([0.0, 0.5, 0.999], device=torch_dev), min_p=1.5)
+        assert got.tolist() == [7, 1, 0], vocab
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab,k", [(600, 555), (1644, 1100), (4096, 2500), (7168, 7000), (7169, 4096), (40000, 1500),
+                                     (131072, 4000)])
+def test_many_candidates(torch_dev, kind, vocab, k):
+    """More than are put in order, up to all that can be listed, and past that; equal
+    logits at the cut, all in a narrow range, and of very different size."""
+    g = torch.Generator().manual_seed(vocab)
+    x = torch.cat([torch.randn(4, vocab, generator=g), torch.randn(2, vocab, generator=g) * 1e-3,
+                   torch.randint(-3, 3, (2, vocab), generator=g).float(), torch.randn(2, vocab, generator=g) * 1e3,
+                   torch.randn(2, vocab, generator=g) - 50.0])
+    n = len(x)
+    t = torch.tensor([1.0, 2.0, 0.7]).repeat(n // 3)
+    p = torch.tensor([1.0, 0.9, 0.5, 0.999]).repeat(n // 4)
+    least = torch.where(torch.arange(n) % 3 == 2, 0.004, 0.0)
+    for ks in (torch.full((n,), k), torch.where(torch.arange(n) % 2 == 0, 0, k // 2)):
+        check(x.to(TYPES[kind]), torch.rand(n, generator=g), t, ks.int(), p, least, dev=torch_dev)
+
+
 def test_infinite_and_nan_logits(torch_dev):
     for vocab in (40, 6000):
         g = torch.Generator().manual_seed(vocab)
