@@ -647,19 +647,22 @@ Plan make_plan(const PagedAttnDesc &d) {
     // Keys per workgroup of the few-row launch.  One round of the workgroups that fit the
     // CUs (three; fp32 q's two make more rounds, of as much workspace; lengths are not all
     // the longest: 3/4), where a row's parts, which are joined one after the other, are then
-    // at most 32 of at least 256 keys.  Four heads to a
-    // workgroup (us of a call, bf16, 32 heads over 8 of 128: 64 sequences of 1024 .. 4096
-    // keys 77 / one head 88, all of 4096 120 / 124), unless their waves then have few tiles
-    // each (16 of 500 .. 2000 keys 29 / 24, one of 16384 32 / 22) or one head needs no
-    // second part (256 of 175 .. 700 keys 70 / 64).
+    // at most 32 of at least 256 keys, or 512 where that leaves every CU one (us of a call,
+    // 256 / 512: 16 sequences of up to 2000 25.3 / 23.5, 25 of 1558 under a window of 1112, fp32,
+    // 28.3 / 25.4; one of 11476, 20 heads over 5 of 80, 18.9 / 21.2).  Four heads to a workgroup
+    // (bf16, 32 heads over 8 of 128: 64 sequences of 1024 .. 4096 keys 77 / one head 88, all
+    // of 4096 120 / 124), unless their waves then have few tiles each (16 of 500 .. 2000 keys
+    // 29 / 24, one of 16384 32 / 22) or one head needs no second part (256 of 175 .. 700 keys
+    // 70 / 64).
     {
         const bool apart = d.tokens == d.kv.num_seqs && 16 % group == 0;  // no row beyond a sequence's first tile
         const int64_t tiles = apart ? d.kv.num_seqs : few_tiles, slots = 3 * cus;
-        int64_t keys = tiles * d.kv.kv_heads * sees * 3 / 4 / slots;
+        const int64_t most = tiles * d.kv.kv_heads * sees * 3 / 4;
+        int64_t keys = most / slots;
         pl.side = 1;
         if (keys >= 1024 && keys * 3 / 2 < sees)
             while (pl.side < kDecodeWaves && d.kv.kv_heads % (2 * pl.side) == 0) pl.side *= 2;
-        keys = std::max<int64_t>({256, keys / pl.side, sees / 32});
+        keys = std::max<int64_t>({pl.side == 1 && most >= 512 * cus ? 512 : 256, keys / pl.side, sees / 32});
         cut(few_tiles, kAll, keys, 64, pl.few_split, pl.few_chunk);
     }
     pl.wide = pl.few_split > 1 && few_tiles * d.kv.kv_heads <= cus &&
