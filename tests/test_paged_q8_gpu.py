@@ -177,6 +177,48 @@ def test_what_cannot_be_written(torch_dev):
     assert int(status) == 1 and (k[:2] == 5).all() and (k[2:4] != 5).any() and (k[5:] == 5).all()
 
 
+@pytest.mark.parametrize("cache,kind,kv_heads,d", [("u8", "bf16", 2, 64), ("u8", "f32", 1, 16), ("u8", "f16", 3, 80),
+                                                   ("bf16", "f32", 2, 64), ("f16", "f16", 4, 128), ("f32", "bf16", 1, 24)])
+@pytest.mark.parametrize("page", [16, 5])
+def test_many_small_rows_read(torch_dev, cache, kind, kv_heads, d, page):
+    """Enough tokens of few heads that waves take several: neighbours of one sequence
+    and of others, empty ones between, tokens before position 0, pages outside the
+    cache, rows of no sequence in front of the first and behind the last."""
+    g = torch.Generator().manual_seed(page)
+    i = lambda a, b, *n: torch.randint(a, b, n, generator=g, dtype=torch.int32)  # noqa: E731
+    seqs, num_pages, width = 3000, 50, 9
+    q = i(0, 12, seqs) * (i(0, 4, seqs) > 0)
+    q[100], q[101:400] = 200, 0
+    kv = torch.clamp(q + i(-2, 2 * page, seqs), min=0, max=width * page)
+    table = i(-1, num_pages + 1, seqs, width)
+    off = torch.cat([torch.zeros(1, dtype=torch.int32), q.cumsum(0).int()]) + 3
+    tokens = int(off[-1]) + 6
+    assert tokens > 8192
+    if cache == "u8":
+        kp, vp = (i(0, 256, num_pages, page, kv_heads, d).to(torch.uint8) for _ in "kv")
+        ks, vs = (i(0, 256, num_pages, kv_heads, page).to(torch.uint8) for _ in "kv")
+        whole = [Q.values(p, s.transpose(1, 2)) for p, s in ((kp, ks), (vp, vs))]
+        extra = {"k_scales": ks.to(torch_dev), "v_scales": vs.to(torch_dev)}
+    else:
+        kp, vp = (torch.randn(num_pages, page, kv_heads, d, generator=g).to(P.TYPES[cache]) for _ in "kv")
+        whole, extra = [kp.float(), vp.float()], {}
+    seq = torch.repeat_interleave(torch.arange(seqs), q.long())
+    pos = kv[seq] - (off[seq + 1] - torch.arange(3, tokens - 6))
+    there = pos >= 0
+    at = table[seq, pos.clamp(min=0) // page].long()
+    good = there & (at >= 0) & (at < num_pages)
+    status = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+    out = [torch.full((tokens, kv_heads, d), 7.0, dtype=P.TYPES[kind], device=torch_dev) for _ in "kv"]
+    _gh().paged_read(kp.to(torch_dev), vp.to(torch_dev), table.to(torch_dev), off.to(torch_dev), kv.to(torch_dev),
+                     k_out=out[0], v_out=out[1], status=status, **extra)
+    for got, values in zip(out, whole):
+        want = torch.full((tokens, kv_heads, d), 7.0)
+        rows = torch.where(good[:, None, None], values[at.clamp(0, num_pages - 1), pos.clamp(min=0) % page], 0.0)
+        want[3:-6] = torch.where(there[:, None, None], rows, 7.0)
+        assert torch.equal(got.cpu(), want.to(P.TYPES[kind]))
+    assert int(status) == (0 if there.all() else 1) + (0 if (good | ~there).all() else 2) == 3
+
+
 @pytest.mark.parametrize("layout,steps_like", [("heads", "rows"), ("rows", "pages"), ("heads", "pages")])
 def test_layouts(torch_dev, layout, steps_like):
     b = Q.batch([5, 1], [21, 9], kind="f16", heads=4, kv_heads=2, d=64, page=8, seed=3, layout=layout, steps_like=steps_like)
