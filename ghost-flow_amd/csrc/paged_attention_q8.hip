@@ -608,6 +608,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_chunk_kernel(Q8Params 
 
 // What a call launches: a few-row launch, a chunk launch or both (as in
 // paged_attention.hip).
+constexpr int64_t kKeptBytes = (int64_t)64 << 20;  // that a call without a workspace finds kept
 struct Plan {
     bool few, chunk;
     bool wide;    // the few-row launch has wide workgroups
@@ -673,7 +674,21 @@ Plan make_plan(const PagedAttnDesc &d) {
     // tokens over 16384 keys bf16 608 / 550, fp32 942 / 902; over 2048 69 / 70 and 96 / 101; six
     // chunks of up to 700 over a window of 1024, fp32, 74 / 90).
     pl.chunk_rows = rows * d.kv.kv_heads >= 256 * cus && sees >= 4096 ? 256 : 128;
-    cut(rows / pl.chunk_rows + 1, 256 / pl.chunk_rows * cus, 512, 64, pl.chunk_split, pl.chunk_chunk);
+    // One round of them on the keys of their rows (two to a CU of 128 rows), or, where these
+    // are cut anyway and the parts are few enough for the stream's kept block, two rounds of
+    // half as many keys (or one and a half), which even out better (us of a call, one / two: 59
+    // sequences of up to 83 tokens over up to 5136 keys, 16 heads over 4 of 64, fp32, 203 / 169;
+    // 11 of 183 over 5536, 32 over 8 of 128, bf16, 146 / 130; what was not cut loses by the
+    // join: 6 of 700 under a window of 1024, fp32, 75 / 123).
+    const int64_t tiles = rows / pl.chunk_rows + 1, round = 256 / pl.chunk_rows * cus;
+    cut(tiles, round, 512, 64, pl.chunk_split, pl.chunk_chunk);
+    for (int64_t target : {2 * round, 3 * round / 2}) {
+        int nsplit, keys;
+        cut(tiles, target, 512, 64, nsplit, keys);
+        if (pl.chunk_split == 1 || rows * d.kv.kv_heads * nsplit * (d.kv.head_dim + 2) * 4 > kKeptBytes) continue;
+        pl.chunk_split = nsplit, pl.chunk_chunk = keys;
+        break;
+    }
     if (pl.chunk && 64 * d.kv.num_seqs <= rows && std::min<int64_t>(sees, pl.chunk_chunk) <= 2048) pl.few = false;
     auto floats = [&](bool on, int64_t nsplit, int64_t part_rows) {
         return on && nsplit > 1 ? part_rows * nsplit * (d.kv.head_dim + 2) : 0;
