@@ -632,7 +632,19 @@ Plan make_plan(const PagedAttnDesc &d) {
     // the keys that a row of a tile sees at most
     const int64_t sees = std::max<int64_t>(1, d.window > 0 ? std::min(d.max_kv_len, d.window + 127) : d.max_kv_len);
     pl.few_max = kFewRows;
-    pl.chunk = rows > (sees <= 2048 ? 128 : kFewRows) && d.tokens > d.kv.num_seqs;
+    // Tiles of 128 rows, or of 16 for all.  Over the same keys the first take about 1.6 times
+    // the second's time, of which there are up to eight times as many, and 9 us more for
+    // their launches: some 100000 keys of 16 rows, 150000 of up to 64 dims.  (us of a call,
+    // 128 / 16, bf16, 32 heads over 8 of 128: 32 sequences of 2 tokens over 4000 keys 112 / 70,
+    // of 5 115 / 127; 8 of 5 over 600 24 / 14, of 17 23 / 23, of 33 24 / 31; 1 of 65 over 600
+    // 24 / 13, of 33 over 4000 25 / 33.)
+    {
+        const int64_t seqs = d.kv.num_seqs;
+        // in quarters; a sequence's last tile is partly empty
+        const int64_t small = std::max(4 * seqs, rows / 4 + 3 * seqs), large = std::max(4 * seqs, rows / 32 + 2 * seqs);
+        const int64_t keys = d.kv.kv_heads * (sees * 3 / 4);
+        pl.chunk = d.tokens > seqs && keys * (5 * small - 8 * large) > 20 * (d.kv.head_dim <= 64 ? 150000 : 100000);
+    }
     pl.few = !pl.chunk || d.kv.num_seqs > 1;
     if (!pl.chunk) pl.few_max = kAll;
     auto cut = [&](int64_t tiles, int64_t target, int64_t least, int64_t unit, int &nsplit, int &chunk) {

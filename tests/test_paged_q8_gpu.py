@@ -282,6 +282,16 @@ def test_chunks(torch_dev, kind, heads, kv_heads, d, causal, window):
         _check(b, torch_dev, causal=causal, window=window)
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,d", [(4, 4, 64), (8, 2, 128), (5, 1, 80), (6, 2, 96), (4, 1, 16), (7, 1, 32)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 300)])
+def test_chunks_over_many_keys(torch_dev, kind, heads, kv_heads, d, causal, window):
+    """Enough rows and keys for tiles of many rows whatever the heads, beside single
+    tokens and an empty sequence."""
+    b = Q.batch([701, 1, 0, 303, 2], [2500, 900, 0, 310, 2], kind=kind, heads=heads, kv_heads=kv_heads, d=d, page=16)
+    _check(b, torch_dev, causal=causal, window=window)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("q,kv", [([1], [9000]), ([3, 1], [5000, 40]), ([600], [3000]), ([300, 1, 1], [2500, 2600, 8])])
 def test_long_axes_in_parts(torch_dev, kind, q, kv):
