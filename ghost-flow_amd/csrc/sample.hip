@@ -21,9 +21,9 @@
 //  * no filter: the sums find the 4096 that hold the token;
 //  * top-k, min_p (pick_from_few): the k-th largest of the 16s' maxima bounds the k-th
 //    largest logit from below, so a few groups, found without reading the row, hold all
-//    candidates; up to 512 are put in order, each counting those before it, of up to 7168
-//    the cut is found by radix (1000 of 131072: 32 us of a call for 64 rows; 1644 logits
-//    under all kinds of settings 26, in order by counting 114);
+//    candidates; up to 512 (or what one histogram leaves of more) are put in order, each
+//    counting those before it, and of up to 7168 the cut is found by radix (a call for 64
+//    rows: top-k 400 of 1644 22 us, in order by counting 100; 1000 of 131072 32);
 //  * top-p (pick_by_bins): the bins say which one is cut, one pass over the row collects
 //    its logits, and their bits say the cut;
 //  * anything else, such as a larger k or one bin of equal logits (pick_from_row): the row
@@ -463,15 +463,25 @@ __device__ __forceinline__ void put_in_order(PickShared &sh, Few &few, int n, in
     static_assert(64 * 64 >= 4 * kPickThreads && kFew <= kPickThreads, "four keys at a time");
     typedef uint32_t four __attribute__((ext_vector_type(4)));
     if (i < n) {
+        // (equal ones count where they lie before; for most of the list the wave's 64 agree on that)
         const uint32_t mine = sh.list.key[i];
-        const int first = tid / size * per;
+        const int first = tid / size * per, end = first + per, i0 = __builtin_amdgcn_readfirstlane(i & ~63);
         int before = 0;
+        const auto count = [&](int from, int to, uint32_t least) {
 #pragma unroll 4
-        for (int j = first; j < first + per; j += 4) {
+            for (int j = from; j < to; j += 4) {
+                const four k = *reinterpret_cast<const four *>(&sh.list.key[j]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) before += k[e] < least;
+            }
+        };
+        count(first, min(end, i0), mine + 1);
+        for (int j = max(first, i0); j < min(end, i0 + 64); j += 4) {
             const four k = *reinterpret_cast<const four *>(&sh.list.key[j]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) before += k[e] < mine + (uint32_t)(j + e < i);
         }
+        count(max(first, i0 + 64), end, mine);
         atomicAdd(&few.rank[i], before);
     }
     __syncthreads();
@@ -552,6 +562,56 @@ __device__ __forceinline__ ListCut cut_list(const Row &r, PickShared &sh, int &t
             return {lo, hi, ties, sum + ties * w, false};
         }
     }
+}
+
+// The listed logits of the 2048ths of the range of z up to the one where the first k end, or
+// the first with `limit`, are moved together, if they are kFew at most; returns how many are
+// listed then.  (They hold all that stays: the cut lies in the last part.)
+__device__ __forceinline__ int narrow_list(const Row &r, PickShared &sh, int &turn, int tid, int n, int bins, uint64_t limit) {
+    const float end = r.top + 1.f, per = (float)kDigits / (float)bins;
+    const auto digit_of = [&](uint32_t key) {
+        return (int)fminf(fmaxf(fmaf(-logit_of(key), r.per, end) * per, 0.f), (float)(kDigits - 1));
+    };
+    for (int i = tid; i < kDigits; i += kPickThreads) sh.count[i] = 0, sh.sum[i] = 0;
+    if (tid == 0) sh.found = -1;
+    __syncthreads();
+    constexpr int kMost = kListed / kPickThreads;
+    static_assert(kMost * kPickThreads == kListed);
+    const int each = (n + kPickThreads - 1) / kPickThreads, from = tid * each;
+    uint32_t key[kMost];
+    int at[kMost], digit[kMost];
+#pragma unroll
+    for (int e = 0; e < kMost; ++e) {
+        digit[e] = kDigits;
+        if (e >= each || from + e >= n) continue;
+        key[e] = sh.list.key[from + e], at[e] = sh.list.at[from + e];
+        digit[e] = digit_of(key[e]);
+        atomicAdd(&sh.count[digit[e]], 1u);
+        if (!r.k)
+            atomicAdd((unsigned long long *)&sh.sum[digit[e]],
+                      (unsigned long long)weight(logit_of(key[e]), r.most, r.scale, sh.table));
+    }
+    __syncthreads();
+    uint64_t total;
+    const uint64_t c0 = sh.count[2 * tid], c1 = sh.count[2 * tid + 1], s0 = sh.sum[2 * tid], s1 = sh.sum[2 * tid + 1];
+    const uint64_t cn = block_scan(c0 + c1, sh, turn, tid, total), sn = r.k ? 0 : block_scan(s0 + s1, sh, turn, tid, total);
+    // the first digit up to which there are enough (found by one thread)
+    const uint64_t k = (uint64_t)r.k;
+    const bool before = r.k ? cn - c0 - c1 >= k : sn - s0 - s1 >= limit, half = r.k ? cn - c1 >= k : sn - s1 >= limit,
+               here = r.k ? cn >= k : sn >= limit;
+    if (!before && here) sh.found = half ? 2 * tid : 2 * tid + 1, sh.found_count = half ? cn - c1 : cn;
+    __syncthreads();
+    if (sh.found < 0 || sh.found_count > kFew) return n;
+    const int last = sh.found, left = (int)sh.found_count;
+    uint64_t mine = 0;
+#pragma unroll
+    for (int e = 0; e < kMost; ++e) mine += digit[e] <= last;
+    int to = (int)(block_scan(mine, sh, turn, tid, total) - mine);
+#pragma unroll
+    for (int e = 0; e < kMost; ++e)
+        if (digit[e] <= last) sh.list.key[to] = key[e], sh.list.at[to] = at[e], ++to;
+    __syncthreads();
+    return left;
 }
 
 // Candidates, if they are few enough: the logits in bins up to the one that holds
@@ -657,6 +717,8 @@ __device__ __forceinline__ bool pick_from_few(const SampleParams &s, int row, co
         return most > 0.0 ? (uint64_t)ceil(most) : 0;
     };
     const uint64_t none = ~(uint64_t)0;
+    if (n > kFew && (r.k ? r.k < n && r.k <= kFew : r.p < 1.0) && fabsf(r.top) < 0x1p22f && r.per > 0.f)
+        n = narrow_list(r, sh, turn, tid, n, last + 1, r.k ? none : limit_of(all));
     if (n <= kFew) {
         Few &few = *reinterpret_cast<Few *>(sh.sum);
         if (tid < n) few.weight[tid] = weight(logit_of(sh.list.key[tid]), r.most, r.scale, sh.table);
