@@ -9,8 +9,8 @@
 // places once; a lane takes 16 bytes of the output per step, so that stores cover whole
 // lines, with kAhead steps' loads on their way at once.  Stores are nontemporal: nothing
 // reads them here, and lines of the cache stay (16 sequences of up to 4096 positions, 8
-// heads of 128, codes to fp32, 349 MB: 51 us, 6.8 TB/s as part of the codes is in the last
-// cache; 512 positions 4.3 us).
+// heads of 128, codes to fp32, 349 MB: 52 us, 6.7 TB/s as part of the codes is in the last
+// cache; 512 positions 4.0 us).
 #include "common.hpp"
 #include "kernels.hpp"
 #include "paged_kv.hpp"
