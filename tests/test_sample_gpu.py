@@ -189,6 +189,20 @@ def test_infinite_and_nan_logits(torch_dev):
         check(x, torch.rand(len(x), generator=g), *settings(), dev=torch_dev)
 
 
+@pytest.mark.parametrize("vocab", [700, 3000, 7000])
+def test_infinite_and_nan_among_many_candidates(torch_dev, vocab):
+    g = torch.Generator().manual_seed(vocab)
+    for filled in (0.3, 0.95):
+        x = logits(len(SETTINGS), vocab, "f32", g)
+        x[torch.rand(x.shape, generator=g) < filled] = -INF
+        x[torch.rand(x.shape, generator=g) < 0.05] = NAN
+        check(x, torch.rand(len(x), generator=g), *settings(), dev=torch_dev)
+        x[:, 11] = -3e38
+        x[::2, 600:620] = INF
+        check(x, torch.rand(len(x), generator=g), *settings(), dev=torch_dev)
+        check(x * 1e-38, torch.rand(len(x), generator=g), *settings(), dev=torch_dev)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 def test_rows_that_begin_anywhere(torch_dev, kind):
     g = torch.Generator().manual_seed(3)
