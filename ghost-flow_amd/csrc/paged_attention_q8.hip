@@ -8,7 +8,8 @@
 // factor per key in the scores or the weights; the two factors of 4 go into the
 // softmax's scale and into l.  q is brought to [2^14, 2^15) by a power of two per row:
 // bf16 and f16 are then f16 with all their bits down to 2^-39 of the row's largest
-// magnitude, fp32 two f16 pieces (22 bits).  P is one or two f16 pieces as there.
+// magnitude, fp32 two f16 pieces (22 bits).  P is two f16 pieces, or one where the output's
+// own rounding is eight times as coarse (bf16 prompts).
 //
 // Nothing in the cache is infinite or NaN, whatever its bytes, so keys that a row does
 // not see need no look; a row of q that is not finite gets NaN.
@@ -390,12 +391,17 @@ __global__ __launch_bounds__(64 * WAVES, NQ > 1 ? 2 : 3) void paged_q8_decode_ke
 // 90 vector instructions per wave and tile more for the codes (of 290; half as many in tiles
 // of 256 rows): 2048 tokens over 16384 keys, 32 heads over 8 of 128, 515 GFLOP, bf16 532 us
 // (0.97 PFLOP/s; 515 over an f16 cache), fp32 in two pieces 902 (1.14 PFLOP/s of products).
+//
+// P is rounded to f16 for bf16 q, and is two pieces (22 bits) for f16 and fp32.  Relative errors
+// against 64 bits there (root of the mean square) and us, one piece / two: bf16 1.67e-3 / 1.66e-3,
+// the output's own rounding, and 552 / 750; f16 2.94e-4 / 2.07e-4, its own, and 559 / 756: a bf16
+// output hides that rounding, an f16 one would be 42% further off.  One piece is also what l sums.
 template <typename TA, int DP, int ND, int NQ, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void paged_q8_chunk_kernel(Q8Params pp) {
     using H = Half<_Float16>;
     static_assert(DP % 16 == 0 && (WAVES == 4 || WAVES == 8));
     constexpr int NU = 2 * ND, NB = ND, kTile = 64 * DP * 2;  // ND: 32-dim blocks computed
-    constexpr int NP = NQ;                                    // pieces of P
+    constexpr int NP = std::is_same_v<TA, __bf16> ? 1 : 2;    // pieces of P (see above)
     constexpr float kLate = 6.f, kBias = 9.f;
     constexpr int kAheadK = NQ > 1 ? 1 : 2, kAheadV = NQ > 1 ? 1 : 3;  // steps that fragments are read ahead
     constexpr int kRowUnits = DP / 16, kStep = 64 * WAVES / kRowUnits;

@@ -555,8 +555,8 @@ GFH_API int gfh_paged_read(const gfh_paged_kv *kv, const gfh_paged_scales *scale
 /* gfh_paged_attention over a GFH_U8 cache, q and out of any dtype.  Keys and values
  * meet q and P as the exact values that the codes stand for; fp32 q as two f16 pieces
  * of its row's range (22 bits, and 2^-39 of the row's largest magnitude), 16-bit q
- * with all its bits down to that.  P meets V as two f16 pieces, and for q of 16 bits in
- * tiles of 128 rows (prompts) rounded to f16, in its sum too.  The cache holds nothing
+ * with all its bits down to that.  P meets V as two f16 pieces, and for bf16 q in tiles of
+ * 128 or 256 rows (prompts) rounded to f16, in its sum too.  The cache holds nothing
  * infinite or NaN; a row of q that does gets NaN (zeros where all its scores are
  * -inf).  Scores, softmax and sums in fp32, out rounded once. */
 GFH_API size_t gfh_paged_attention_q8_workspace_size(const gfh_paged_kv *kv, int64_t tokens, int64_t heads,

@@ -578,3 +578,26 @@ def test_offsets_beyond_32_bits(torch_dev):
         ref = torch.einsum("hqk,khd->qhd", p, want[1].double())
         # scores: sums of 128 terms of at most some 4 x 4 in fp32, over sqrt(128)
         assert (o - ref).abs().max() <= 2 * 136 * 2.0 ** -24 * 16 * 128 / math.sqrt(d)
+
+
+# ---- what has one answer whatever the sizes ---------------------------------------------
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,kv_heads,d,q,kv", [(8, 2, 128, 600, 2500), (8, 4, 64, 700, 2600), (32, 8, 128, 2048, 4200)])
+def test_prompts_round_as_their_type_does(torch_dev, kind, heads, kv_heads, d, q, kv):
+    """The mean square error against 64 bits is that of the output's own rounding.  What a
+    rounding of the weights to f16 adds: a value with mantissa m is off by 2^-10 / sqrt(12) / m
+    (root of the mean square), a bf16 output by 2^-7 / sqrt(12) / m, so at most (2.8e-4 / 1.1e-3)^2
+    / 2 = 3.2% where every weight has the smallest mantissa and every output the largest, and
+    0.8% for mantissas alike; for an f16 output it would be 41%."""
+    b = Q.batch([q], [kv], kind=kind, heads=heads, kv_heads=kv_heads, d=d, page=32, seed=d + q)
+    x = Q.to(b, torch_dev)
+    got = _gh().paged_attention(x["q"], *P.args(x), **Q.scales(x)).double()
+    k, v = (t.to(torch_dev) for t in P.rows_of(Q.plain(b), 0))
+    hidden = torch.arange(kv, device=torch_dev)[None] > torch.arange(kv - q, kv, device=torch_dev)[:, None]
+    for i in range(0, heads, 3):
+        kk, vv = k[:, i * kv_heads // heads].t().contiguous(), v[:, i * kv_heads // heads].contiguous()
+        p = torch.softmax((x["q"][:, i].double() @ kk / math.sqrt(d)).masked_fill(hidden, -math.inf), -1)
+        want = p @ vv
+        own = (want.to(P.TYPES[kind]).double() - want).norm()
+        assert (got[:, i] - want).norm() <= 1.04 * own, (i, float((got[:, i] - want).norm() / own))
