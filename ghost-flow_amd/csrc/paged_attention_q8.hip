@@ -116,11 +116,12 @@ __device__ __forceinline__ float load_q8(const AttnParams &p, const Rows &t, int
     }
     return down;
 }
-// The softmax's factor of a row whose q was scaled by 1 / down.  (Kept finite: 0 times it is
-// 0; max_nan keeps a NaN.)
+// The softmax's factor of a row whose q was scaled by 1 / down.  Kept finite, as 0 times it has to
+// be 0, and above 0, as a masked score's -inf times it has to be -inf: sums of products here are
+// below 2^35, which 1e-38 takes to nothing.  (A NaN passes either comparison.)
 __device__ __forceinline__ float row_scale(const AttnParams &p, float down) {
-    const float s = p.sc2 * 4.f * down;
-    return s > 3e38f ? 3e38f : s;
+    const float s = p.sc2 * (4.f * down);
+    return s > 3e38f ? 3e38f : s < 1e-38f ? 1e-38f : s;
 }
 
 __device__ __forceinline__ f16x8 as_operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -730,8 +731,7 @@ int launch_paged_attention_q8(const PagedAttnDesc &d, const gfh_paged_scales &sc
     p.q = static_cast<const char *>(d.q);
     p.out = static_cast<char *>(d.out);
     p.ldq = d.ldq, p.ldo = d.ldo;
-    // (a scale of 0 keeps masked scores at -inf)
-    p.sc2 = d.scale == 0.f ? 1e-38f : std::fabs(d.scale) * 0x1.715476p+0f;
+    p.sc2 = std::fabs(d.scale) * 0x1.715476p+0f;
     p.negate = d.scale < 0.f;
     p.causal = d.causal;
     p.window = d.window >= p.c.capacity ? 0 : (int)d.window;

@@ -601,3 +601,29 @@ def test_prompts_round_as_their_type_does(torch_dev, kind, heads, kv_heads, d, q
         want = p @ vv
         own = (want.to(P.TYPES[kind]).double() - want).norm()
         assert (got[:, i] - want).norm() <= 1.04 * own, (i, float((got[:, i] - want).norm() / own))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale", [0.0, 1e-30, -1e-38])
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-6, 1e-30, 1e30, 1e37])
+def test_scales_of_next_to_nothing(torch_dev, kind, scale, size):
+    """Every row is the mean of the values that it sees, whatever its queries' size: equal
+    weights, which lose nothing in any type; their sum in fp32, one rounding."""
+    if kind == "f16" and size > 1e4 or scale and size > 1:
+        return
+    for q, kv, page in (([1, 1], [200, 33], 16), ([1, 140], [200, 301], 12), ([400], [1501], 16)):
+        b = Q.batch(q, kv, kind=kind, heads=8, kv_heads=4, d=64, page=page, seed=21)
+        b["q"] = (b["q"].float() * size).to(b["q"].dtype)
+        x, flat = Q.to(b, torch_dev), Q.plain(b)
+        for window in (0, 70):
+            got = _gh().paged_attention(x["q"], *P.args(x), scale=scale, window=window, **Q.scales(x)).cpu().double()
+            at = 0
+            for s, (m, n) in enumerate(zip(q, kv)):
+                v = P.rows_of(flat, s)[1].repeat_interleave(2, 1)
+                hi = torch.arange(n - m + 1, n + 1)
+                lo = (hi - window).clamp(min=0) if window else 0 * hi
+                sums = [torch.cat((0 * t[:1], t)).cumsum(0) for t in (v, v.abs())]
+                want, mean = ((t[hi] - t[lo]) / (hi - lo)[:, None, None] for t in sums)
+                bound = P.half_step(b["q"].dtype) * want.abs() + mean * (2.0 ** -21 + n * 2.0 ** -24) + 2.0 ** -25
+                assert ((got[at:at + m] - want).abs() <= bound).all(), (s, window)
+                at += m
