@@ -627,3 +627,55 @@ def test_scales_of_next_to_nothing(torch_dev, kind, scale, size):
                 bound = P.half_step(b["q"].dtype) * want.abs() + mean * (2.0 ** -21 + n * 2.0 ** -24) + 2.0 ** -25
                 assert ((got[at:at + m] - want).abs() <= bound).all(), (s, window)
                 at += m
+
+
+def _many(seqs, longest, heads, kv_heads, d, page, kind, dev, seed):
+    """One new token each of ragged sequences whose pages lie anywhere, the cache any codes
+    and steps of usual values, made on the device."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    i = lambda lo, hi, *n: torch.randint(lo, hi, n, generator=g, device=dev)  # noqa: E731
+    lens = i(longest // 4, longest + 1, seqs)
+    lens[0], lens[1] = longest, 1
+    pages = (lens + page - 1) // page
+    total, width = int(pages.sum()), int(pages.max())
+    order = torch.randperm(total, generator=g, device=dev).int()
+    col = torch.arange(width, device=dev)
+    table = torch.full((seqs, width), -1, dtype=torch.int32, device=dev)
+    used = col < pages[:, None]
+    table[used] = order[((pages.cumsum(0) - pages)[:, None] + col)[used]]
+    x = {"page_table": table, "kv_lens": lens.int(), "q_offsets": torch.arange(seqs + 1, device=dev).int()}
+    for n in "kv":
+        x[n + "_pages"] = i(0, 256, total, page, kv_heads, d).to(torch.uint8)
+        x[n + "_scales"] = i(96, 104, total, kv_heads, page).to(torch.uint8)
+    x["q"] = torch.randn(seqs, heads, d, generator=g, device=dev).to(P.TYPES[kind])
+    return x
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("seqs,longest,heads,kv_heads,d,window", [
+    (64, 4096, 32, 8, 128, 0), (64, 4096, 32, 8, 128, 2500), (70, 4300, 16, 8, 64, 0), (100, 2600, 12, 6, 80, 0),
+    (310, 2300, 8, 2, 64, 0), (150, 3000, 16, 4, 96, 2200)])
+def test_heads_side_by_side(torch_dev, kind, page, seqs, longest, heads, kv_heads, d, window):
+    """Single tokens of so many long sequences that four, or two, key/value heads share a
+    workgroup: three workgroups to a CU leave each 1024 keys of a head and more.  Every head
+    of every sequence against 64 bits, with the bound of _paged.attention."""
+    x = _many(seqs, longest, heads, kv_heads, d, page, kind, torch_dev, seqs + page)
+    status = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+    got = _gh().paged_attention(x["q"], *P.args(x), window=window, max_kv_len=longest, status=status, **Q.scales(x))
+    steps = Q.STEPS.double().to(torch_dev)
+    u, h = 2.0 ** -24, P.half_step(x["q"].dtype)
+    for s in range(seqs):
+        n = int(x["kv_lens"][s])
+        lo = max(0, n - window) if window else 0
+        at = x["page_table"][s, :-(-n // page)].long()
+        k, v = (((x[c + "_pages"][at].double() - 128) * steps[x[c + "_scales"][at].transpose(1, 2).long()][..., None])
+                .flatten(0, 1)[lo:n].transpose(0, 1).contiguous() for c in "kv")  # [kv_heads, keys, d]
+        q = x["q"][s].double().view(kv_heads, -1, d)
+        kt = k.transpose(1, 2).contiguous()
+        p = torch.softmax(q @ kt / math.sqrt(d), -1)
+        want, size = p @ v, p @ v.abs()
+        delta = u * (d + 8) / math.sqrt(d) * (q.abs() @ kt.abs()).amax(-1, keepdim=True)
+        bound = h * want.abs() + size * (h + 2 * delta + 2.0 ** -21 + (n - lo) * u)
+        assert ((got[s].double().view(kv_heads, -1, d) - want).abs() <= bound).all(), s
+    assert int(status) == 0
