@@ -679,3 +679,20 @@ def test_heads_side_by_side(torch_dev, kind, page, seqs, longest, heads, kv_head
         bound = h * want.abs() + size * (h + 2 * delta + 2.0 ** -21 + (n - lo) * u)
         assert ((got[s].double().view(kv_heads, -1, d) - want).abs() <= bound).all(), s
     assert int(status) == 0
+
+
+def test_every_border_between_steps(torch_dev):
+    """Rows whose largest magnitude is 127 of each of the 208 steps, and its neighbours in fp32."""
+    g = torch.Generator().manual_seed(22)
+    most = 127.0 * Q.STEPS
+    most = torch.stack((most, torch.nextafter(most, torch.tensor(0.0)), torch.nextafter(most, torch.tensor(1e6))), 1).flatten()[:-1]
+    n, d = len(most), 32  # (but the largest's upper neighbour, which no step holds)
+    rows = (torch.rand(n, 2, d, generator=g) * 2 - 1) * most[:, None, None]
+    rows[torch.arange(n), :, torch.arange(n) % d] = torch.stack((most, -most), 1)
+    b = Q.batch([n], [n], kind="f32", heads=2, kv_heads=2, d=d, page=16, seed=22)
+    b["k"], b["v"] = rows, rows.flip(0)
+    status = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+    _, x = _append(b, torch_dev, status=status)
+    for name, t in _expected(b).items():
+        assert torch.equal(x[name].cpu(), t), name
+    assert int(status) == 0
