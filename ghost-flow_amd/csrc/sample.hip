@@ -397,7 +397,9 @@ __device__ __forceinline__ uint64_t target_of(double u, uint64_t total) {
 }
 
 // The slice that holds the token, by the slices' running sums of what stays, then the token
-// in it; stays(l, first, b) says which of a thread's logits do.
+// in it; stays(l, first, b) says which of a thread's logits do.  A slice far below the largest
+// has a sum, if a small one, and no weight that is not 0 here: then the token is the first
+// behind it that has one, or, where none does, the last before it.
 template <typename T, typename F>
 __device__ __forceinline__ void pick_in_slice(const SampleParams &s, int row, const Row &r, PickShared &sh, int &turn,
                                               int tid, const double *sums, F &&stays) {
@@ -414,38 +416,38 @@ __device__ __forceinline__ void pick_in_slice(const SampleParams &s, int row, co
         if (tid == 0) sh.found = min(n, last);
     }
     __syncthreads();
-    const int slice = sh.found;
-    const double target = aim - (slice ? sums[slice - 1] : 0.0);
+    const int found = sh.found;
     const T *const x = reinterpret_cast<const T *>(s.logits) + row * s.ld;
     constexpr int kPer = kPerPick;
-    const int first = slice * kSlice + tid * kPer;
-    float l[kPer];
-    bool in[kPer];
-    uint64_t w[kPer], sum = 0;
+    for (int i = 0; i < s.slices; ++i) {  // (ends at the first, or where the row's largest is)
+        const bool back = found + i >= s.slices;
+        const int slice = back ? s.slices - 1 - i : found + i, first = slice * kSlice + tid * kPer;
+        float l[kPer];
+        bool in[kPer];
+        uint64_t w[kPer], sum = 0;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const float v = first + e < s.vocab ? (float)x[first + e] : -INFINITY;
-        l[e] = v == v ? v : -INFINITY;
-    }
-    stays(l, first, in);
+        for (int e = 0; e < kPer; ++e) {
+            const float v = first + e < s.vocab ? (float)x[first + e] : -INFINITY;
+            l[e] = v == v ? v : -INFINITY;
+        }
+        stays(l, first, in);
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        w[e] = in[e] ? weight(l[e], r.most, r.scale, sh.table) : 0;
-        sum += w[e];
-    }
-    uint64_t all;
-    uint64_t before = block_scan(sum, sh, turn, tid, all) - sum;
-    if (all == 0) {  // weights so small that all are 0 here: the slice's largest
-        const Slice sl = s.slice[(int64_t)row * s.slices + slice];
-        if (tid == 0) answer(s, row, sl.at, sl.most, r, total);
+        for (int e = 0; e < kPer; ++e) {
+            w[e] = in[e] ? weight(l[e], r.most, r.scale, sh.table) : 0;
+            sum += w[e];
+        }
+        uint64_t all;
+        uint64_t before = block_scan(sum, sh, turn, tid, all) - sum;
+        if (all == 0) continue;
+        const double target = aim - (slice ? sums[slice - 1] : 0.0);
+        uint64_t n = back ? all - 1 : i == 0 && target > 0.0 ? (uint64_t)target : 0;
+        n = n < all ? n : all - 1;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            if (before <= n && n < before + w[e]) answer(s, row, first + e, l[e], r, total);
+            before += w[e];
+        }
         return;
-    }
-    uint64_t n = target > 0.0 ? (uint64_t)target : 0;
-    n = n < all ? n : all - 1;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        if (before <= n && n < before + w[e]) answer(s, row, first + e, l[e], r, total);
-        before += w[e];
     }
 }
 

@@ -343,3 +343,36 @@ def test_numbers_past_fp32(torch_dev):
         assert torch.equal(gh.sample(x, u, **a), gh.sample(x, u, **b)), a
     with pytest.raises(gh.GhostFlowError):
         gh.sample(x, u, temperature=NAN)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("low", [-31.5, -40.0, -100.0, -600.0])
+@pytest.mark.parametrize("filters", [{}, {"top_p": 0.97}, {"top_k": 700}, {"min_p": 1e-6}, {"top_k": 5000, "top_p": 0.9999}])
+def test_what_weighs_nothing_is_not_drawn(torch_dev, kind, low, filters):
+    """Weights are held to 2^-45 of the largest, and e^-31.5 is less: u = 0 draws the first token
+    that has one, numbers up to 1 and above the last, past whole runs of 4096 that have none."""
+    g = torch.Generator().manual_seed(31)
+    vocab = 6 * 4096 - 100
+    x = torch.full((5, vocab), low)
+    x[:, 9000:14000] = torch.randn(5, 5000, generator=g).clamp(-2, 2)
+    x[1, :] = low
+    x[1, 13000] = 0.0   # one alone
+    x[2, 20000] = 0.5   # and one behind two runs without any
+    x[3, 4096] = 1.0
+    x[4, :9000] = -INF
+    x = x.to(TYPES[kind])
+    z = x.double() - x.double().amax(1, keepdim=True)
+    w = torch.exp(z)
+    order = torch.sort(x.float(), dim=1, descending=True, stable=True).indices
+    for r in range(len(x)):
+        s = w[r, order[r]]
+        n = filters.get("top_k", vocab)
+        if "top_p" in filters:
+            n = max(1, int((torch.cumsum(s[:n], 0) - s[:n] < torch.tensor(filters["top_p"]).double() * s[:n].sum()).sum()))
+        w[r, order[r, n:]] = 0
+    w[w < max(filters.get("min_p", 0.0), 2.0 ** -45)] = 0
+    first = (w > 0).int().argmax(1)
+    last = vocab - 1 - (w > 0).flip(1).int().argmax(1)
+    for u, want in ((0.0, first), (-1.0, first), (1.0, last), (3.0, last)):
+        got = _gh().sample(x.to(torch_dev), torch.full((5,), u, device=torch_dev), **filters)
+        assert got.tolist() == want.tolist(), u
