@@ -644,7 +644,10 @@ def _paged_kv(k_pages, v_pages, page_table, q_offsets, kv_lens, status, dev):
             or page_table.get_device() != index or q_offsets.get_device() != index or kv_lens.get_device() != index
             or not (tstride[1] == 1 or page_table.is_contiguous()) or not q_offsets.is_contiguous()
             or not kv_lens.is_contiguous()):
-        raise GhostFlowError(_lib.INVALID_DATA, f"page_table, q_offsets and kv_lens must be contiguous int32 tensors on {dev}")
+        bad = next(n for t, n in ((page_table, "page_table"), (q_offsets, "q_offsets"), (kv_lens, "kv_lens"))
+                   if t.dtype is not i32 or t.get_device() != index
+                   or not (t.is_contiguous() or (t is page_table and tstride[1] == 1)))
+        raise GhostFlowError(_lib.INVALID_DATA, f"{bad} must be a contiguous int32 tensor on {dev}")
     if status is not None and (status.dtype is not i32 or status.get_device() != index or status.numel() < 1):
         raise GhostFlowError(_lib.INVALID_DATA, f"status must be an int32 tensor on {dev}")
     # (a stride over a single element says nothing)

@@ -696,3 +696,17 @@ def test_every_border_between_steps(torch_dev):
     for name, t in _expected(b).items():
         assert torch.equal(x[name].cpu(), t), name
     assert int(status) == 0
+
+
+@pytest.mark.parametrize("name", ["page_table", "q_offsets", "kv_lens"])
+def test_the_wrong_argument_is_named(torch_dev, name):
+    gh = _gh()
+    b = Q.to(Q.batch([1, 1], [20, 9], kind="bf16", heads=2, kv_heads=1, d=32, page=16, seed=23), torch_dev)
+    twice = torch.stack((b[name], b[name]), -1)
+    for bad in (b[name].long(), b[name].cpu(), twice[..., 0]):
+        x = {**b, name: bad}
+        for call in (lambda: gh.paged_attention(x["q"], *P.args(x), **Q.scales(x)),
+                     lambda: gh.paged_append(*P.args(x), x["k"], x["v"], **Q.scales(x)),
+                     lambda: gh.paged_read(*P.args(x), tokens=2, **Q.scales(x))):
+            with pytest.raises(gh.GhostFlowError, match=rf"(?<!and ){name} must be a contiguous int32 tensor"):
+                call()
