@@ -267,14 +267,17 @@ class MultiHeadAttention:
                         ((self.q_weight, self.q_bias), (self.k_weight, self.k_bias), (self.v_weight, self.v_bias),
                          (self.out_weight, self.out_bias)))
 
-    def step_paged(self, x, cache: PagedKVCache, batch: PagedBatch, *, cos=None, sin=None, interleaved=False, window=0):
+    def step_paged(self, x, cache: PagedKVCache, batch: PagedBatch, *, cos=None, sin=None, interleaved=False, window=0,
+                   status=None):
         """Self-attention of the batch's new tokens x [tokens, E] over their
         sequences, causal, their keys and values appended to the pages: a
         prompt's chunks and single tokens in one call.  cos and sin
         [positions, rotary_dim / 2] turn queries and keys; they cover whole
         pages of the longest sequence.  fp32, or after quantize_grouped() any
         type that the cache takes.  After enable_qk_norm() queries and keys are
-        normed first."""
+        normed first.  status (int32, on the device) gets the bits of what could
+        not be written or read, as in paged_append: 4 for keys and values that
+        8 bits cut, or NaN."""
         weights = self._weights(norms=True)
         if x.dim() != 2 or tuple(x.shape) != (batch.tokens, self.embed_dim):
             raise GhostFlowError(_lib.INVALID_SHAPE, f"x must be [{batch.tokens}, {self.embed_dim}], got {list(x.shape)}")
@@ -284,10 +287,10 @@ class MultiHeadAttention:
             project = lambda i, t: linear(t, weights[2 * i], weights[2 * i + 1])  # noqa: E731
         q, k, v = (project(i, x).view(-1, self.num_heads, self.head_dim) for i in range(3))
         pages = (cache.k_pages, cache.v_pages, batch.page_table, batch.q_offsets, batch.kv_lens)
-        scales = {"k_scales": cache.k_scales, "v_scales": cache.v_scales}
+        rest = {"k_scales": cache.k_scales, "v_scales": cache.v_scales, "status": status}
         paged_append(*pages, k, v, q=q, q_out=q, cos=cos, sin=sin, interleaved=interleaved, q_norm=self.q_norm,
-                     k_norm=self.k_norm, norm_eps=self.norm_eps, **scales)
-        y = paged_attention(q, *pages, window=window, max_kv_len=batch.max_kv_len, out=q, **scales)
+                     k_norm=self.k_norm, norm_eps=self.norm_eps, **rest)
+        y = paged_attention(q, *pages, window=window, max_kv_len=batch.max_kv_len, out=q, **rest)
         return project(3, y.view(-1, self.embed_dim))
 
     def parameters(self):

@@ -710,3 +710,25 @@ def test_the_wrong_argument_is_named(torch_dev, name):
                      lambda: gh.paged_read(*P.args(x), tokens=2, **Q.scales(x))):
             with pytest.raises(gh.GhostFlowError, match=rf"(?<!and ){name} must be a contiguous int32 tensor"):
                 call()
+
+
+def test_a_layer_says_what_it_could_not_write(torch_dev):
+    """step_paged's status: values past the largest code's, and NaN, set bit 2; a page outside
+    the cache bit 1."""
+    gh = _gh()
+    torch.manual_seed(24)
+    m = gh.MultiHeadAttention(64, 2)
+    m.eval()
+    status = torch.zeros(1, dtype=torch.int32, device=torch_dev)
+    for scale, bits in ((1.0, 0), (1e7, 4), (float("nan"), 4)):
+        c = gh.PagedKVCache(4, 8, 2, 32, dtype=torch.uint8)
+        x = torch.randn(3, 64, device=torch_dev) * scale
+        status.zero_()
+        m.step_paged(x, c, c.extend([c.add()], [3]), status=status)
+        assert int(status) == bits, scale
+    c = gh.PagedKVCache(4, 8, 2, 32)
+    batch = c.extend([c.add()], [3])
+    batch.page_table.fill_(9)
+    status.zero_()
+    m.step_paged(torch.randn(3, 64, device=torch_dev), c, batch, status=status)
+    assert int(status) == 2
