@@ -1185,8 +1185,8 @@ int launch_paged_attention(const PagedAttnDesc &d, void *workspace, hipStream_t 
     p.q = static_cast<const char *>(d.q);
     p.out = static_cast<char *>(d.out);
     p.ldq = d.ldq, p.ldo = d.ldo;
-    // (a scale of 0 keeps masked scores at -inf)
-    p.sc2 = d.scale == 0.f ? 1e-38f : std::fabs(d.scale) * 0x1.715476p+0f;
+    // (for a scale of 0 the smallest number: masked scores stay at -inf, and no finite one reaches 2^-20)
+    p.sc2 = d.scale == 0.f ? 0x1p-149f : std::fabs(d.scale) * 0x1.715476p+0f;
     p.negate = d.scale < 0.f;
     p.causal = d.causal;
     p.window = d.window >= p.c.capacity ? 0 : (int)d.window;

@@ -619,3 +619,12 @@ def test_rows_one_by_one_over_a_page_outside_the_cache(torch_dev, types, lens, d
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.isnan(got[-1, 2:, 2]).all()
     fine = torch.isfinite(want)
     assert (got - want).abs()[fine].le(bound[fine]).all()
+
+
+@pytest.mark.parametrize("types", [t for t in P.PAIRS if t[0] != "f16"], ids="/".join)
+def test_attention_scale_of_nothing_over_huge_scores(torch_dev, types):
+    """All weights are equal where the scale is 0, however large the products."""
+    b = P.batch([1, 60, 400], [200, 150, 900], heads=4, kv_heads=2, d=64, page=16, types=types, seed=41)
+    b["q"] *= 1e36
+    _check(_attend(torch_dev, b, scale=0.0), *P.attention(b, scale=0.0))
+    _check(_attend(torch_dev, b, scale=0.0, window=40), *P.attention(b, scale=0.0, window=40))
