@@ -13,7 +13,7 @@
 // everything is read and written once.
 //
 // Bound by bytes where there are many tokens (16000 of 32 heads over 8 of 128, fp32 into
-// codes: 73 us; 20000 of 16 over 4, bf16 with norms: 145 MB in 36 us, 4.0 TB/s), by the way
+// codes: 73 to 77 us; 20000 of 16 over 4, bf16 with norms: 145 MB in 36 us, 4.0 TB/s), by the way
 // from offsets to length to page where there are few (64 tokens 5.5 us).  A wave's values are
 // on their way while it finds its page (after it: 38.5 instead of 36.4 us).
 #include "common.hpp"

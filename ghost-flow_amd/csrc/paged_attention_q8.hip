@@ -144,8 +144,9 @@ __device__ __forceinline__ f16x8 as_operand(uint32_t a, uint32_t b, uint32_t c, 
 // The next tile's K is asked for when this one's has been multiplied, V likewise: half
 // a tile per wave is on its way at any time, in registers that are free anyway.
 //
-// Bound by bytes: 64 sequences of up to 4096 keys, 32 heads over 8 of 128, bf16, 333 MB: 72 us
-// (4.6 TB/s) and 5 for the join.  Two tiles ahead (234 registers) gained nothing, four waves
+// Bound by bytes, and by their latency: 64 sequences of up to 4096 keys, 32 heads over 8 of 128,
+// 333 MB: bf16 72 to 79 us (4.2 to 4.6 TB/s) and 5 for the join, fp32 with two workgroups to a CU
+// 96 with it; pages of 100 rows, a look-up and a byte of steps per key, 100 and 146.  Two tiles ahead (234 registers) gained nothing, four waves
 // per SIMD spill (134 us), loads that stay in the caches took 82.  One token over 517 keys:
 // 9.7 us, the way from offsets to length to page to codes and the waves' join.
 template <typename TA, int DP, int NQ, int WAVES>
@@ -390,8 +391,9 @@ __global__ __launch_bounds__(64 * WAVES, NQ > 1 ? 2 : 3) void paged_q8_decode_ke
 //
 // Bound by the vector ALU and the matrix units together, as the 16-bit kernel is, with some
 // 90 vector instructions per wave and tile more for the codes (of 290; half as many in tiles
-// of 256 rows): 2048 tokens over 16384 keys, 32 heads over 8 of 128, 515 GFLOP, bf16 532 us
-// (0.97 PFLOP/s; 515 over an f16 cache), fp32 in two pieces 902 (1.14 PFLOP/s of products).
+// of 256 rows): 2048 tokens over 16384 keys, 32 heads over 8 of 128, 515 GFLOP, bf16 537 to 566 us
+// from card to card (0.91 to 0.96 PFLOP/s; 542 where a bf16 cache takes 511), f16 738 to 756 (773
+// GFLOP with two pieces of P, 1.04), fp32 in two pieces 885 to 904 (1.15).
 //
 // P is rounded to f16 for bf16 q, and is two pieces (22 bits) for f16 and fp32.  Relative errors
 // against 64 bits there (root of the mean square) and us, one piece / two: bf16 1.67e-3 / 1.66e-3,

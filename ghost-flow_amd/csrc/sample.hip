@@ -8,11 +8,11 @@
 // total.
 //
 // Weights are integers, round(w 2^44): sums are exact in 64 bits (up to 2^19 entries),
-// the same in any order, and a border between two tokens lies within 2^-35 of its
-// place whatever the vocabulary, so no u meets another token than in a longer format
-// but for one in 10^10.  An exponential is a table of 2^(j / 128), a polynomial of four
-// terms beyond (2e-15) and the exponent: 17 operations without a branch, 9 of them fp64,
-// which this card issues at the rate of fp32.
+// the same in any order.  A border between two tokens is off by what the roundings before
+// it add up to: some 2^-35 of the largest weight where they are independent, and n 2^-45 for
+// n logits that are equal, 2^-26 at worst (a step of u is 2^-24).  An exponential is a table
+// of 2^(j / 128), a polynomial of four terms beyond (2e-15) and the exponent: 17 operations
+// without a branch, 9 of them fp64, which this card issues at the rate of fp32.
 //
 // Two launches.  The first (a workgroup per 4096 logits, read once) leaves the largest of
 // every 16, of its 4096 and where it is, and, where the row's settings need the sum of all
@@ -30,10 +30,12 @@
 //    is searched whole, by bins, then the cut's 32 bits by eleven, eleven and ten.
 //
 // Bound by the way through a row's single workgroup, and the first launch of many rows by the
-// exponentials' operations beside the bytes.  Launches, us: one row of 32000, top-k and top-p,
-// fp32 3.3 and 12; 64 rows of 131072, settings of all kinds, bf16 11 and 26; 256 rows of 50257
-// without filters, fp32 18 (2.8 TB/s) and 7.  Per stage of top-p over 131072: 3 to the cut
-// cell and bin, 9 to list the bin, 5 to the cut's key, 4 to the token.
+// vector ALU: some 36 instructions to a logit without filters, 12.6 us of issue of the 13.7 that
+// the CUs are busy with 256 rows of 50257 (2.5 are an empty launch's; LDS 2.6, half of that
+// conflicts of the table's look-ups).  Launches, us: one row of 32000, top-k and top-p, fp32 3.3
+// and 12; 64 rows of 131072, settings of all kinds, bf16 10 and 26; 256 rows of 50257 without
+// filters, fp32 18 (2.8 TB/s) and 7.  Per stage of top-p over 131072: 3 to the cut cell and
+// bin, 9 to list the bin, 5 to the cut's key, 4 to the token.
 #include <climits>
 #include <cmath>
 #include <type_traits>

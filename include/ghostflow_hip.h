@@ -313,9 +313,9 @@ typedef struct gfh_sampling {
  * of those the ones with w >= min_p.  tokens[row] is the first of them, by index, whose
  * running sum of w exceeds u times their total; logprobs (nullable) gets the logarithm of
  * its w over that total.  Weights are held to 2^-45 of the largest and summed exactly,
- * so results do not depend on the order of sums.  A logit of -inf or NaN is never
- * drawn; of infinite ones all are alike and the others have w = 0; a row with none to draw
- * gets -1 (and NaN).  vocab <= 2^19.  workspace (nullable, 16-byte aligned) of at least
+ * so results do not depend on the order of sums.  A logit of -inf or NaN, or whose w is
+ * held as 0, is never drawn; of infinite ones all are alike and the others have w = 0; a row
+ * with none to draw gets -1 (and NaN).  vocab <= 2^19.  workspace (nullable, 16-byte aligned) of at least
  * gfh_sample_workspace_size(rows, vocab) bytes, any contents. */
 GFH_API size_t gfh_sample_workspace_size(int64_t rows, int64_t vocab);
 GFH_API int gfh_sample(int dtype, const void *logits, int64_t ld, int64_t rows, int64_t vocab, const float *u,
